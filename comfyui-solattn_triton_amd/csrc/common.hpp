@@ -183,4 +183,16 @@ int fwd_int8(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const 
              uint16_t* o, int64_t so_b, int64_t so_t, int64_t so_h, solattn_stream_t stream,
              bool uniform_ks, bool ks_head_major = false);
 
+// Attention of one token per sequence over a cache, split over its length (paged.hip).
+// table null: sequence b is page b, and the token sits at position length - 1 of the
+// sequences that lengths (if any) says are that long.
+int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k, int64_t sk_p, int64_t sk_s,
+               int64_t sk_h, const uint16_t* v, int64_t sv_p, int64_t sv_s, int64_t sv_h, int64_t pages,
+               int64_t page_size, const int32_t* table, int64_t table_stride, int64_t max_pages,
+               const int32_t* lengths, int64_t length, int64_t B, int64_t H, int64_t Hkv, int64_t D, int dtype,
+               int64_t window, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, uint16_t* o,
+               int64_t so_b, int64_t so_h, hipStream_t s, const char* what);
+int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
+                             int64_t sinks);
+
 }  // namespace solattn

@@ -1,0 +1,389 @@
+// Sliding-window attention with sinks: forward and gradients, causal or symmetric,
+// kv heads shared by a group of query heads, padded batches (window_common.hpp has
+// the rule of what a row sees).
+//
+//   o_i = sum_j P_ij v_j,  P_ij = exp(scale q_i.k_j - lse_i)
+//   D_i = do_i . o_i,  dS = P (do_i . v_j - D_i)
+//   dv_j = sum_i P do_i,  dq_i = scale sum_j dS k_j,  dk_j = scale sum_i dS q_i
+//
+// Bound: the matrix instructions and, beside them, the exps. Everything between
+// the products stays in registers: S^T = K Q^T puts a row on a lane column, so its
+// statistics need one exchange (lanes 32 apart) and P converts in place into the B
+// operand of the next product, whose A operand is read transposed from LDS
+// (ds_read_b64_tr_b16). P and dS are rounded to the inputs' type for the matrix
+// instruction; row sums add P as rounded, every other sum is fp32.
+#include "window_common.hpp"
+
+namespace solattn {
+namespace {
+
+constexpr int kRows = 128;            // query rows (or keys) of a workgroup
+constexpr int kThreads = 2 * kRows;   // a wave for 32 of them
+
+// Running maximum before any visible key: finite, so that exp2 of a masked score
+// stays 0, and below every score that counts.
+constexpr float kNoMax = -1e30f;
+
+// Workgroup -> (batch, kv head, block of rows, query head): the query heads of one
+// kv head and block run side by side.
+__device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, int& qb) {
+  uint32_t w = xcd_run(blockIdx.x, gridDim.x);
+  const int g = w % a.group;
+  w /= a.group;
+  qb = w % a.nqb;
+  w /= a.nqb;
+  h = (w % a.Hkv) * a.group + g;
+  b = w / a.Hkv;
+}
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
+window_fwd_kernel(const WindowArgs a) {
+  constexpr int ND = D / 32, NC = D / 16;
+  __shared__ __align__(256) uint16_t kbuf[kKeys * D];
+  __shared__ __align__(256) uint16_t vbuf[kKeys * D];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  int b, h, qb;
+  row_item(a, b, h, qb);
+  const int len = sequence_length(a, b), hk = h / a.group;
+  const int r0 = qb * kRows, row = r0 + wave_id() * 32 + (lane & 31);
+  const int p = a.q_start + min(row, a.Tq - 1);
+  const KeyTiles kt = key_tiles(a, a.q_start + r0, a.q_start + min(r0 + kRows, a.Tq) - 1, len);
+  const RowKeys rk = row_keys(a, p, len);
+  const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
+  const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
+  const uint32_t kb = lds_addr(kbuf), vb = lds_addr(vbuf);
+  const TileAddr<D, kByRow> ka(kb, lane);
+  const TileAddr<D, kTransposed> va(vb, lane);
+  bf16x8 q[NC];
+  load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(min(row, a.Tq - 1)) * a.q.t + h * a.q.h, half);
+
+  f32x16 acc[ND] = {};
+  float m = kNoMax, l = 0.f;
+  for (int t = 0; t < kt.n; ++t) {
+    const int j0 = kt.first(t);
+    const auto safe = [&](int r) { return kt.safe(j0 + r); };
+    __syncthreads();
+    copy_tile<kThreads, D, kByRow>(kb, kp, a.k.t, safe);
+    copy_tile<kThreads, D, kTransposed>(vb, vp, a.v.t, safe);
+    wait_tile_copies();
+    __syncthreads();
+#pragma unroll
+    for (int m2 = 0; m2 < 2; ++m2) {
+      f32x16 s = {};
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc), q[cc], s);
+      mask_keys(s, rk, j0 + 32 * m2, half);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      const float m_new = fmaxf(m, xhalf_max(mx) * a.c);
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -m));
+      bf16x8 pb[2];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        pb[ks] = pack8<E>(s, ks);
+        const uint4 w = __builtin_bit_cast(uint4, pb[ks]);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += E::lo(u[i]) + E::hi(u[i]);
+      }
+      l = fmaf(l, alpha, sum);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) acc[dt] *= alpha;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(va.transposed(2 * m2 + ks, dt), pb[ks], acc[dt]);
+    }
+  }
+  l = xhalf_sum(l);
+  const bool on = row < a.Tq;
+  store_row<E>(acc, l == 0.f ? 0.f : 1.f / l, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h,
+               on, half);
+  if (a.lse && on && half == 0)
+    a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
+window_dq_kernel(const WindowArgs a) {
+  constexpr int ND = D / 32, NC = D / 16;
+  __shared__ __align__(256) uint16_t kbuf[kKeys * D];
+  __shared__ __align__(256) uint16_t vbuf[kKeys * D];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  int b, h, qb;
+  row_item(a, b, h, qb);
+  const int len = sequence_length(a, b), hk = h / a.group;
+  const int r0 = qb * kRows, row = r0 + wave_id() * 32 + (lane & 31), rr = min(row, a.Tq - 1);
+  const int p = a.q_start + rr;
+  const KeyTiles kt = key_tiles(a, a.q_start + r0, a.q_start + min(r0 + kRows, a.Tq) - 1, len);
+  const RowKeys rk = row_keys(a, p, len);
+  const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
+  const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
+  const uint32_t kb = lds_addr(kbuf), vb = lds_addr(vbuf);
+  const TileAddr<D, kBoth> ka(kb, lane);
+  const TileAddr<D, kByRow> va(vb, lane);
+  bf16x8 q[NC], g[NC];
+  load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
+  load_row<D>(g, a.d_o.p + b * a.d_o.b + static_cast<int64_t>(rr) * a.d_o.t + h * a.d_o.h, half);
+  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.Tq + rr;
+  float delta = 0.f;
+  {
+    bf16x8 o[NC];
+    load_row<D>(o, a.o.p + b * a.o.b + static_cast<int64_t>(rr) * a.o.t + h * a.o.h, half);
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) {
+      const uint4 x = __builtin_bit_cast(uint4, o[cc]), y = __builtin_bit_cast(uint4, g[cc]);
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) delta = fmaf(E::lo(u[i]), E::lo(w[i]), fmaf(E::hi(u[i]), E::hi(w[i]), delta));
+    }
+    delta = xhalf_sum(delta);
+  }
+  const float neg = -a.lse[at];  // -inf for a row that sees nothing
+  if (row < a.Tq && half == 0) a.delta[at] = delta;
+
+  f32x16 acc[ND] = {};
+  for (int t = 0; t < kt.n; ++t) {
+    const int j0 = kt.first(t);
+    const auto safe = [&](int r) { return kt.safe(j0 + r); };
+    __syncthreads();
+    copy_tile<kThreads, D, kBoth>(kb, kp, a.k.t, safe);
+    copy_tile<kThreads, D, kByRow>(vb, vp, a.v.t, safe);
+    wait_tile_copies();
+    __syncthreads();
+#pragma unroll
+    for (int m2 = 0; m2 < 2; ++m2) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc), q[cc], s);
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(va.by_row(m2, cc), g[cc], dp);
+      mask_keys(s, rk, j0 + 32 * m2, half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, neg));
+        s[r] = s[r] == -INFINITY ? 0.f : pr * (dp[r] - delta);  // (a masked dp may be anything)
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const bf16x8 ds = pack8<E>(s, ks);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(ka.transposed(2 * m2 + ks, dt), ds, acc[dt]);
+      }
+    }
+  }
+  store_row<E>(acc, a.scale, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h, row < a.Tq,
+               half);
+}
+
+// dk and dv: a workgroup owns 128 keys of a kv head and walks the rows that see
+// any of them, head by head of the group; a wave's 32 keys stay in registers.
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+window_dkv_kernel(const WindowArgs a) {
+  constexpr int ND = D / 32, NC = D / 16;
+  __shared__ __align__(256) uint16_t qbuf[kKeys * D];
+  __shared__ __align__(256) uint16_t gbuf[kKeys * D];
+  __shared__ float lse[kKeys], delta[kKeys];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  uint32_t w = xcd_run(blockIdx.x, gridDim.x);
+  const int kblk = w % a.nkb;
+  w /= a.nkb;
+  const int hk = w % a.Hkv, b = w / a.Hkv;
+  const int len = sequence_length(a, b);
+  const int j0 = kblk * kRows, j = j0 + wave_id() * 32 + (lane & 31), jj = min(j, a.Tk - 1);
+  const KeyRows kr = key_rows(a, j < a.Tk ? j : len, len);
+  // rows that see a key of the block: a key's interval only moves up with it, but that a sink's has no end
+  const int jlast = min(min(j0 + kRows, a.Tk), len) - 1;
+  const KeyRows k0 = key_rows(a, j0, len), k1 = key_rows(a, max(jlast, j0), len);
+  const int i0 = k0.pl - a.q_start, i1 = (j0 < a.sinks ? k0.ph : k1.ph) - a.q_start;  // rows [i0, i1]
+  const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf);
+  const TileAddr<D, kBoth> qa(qb, lane), ga(gb, lane);
+  bf16x8 k[NC], v[NC];
+  load_row<D>(k, a.k.p + b * a.k.b + static_cast<int64_t>(jj) * a.k.t + hk * a.k.h, half);
+  load_row<D>(v, a.v.p + b * a.v.b + static_cast<int64_t>(jj) * a.v.t + hk * a.v.h, half);
+
+  f32x16 dk[ND] = {}, dv[ND] = {};
+  if (j0 < len && i0 <= i1) {
+    for (int g = 0; g < a.group; ++g) {
+      const int h = hk * a.group + g;
+      const uint16_t* qp = a.q.p + b * a.q.b + h * a.q.h;
+      const uint16_t* gp = a.d_o.p + b * a.d_o.b + h * a.d_o.h;
+      const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Tq;
+      for (int t0 = i0 & ~(kKeys - 1); t0 <= i1; t0 += kKeys) {
+        const auto safe = [&](int r) { return min(max(t0 + r, i0), i1); };
+        __syncthreads();
+        copy_tile<kThreads, D, kBoth>(qb, qp, a.q.t, safe);
+        copy_tile<kThreads, D, kBoth>(gb, gp, a.d_o.t, safe);
+        if (threadIdx.x < kKeys)
+          lse[threadIdx.x] = a.lse[stat + safe(threadIdx.x)];
+        else if (threadIdx.x < 2 * kKeys)
+          delta[threadIdx.x - kKeys] = a.delta[stat + safe(threadIdx.x - kKeys)];
+        wait_tile_copies();
+        __syncthreads();
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          f32x16 s = {}, dp = {};
+#pragma unroll
+          for (int cc = 0; cc < NC; ++cc) s = E::mfma32(qa.by_row(m2, cc), k[cc], s);
+#pragma unroll
+          for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(ga.by_row(m2, cc), v[cc], dp);
+          const int off = a.q_start + t0 + 32 * m2 + 4 * half - kr.pl;
+          const uint32_t span = static_cast<uint32_t>(kr.ph - kr.pl);
+          const bool none = kr.ph < kr.pl;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = 8 * (r >> 2) + (r & 3);
+            const bool on = !none && static_cast<uint32_t>(off + i) <= span;
+            const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse[32 * m2 + 4 * half + i]));
+            s[r] = on ? pr : 0.f;
+            dp[r] = on ? pr * (dp[r] - delta[32 * m2 + 4 * half + i]) : 0.f;
+          }
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const bf16x8 pb = pack8<E>(s, ks), ds = pack8<E>(dp, ks);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dv[dt] = E::mfma32(ga.transposed(2 * m2 + ks, dt), pb, dv[dt]);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dk[dt] = E::mfma32(qa.transposed(2 * m2 + ks, dt), ds, dk[dt]);
+          }
+        }
+      }
+    }
+  }
+  const bool on = j < a.Tk;
+  store_row<E>(dk, a.scale, a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h, on, half);
+  store_row<E>(dv, 1.f, a.dv + b * a.dv_b + static_cast<int64_t>(j) * a.dv_t + hk * a.dv_h, on, half);
+}
+
+int check_mat(const Mat& m, const char* what, const char* name) {
+  SOLATTN_REQUIRE(m.p, SOLATTN_EINVAL, "%s: null %s", what, name);
+  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.b % 8 == 0 && m.t % 8 == 0 && m.h % 8 == 0,
+                  SOLATTN_EINVAL, "%s: %s must be 16-byte aligned with strides multiple of 8", what, name);
+  return 0;
+}
+
+int setup(WindowArgs& a, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv, int64_t D, int dtype,
+          int64_t q_start, int64_t window, int64_t sinks, int causal, float scale, const char* what) {
+  SOLATTN_REQUIRE(dtype == SOLATTN_BF16 || dtype == SOLATTN_FP16, SOLATTN_EINVAL, "%s: dtype %d", what, dtype);
+  SOLATTN_REQUIRE(B > 0 && Tq > 0 && Tk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0, SOLATTN_EINVAL,
+                  "%s: bad sizes (%lld query heads over %lld kv heads)", what, (long long)H, (long long)Hkv);
+  SOLATTN_REQUIRE(D == 64 || D == 128, SOLATTN_EUNSUPPORTED, "%s: head_dim %lld not in {64, 128}", what, (long long)D);
+  SOLATTN_REQUIRE(Tk < (1ll << 29), SOLATTN_EUNSUPPORTED, "%s: %lld keys", what, (long long)Tk);
+  SOLATTN_REQUIRE(q_start >= 0 && q_start + Tq <= Tk, SOLATTN_EINVAL, "%s: rows %lld + %lld past %lld keys", what,
+                  (long long)q_start, (long long)Tq, (long long)Tk);
+  SOLATTN_REQUIRE(window > 0 && sinks >= 0, SOLATTN_EINVAL, "%s: window %lld, sinks %lld", what, (long long)window,
+                  (long long)sinks);
+  SOLATTN_REQUIRE(scale > 0.f, SOLATTN_EINVAL, "%s: scale %g", what, static_cast<double>(scale));
+  a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.Hkv = static_cast<int>(Hkv);
+  a.group = static_cast<int>(H / Hkv);
+  a.Tq = static_cast<int>(Tq), a.Tk = static_cast<int>(Tk), a.q_start = static_cast<int>(q_start);
+  // wider than the sequence is the same as wide as it
+  a.window = static_cast<int>(window < Tk ? window : Tk), a.sinks = static_cast<int>(sinks < Tk ? sinks : Tk);
+  a.causal = causal;
+  a.nqb = static_cast<int>(cdiv(Tq, kRows)), a.nkb = static_cast<int>(cdiv(Tk, kRows));
+  a.c = scale * kLog2e, a.scale = scale;
+  SOLATTN_REQUIRE(B * H * a.nqb < (1ll << 31) && B * Hkv * a.nkb < (1ll << 31), SOLATTN_EUNSUPPORTED,
+                  "%s: grid too large", what);
+  return 0;
+}
+
+}  // namespace
+}  // namespace solattn
+
+using namespace solattn;
+
+// One causal row per sequence: the kernel of single tokens, which splits the keys.
+static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq == 1 && causal && !lse; }
+
+extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t H, int64_t Hkv, int64_t D,
+                                                       int64_t q_start, int64_t window, int64_t sinks, int causal) {
+  return single_token(Tq, causal, nullptr) ? paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks) : 0;
+}
+
+extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k,
+                                   int64_t sk_b, int64_t sk_t, int64_t sk_h, const uint16_t* v, int64_t sv_b,
+                                   int64_t sv_t, int64_t sv_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                                   int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths,
+                                   int64_t window, int64_t sinks, int causal, float scale, uint16_t* o, int64_t so_b,
+                                   int64_t so_t, int64_t so_h, float* lse, void* workspace, int64_t workspace_bytes,
+                                   solattn_stream_t stream) {
+  clear_error();
+  const char* what = "window_attn";
+  if (single_token(Tq, causal, lse)) {
+    SOLATTN_REQUIRE(window > 0 && q_start >= 0 && q_start < Tk, SOLATTN_EINVAL, "%s: row %lld of %lld keys, window %lld",
+                    what, (long long)q_start, (long long)Tk, (long long)window);
+    return paged_attn(q, sq_b, sq_h, k, sk_b, sk_t, sk_h, v, sv_b, sv_t, sv_h, B, q_start + 1, nullptr, 0, 1, lengths,
+                      q_start + 1, B, H, Hkv, D, dtype, window, sinks, scale, workspace, workspace_bytes, o, so_b, so_h,
+                      reinterpret_cast<hipStream_t>(stream), what);
+  }
+  WindowArgs a{};
+  a.q = {q, sq_b, sq_t, sq_h}, a.k = {k, sk_b, sk_t, sk_h}, a.v = {v, sv_b, sv_t, sv_h};
+  a.out = o, a.out_b = so_b, a.out_t = so_t, a.out_h = so_h;
+  a.lse = lse, a.lengths = lengths;
+  int rc = setup(a, B, Tq, Tk, H, Hkv, D, dtype, q_start, window, sinks, causal, scale, what);
+  if (!rc) rc = check_mat(a.q, what, "q");
+  if (!rc) rc = check_mat(a.k, what, "k");
+  if (!rc) rc = check_mat(a.v, what, "v");
+  if (!rc) rc = check_mat({o, so_b, so_t, so_h}, what, "o");
+  if (rc) return rc;
+  const bool bf = dtype == SOLATTN_BF16;
+  const auto kern = D == 128 ? (bf ? window_fwd_kernel<Bf16, 128> : window_fwd_kernel<Fp16, 128>)
+                             : (bf ? window_fwd_kernel<Bf16, 64> : window_fwd_kernel<Fp16, 64>);
+  hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(B * H * a.nqb)), dim3(kThreads), 0,
+                     reinterpret_cast<hipStream_t>(stream), a);
+  return check_launch(what);
+}
+
+extern "C" int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t H) {
+  return B <= 0 || Tq <= 0 || H <= 0 ? 0 : cdiv(B * H * Tq * 4, 256) * 256;
+}
+
+extern "C" int solattn_window_attn_bwd(
+    const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k, int64_t sk_b, int64_t sk_t,
+    int64_t sk_h, const uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, const uint16_t* o, int64_t so_b,
+    int64_t so_t, int64_t so_h, const uint16_t* d_o, int64_t sg_b, int64_t sg_t, int64_t sg_h, const float* lse,
+    int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t q_start,
+    const int32_t* lengths, int64_t window, int64_t sinks, int causal, float scale, uint16_t* dq, int64_t sdq_b,
+    int64_t sdq_t, int64_t sdq_h, uint16_t* dk, int64_t sdk_b, int64_t sdk_t, int64_t sdk_h, uint16_t* dv,
+    int64_t sdv_b, int64_t sdv_t, int64_t sdv_h, void* workspace, int64_t workspace_bytes, solattn_stream_t stream) {
+  clear_error();
+  const char* what = "window_attn_bwd";
+  WindowArgs a{};
+  a.q = {q, sq_b, sq_t, sq_h}, a.k = {k, sk_b, sk_t, sk_h}, a.v = {v, sv_b, sv_t, sv_h};
+  a.o = {o, so_b, so_t, so_h}, a.d_o = {d_o, sg_b, sg_t, sg_h};
+  a.out = dq, a.out_b = sdq_b, a.out_t = sdq_t, a.out_h = sdq_h;
+  a.dk = dk, a.dk_b = sdk_b, a.dk_t = sdk_t, a.dk_h = sdk_h;
+  a.dv = dv, a.dv_b = sdv_b, a.dv_t = sdv_t, a.dv_h = sdv_h;
+  a.lse = const_cast<float*>(lse), a.lengths = lengths;
+  int rc = setup(a, B, Tq, Tk, H, Hkv, D, dtype, q_start, window, sinks, causal, scale, what);
+  const Mat outs[3] = {{dq, sdq_b, sdq_t, sdq_h}, {dk, sdk_b, sdk_t, sdk_h}, {dv, sdv_b, sdv_t, sdv_h}};
+  const Mat* mats[8] = {&a.q, &a.k, &a.v, &a.o, &a.d_o, &outs[0], &outs[1], &outs[2]};
+  const char* names[8] = {"q", "k", "v", "o", "do", "dq", "dk", "dv"};
+  for (int i = 0; i < 8 && !rc; ++i) rc = check_mat(*mats[i], what, names[i]);
+  if (rc) return rc;
+  SOLATTN_REQUIRE(lse, SOLATTN_EINVAL, "%s: null lse", what);
+  SOLATTN_REQUIRE(workspace && workspace_bytes >= solattn_window_attn_bwd_workspace_bytes(B, Tq, H), SOLATTN_ESIZE,
+                  "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes,
+                  (long long)solattn_window_attn_bwd_workspace_bytes(B, Tq, H));
+  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SOLATTN_EINVAL,
+                  "%s: workspace must be 256-byte aligned", what);
+  a.delta = static_cast<float*>(workspace);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool bf = dtype == SOLATTN_BF16;
+  const auto kq = D == 128 ? (bf ? window_dq_kernel<Bf16, 128> : window_dq_kernel<Fp16, 128>)
+                           : (bf ? window_dq_kernel<Bf16, 64> : window_dq_kernel<Fp16, 64>);
+  hipLaunchKernelGGL(kq, dim3(static_cast<uint32_t>(B * H * a.nqb)), dim3(kThreads), 0, s, a);
+  if ((rc = check_launch(what))) return rc;
+  const auto kk = D == 128 ? (bf ? window_dkv_kernel<Bf16, 128> : window_dkv_kernel<Fp16, 128>)
+                           : (bf ? window_dkv_kernel<Bf16, 64> : window_dkv_kernel<Fp16, 64>);
+  hipLaunchKernelGGL(kk, dim3(static_cast<uint32_t>(B * Hkv * a.nkb)), dim3(kThreads), 0, s, a);
+  return check_launch(what);
+}

@@ -1,0 +1,226 @@
+// What the sliding-window kernels share: which keys a row sees, the 64-key tiles
+// of a block of rows, their copies into LDS and the 16-bit MFMA products.
+//
+// Row i sits at position p = q_start + i. With a window of W keys and S sinks it
+// sees, of the keys j < len, those of
+//   causal:    j <= p and (p - j < W or j < S)
+//   symmetric: |p - j| < W or j < S
+// and none when p >= len. Seen from a row the keys are the interval [jl, jh] and
+// those below sk; seen from a key the rows are one interval [pl, ph].
+#pragma once
+
+#include "elem.hpp"
+#include "fwd_common.hpp"
+
+namespace solattn {
+
+struct Mat {  // a BTHD tensor of 16-bit values, strides in elements
+  const uint16_t* p;
+  int64_t b, t, h;
+};
+
+struct WindowArgs {
+  Mat q, k, v, o, d_o;       // (o, d_o: backward's inputs)
+  uint16_t* out;             // forward: o; backward: dq
+  int64_t out_b, out_t, out_h;
+  uint16_t* dk;
+  int64_t dk_b, dk_t, dk_h;
+  uint16_t* dv;
+  int64_t dv_b, dv_t, dv_h;
+  float* lse;                // [B][H][Tq], log2 domain; +inf for a row that sees nothing
+  float* delta;              // [B][H][Tq]
+  const int32_t* lengths;    // null: Tk
+  int B, H, Hkv, group, Tq, Tk, q_start;
+  int window, sinks, causal; // window <= 2^30
+  int nqb, nkb;              // blocks of rows and of keys
+  float c, scale;            // c = scale log2(e)
+};
+
+__device__ __forceinline__ int sequence_length(const WindowArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+}
+
+// The keys of one row (see above): j in [jl, jh] or j < sk.
+struct RowKeys {
+  int jl, jh, sk;
+};
+__device__ __forceinline__ RowKeys row_keys(const WindowArgs& a, int p, int len) {
+  RowKeys r;
+  r.jl = p - a.window + 1;
+  r.jh = a.causal ? p : p + a.window - 1;
+  r.sk = a.causal ? min(a.sinks, p + 1) : a.sinks;
+  r.jh = min(r.jh, len - 1);
+  r.sk = min(r.sk, len);
+  if (p >= len) r.jl = 0, r.jh = -1, r.sk = 0;
+  return r;
+}
+
+// The rows of one key: p in [pl, ph]; none when pl > ph.
+struct KeyRows {
+  int pl, ph;
+};
+__device__ __forceinline__ KeyRows key_rows(const WindowArgs& a, int j, int len) {
+  KeyRows r;
+  const int end = min(len, a.q_start + a.Tq) - 1;
+  r.pl = a.causal ? j : j < a.sinks ? 0 : j - a.window + 1;
+  r.ph = j < a.sinks ? end : min(j + a.window - 1, end);
+  r.pl = max(r.pl, a.q_start);
+  if (j >= len) r.pl = 1, r.ph = 0;
+  return r;
+}
+
+// The 64-key tiles that rows [p0, p1] see: those of the sinks below the window,
+// then the window's. Keys of a tile that none of these rows sees are not read:
+// safe(j) is a key that is.
+struct KeyTiles {
+  int lo, hi;     // window keys of the rows, [lo, hi)
+  int s_end;      // sink keys below them
+  int ns, n, w0;  // sink tiles, tiles, first key of the first window tile
+  __device__ __forceinline__ int first(int t) const { return t < ns ? kKeys * t : w0 + kKeys * (t - ns); }
+  __device__ __forceinline__ int safe(int j) const { return j < s_end ? j : min(max(j, lo), hi - 1); }
+  __device__ __forceinline__ bool whole(int t) const {  // every key of the tile is some row's
+    const int j = first(t);
+    return j + kKeys <= s_end || (j >= lo && j + kKeys <= hi);
+  }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const WindowArgs& a, int p0, int p1, int len) {
+  KeyTiles k;
+  if (p0 >= len) {
+    k.lo = k.hi = k.s_end = k.ns = k.n = k.w0 = 0;
+    return k;
+  }
+  p1 = min(p1, len - 1);
+  k.lo = max(p0 - a.window + 1, 0);
+  k.hi = min(a.causal ? p1 + 1 : max(p1 + a.window, a.sinks), len);
+  k.s_end = min(a.sinks, k.lo);
+  k.w0 = k.lo & ~(kKeys - 1);
+  k.ns = min((k.s_end + kKeys - 1) / kKeys, k.w0 / kKeys);
+  k.n = k.ns + (k.hi - k.w0 + kKeys - 1) / kKeys;
+  return k;
+}
+
+// Workgroup id -> item of the launch, so that each of the 8 XCDs (dealt round
+// robin) walks a contiguous run: neighbouring items share their keys in its L2.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t w, uint32_t total) {
+  const uint32_t x = w & 7u, q8 = total >> 3, rem = total & 7u;
+  return x * q8 + min(x, rem) + (w >> 3);
+}
+
+// ------------------------------------------------------------------- LDS tiles
+// Tiles that are read both by rows (16-byte pieces of 16 rows) and transposed
+// (ds_read_b64_tr_b16: 4 rows x 4 consecutive pieces) need one swizzle that keeps
+// both free of conflicts: the row's low bits pick a quarter of the row for the
+// transposed read, the next ones a place within it.
+template <int D>
+__device__ __forceinline__ int swz_both(int row, int chunk) {
+  const int r = D == 128 ? row : row >> 1;
+  return D == 128 ? chunk ^ (((r & 3) << 2) | ((r >> 2) & 3)) : chunk ^ (((r & 1) << 2) | ((r >> 1) & 3));
+}
+
+// How a tile is read: by rows (K of the forward), transposed (its V) or both.
+enum { kByRow, kTransposed, kBoth };
+template <int D, int HOW>
+__device__ __forceinline__ int swz(int row, int chunk) {
+  return HOW == kByRow ? swz_k<D>(row, chunk) : HOW == kTransposed ? swz_v<D>(row, chunk) : swz_both<D>(row, chunk);
+}
+
+// 64 rows of D values into the LDS tile at dst, row i from base + row_of(i) stride.
+template <int NTHREADS, int D, int HOW, typename RowOf>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const uint16_t* base, int64_t stride, RowOf&& row_of) {
+  constexpr int C = D / 8, U = kKeys * C / NTHREADS;
+  const uint32_t l0 = dst + wave_id() * 64 * 16;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = threadIdx.x + NTHREADS * u, row = e / C, pc = e % C;
+    g2l16(base + static_cast<int64_t>(row_of(row)) * stride + swz<D, HOW>(row, pc) * 8, l0 + NTHREADS * u * 16);
+  }
+}
+
+// Operands of an LDS tile (256-byte aligned): the row operand (m, cc) is rows
+// 32 m + lane % 32, channels 16 cc + 8 (lane / 32) ..; the transposed operand
+// (ks, dt) is channel 32 dt + lane % 32 of rows 16 ks + 8 (e / 4) + 4 (lane / 32)
+// + e % 4. A lane keeps one address for the first and two for the second.
+template <int D, int HOW>
+struct TileAddr {
+  uint32_t row, tr0, tr1;
+  __device__ __forceinline__ TileAddr(uint32_t tile, int lane) {
+    const int col = lane & 31, half = lane >> 5;
+    row = tile + col * (2 * D) + 16 * swz<D, HOW>(col, half);
+    const int g = lane >> 4, sl = lane & 15, r0 = 4 * (g >> 1) + (sl >> 2), cp = 2 * (g & 1) + ((sl & 3) >> 1);
+    tr0 = tile + r0 * (2 * D) + 16 * swz<D, HOW>(r0, cp) + 8 * (sl & 1);
+    tr1 = tile + (r0 + 8) * (2 * D) + 16 * swz<D, HOW>(r0 + 8, cp) + 8 * (sl & 1);
+  }
+  __device__ __forceinline__ bf16x8 by_row(int m, int cc) const {
+    const uint32_t x = (row ^ static_cast<uint32_t>(cc << 5)) + m * (64 * D);
+    return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(static_cast<uintptr_t>(x));
+  }
+  __device__ __forceinline__ bf16x8 transposed(int ks, int dt) const {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    const uint32_t x0 = (tr0 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D);
+    const uint32_t x1 = (tr1 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D);
+    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) v4i16*>(static_cast<uintptr_t>(x0)));
+    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) v4i16*>(static_cast<uintptr_t>(x1)));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// This lane's row of a B operand straight from memory: channels 16 cc + 8 (lane / 32) ...
+template <int D>
+__device__ __forceinline__ void load_row(bf16x8 (&x)[D / 16], const uint16_t* row, int half) {
+#pragma unroll
+  for (int cc = 0; cc < D / 16; ++cc)
+    x[cc] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(row + 16 * cc + 8 * half));
+}
+
+// Rows of 32 columns of an accumulator pair-packed into a B operand: elements 8 ks .. 8 ks + 7.
+template <typename E>
+__device__ __forceinline__ bf16x8 pack8(const f32x16& s, int ks) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = E::pack(s[8 * ks + 2 * i], s[8 * ks + 2 * i + 1]);
+  return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// acc^T (channel 32 dt + 8 (r / 4) + 4 half + r % 4 of row `lane % 32`) times f into a row of D values.
+template <typename E, int ND>
+__device__ __forceinline__ void store_row(const f32x16 (&acc)[ND], float f, uint16_t* row, bool on, int half) {
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int ip = 0; ip < 2; ++ip) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = 4 * (2 * ip + u);
+        w[u][0] = E::pack(acc[dt][i] * f, acc[dt][i + 1] * f);
+        w[u][1] = E::pack(acc[dt][i + 2] * f, acc[dt][i + 3] * f);
+      }
+      uint32_t y[2];  // the two lanes of a row swap halves, so each writes 16 contiguous bytes
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t x = half ? w[0][e] : w[1][e];
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        y[e] = half ? r[0] : r[1];
+      }
+      const uint4 v = half ? make_uint4(y[0], y[1], w[1][0], w[1][1]) : make_uint4(w[0][0], w[0][1], y[0], y[1]);
+      if (on) *reinterpret_cast<uint4*>(row + 32 * dt + 16 * ip + 8 * half) = v;
+    }
+}
+
+// Scores of 32 keys (first + the key of element r) for this lane's row: those it does not see become -inf.
+__device__ __forceinline__ void mask_keys(f32x16& s, const RowKeys& rk, int first, int half) {
+  const int base = first + 4 * half;
+  const uint32_t span = static_cast<uint32_t>(rk.jh - rk.jl);
+  const int off = base - rk.jl, sk = rk.sk - base;
+  const bool none = rk.jh < rk.jl;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int k0 = 8 * (r >> 2) + (r & 3);
+    const bool on = (!none && static_cast<uint32_t>(off + k0) <= span) || k0 < sk;
+    s[r] = on ? s[r] : -INFINITY;
+  }
+}
+
+}  // namespace solattn

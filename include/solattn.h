@@ -359,6 +359,120 @@ int solattn_sol_attn_noalloc(const uint16_t* q, int64_t sq_b, int64_t sq_t, int6
                              int64_t sink_q_lo, int64_t sink_q_hi, uint16_t* o, int64_t so_b,
                              int64_t so_t, int64_t so_h, solattn_stream_t stream);
 
+/* ------------------------------------------------ operators around attention --
+ * Norms and rotation of queries and keys, sliding-window attention with sinks
+ * and attention of one new token over a paged cache: no counterpart in the
+ * reference. q, o: BTHD with H query heads; k, v: BTHD with Hkv kv heads, each
+ * shared by the H / Hkv query heads behind one another (H % Hkv == 0). Rows
+ * (the last dim) are contiguous, 16-byte aligned, and every stride keeps them
+ * so; strides may be 0 or negative for inputs. Sums, softmax statistics and
+ * accumulators are fp32; outputs are rounded once. */
+enum { SOLATTN_BF16 = 0, SOLATTN_FP16 = 1, SOLATTN_FP32 = 2 }; /* dtype arguments */
+
+/* Per (batch, token, head) row x of q and k, D channels (a multiple of 8 up to 128):
+ *   n = x / sqrt(mean(x^2) + eps) * weight        (weight null: 1)
+ *   y[i1] = n[i1] cos - n[i2] sin, y[i2] = n[i2] cos + n[i1] sin for the R / 2 pairs
+ *   of the first R channels, (i, i + R/2), or (2i, 2i + 1) when interleaved; the
+ *   other channels are n. R: a multiple of 16 (interleaved: 8), 0 for none.
+ * cos, sin: fp32 [P][R/2] by position. positions: int32 [B][T] with row stride
+ * pos_stride_b (0: shared), clamped to [0, P); null: token t is at t (T <= P).
+ * weights: fp32 [D]. dtype of q, k and the outputs: any SOLATTN_*; weights and
+ * tables 16-byte aligned. Hkv may be 0 (q alone). Outputs may be the inputs. */
+int solattn_qk_norm_rope(const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k,
+                         int64_t sk_b, int64_t sk_t, int64_t sk_h, int64_t B, int64_t T, int64_t H,
+                         int64_t Hkv, int64_t D, int dtype, const float* q_weight,
+                         const float* k_weight, const float* cos, const float* sin, int64_t P,
+                         int64_t R, int interleaved, const int32_t* positions,
+                         int64_t pos_stride_b, float eps, void* qo, int64_t sqo_b, int64_t sqo_t,
+                         int64_t sqo_h, void* ko, int64_t sko_b, int64_t sko_t, int64_t sko_h,
+                         solattn_stream_t stream);
+
+/* The same for the newest T tokens of sequences of lengths[b] tokens (these
+ * included): token t is at position lengths[b] - T + t; its k goes, turned, and its
+ * v as it is, to slot position % page_size of page page_table[b][position /
+ * page_size]. k_cache, v_cache: [pages][page_size][Hkv][D] with the strides given.
+ * Tokens before position 0, past the table, or whose page id is not in
+ * [0, pages) are not written (their rows of qo are finite but mean nothing). */
+int solattn_qk_norm_rope_append(
+    const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_b,
+    int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int64_t B,
+    int64_t T, int64_t H, int64_t Hkv, int64_t D, int dtype, const float* q_weight,
+    const float* k_weight, const float* cos, const float* sin, int64_t P, int64_t R, int interleaved,
+    float eps, void* qo, int64_t sqo_b, int64_t sqo_t, int64_t sqo_h, void* k_cache, int64_t skc_p,
+    int64_t skc_s, int64_t skc_h, void* v_cache, int64_t svc_p, int64_t svc_s, int64_t svc_h,
+    int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_stride,
+    int64_t max_pages, const int32_t* lengths, solattn_stream_t stream);
+
+/* Gradients of solattn_qk_norm_rope: dq, dk from the inputs q, k and the outputs'
+ * gradients dqo, dko; dq_weight, dk_weight: fp32 [D], null to leave out (with either,
+ * a 256-byte aligned workspace of the size below; the order of every sum is fixed). */
+int64_t solattn_qk_norm_rope_bwd_workspace_bytes(int64_t D);
+int solattn_qk_norm_rope_bwd(
+    const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_b,
+    int64_t sk_t, int64_t sk_h, const void* dqo, int64_t sdq_b, int64_t sdq_t, int64_t sdq_h,
+    const void* dko, int64_t sdk_b, int64_t sdk_t, int64_t sdk_h, int64_t B, int64_t T, int64_t H,
+    int64_t Hkv, int64_t D, int dtype, const float* q_weight, const float* k_weight, const float* cos,
+    const float* sin, int64_t P, int64_t R, int interleaved, const int32_t* positions,
+    int64_t pos_stride_b, float eps, void* dq, int64_t sgq_b, int64_t sgq_t, int64_t sgq_h, void* dk,
+    int64_t sgk_b, int64_t sgk_t, int64_t sgk_h, float* dq_weight, float* dk_weight, void* workspace,
+    int64_t workspace_bytes, solattn_stream_t stream);
+
+/* Row t of q sits at position p = q_start + t (q_start + Tq <= Tk) and sees the keys
+ *   causal:    j <= p and (p - j < window or j < sinks)
+ *   otherwise: |p - j| < window or j < sinks
+ * of j < len, len = lengths[b] clamped to [0, Tk] (int32 [B]; null: Tk).
+ *   o = sum_j softmax_j(scale q.k_j) v_j; rows at p >= len are zeros.
+ * lse: fp32 [B][H][Tq], log2 of the row's softmax sum (+inf for a row without keys),
+ * what the backward reads; null: not written. dtype bf16 or fp16, D 64 or 128
+ * (D: multiples of 8 up to 128 for the call below). Keys that no row of a call sees
+ * are never read; what k holds at a key reaches the rows that see it only, but a
+ * NaN or infinity in v (backward: also in k, q, do) can reach rows that do not see
+ * it within the same 128 rows.
+ * One causal row per sequence without lse (Tq = 1) runs split over the keys, as
+ * solattn_paged_attn, on a 256-byte aligned workspace of the size below (which is 0
+ * for other calls, and the workspace null). */
+int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t H, int64_t Hkv, int64_t D,
+                                            int64_t q_start, int64_t window, int64_t sinks, int causal);
+int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k,
+                        int64_t sk_b, int64_t sk_t, int64_t sk_h, const uint16_t* v, int64_t sv_b,
+                        int64_t sv_t, int64_t sv_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                        int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths,
+                        int64_t window, int64_t sinks, int causal, float scale, uint16_t* o,
+                        int64_t so_b, int64_t so_t, int64_t so_h, float* lse, void* workspace,
+                        int64_t workspace_bytes, solattn_stream_t stream);
+
+/* Gradients of solattn_window_attn from its inputs, o, lse and do: dq like q, dk and dv
+ * like k (every row written, zeros where nothing is seen). workspace: 256-byte
+ * aligned. No atomics: the same inputs give the same bits. */
+int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t H);
+int solattn_window_attn_bwd(
+    const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k, int64_t sk_b,
+    int64_t sk_t, int64_t sk_h, const uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h,
+    const uint16_t* o, int64_t so_b, int64_t so_t, int64_t so_h, const uint16_t* d_o, int64_t sg_b,
+    int64_t sg_t, int64_t sg_h, const float* lse, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+    int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths, int64_t window,
+    int64_t sinks, int causal, float scale, uint16_t* dq, int64_t sdq_b, int64_t sdq_t, int64_t sdq_h,
+    uint16_t* dk, int64_t sdk_b, int64_t sdk_t, int64_t sdk_h, uint16_t* dv, int64_t sdv_b,
+    int64_t sdv_t, int64_t sdv_h, void* workspace, int64_t workspace_bytes, solattn_stream_t stream);
+
+/* One new token of each sequence, the last of its lengths[b] (int32 [B], clamped to
+ * [0, max_pages page_size]): o[b][h] over the keys j < len, with a window (0: none)
+ * those of j >= len - window or j < sinks. Key j is slot j % page_size of page
+ * page_table[b][j / page_size] of k_cache, v_cache [pages][page_size][Hkv][D]
+ * (strides given; page_size a multiple of 8); keys of a page id outside
+ * [0, pages) are not visible. A sequence without visible keys gives zeros. Slots
+ * behind a sequence's last key may hold anything. dtype bf16 or fp16, D a multiple
+ * of 8 up to 128. workspace: 256-byte aligned, of the size below (0: may be null). */
+int64_t solattn_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
+                                           int64_t page_size, int64_t window, int64_t sinks);
+int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k_cache, int64_t sk_p,
+                       int64_t sk_s, int64_t sk_h, const uint16_t* v_cache, int64_t sv_p, int64_t sv_s,
+                       int64_t sv_h, int64_t pages, int64_t page_size, const int32_t* page_table,
+                       int64_t table_stride, int64_t max_pages, const int32_t* lengths, int64_t B,
+                       int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t window, int64_t sinks,
+                       float scale, void* workspace, int64_t workspace_bytes, uint16_t* o, int64_t so_b,
+                       int64_t so_h, solattn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,516 @@
+"""The operators around attention on the GPU, against float64: norms with rotation
+(forward, gradients, the form that fills a paged cache), sliding-window attention
+with sinks (forward and gradients) and attention of one token over pages. Bounds
+are those of tests/_operators.py."""
+
+import importlib
+
+import pytest
+import torch
+
+import _operators as ref
+
+pytestmark = pytest.mark.gpu
+
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def rope(pkg):
+    return importlib.import_module(f"{pkg.__name__}._qk_rope")
+
+
+@pytest.fixture(scope="module")
+def window(pkg):
+    return importlib.import_module(f"{pkg.__name__}._window")
+
+
+@pytest.fixture(scope="module")
+def paged(pkg):
+    return importlib.import_module(f"{pkg.__name__}._paged")
+
+
+def randn(shape, seed, dev, dtype=BF, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(dev)
+
+
+def tables(P, R, dev):
+    if not R:
+        return None, None
+    f = 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    a = torch.arange(P, dtype=torch.float64)[:, None] * f
+    return a.cos().float().to(dev), a.sin().float().to(dev)
+
+
+# ------------------------------------------------------- norms and rotation
+# B, T, H, Hkv, D, R, interleaved, dtype, weights, positions
+ROPE = [
+    (1, 1, 1, 1, 128, 128, False, BF, True, None),
+    (2, 5, 3, 1, 128, 128, True, FP, True, "shared"),
+    (1, 333, 24, 8, 128, 64, False, BF, True, None),
+    (3, 17, 16, 4, 64, 64, False, FP, True, "batch"),
+    (1, 50, 5, 5, 64, 32, True, F32, True, None),
+    (2, 9, 7, 7, 80, 80, True, BF, False, "batch"),
+    (1, 40, 2, 1, 96, 48, False, F32, True, "shared"),
+    (1, 70, 40, 40, 8, 0, False, BF, True, None),
+    (4, 1, 33, 11, 120, 16, False, FP, False, "batch"),
+    (1, 2000, 2, 2, 128, 128, True, BF, True, None),
+]
+
+
+def rope_case(c, dev, seed=0):
+    B, T, H, Hkv, D, R, interleaved, dtype, weights, positions = c
+    P = T + 7
+    q, k = randn((B, T, H, D), seed, dev, dtype, 2.0), randn((B, T, Hkv, D), seed + 1, dev, dtype, 0.5)
+    qw = 1 + 0.2 * randn((D,), seed + 2, dev, F32) if weights else None
+    kw = 1 + 0.2 * randn((D,), seed + 3, dev, F32) if weights else None
+    cos, sin = tables(P, R, dev)
+    g = torch.Generator().manual_seed(seed + 4)
+    pos = None
+    if positions:
+        pos = torch.randint(0, P, (T,) if positions == "shared" else (B, T), generator=g).to(dev)
+    at = torch.arange(T, device=dev).expand(B, T) if pos is None else pos.expand(B, T)
+    return q, k, qw, kw, cos, sin, pos, at
+
+
+def rope_bound(y, x, w, dtype):
+    """One rounding of y; in fp32: the sum of squares and the root (at most 16
+    roundings), two factors, two products and their sum, on values up to the row's
+    largest."""
+    top = y.abs().amax(-1, keepdim=True) * 2
+    return (ref.half_step(dtype) * y.abs() + 32 * ref.U32 * top) * 1.01
+
+
+@pytest.mark.parametrize("case", ROPE, ids=[str(i) for i in range(len(ROPE))])
+def test_norm_rope(rope, dev, case):
+    q, k, qw, kw, cos, sin, pos, at = rope_case(case, dev)
+    print("[rope]", case, flush=True)
+    qo, ko = rope.qk_norm_rope(q, k, qw, kw, cos, sin, eps=1e-5, positions=pos, interleaved=case[6])
+    for got, x, w in ((qo, q, qw), (ko, k, kw)):
+        want = ref.norm_rope(x, w, cos, sin, at, case[6], 1e-5)
+        assert got.dtype == x.dtype and got.is_contiguous()
+        ref.close(got, want, rope_bound(want, x, w, case[7]), "row")
+
+
+@pytest.mark.parametrize("case", ROPE, ids=[str(i) for i in range(len(ROPE))])
+def test_norm_rope_gradients(rope, dev, case):
+    """Against the formula in float64 (autograd of the float64 form) and, in the
+    same form, against differences along a direction."""
+    q, k, qw, kw, cos, sin, pos, at = rope_case(case, dev, seed=20)
+    leaves = [t for t in (q, k, qw, kw) if t is not None]
+    for t in leaves:
+        t.requires_grad_(True)
+    print("[rope grad]", case, flush=True)
+    dqo, dko = randn(q.shape, 31, dev, case[7]), randn(k.shape, 32, dev, case[7])
+    out = rope.qk_norm_rope(q, k, qw, kw, cos, sin, eps=1e-5, positions=pos, interleaved=case[6])
+    got = torch.autograd.grad(out, leaves, (dqo, dko))
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    full = wide if qw is not None else [*wide, None, None]
+
+    def loss(x):
+        y = [ref.norm_rope(x[i], x[i + 2], cos, sin, at, case[6], 1e-5) for i in (0, 1)]
+        return (y[0] * dqo.double()).sum() + (y[1] * dko.double()).sum()
+
+    want = torch.autograd.grad(loss(full), wide)
+    u = ref.half_step(case[7])
+    for g, w, x, dy in zip(got[:2], want[:2], (q, k), (dqo, dko)):
+        # fp32 before the one rounding: values up to the row's largest |r u| (r up to its inverse norm)
+        r = 1 / (x.detach().double().pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
+        scale = r * dy.double().abs().amax(-1, keepdim=True) * 3 * (1 + x.detach().double().abs() * r)
+        assert g.dtype == x.dtype
+        ref.close(g, w, (u * w.abs() + 64 * ref.U32 * scale) * 1.01, "dx")
+    for i, x, dy in ((2, q, dqo), (3, k, dko)):
+        if qw is None:
+            continue
+        xd = x.detach().double()
+        r = 1 / (xd.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
+        terms = (dy.double().abs().amax(-1, keepdim=True) * 1.5 * (xd * r).abs()).sum((0, 1, 2))
+        # at most 128 additions behind one another, and 32 roundings inside a term
+        ref.close(got[i], want[i], 160 * ref.U32 * terms + 1e-30, "dw")
+    d = [randn(t.shape, 40 + i, dev, F32).double() for i, t in enumerate(wide)]
+    with torch.no_grad():
+        h = 1e-6
+        step = [[t + s * h * x for t, x in zip(wide, d)] for s in (1, -1)]
+        step = [x if qw is not None else [*x, None, None] for x in step]
+        slope = (loss(step[0]) - loss(step[1])) / (2 * h)
+        along = sum((g.double() * x).sum() for g, x in zip(got, d))
+        size = sum((g.double() * x).pow(2).sum() for g, x in zip(got, d)).sqrt()
+    # the type's roundings are independent: a sum of n of them is off by about u sqrt(sum squares)
+    assert (slope - along).abs() <= 8 * u * size + 1e-5 * size + 1e-6, (slope, along)
+
+
+def test_norm_rope_strides_and_types(rope, dev):
+    """Views of one projection, a batch expanded from one sequence, weights of another
+    type, rows that are not 16-byte aligned and shifted tables."""
+    B, T, H, D = 2, 19, 4, 64
+    qkv = randn((B, T, 3, H, D), 1, dev)
+    q, k = qkv[:, :, 0], qkv[:, :, 1]
+    w = (1 + 0.1 * randn((D + 1,), 2, dev, F32))[1:]
+    cos, sin = tables(T, D, dev)
+    want = rope.qk_norm_rope(q.contiguous(), k.contiguous(), w.clone(), w.clone(), cos, sin)
+    for got, x in zip(rope.qk_norm_rope(q, k, w, w, cos, sin), want):
+        assert torch.equal(got, x)
+    odd = torch.empty(B * T * H * D + 1, device=dev, dtype=BF)[1:].view(B, T, H, D).copy_(q)
+    assert torch.equal(rope.qk_norm_rope(odd, k, w, w, cos, sin)[0], want[0])
+    one = q[:1].expand(3, T, H, D)
+    got = rope.qk_norm_rope(one, one, w, w, cos, sin)[0]
+    assert torch.equal(got, want[0][:1].expand_as(got))
+    got = rope.qk_norm_rope(q, k, w.to(BF), None, cos, sin)
+    assert torch.equal(got[0], rope.qk_norm_rope(q, k, w.to(BF).float(), None, cos, sin)[0])
+    pos = torch.tensor([5, -3, 10 ** 6], device=dev)
+    got = rope.qk_norm_rope(q[:, :3], k[:, :3], w, w, cos, sin, positions=pos)  # clamped to the table
+    pos = torch.tensor([5, 0, T - 1], device=dev)
+    assert torch.equal(got[0], rope.qk_norm_rope(q[:, :3], k[:, :3], w, w, cos, sin, positions=pos)[0])
+    empty = rope.qk_norm_rope(q[:, :0], k[:, :0], w, w, cos, sin)
+    assert empty[0].shape == (B, 0, H, D)
+
+
+def cache_of(B, max_len, page, Hkv, D, dev, dtype=BF, seed=7, fill=float("nan")):
+    """An empty cache of NaN, its pages dealt at random, one page more than used."""
+    most = -(-max_len // page)
+    n = B * most + 1
+    g = torch.Generator().manual_seed(seed)
+    table = (torch.randperm(n, generator=g)[:B * most]).to(torch.int32).reshape(B, most).to(dev)
+    shape = (n, page, Hkv, D)
+    return torch.full(shape, fill, device=dev, dtype=dtype), torch.full(shape, fill, device=dev, dtype=dtype), table
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,D,page,lengths,dtype", [
+    (1, 1, 24, 8, 128, 64, [1], BF), (3, 1, 4, 4, 64, 16, [17, 0, 64], FP), (2, 70, 6, 2, 96, 32, [70, 95], BF),
+    (2, 5, 2, 1, 128, 8, [3, 40], F32),
+])
+def test_append(rope, dev, B, T, H, Hkv, D, page, lengths, dtype):
+    """Rows land at their places, turned by their positions; every other slot, an
+    idle sequence's and those of tokens before position 0 among them, stays."""
+    q, k, v = (randn((B, T, h, D), s, dev, dtype) for h, s in ((H, 1), (Hkv, 2), (Hkv, 3)))
+    kc, vc, table = cache_of(B, 100, page, Hkv, D, dev, dtype, fill=3.0)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    cos, sin = tables(100, 16 * (D // 16), dev)
+    w = 1 + 0.2 * randn((D,), 4, dev, F32)
+    kc0, vc0 = kc.clone(), vc.clone()
+    print("[append]", B, T, H, Hkv, D, page, lengths, dtype, flush=True)
+    qo = rope.qk_norm_rope_append(q, k, v, kc, vc, table, n, w, w, cos, sin)
+    at = n[:, None] - T + torch.arange(T, device=dev)
+    want_q, want_k = rope.qk_norm_rope(q, k, w, w, cos, sin, positions=at)
+    for b in range(B):
+        for t in range(T):
+            p = int(at[b, t])
+            if p < 0:
+                continue
+            page_id = int(table[b, p // page])
+            assert torch.equal(qo[b, t], want_q[b, t])
+            assert torch.equal(kc[page_id, p % page], want_k[b, t])
+            assert torch.equal(vc[page_id, p % page], v[b, t])
+            kc0[page_id, p % page], vc0[page_id, p % page] = kc[page_id, p % page], vc[page_id, p % page]
+    assert torch.equal(kc, kc0) and torch.equal(vc, vc0)
+
+
+def test_append_bad_pages(rope, dev):
+    """Page ids outside the cache and tokens past the table write nothing."""
+    q, k, v = (randn((3, 1, 2, 64), s, dev) for s in (1, 2, 3))
+    kc, vc, _ = cache_of(3, 16, 8, 2, 64, dev, fill=3.0)
+    table = torch.tensor([[-1, 0], [kc.shape[0], 0], [0, 0]], dtype=torch.int32, device=dev)
+    n = torch.tensor([3, 4, 17], dtype=torch.int32, device=dev)
+    rope.qk_norm_rope_append(q, k, v, kc, vc, table, n)
+    assert (kc == 3).all() and (vc == 3).all()
+    none = kc[:0]
+    assert rope.qk_norm_rope_append(q, k, v, none, none, table, n).shape == q.shape
+
+
+# ------------------------------------------------------------------- windows
+# B, Tq, Tk, H, Hkv, D, window, sinks, causal, lengths, dtype
+WINDOW = [
+    (1, 1, 1, 1, 1, 128, 1, 0, True, None, BF),
+    (1, 1, 700, 6, 2, 128, 300, 4, True, None, BF),
+    (2, 1, 65, 4, 4, 64, 9, 70, True, [65, 30], FP),
+    (1, 63, 63, 2, 1, 64, 7, 2, True, None, BF),
+    (1, 130, 130, 2, 2, 128, None, 0, True, None, FP),
+    (2, 200, 200, 4, 2, 128, 50, 3, True, [200, 77], BF),
+    (1, 257, 1000, 3, 1, 64, 300, 130, True, None, BF),
+    (2, 300, 300, 2, 2, 128, 40, 0, False, [0, 261], FP),
+    (1, 400, 400, 2, 1, 128, 65, 333, False, None, BF),
+    (1, 190, 500, 2, 2, 64, 1, 1, False, None, FP),
+    (1, 500, 500, 16, 2, 64, 128, 64, True, None, BF),
+    (3, 129, 129, 1, 1, 80, 64, 5, True, [129, 1, 64], BF),
+    (1, 70, 90, 3, 3, 24, 33, 2, False, None, FP),
+    (1, 1100, 1100, 2, 1, 128, 256, 4, True, None, FP),
+    (1, 640, 640, 1, 1, 128, None, 0, False, None, BF),
+]
+
+
+def window_case(c, dev, seed=0):
+    B, Tq, Tk, H, Hkv, D, w, sinks, causal, lengths, dtype = c
+    q = randn((B, Tq, H, D), seed, dev, dtype, 2.0)
+    k, v = randn((B, Tk, Hkv, D), seed + 1, dev, dtype), randn((B, Tk, Hkv, D), seed + 2, dev, dtype)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev)
+    if n is not None:  # what lies behind a sequence may be anything
+        for b, e in enumerate(lengths):
+            k[b, e:], v[b, e:] = float("nan"), float("inf")
+            q[b, max(0, e - (Tk - Tq)):] = float("nan")
+    on = ref.seen(Tq, Tk, Tk - Tq, w, sinks, causal, n, B, dev)
+    return q, k, v, n, on, dict(window=w, sinks=sinks, causal=causal, lengths=n)
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=[str(i) for i in range(len(WINDOW))])
+def test_window(window, dev, case):
+    q, k, v, n, on, kw = window_case(case, dev)
+    print("[window]", case, flush=True)
+    got = window.window_attn(q, k, v, **kw)
+    o, p, (_, _, vh) = ref.attention(q, k, v, on, q.shape[-1] ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, q.dtype), "o")
+    assert (got.masked_select(~on.any(2)[:, :, None, None].expand_as(got)) == 0).all()
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=[str(i) for i in range(len(WINDOW))])
+def test_window_gradients(window, dev, case):
+    q, k, v, n, on, kw = window_case(case, dev, seed=50)
+    do = randn(q.shape, 60, dev, q.dtype)
+    if n is not None:
+        do.masked_fill_(~on.any(2)[:, :, None, None], float("nan"))  # gradients of rows that nothing reads
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    print("[window grad]", case, flush=True)
+    out = window.window_attn(q, k, v, scale=0.11, **kw)
+    got = torch.autograd.grad(out, (q, k, v), do)
+    want, bound = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.11, do, q.dtype)
+    for name, g, w, b in zip(("dq", "dk", "dv"), got, want, bound):
+        ref.close(g, w, b, name)
+    again = torch.autograd.grad(window.window_attn(q, k, v, scale=0.11, **kw), (q, k, v), do)
+    for x, y in zip(got, again):
+        assert torch.equal(x, y)
+
+
+def test_window_gradients_against_differences(window, dev):
+    """Along a direction, the float64 form's differences against the kernels' gradients."""
+    c = (1, 150, 150, 4, 2, 64, 60, 3, True, None, FP)
+    q, k, v, n, on, kw = window_case(c, dev, seed=70)
+    do = randn(q.shape, 80, dev, FP)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    got = torch.autograd.grad(window.window_attn(q, k, v, **kw), (q, k, v), do)
+    _, bound = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.125, do, FP)
+    d = [randn(t.shape, 90 + i, dev, F32).double() for i, t in enumerate((q, k, v))]
+    h = 1e-5
+
+    def loss(s):
+        x = [t.detach().double() + s * h * y for t, y in zip((q, k, v), d)]
+        return (ref.attention(*x, on, 0.125)[0] * do.double()).sum()
+
+    slope = (loss(1) - loss(-1)) / (2 * h)
+    along = sum((g.double() * y).sum() for g, y in zip(got, d))
+    room = sum((b * y.abs()).sum() for b, y in zip(bound, d))
+    assert (slope - along).abs() <= room + 1e-4, (slope, along, room)
+    size = sum((g.double() * y).pow(2).sum() for g, y in zip(got, d)).sqrt()
+    assert (slope - along).abs() <= 0.02 * size, (slope, along, size)  # roundings of 2^-11 that average out
+
+
+def test_window_strides(window, dev):
+    """Interleaved views, BHTD storage, one sequence's keys for a whole batch, heads
+    expanded from one, rows that are not aligned: the same bits as dense copies."""
+    B, T, H, D = 2, 150, 4, 64
+    qkv = randn((B, T, 3, H, D), 3, dev)
+    q, k, v = qkv.unbind(2)
+    kw = dict(window=40, sinks=2)
+    want = window.window_attn(*(t.contiguous() for t in (q, k, v)), **kw)
+    assert torch.equal(window.window_attn(q, k, v, **kw), want)
+    bh = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert torch.equal(window.window_attn(*bh, **kw), want)
+    odd = [torch.empty(t.numel() + 1, device=dev, dtype=BF)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    assert torch.equal(window.window_attn(*odd, **kw), want)
+    k1, v1 = k[:1].expand_as(k), v[:1].expand_as(v)
+    assert torch.equal(window.window_attn(q, k1, v1, **kw), window.window_attn(q, k1.contiguous(), v1.contiguous(), **kw))
+    kh, vh = (t[:, :, :1].expand_as(t) for t in (k, v))
+    got = window.window_attn(q, kh, vh, **kw)
+    assert torch.equal(got, window.window_attn(q, k[:, :, :1], v[:, :, :1], **kw))
+    # gradients of broadcast inputs: those of the copies, summed
+    leaf = k[:1].detach().clone().requires_grad_(True)
+    g, = torch.autograd.grad(window.window_attn(q, leaf.expand_as(k), v, **kw), leaf, want)
+    dense = k[:1].expand_as(k).contiguous().requires_grad_(True)
+    gd, = torch.autograd.grad(window.window_attn(q, dense, v, **kw), dense, want)
+    assert torch.equal(g, gd.sum(0, keepdim=True))
+    # an expanded gradient of the output
+    leaf = q.detach().clone().requires_grad_(True)
+    window.window_attn(leaf, k, v, **kw).sum().backward()
+    ones = q.detach().clone().requires_grad_(True)
+    window.window_attn(ones, k, v, **kw).backward(torch.ones_like(q))
+    assert torch.equal(leaf.grad, ones.grad)
+
+
+def test_window_unread_keys(window, dev):
+    """Keys that no row of a call sees are not read: those past the last row (a
+    buffer longer than the sequence) and those that slid out of every window."""
+    B, T, H, D = 1, 90, 2, 128
+    q, k, v = (randn((B, s, H, D), i, dev) for i, s in enumerate((T, 600, 600)))
+    kw = dict(window=20, sinks=3)
+    clean = window.window_attn(q, k, v, q_start=300, **kw)
+    bad = torch.ones(600, dtype=torch.bool, device=dev)
+    bad[:3] = False
+    bad[300 - 19:300 + T] = False
+    for x in (float("nan"), float("inf"), torch.finfo(BF).min):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, bad], v2[:, bad] = x, x
+        assert torch.equal(window.window_attn(q, k2, v2, q_start=300, **kw), clean)
+        one = window.window_attn(q[:, :1], k2, v2, q_start=300, **kw)
+        assert torch.isfinite(one).all()
+    # a key's own values reach the rows that see it only, also in k's case within a block
+    k2 = k.clone()
+    k2[:, 320] = float("nan")
+    got = window.window_attn(q, k2, v, q_start=300, **kw)
+    rows = torch.arange(T, device=dev) + 300
+    hit = (rows >= 320) & (rows < 340)
+    assert torch.isnan(got[:, hit]).all() and torch.equal(got[:, ~hit], clean[:, ~hit])
+
+
+def test_window_empty(window, dev):
+    q = torch.zeros((2, 0, 2, 64), device=dev, dtype=BF, requires_grad=True)
+    k = torch.zeros((2, 5, 2, 64), device=dev, dtype=BF, requires_grad=True)
+    out = window.window_attn(q, k, k, window=3)
+    assert out.shape == q.shape
+    gq, gk = torch.autograd.grad(out.sum(), (q, k))
+    assert gq.shape == q.shape and (gk == 0).all()
+
+
+# --------------------------------------------------------------------- pages
+# lengths, page, H, Hkv, D, window, sinks, dtype
+PAGED = [
+    ([1], 16, 1, 1, 128, None, 0, BF),
+    ([0, 7, 64], 8, 24, 8, 128, None, 0, BF),
+    ([1000, 333, 31, 32, 33], 16, 16, 4, 64, None, 0, FP),
+    ([5000], 64, 24, 8, 128, 700, 4, BF),
+    ([130, 4097], 24, 40, 2, 128, 100, 33, FP),
+    ([900, 20], 136, 3, 3, 96, 64, 0, BF),
+    ([70], 32, 34, 1, 80, 33, 40, FP),
+    ([300] * 9, 256, 8, 8, 24, None, 0, BF),
+    ([20000], 64, 4, 4, 64, None, 0, BF),
+]
+
+
+@pytest.mark.parametrize("case", PAGED, ids=[str(i) for i in range(len(PAGED))])
+def test_paged(paged, dev, case):
+    lengths, page, H, Hkv, D, w, sinks, dtype = case
+    B, L = len(lengths), max(lengths)
+    k, v = randn((B, L, Hkv, D), 1, dev, dtype), randn((B, L, Hkv, D), 2, dev, dtype)
+    q = randn((B, 1, H, D), 3, dev, dtype, 2.0)
+    kc, vc, table = cache_of(B, L + page, page, Hkv, D, dev, dtype)  # slots not written stay NaN
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    on = torch.zeros((B, 1, L), dtype=torch.bool, device=dev)
+    for b, e in enumerate(lengths):
+        for p in range(0, e, page):
+            m = min(page, e - p)
+            kc[table[b, p // page], :m], vc[table[b, p // page], :m] = k[b, p:p + m], v[b, p:p + m]
+        table[b, -(-e // page):] = -1 if b % 2 else 10 ** 9
+        on[b, 0, :e] = True
+        if w:
+            on[b, 0, min(sinks, e):max(0, e - w)] = False
+    print("[paged]", case, flush=True)
+    got = paged.paged_attn(q, kc, vc, table, n, window=w, sinks=sinks)
+    o, p, (_, _, vh) = ref.attention(q, k, v, on, D ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, dtype), "o")
+    assert (got[n == 0] == 0).all()
+
+
+def test_paged_bad_pages_and_long_lengths(paged, dev):
+    """Keys on page ids that the cache lacks are not visible; a length past the table
+    is the table's; a cache without pages gives zeros."""
+    B, page, Hkv, D = 2, 16, 2, 64
+    kc, vc = randn((7, page, Hkv, D), 1, dev), randn((7, page, Hkv, D), 2, dev)
+    q = randn((B, 1, 4, D), 3, dev)
+    table = torch.tensor([[3, 99, 1], [0, -5, 2]], dtype=torch.int32, device=dev)
+    n = torch.tensor([41, 48], dtype=torch.int32, device=dev)
+    got = paged.paged_attn(q, kc, vc, table, n)
+    k = torch.stack([torch.cat([kc[3], kc[1]]), torch.cat([kc[0], kc[2]])])
+    v = torch.stack([torch.cat([vc[3], vc[1]]), torch.cat([vc[0], vc[2]])])
+    on = torch.arange(32, device=dev)[None, None] < torch.tensor([25, 32], device=dev)[:, None, None]
+    o, p, (_, _, vh) = ref.attention(q, k, v, on, D ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, BF), "o")
+    long = torch.tensor([41, 2 ** 31 - 1], dtype=torch.int32, device=dev)
+    assert torch.equal(paged.paged_attn(q, kc, vc, table, long), got)
+    neg = torch.tensor([-4, 48], dtype=torch.int32, device=dev)
+    assert (paged.paged_attn(q, kc, vc, table, neg)[0] == 0).all()
+    assert (paged.paged_attn(q, kc[:0], vc[:0], table, n) == 0).all()
+
+
+# ------------------------------------------------------------------- together
+@pytest.mark.parametrize("H,Hkv,D,w,sinks", [(6, 2, 128, 100, 4), (4, 4, 64, None, 0)])
+def test_prompt_then_tokens(rope, window, paged, dev, H, Hkv, D, w, sinks):
+    """A prompt and its next tokens as they are used: norms and rotation into the
+    cache, windowed attention over the prompt, then token by token over the pages;
+    the whole against one windowed call over all tokens."""
+    B, T, new, page = 2, 150, 20, 16
+    total = T + new
+    x = randn((B, total, H + 2 * Hkv, D), 5, dev)
+    q, k, v = x.split([H, Hkv, Hkv], 2)
+    qw, kw = 1 + 0.1 * randn((D,), 6, dev, F32), 1 + 0.1 * randn((D,), 7, dev, F32)
+    cos, sin = tables(total, D, dev)
+    kc, vc, table = cache_of(B, total, page, Hkv, D, dev)
+    rows = []
+
+    def lengths(n):
+        return torch.full((B,), n, dtype=torch.int32, device=dev)
+
+    qp = rope.qk_norm_rope_append(q[:, :T], k[:, :T], v[:, :T], kc, vc, table, lengths(T), qw, kw, cos, sin)
+    qr, kr = rope.qk_norm_rope(q, k, qw, kw, cos, sin)
+    assert torch.equal(qp, qr[:, :T])
+    rows.append(window.window_attn(qp, kr[:, :T], v[:, :T], window=w, sinks=sinks))
+    for t in range(T, total):
+        s = slice(t, t + 1)
+        qt = rope.qk_norm_rope_append(q[:, s], k[:, s], v[:, s], kc, vc, table, lengths(t + 1), qw, kw, cos, sin)
+        assert torch.equal(qt, qr[:, s])
+        rows.append(paged.paged_attn(qt, kc, vc, table, lengths(t + 1), window=w, sinks=sinks))
+        # the same token against the contiguous keys so far
+        flat = window.window_attn(qt, kr[:, :t + 1], v[:, :t + 1], window=w, sinks=sinks)
+        u = ref.half_step(BF)
+        assert ((flat.double() - rows[-1].double()).abs() <= 4 * u * (flat.double().abs() + 1)).all()
+    got = torch.cat(rows, 1)
+    on = ref.seen(total, total, 0, w, sinks, True, None, B, dev)
+    o, p, (_, _, vh) = ref.attention(qr, kr, v, on, D ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, BF), "o")
+
+
+def test_other_stream_and_graph(rope, window, paged, dev):
+    """On a stream of its own, and captured once and replayed on new contents with
+    eager work between the replays: the eager bits every time."""
+    B, T, H, Hkv, D, page = 2, 200, 4, 2, 64, 16
+    q, k, v = randn((B, T, H, D), 1, dev), randn((B, T, Hkv, D), 2, dev), randn((B, T, Hkv, D), 3, dev)
+    w = 1 + 0.1 * randn((D,), 4, dev, F32)
+    cos, sin = tables(T, D, dev)
+    kc, vc, table = cache_of(B, T, page, Hkv, D, dev)
+    n = torch.full((B,), T, dtype=torch.int32, device=dev)
+    do = randn(q.shape, 5, dev)
+
+    def step():
+        qp = rope.qk_norm_rope_append(q, k, v, kc, vc, table, n, w, w, cos, sin)
+        _, kr = rope.qk_norm_rope(q, k, w, w, cos, sin)
+        o = window.window_attn(qp, kr, v, window=50, sinks=2)
+        one = paged.paged_attn(qp[:, -1:], kc, vc, table, n, window=50, sinks=2)
+        leaves = [t.detach().requires_grad_(True) for t in (qp, kr, v)]
+        grads = torch.autograd.grad(window.window_attn(*leaves, window=50, sinks=2), leaves, do)
+        return [qp, kr, o, one, *grads]
+
+    eager = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(got, eager):
+        assert torch.equal(x, y)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs live at once
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for rep in range(3):
+        print("[graph] replay", rep, flush=True)
+        for i, t in enumerate((q, k, v, do)):
+            t.copy_(randn(t.shape, 100 + 10 * rep + i, dev))
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            kc.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(out, step()):
+                assert torch.equal(x, y)
