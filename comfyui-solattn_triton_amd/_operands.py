@@ -21,7 +21,8 @@ def row_ready(t: torch.Tensor) -> bool:
     row 16-byte aligned."""
     whole = 16 // t.element_size()
     return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and t.stride(0) % whole == 0 and t.stride(1) % whole == 0 and t.stride(2) % whole == 0)
+            and t.stride(0) % whole == 0 and t.stride(1) % whole == 0 and t.stride(2) % whole == 0
+            and t.stride(1) < 1 << 24)
 
 
 def as_rows(t: torch.Tensor) -> torch.Tensor:

@@ -51,7 +51,7 @@ class _WindowAttn(torch.autograd.Function):
         dk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
         dv = torch.empty(k.shape, device=q.device, dtype=q.dtype)
         with torch.cuda.device(q.device):
-            ws = workspace(LIB.solattn_window_attn_bwd_workspace_bytes(B, Tq, H), q.device)
+            ws = workspace(LIB.solattn_window_attn_bwd_workspace_bytes(B, Tq, Tk, H, Hkv, D, window, sinks, causal), q.device)
             call("solattn_window_attn_bwd", ptr(q), *strides(q), ptr(k), *strides(k), ptr(v), *strides(v), ptr(out),
                  *strides(out), ptr(grad), *strides(grad), ptr(lse), B, Tq, Tk, H, Hkv, D, DTYPES[q.dtype], q_start,
                  ptr(lengths), window, sinks, causal, scale, ptr(dq), *strides(dq), ptr(dk), *strides(dk), ptr(dv),

@@ -109,13 +109,21 @@ window_fwd_kernel(const WindowArgs a) {
     a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// Wave-wide minimum and maximum of a lane value, as scalars.
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dq_kernel(const WindowArgs a) {
   constexpr int ND = D / 32, NC = D / 16;
-  __shared__ __align__(256) uint16_t kbuf[kKeys * D];
-  __shared__ __align__(256) uint16_t vbuf[kKeys * D];
+  constexpr uint32_t kBuf = kKeys * D * 2;  // bytes of a tile
+  __shared__ __align__(256) uint16_t kbuf[2 * kKeys * D];
+  __shared__ __align__(256) uint16_t vbuf[2 * kKeys * D];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   int b, h, qb;
   row_item(a, b, h, qb);
@@ -127,8 +135,24 @@ window_dq_kernel(const WindowArgs a) {
   const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
   const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
   const uint32_t kb = lds_addr(kbuf), vb = lds_addr(vbuf);
-  const TileAddr<D, kBoth> ka(kb, lane);
-  const TileAddr<D, kByRow> va(vb, lane);
+  TileAddr<D, kBoth> ka(kb, lane);
+  TileAddr<D, kByRow> va(vb, lane);
+  const uint32_t off_k = copy_offset<kThreads, D, kBoth>(a.k.t), off_v = copy_offset<kThreads, D, kByRow>(a.v.t);
+  const auto issue = [&](int t) __attribute__((always_inline)) {
+    const int j0 = kt.first(t);
+    const uint32_t at = (t & 1) * kBuf;
+    if (kt.whole(t)) {
+      copy_whole<kThreads, D>(kb + at, kp + j0 * a.k.t, a.k.t, off_k);
+      copy_whole<kThreads, D>(vb + at, vp + j0 * a.v.t, a.v.t, off_v);
+    } else {
+      const auto safe = [&](int r) { return kt.safe(j0 + r); };
+      copy_tile<kThreads, D, kBoth>(kb + at, kp, a.k.t, safe);
+      copy_tile<kThreads, D, kByRow>(vb + at, vp, a.v.t, safe);
+    }
+  };
+  // keys that every row of the wave sees
+  const int all_lo = -wave_min(-rk.jl), all_hi = wave_min(rk.jh), all_sk = wave_min(rk.sk);
+  if (kt.n) issue(0);
   bf16x8 q[NC], g[NC];
   load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
   load_row<D>(g, a.d_o.p + b * a.d_o.b + static_cast<int64_t>(rr) * a.d_o.t + h * a.d_o.h, half);
@@ -152,30 +176,34 @@ window_dq_kernel(const WindowArgs a) {
   f32x16 acc[ND] = {};
   for (int t = 0; t < kt.n; ++t) {
     const int j0 = kt.first(t);
-    const auto safe = [&](int r) { return kt.safe(j0 + r); };
-    __syncthreads();
-    copy_tile<kThreads, D, kBoth>(kb, kp, a.k.t, safe);
-    copy_tile<kThreads, D, kByRow>(vb, vp, a.v.t, safe);
     wait_tile_copies();
-    __syncthreads();
+    __syncthreads();  // this tile is in, and every wave is done with the buffers of the last
+    if (t + 1 < kt.n) issue(t + 1);
+    const bool masked = !((j0 >= all_lo && j0 + kKeys - 1 <= all_hi) || j0 + kKeys <= all_sk);
+    const uint32_t at = (t & 1) * kBuf;
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
+      ka.remade();
+      va.remade();
       f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc), q[cc], s);
+      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc, at), q[cc], s);
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(va.by_row(m2, cc), g[cc], dp);
-      mask_keys(s, rk, j0 + 32 * m2, half);
+      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(va.by_row(m2, cc, at), g[cc], dp);
+      if (masked) mask_keys(s, rk, j0 + 32 * m2, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, neg));
-        s[r] = s[r] == -INFINITY ? 0.f : pr * (dp[r] - delta);  // (a masked dp may be anything)
+        dp[r] = pr * (dp[r] - delta);
       }
+      if (masked)  // (a masked dp may be anything)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 ds = pack8<E>(s, ks);
+        const bf16x8 ds = pack8<E>(dp, ks);
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(ka.transposed(2 * m2 + ks, dt), ds, acc[dt]);
+        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(ka.transposed(2 * m2 + ks, dt, at), ds, acc[dt]);
       }
     }
   }
@@ -183,87 +211,203 @@ window_dq_kernel(const WindowArgs a) {
                half);
 }
 
-// dk and dv: a workgroup owns 128 keys of a kv head and walks the rows that see
-// any of them, head by head of the group; a wave's 32 keys stay in registers.
+// dk and dv: a workgroup owns 128 keys of a kv head and walks, head by head of the
+// group, the tiles of 64 rows that see any of them; a wave's 32 keys (k, v and the
+// sums) stay in registers: S = Q K^T and dP = dO V^T put a key on a lane column, and
+// P and dS convert in place into B operands of dv^T += dO^T P and dk^T += Q^T dS.
+// Q and dO tiles are double buffered: the next one lands while this one is used.
+//
+// Parts: the steps (heads x tiles) of a block of keys are cut into parts of their
+// own workgroups, sinks' blocks into `ks` and the others into `kn`: every row sees
+// the sinks, and few or short heads leave CUs without a block. A part's sums go to
+// the workspace in fp32 and window_dkv_join_kernel adds them up in order; a block
+// of one part is stored straight.
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dkv_kernel(const WindowArgs a) {
   constexpr int ND = D / 32, NC = D / 16;
-  __shared__ __align__(256) uint16_t qbuf[kKeys * D];
-  __shared__ __align__(256) uint16_t gbuf[kKeys * D];
-  __shared__ float lse[kKeys], delta[kKeys];
-  const int lane = threadIdx.x & 63, half = lane >> 5;
+  constexpr uint32_t kBuf = kKeys * D * 2;  // bytes of a tile
+  __shared__ __align__(256) uint16_t qbuf[2 * kKeys * D];
+  __shared__ __align__(256) uint16_t gbuf[2 * kKeys * D];
+  __shared__ __align__(16) float stat[2][2][kKeys];  // [buffer][lse, delta]
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = wave_id();
   uint32_t w = xcd_run(blockIdx.x, gridDim.x);
-  const int kblk = w % a.nkb;
-  w /= a.nkb;
-  const int hk = w % a.Hkv, b = w / a.Hkv;
+  const KeyPart kp = key_part(a, w);
+  const int hk = kp.bh % a.Hkv, b = kp.bh / a.Hkv;
   const int len = sequence_length(a, b);
-  const int j0 = kblk * kRows, j = j0 + wave_id() * 32 + (lane & 31), jj = min(j, a.Tk - 1);
+  const int j0 = kp.block * kRows, j = j0 + wave * 32 + (lane & 31), jj = min(j, a.Tk - 1);
   const KeyRows kr = key_rows(a, j < a.Tk ? j : len, len);
-  // rows that see a key of the block: a key's interval only moves up with it, but that a sink's has no end
+  // rows that see a key of the block: a key's interval moves up with it, but that a sink's has no end
   const int jlast = min(min(j0 + kRows, a.Tk), len) - 1;
   const KeyRows k0 = key_rows(a, j0, len), k1 = key_rows(a, max(jlast, j0), len);
   const int i0 = k0.pl - a.q_start, i1 = (j0 < a.sinks ? k0.ph : k1.ph) - a.q_start;  // rows [i0, i1]
-  const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf);
-  const TileAddr<D, kBoth> qa(qb, lane), ga(gb, lane);
+  const int tile0 = i0 & ~(kKeys - 1);
+  const int tiles = j0 < len && i0 <= i1 ? (i1 - tile0) / kKeys + 1 : 0;
+  const int per = (tiles * a.group + kp.parts - 1) / kp.parts;
+  const int s0 = min(kp.part * per, tiles * a.group), s1 = min(s0 + per, tiles * a.group);
+  // rows that every key of the wave is seen by
+  const int all_lo = -wave_min(-kr.pl) - a.q_start, all_hi = wave_min(kr.ph) - a.q_start;
+
+  const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf), sb = lds_addr(stat);
+  TileAddr<D, kBoth> qa(qb, lane), ga(gb, lane);
   bf16x8 k[NC], v[NC];
   load_row<D>(k, a.k.p + b * a.k.b + static_cast<int64_t>(jj) * a.k.t + hk * a.k.h, half);
   load_row<D>(v, a.v.p + b * a.v.b + static_cast<int64_t>(jj) * a.v.t + hk * a.v.h, half);
 
+  const uint32_t off_q = copy_offset<kThreads, D, kBoth>(a.q.t), off_g = copy_offset<kThreads, D, kBoth>(a.d_o.t);
+  // The next step to copy: head g of the group, rows from t0 on.
+  int g = tiles ? s0 / tiles : 0, t0 = tiles ? tile0 + (s0 - g * tiles) * kKeys : 0;
+  const auto issue = [&](int buf) __attribute__((always_inline)) {
+    const int h = hk * a.group + g;
+    const uint16_t* qp = a.q.p + b * a.q.b + h * a.q.h;
+    const uint16_t* gp = a.d_o.p + b * a.d_o.b + h * a.d_o.h;
+    const auto safe = [&](int r) { return min(max(t0 + r, i0), i1); };
+    if (t0 >= i0 && t0 + kKeys - 1 <= i1) {
+      copy_whole<kThreads, D>(qb + buf * kBuf, qp + t0 * a.q.t, a.q.t, off_q);
+      copy_whole<kThreads, D>(gb + buf * kBuf, gp + t0 * a.d_o.t, a.d_o.t, off_g);
+    } else {
+      copy_tile<kThreads, D, kBoth>(qb + buf * kBuf, qp, a.q.t, safe);
+      copy_tile<kThreads, D, kBoth>(gb + buf * kBuf, gp, a.d_o.t, safe);
+    }
+    const float* st = wave == 0 ? a.lse : a.delta;
+    if (wave < 2)
+      g2l4(st + (static_cast<int64_t>(b) * a.H + h) * a.Tq + safe(lane), sb + (2 * buf + wave) * kKeys * 4);
+    t0 += kKeys;
+    if (t0 >= tile0 + tiles * kKeys) t0 = tile0, ++g;
+  };
+
   f32x16 dk[ND] = {}, dv[ND] = {};
-  if (j0 < len && i0 <= i1) {
-    for (int g = 0; g < a.group; ++g) {
-      const int h = hk * a.group + g;
-      const uint16_t* qp = a.q.p + b * a.q.b + h * a.q.h;
-      const uint16_t* gp = a.d_o.p + b * a.d_o.b + h * a.d_o.h;
-      const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Tq;
-      for (int t0 = i0 & ~(kKeys - 1); t0 <= i1; t0 += kKeys) {
-        const auto safe = [&](int r) { return min(max(t0 + r, i0), i1); };
-        __syncthreads();
-        copy_tile<kThreads, D, kBoth>(qb, qp, a.q.t, safe);
-        copy_tile<kThreads, D, kBoth>(gb, gp, a.d_o.t, safe);
-        if (threadIdx.x < kKeys)
-          lse[threadIdx.x] = a.lse[stat + safe(threadIdx.x)];
-        else if (threadIdx.x < 2 * kKeys)
-          delta[threadIdx.x - kKeys] = a.delta[stat + safe(threadIdx.x - kKeys)];
-        wait_tile_copies();
-        __syncthreads();
+  if (s0 < s1) issue(0);
+  for (int st = s0; st < s1; ++st) {
+    const int buf = (st - s0) & 1;
+    // the rows of this step (the copy that was issued last)
+    const int r0 = t0 == tile0 ? tile0 + (tiles - 1) * kKeys : t0 - kKeys;
+    wait_tile_copies();
+    __syncthreads();  // this step's tiles are in, and every wave is done with the buffers of the last
+    if (st + 1 < s1) issue(buf ^ 1);
+    const bool masked = r0 < all_lo || r0 + kKeys - 1 > all_hi;
+    const uint32_t at = buf * kBuf;
 #pragma unroll
-        for (int m2 = 0; m2 < 2; ++m2) {
-          f32x16 s = {}, dp = {};
+    for (int m2 = 0; m2 < 2; ++m2) {
+      qa.remade();
+      ga.remade();
+      f32x16 s = {}, dp = {};
 #pragma unroll
-          for (int cc = 0; cc < NC; ++cc) s = E::mfma32(qa.by_row(m2, cc), k[cc], s);
+      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(qa.by_row(m2, cc, at), k[cc], s);
 #pragma unroll
-          for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(ga.by_row(m2, cc), v[cc], dp);
-          const int off = a.q_start + t0 + 32 * m2 + 4 * half - kr.pl;
-          const uint32_t span = static_cast<uint32_t>(kr.ph - kr.pl);
-          const bool none = kr.ph < kr.pl;
+      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(ga.by_row(m2, cc, at), v[cc], dp);
+      const float* lse = stat[buf][0] + 32 * m2 + 4 * half;
+      const float* delta = stat[buf][1] + 32 * m2 + 4 * half;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = 8 * (r >> 2) + (r & 3);
-            const bool on = !none && static_cast<uint32_t>(off + i) <= span;
-            const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse[32 * m2 + 4 * half + i]));
-            s[r] = on ? pr : 0.f;
-            dp[r] = on ? pr * (dp[r] - delta[32 * m2 + 4 * half + i]) : 0.f;
-          }
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const float4 l4 = *reinterpret_cast<const float4*>(lse + 8 * r4);
+        const float4 d4 = *reinterpret_cast<const float4*>(delta + 8 * r4);
+        const float lx[4] = {l4.x, l4.y, l4.z, l4.w}, dx[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const bf16x8 pb = pack8<E>(s, ks), ds = pack8<E>(dp, ks);
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) dv[dt] = E::mfma32(ga.transposed(2 * m2 + ks, dt), pb, dv[dt]);
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) dk[dt] = E::mfma32(qa.transposed(2 * m2 + ks, dt), ds, dk[dt]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * r4 + i;
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lx[i]));
+          dp[r] = s[r] * (dp[r] - dx[i]);
         }
+      }
+      if (masked) {  // (what a key does not see may be anything up to here)
+        const int off = a.q_start + r0 + 32 * m2 + 4 * half - kr.pl;
+        const uint32_t span = static_cast<uint32_t>(kr.ph - kr.pl);
+        const bool none = kr.ph < kr.pl;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool on = !none && static_cast<uint32_t>(off + 8 * (r >> 2) + (r & 3)) <= span;
+          s[r] = on ? s[r] : 0.f;
+          dp[r] = on ? dp[r] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const bf16x8 pb = pack8<E>(s, ks);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dv[dt] = E::mfma32(ga.transposed(2 * m2 + ks, dt, at), pb, dv[dt]);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const bf16x8 ds = pack8<E>(dp, ks);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dk[dt] = E::mfma32(qa.transposed(2 * m2 + ks, dt, at), ds, dk[dt]);
       }
     }
   }
-  const bool on = j < a.Tk;
-  store_row<E>(dk, a.scale, a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h, on, half);
-  store_row<E>(dv, 1.f, a.dv + b * a.dv_b + static_cast<int64_t>(j) * a.dv_t + hk * a.dv_h, on, half);
+  if (kp.parts == 1) {
+    const bool on = j < a.Tk;
+    store_row<E>(dk, a.scale, a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h, on, half);
+    store_row<E>(dv, 1.f, a.dv + b * a.dv_b + static_cast<int64_t>(j) * a.dv_t + hk * a.dv_h, on, half);
+    return;
+  }
+  // [dk, dv][key][channel]: a lane has 4 consecutive channels of its key at a time
+  float* part = a.part + static_cast<int64_t>(kp.slot) * (2 * kRows * D) + (wave * 32 + (lane & 31)) * D + 4 * half;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x16 &x = dk[dt], &y = dv[dt];
+      *reinterpret_cast<float4*>(part + 32 * dt + 8 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      *reinterpret_cast<float4*>(part + kRows * D + 32 * dt + 8 * i) =
+          make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+    }
+}
+
+// The parts of the cut blocks added up: a thread has 8 channels of a key, dk or dv.
+template <typename E, int D>
+__global__ void __launch_bounds__(256) window_dkv_join_kernel(const WindowArgs a, int blocks) {
+  constexpr int C = D / 8;
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int ch = static_cast<int>(e % C) * 8, key = static_cast<int>(e / C % kRows);
+  const int which = static_cast<int>(e / (C * kRows) & 1);
+  const int64_t bk = e / (C * kRows * 2);
+  const int bh = static_cast<int>(bk / blocks), block = static_cast<int>(bk % blocks);
+  const int j = block * kRows + key;
+  if (bh >= a.B * a.Hkv || j >= a.Tk) return;
+  const bool sink = block < a.nsb;
+  const int parts = sink ? a.ks : a.kn;
+  const int64_t slot = static_cast<int64_t>(bh) * a.slots + (sink ? block * a.ks : a.nsb * a.ks + (block - a.nsb) * a.kn);
+  const float* p = a.part + (slot * 2 + which) * (kRows * D) + key * D + ch;
+  float x[8] = {};
+  for (int i = 0; i < parts; ++i) {
+    const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
+    x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w, x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
+    p += 2 * kRows * D;
+  }
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  uint16_t* out = which ? a.dv + b * a.dv_b + static_cast<int64_t>(j) * a.dv_t + hk * a.dv_h
+                        : a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h;
+  if (!which)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= a.scale;
+  Row8<E>::store(out + ch, x);
+}
+
+// How the key blocks of the backward are cut (WindowArgs::nsb, ks, kn, slots): the
+// sinks' blocks into parts no longer than another block, and every block further
+// where the launch would leave the CUs' two workgroups each empty, as long as a
+// part keeps eight steps.
+void cut_keys(WindowArgs& a) {
+  const int64_t tiles_all = cdiv(a.Tq, kKeys) + 1;
+  int64_t tiles = cdiv(static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + kRows, kKeys) + 1;
+  if (tiles > tiles_all) tiles = tiles_all;
+  const int64_t steps = tiles * a.group;
+  a.nsb = static_cast<int>(cdiv(a.sinks, kRows));
+  int64_t kn = cdiv(512, static_cast<int64_t>(a.B) * a.Hkv * a.nkb);
+  if (kn > steps / 8) kn = steps / 8;
+  if (kn < 1) kn = 1;
+  int64_t ks = cdiv(tiles_all * a.group, cdiv(steps, kn));
+  a.kn = static_cast<int>(kn);
+  a.ks = static_cast<int>(ks);
+  if (a.nsb == a.nkb) a.kn = a.ks;  // (only sinks' blocks)
+  a.slots = (a.ks > 1 ? a.nsb * a.ks : 0) + (a.kn > 1 ? (a.nkb - a.nsb) * a.kn : 0);
 }
 
 int check_mat(const Mat& m, const char* what, const char* name) {
+  // (a copy's lane offsets are 32-bit bytes)
+  SOLATTN_REQUIRE(m.t >= 0 && m.t < (1ll << 24), SOLATTN_EUNSUPPORTED, "%s: %s token stride %lld beyond 2^24 elements",
+                  what, name, (long long)m.t);
   SOLATTN_REQUIRE(m.p, SOLATTN_EINVAL, "%s: null %s", what, name);
   SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.b % 8 == 0 && m.t % 8 == 0 && m.h % 8 == 0,
                   SOLATTN_EINVAL, "%s: %s must be 16-byte aligned with strides multiple of 8", what, name);
@@ -342,8 +486,18 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   return check_launch(what);
 }
 
-extern "C" int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t H) {
-  return B <= 0 || Tq <= 0 || H <= 0 ? 0 : cdiv(B * H * Tq * 4, 256) * 256;
+static int64_t bwd_workspace(const WindowArgs& a, int64_t D) {
+  return cdiv(static_cast<int64_t>(a.B) * a.H * a.Tq * 4, 256) * 256 +
+         static_cast<int64_t>(a.B) * a.Hkv * a.slots * 2 * kRows * D * 4;
+}
+
+extern "C" int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
+                                                           int64_t D, int64_t window, int64_t sinks, int causal) {
+  clear_error();
+  WindowArgs a{};
+  if (setup(a, B, Tq, Tk, H, Hkv, D, SOLATTN_BF16, Tk - Tq, window, sinks, causal, 1.f, "window_attn_bwd")) return 0;
+  cut_keys(a);
+  return bwd_workspace(a, D);
 }
 
 extern "C" int solattn_window_attn_bwd(
@@ -370,12 +524,18 @@ extern "C" int solattn_window_attn_bwd(
   for (int i = 0; i < 8 && !rc; ++i) rc = check_mat(*mats[i], what, names[i]);
   if (rc) return rc;
   SOLATTN_REQUIRE(lse, SOLATTN_EINVAL, "%s: null lse", what);
-  SOLATTN_REQUIRE(workspace && workspace_bytes >= solattn_window_attn_bwd_workspace_bytes(B, Tq, H), SOLATTN_ESIZE,
-                  "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes,
-                  (long long)solattn_window_attn_bwd_workspace_bytes(B, Tq, H));
+  cut_keys(a);
+  const int64_t need = bwd_workspace(a, D);
+  SOLATTN_REQUIRE(workspace && workspace_bytes >= need, SOLATTN_ESIZE, "%s: workspace %lld < %lld bytes", what,
+                  (long long)workspace_bytes, (long long)need);
   SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SOLATTN_EINVAL,
                   "%s: workspace must be 256-byte aligned", what);
   a.delta = static_cast<float*>(workspace);
+  a.part = a.delta + cdiv(B * H * Tq * 4, 256) * 64;
+  const int64_t items = B * Hkv * (static_cast<int64_t>(a.nsb) * a.ks + static_cast<int64_t>(a.nkb - a.nsb) * a.kn);
+  const int64_t cut = a.kn > 1 ? a.nkb : a.ks > 1 ? a.nsb : 0;  // blocks of keys to join
+  const int64_t join = cdiv(B * Hkv * cut * 2 * kRows * (D / 8), 256);
+  SOLATTN_REQUIRE(items < (1ll << 31) && join < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf = dtype == SOLATTN_BF16;
   const auto kq = D == 128 ? (bf ? window_dq_kernel<Bf16, 128> : window_dq_kernel<Fp16, 128>)
@@ -384,6 +544,10 @@ extern "C" int solattn_window_attn_bwd(
   if ((rc = check_launch(what))) return rc;
   const auto kk = D == 128 ? (bf ? window_dkv_kernel<Bf16, 128> : window_dkv_kernel<Fp16, 128>)
                            : (bf ? window_dkv_kernel<Bf16, 64> : window_dkv_kernel<Fp16, 64>);
-  hipLaunchKernelGGL(kk, dim3(static_cast<uint32_t>(B * Hkv * a.nkb)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(kk, dim3(static_cast<uint32_t>(items)), dim3(kThreads), 0, s, a);
+  if ((rc = check_launch(what)) || cut == 0) return rc;
+  const auto kj = D == 128 ? (bf ? window_dkv_join_kernel<Bf16, 128> : window_dkv_join_kernel<Fp16, 128>)
+                           : (bf ? window_dkv_join_kernel<Bf16, 64> : window_dkv_join_kernel<Fp16, 64>);
+  hipLaunchKernelGGL(kj, dim3(static_cast<uint32_t>(join)), dim3(256), 0, s, a, static_cast<int>(cut));
   return check_launch(what);
 }

@@ -33,6 +33,8 @@ struct WindowArgs {
   int B, H, Hkv, group, Tq, Tk, q_start;
   int window, sinks, causal; // window <= 2^30
   int nqb, nkb;              // blocks of rows and of keys
+  int nsb, ks, kn, slots;    // backward: blocks with sinks; parts of these and of the others; cut blocks' slots a head
+  float* part;               // [B Hkv][slots][dk, dv][128][D]
   float c, scale;            // c = scale log2(e)
 };
 
@@ -106,6 +108,28 @@ __device__ __forceinline__ uint32_t xcd_run(uint32_t w, uint32_t total) {
   return x * q8 + min(x, rem) + (w >> 3);
 }
 
+// Item of the dk, dv launch -> (batch, kv head), block of keys and part; slot: its
+// place in the workspace, when its block is cut.
+struct KeyPart {
+  int bh, block, part, parts;
+  int64_t slot;
+};
+__device__ __forceinline__ KeyPart key_part(const WindowArgs& a, uint32_t w) {
+  const int sink_items = a.nsb * a.ks, items = sink_items + (a.nkb - a.nsb) * a.kn;
+  KeyPart k;
+  k.bh = static_cast<int>(w / items);
+  const int i = static_cast<int>(w % items);
+  if (i < sink_items) {
+    k.block = i / a.ks, k.part = i % a.ks, k.parts = a.ks;
+    k.slot = static_cast<int64_t>(k.bh) * a.slots + i;
+  } else {
+    const int n = i - sink_items;
+    k.block = a.nsb + n / a.kn, k.part = n % a.kn, k.parts = a.kn;
+    k.slot = static_cast<int64_t>(k.bh) * a.slots + sink_items + n;
+  }
+  return k;
+}
+
 // ------------------------------------------------------------------- LDS tiles
 // Tiles that are read both by rows (16-byte pieces of 16 rows) and transposed
 // (ds_read_b64_tr_b16: 4 rows x 4 consecutive pieces) need one swizzle that keeps
@@ -129,11 +153,30 @@ template <int NTHREADS, int D, int HOW, typename RowOf>
 __device__ __forceinline__ void copy_tile(uint32_t dst, const uint16_t* base, int64_t stride, RowOf&& row_of) {
   constexpr int C = D / 8, U = kKeys * C / NTHREADS;
   const uint32_t l0 = dst + wave_id() * 64 * 16;
+  uint32_t tid = threadIdx.x;  // (hidden: the addresses are made at each copy, not held through a loop)
+  asm volatile("" : "+v"(tid));
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int e = threadIdx.x + NTHREADS * u, row = e / C, pc = e % C;
+    const int e = tid + NTHREADS * u, row = e / C, pc = e % C;
     g2l16(base + static_cast<int64_t>(row_of(row)) * stride + swz<D, HOW>(row, pc) * 8, l0 + NTHREADS * u * 16);
   }
+}
+
+// Whole tiles of consecutive rows need one lane offset: a copy of all threads is
+// NTHREADS / (D / 8) rows, after which a lane's swizzle repeats.
+template <int NTHREADS, int D, int HOW>
+__device__ __forceinline__ uint32_t copy_offset(int64_t stride) {
+  constexpr int C = D / 8;
+  static_assert(NTHREADS / C % 16 == 0, "a lane keeps its piece");
+  const int row = threadIdx.x / C, pc = threadIdx.x % C;
+  return static_cast<uint32_t>((row * stride + swz<D, HOW>(row, pc) * 8) * 2);
+}
+template <int NTHREADS, int D>
+__device__ __forceinline__ void copy_whole(uint32_t dst, const uint16_t* first, int64_t stride, uint32_t off) {
+  constexpr int R = NTHREADS / (D / 8), U = kKeys / R;
+  const uint32_t l0 = dst + wave_id() * 64 * 16;
+#pragma unroll
+  for (int u = 0; u < U; ++u) g2l16_s(first + u * R * stride, off, l0 + NTHREADS * u * 16);
 }
 
 // Operands of an LDS tile (256-byte aligned): the row operand (m, cc) is rows
@@ -150,14 +193,17 @@ struct TileAddr {
     tr0 = tile + r0 * (2 * D) + 16 * swz<D, HOW>(r0, cp) + 8 * (sl & 1);
     tr1 = tile + (r0 + 8) * (2 * D) + 16 * swz<D, HOW>(r0 + 8, cp) + 8 * (sl & 1);
   }
-  __device__ __forceinline__ bf16x8 by_row(int m, int cc) const {
-    const uint32_t x = (row ^ static_cast<uint32_t>(cc << 5)) + m * (64 * D);
+  // Hides the addresses from the optimiser: what is derived from them afterwards is
+  // derived there, not hoisted out of the loop into registers of its own.
+  __device__ __forceinline__ void remade() { asm volatile("" : "+v"(row), "+v"(tr0), "+v"(tr1)); }
+  __device__ __forceinline__ bf16x8 by_row(int m, int cc, uint32_t at = 0) const {  // at: bytes to another buffer
+    const uint32_t x = (row ^ static_cast<uint32_t>(cc << 5)) + m * (64 * D) + at;
     return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(static_cast<uintptr_t>(x));
   }
-  __device__ __forceinline__ bf16x8 transposed(int ks, int dt) const {
+  __device__ __forceinline__ bf16x8 transposed(int ks, int dt, uint32_t at = 0) const {
     typedef short v4i16 __attribute__((ext_vector_type(4)));
-    const uint32_t x0 = (tr0 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D);
-    const uint32_t x1 = (tr1 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D);
+    const uint32_t x0 = (tr0 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D) + at;
+    const uint32_t x1 = (tr1 ^ static_cast<uint32_t>(dt << 6)) + ks * (32 * D) + at;
     const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         reinterpret_cast<__attribute__((address_space(3))) v4i16*>(static_cast<uintptr_t>(x0)));
     const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(

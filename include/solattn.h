@@ -365,7 +365,7 @@ int solattn_sol_attn_noalloc(const uint16_t* q, int64_t sq_b, int64_t sq_t, int6
  * reference. q, o: BTHD with H query heads; k, v: BTHD with Hkv kv heads, each
  * shared by the H / Hkv query heads behind one another (H % Hkv == 0). Rows
  * (the last dim) are contiguous, 16-byte aligned, and every stride keeps them
- * so; strides may be 0 or negative for inputs. Sums, softmax statistics and
+ * so; strides may be 0 for inputs, token strides below 2^24 elements. Sums, softmax statistics and
  * accumulators are fp32; outputs are rounded once. */
 enum { SOLATTN_BF16 = 0, SOLATTN_FP16 = 1, SOLATTN_FP32 = 2 }; /* dtype arguments */
 
@@ -444,7 +444,8 @@ int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t s
 /* Gradients of solattn_window_attn from its inputs, o, lse and do: dq like q, dk and dv
  * like k (every row written, zeros where nothing is seen). workspace: 256-byte
  * aligned. No atomics: the same inputs give the same bits. */
-int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t H);
+int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
+                                                int64_t D, int64_t window, int64_t sinks, int causal);
 int solattn_window_attn_bwd(
     const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k, int64_t sk_b,
     int64_t sk_t, int64_t sk_h, const uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h,
