@@ -59,7 +59,7 @@ SIGNATURES = {
     "solattn_qk_norm_rope_bwd_workspace_bytes": ([_l], _l),
     "solattn_qk_norm_rope_bwd": ([_p, _l, _l, _l] * 4 + [_l] * 5 + [_i] + [_p] * 4 + [_l, _l, _i, _p, _l, _f]
                                  + [_p, _l, _l, _l] * 2 + [_p, _p, _p, _l, _p], _i),
-    "solattn_window_attn_workspace_bytes": ([_l] * 8 + [_i], _l),
+    "solattn_window_attn_workspace_bytes": ([_l] * 9 + [_i, _i], _l),
     "solattn_window_attn": ([_p, _l, _l, _l] * 3 + [_l] * 6 + [_i, _l, _p, _l, _l, _i, _f]
                             + [_p, _l, _l, _l, _p, _p, _l, _p], _i),
     "solattn_window_attn_bwd_workspace_bytes": ([_l] * 8 + [_i], _l),

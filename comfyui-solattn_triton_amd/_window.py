@@ -19,9 +19,8 @@ def _run(q, k, v, lengths, plan, lse):
     window, sinks, causal, scale, q_start = plan
     out = torch.empty((B, Tq, H, D), device=q.device, dtype=q.dtype)
     with torch.cuda.device(q.device):
-        need = 0
-        if Tq == 1:
-            need = LIB.solattn_window_attn_workspace_bytes(B, Tq, H, Hkv, D, q_start, window, sinks, causal)
+        need = LIB.solattn_window_attn_workspace_bytes(B, Tq, Tk, H, Hkv, D, q_start, window, sinks, causal,
+                                                       lse is not None)
         ws = workspace(need, q.device)
         call("solattn_window_attn", ptr(q), *strides(q), ptr(k), *strides(k), ptr(v), *strides(v), B, Tq, Tk, H, Hkv,
              D, DTYPES[q.dtype], q_start, ptr(lengths), window, sinks, causal, scale, ptr(out), *strides(out),

@@ -28,6 +28,36 @@ struct Bf16 {
   static __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  // The instructions of a hand-ordered stream (fwd_common.hpp has the rules that its
+  // writer keeps): MFMAs, and p = exp2(s c + neg) of two scores, rounded, packed and
+  // added to the row sum as rounded.
+  static __device__ __forceinline__ void amfma0(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma_first(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("s_nop 2\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma_tie(f32x16& d, const bf16x8& a, const bf16x8& b, f32x16& s) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\ts_nop 3" : "+v"(d), "+v"(s) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ uint32_t exp_pair(float s0, float s1, float c, float neg, float& sum) {
+    uint32_t p;
+    float t0, t1;
+    asm volatile(
+        "v_fma_f32 %2, %4, %6, %7\n\t"
+        "v_fma_f32 %3, %5, %6, %7\n\t"
+        "v_exp_f32 %2, %2\n\t"
+        "v_exp_f32 %3, %3\n\t"
+        "s_nop 0\n\t"
+        "v_cvt_pk_bf16_f32 %0, %2, %3\n\t"
+        "v_dot2_f32_bf16 %1, %0, %8, %1"
+        : "=&v"(p), "+v"(sum), "=&v"(t0), "=&v"(t1)
+        : "v"(s0), "v"(s1), "v"(c), "v"(neg), "s"(0x3F803F80u));
+    return p;
+  }
 };
 
 struct Fp16 {
@@ -46,6 +76,36 @@ struct Fp16 {
   static __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                   0, 0);
+  }
+  // The instructions of a hand-ordered stream (fwd_common.hpp has the rules that its
+  // writer keeps): MFMAs, and p = exp2(s c + neg) of two scores, rounded, packed and
+  // added to the row sum as rounded.
+  static __device__ __forceinline__ void amfma0(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma_first(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("s_nop 2\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ void amfma_tie(f32x16& d, const bf16x8& a, const bf16x8& b, f32x16& s) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %3, %0\n\ts_nop 3" : "+v"(d), "+v"(s) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ uint32_t exp_pair(float s0, float s1, float c, float neg, float& sum) {
+    uint32_t p;
+    float t0, t1;
+    asm volatile(
+        "v_fma_f32 %2, %4, %6, %7\n\t"
+        "v_fma_f32 %3, %5, %6, %7\n\t"
+        "v_exp_f32 %2, %2\n\t"
+        "v_exp_f32 %3, %3\n\t"
+        "s_nop 0\n\t"
+        "v_cvt_pk_f16_f32 %0, %2, %3\n\t"
+        "v_dot2_f32_f16 %1, %0, %8, %1"
+        : "=&v"(p), "+v"(sum), "=&v"(t0), "=&v"(t1)
+        : "v"(s0), "v"(s1), "v"(c), "v"(neg), "s"(0x3C003C00u));
+    return p;
   }
 };
 

@@ -24,10 +24,12 @@ constexpr int kThreads = 2 * kRows;   // a wave for 32 of them
 // stays 0, and below every score that counts.
 constexpr float kNoMax = -1e30f;
 
-// Workgroup -> (batch, kv head, block of rows, query head): the query heads of one
-// kv head and block run side by side.
-__device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, int& qb) {
+// Workgroup -> (batch, kv head, block of rows, query head, part): the query heads of
+// one kv head and block run side by side.
+__device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, int& qb, int& part) {
   uint32_t w = xcd_run(blockIdx.x, gridDim.x);
+  part = w % a.split;
+  w /= a.split;
   const int g = w % a.group;
   w /= a.group;
   qb = w % a.nqb;
@@ -36,84 +38,256 @@ __device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, in
   b = w / a.Hkv;
 }
 
-template <typename E, int D>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
-window_fwd_kernel(const WindowArgs a) {
-  constexpr int ND = D / 32, NC = D / 16;
-  __shared__ __align__(256) uint16_t kbuf[kKeys * D];
-  __shared__ __align__(256) uint16_t vbuf[kKeys * D];
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  int b, h, qb;
-  row_item(a, b, h, qb);
-  const int len = sequence_length(a, b), hk = h / a.group;
-  const int r0 = qb * kRows, row = r0 + wave_id() * 32 + (lane & 31);
-  const int p = a.q_start + min(row, a.Tq - 1);
-  const KeyTiles kt = key_tiles(a, a.q_start + r0, a.q_start + min(r0 + kRows, a.Tq) - 1, len);
-  const RowKeys rk = row_keys(a, p, len);
-  const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
-  const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
-  const uint32_t kb = lds_addr(kbuf), vb = lds_addr(vbuf);
-  const TileAddr<D, kByRow> ka(kb, lane);
-  const TileAddr<D, kTransposed> va(vb, lane);
-  bf16x8 q[NC];
-  load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(min(row, a.Tq - 1)) * a.q.t + h * a.q.h, half);
-
-  f32x16 acc[ND] = {};
-  float m = kNoMax, l = 0.f;
-  for (int t = 0; t < kt.n; ++t) {
-    const int j0 = kt.first(t);
-    const auto safe = [&](int r) { return kt.safe(j0 + r); };
-    __syncthreads();
-    copy_tile<kThreads, D, kByRow>(kb, kp, a.k.t, safe);
-    copy_tile<kThreads, D, kTransposed>(vb, vp, a.v.t, safe);
-    wait_tile_copies();
-    __syncthreads();
-#pragma unroll
-    for (int m2 = 0; m2 < 2; ++m2) {
-      f32x16 s = {};
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc), q[cc], s);
-      mask_keys(s, rk, j0 + 32 * m2, half);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
-      const float m_new = fmaxf(m, xhalf_max(mx) * a.c);
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -m));
-      bf16x8 pb[2];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        pb[ks] = pack8<E>(s, ks);
-        const uint4 w = __builtin_bit_cast(uint4, pb[ks]);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += E::lo(u[i]) + E::hi(u[i]);
-      }
-      l = fmaf(l, alpha, sum);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) acc[dt] *= alpha;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(va.transposed(2 * m2 + ks, dt), pb[ks], acc[dt]);
-    }
-  }
-  l = xhalf_sum(l);
-  const bool on = row < a.Tq;
-  store_row<E>(acc, l == 0.f ? 0.f : 1.f / l, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h,
-               on, half);
-  if (a.lse && on && half == 0)
-    a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
-}
-
 // Wave-wide minimum and maximum of a lane value, as scalars.
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
   return __builtin_amdgcn_readfirstlane(x);
+}
+
+template <int ND>
+struct RowState {
+  float m, l;      // running max (log2 domain) and this lane's row sum
+  f32x16 acc[ND];  // O^T
+};
+
+// One step of the forward's pipeline over half tiles of 32 keys, in one hand-ordered
+// stream: S(n+1) = K(n+1) Q^T, O += P(n-1) V(n-1) and the softmax of S(n). Slot i
+// issues a score MFMA, two exps and a P.V MFMA; the operands of slot i + 2 are read
+// at its top (the empty asm keeps them there). The running max stays as it is unless
+// a lane's sum of P passes 255 (no sum above 255: no score more than 8 above it), in
+// which case P is made again and O rescaled, behind the products with P(n-1).
+template <typename E, int D>
+__device__ __forceinline__ void window_step(RowState<D / 32>& st, const f32x16& sc, f32x16& sn, const bf16x8 (&pp)[2],
+                                            bf16x8 (&pn)[2], uint32_t kl, uint32_t vl, const bf16x8 (&q)[D / 16],
+                                            float c) {
+  constexpr int ND = D / 32, NM = D / 16, SLOTS = 8 / NM;
+  bf16x8 ka[3], va[3];
+  uint32_t pw[2][4];
+  float psum = 0.f;
+  const float neg = -st.m;
+  ka[0] = k_op_x<D>(kl, 0, 0);
+  ka[1] = k_op_x<D>(kl, 0, 1);
+  va[0] = v_op_x<D>(vl, 0, 0);
+  va[1] = v_op_x<D>(vl, 0, 1);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int j = i / SLOTS;
+    if (i % SLOTS == 0) {
+      if (j + 2 < NM) {
+        ka[(j + 2) % 3] = k_op_x<D>(kl, 0, j + 2);
+        va[(j + 2) % 3] = v_op_x<D>(vl, (j + 2) / ND, (j + 2) % ND);
+        asm volatile("" ::: "memory");
+      }
+      if (j == 0)
+        E::amfma0(sn, ka[0], q[0]);
+      else
+        E::amfma(sn, ka[j % 3], q[j]);
+    }
+    pw[i >> 2][i & 3] = E::exp_pair(sc[2 * i], sc[2 * i + 1], c, neg, psum);
+    if (i % SLOTS == SLOTS - 1) {
+      if (j == 0)
+        E::amfma_first(st.acc[0], va[0], pp[0]);
+      else if (j == NM - 1)
+        E::amfma_tie(st.acc[ND - 1], va[j % 3], pp[1], sn);
+      else
+        E::amfma(st.acc[j % ND], va[j % 3], pp[j / ND]);
+    }
+    if (i == 0) __builtin_amdgcn_s_setprio(1);
+  }
+  __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+    pn[ks] = __builtin_bit_cast(bf16x8, make_uint4(pw[ks][0], pw[ks][1], pw[ks][2], pw[ks][3]));
+  if (__any(!(psum <= 255.f))) {  // (also infinities and NaN)
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+    float alpha;
+    const float m_new = new_max(st.m, xhalf_max(mx) * c, alpha);
+    if (__any(m_new != st.m)) {  // lanes whose max stays make the same P
+      st.m = m_new;
+      st.l *= alpha;
+      psum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pw[i >> 2][i & 3] = E::exp_pair(sc[2 * i], sc[2 * i + 1], c, -m_new, psum);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        pn[ks] = __builtin_bit_cast(bf16x8, make_uint4(pw[ks][0], pw[ks][1], pw[ks][2], pw[ks][3]));
+      mfma_fence(st.acc);  // the rescale reads O
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) st.acc[dt] *= alpha;
+    }
+  }
+  st.l += psum;
+}
+
+// The forward. Two half buffers of 32 rows each for K and V: step n copies K(n+2)
+// over K(n) and V(n) over V(n-2), so a copy has a whole step to land.
+template <typename E, int BLK, int D>
+__global__ void __launch_bounds__(2 * BLK) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
+window_fwd_kernel(const WindowArgs a) {
+  constexpr int ND = D / 32, NC = D / 16, NT = 2 * BLK;
+  constexpr uint32_t kHalf = kKeys * D;  // bytes of half a tile
+  __shared__ __align__(256) uint16_t kbuf[kKeys * D];
+  __shared__ __align__(256) uint16_t vbuf[kKeys * D];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  int b, h, qb, part;
+  row_item(a, b, h, qb, part);
+  const int len = sequence_length(a, b), hk = h / a.group;
+  const int r0 = qb * BLK, row = r0 + wave_id() * 32 + (lane & 31), rr = min(row, a.Tq - 1);
+  const KeyTiles kt = key_tiles(a, a.q_start + r0, a.q_start + min(r0 + BLK, a.Tq) - 1, len);
+  const RowKeys rk = row_keys(a, a.q_start + rr, len);
+  const int per = (kt.n + a.split - 1) / a.split, tile0 = min(part * per, kt.n);
+  const int ntiles = __builtin_amdgcn_readfirstlane(min(per, kt.n - tile0));
+  const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
+  const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
+  const uint32_t kb = lds_addr(kbuf), vb = lds_addr(vbuf);
+  const uint32_t kl = k_lane<D>(kb, lane & 31, half), vl = v_lane<D>(vb, lane);
+
+  RowState<ND> st;
+  st.m = kNoMax;
+  st.l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) st.acc[dt] = f32x16{};
+
+  if (ntiles > 0) {
+    CopyOffsets<NT, D> off;
+    off.init(a.k.t, a.v.t);
+    // Half n of the part's tiles into buffer n & 1.
+    const auto issue = [&](int kv, int n) __attribute__((always_inline)) {
+      const int t = tile0 + (n >> 1), hh = n & 1, j0 = kt.first(t);
+      const uint32_t dst = (kv ? vb : kb) + hh * kHalf;
+      const uint16_t* base = kv ? vp : kp;
+      const int64_t stride = kv ? a.v.t : a.k.t;
+      if (kt.whole(t)) {
+        issue_half<NT, D>(dst, base + (j0 + 32 * hh) * stride, stride, kv ? off.v : off.k);
+      } else {
+        const auto safe = [&](int r) { return kt.safe(j0 + r); };
+        if (kv)
+          copy_half<NT, D, kTransposed>(dst, hh, base, stride, safe);
+        else
+          copy_half<NT, D, kByRow>(dst, hh, base, stride, safe);
+      }
+    };
+    const auto land = [&]() __attribute__((always_inline)) {
+      wait_tile_copies();
+      __syncthreads();
+    };
+    // keys that every row of the wave sees
+    const int all_lo = -wave_min(-rk.jl), all_hi = wave_min(rk.jh), all_sk = wave_min(rk.sk);
+    const auto mask = [&](f32x16& s, int n) __attribute__((always_inline)) {
+      const int j0 = kt.first(tile0 + (n >> 1)) + 32 * (n & 1);
+      if (!((j0 >= all_lo && j0 + 31 <= all_hi) || j0 + 32 <= all_sk)) mask_keys(s, rk, j0, half);
+    };
+    const int last = 2 * ntiles - 1;
+
+    issue(0, 0);
+    issue(0, 1);
+    issue(1, 0);
+    bf16x8 q[NC];
+    load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
+    f32x16 sa, sb;  // scores of even and odd halves
+    bf16x8 pa[2], pb[2];
+    land();
+    // Step 0, without a stream: both halves are scored, the running max is the whole tile's.
+    {
+      f32x16 s0 = {}, s1 = {};
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) s0 = E::mfma32(k_op_x<D>(kl, 0, cc), q[cc], s0);
+      __syncthreads();  // every wave is done with K(0)
+      if (last > 1) issue(0, 2);
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) s1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], s1);
+      mask(s0, 0);
+      f32x16 t = s1;
+      mask(t, 1);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(s0[r], t[r]));
+      st.m = fmaxf(kNoMax, xhalf_max(mx) * a.c);
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = E::exp_pair(s0[2 * i], s0[2 * i + 1], a.c, -st.m, st.l);
+      pa[0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+      pa[1] = __builtin_bit_cast(bf16x8, make_uint4(w[4], w[5], w[6], w[7]));
+      sb = t;
+    }
+    mfma_fence(st.acc);  // O's zeros are in their registers before the asm MFMAs that add to them
+    land();
+    const auto odd = [&](int n) __attribute__((always_inline)) {
+      if (n + 2 <= last) issue(0, n + 2);
+      issue(1, n);
+      window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, a.c);
+      land();
+    };
+    const auto even = [&](int n) __attribute__((always_inline)) {
+      if (n + 2 <= last) issue(0, n + 2);
+      issue(1, n);
+      mask(sa, n);
+      window_step<E, D>(st, sa, sb, pb, pa, kl + kHalf, vl + kHalf, q, a.c);
+      mask(sb, n + 1);
+      land();
+    };
+    int n = 1;
+    for (; n < last; n += 2) {
+      odd(n);
+      even(n + 1);
+    }
+    odd(n);
+    // P.V of the last half
+    mfma_fence(st.acc);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      st.acc[i % ND] = E::mfma32(v_op_x<D>(vl + kHalf, i / ND, i % ND), pb[i / ND], st.acc[i % ND]);
+  }
+
+  const float l = xhalf_sum(st.l);
+  const bool on = row < a.Tq;
+  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.Tq + row;
+  if (a.split > 1) {
+    if (!on) return;
+    float* p = a.part + (at * a.split + part) * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x16& x = st.acc[dt];
+        *reinterpret_cast<float4*>(p + 32 * dt + 8 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      }
+    if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (at * a.split + part)) = make_float2(st.m, l);
+    return;
+  }
+  store_row<E>(st.acc, l == 0.f ? 0.f : 1.f / l, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h,
+               on, half);
+  if (a.lse && on && half == 0) a.lse[at] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
+}
+
+// The parts of the rows joined: a wave per row, two channels a lane.
+template <typename E, int D>
+__global__ void __launch_bounds__(256) window_join_kernel(const WindowArgs a) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (at >= static_cast<int64_t>(a.B) * a.H * a.Tq) return;
+  const int lane = threadIdx.x & 63, ch = 2 * lane;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.split;
+  float top = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int i = 0; i < a.split; ++i) top = fmaxf(top, ml[i].x);
+  const float* p = a.part + at * a.split * D + (ch < D ? ch : 0);
+  for (int i = 0; i < a.split; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
+    const float2 x = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(i) * D);
+    l = fmaf(ml[i].y, f, l);
+    o0 = fmaf(x.x, f, o0);
+    o1 = fmaf(x.y, f, o1);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int row = static_cast<int>(at % a.Tq);
+  const int64_t bh = at / a.Tq;
+  if (ch < D)
+    *reinterpret_cast<uint32_t*>(a.out + (bh / a.H) * a.out_b + static_cast<int64_t>(row) * a.out_t +
+                                 (bh % a.H) * a.out_h + ch) = E::pack(o0 * inv, o1 * inv);
+  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
@@ -125,8 +299,8 @@ window_dq_kernel(const WindowArgs a) {
   __shared__ __align__(256) uint16_t kbuf[2 * kKeys * D];
   __shared__ __align__(256) uint16_t vbuf[2 * kKeys * D];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  int b, h, qb;
-  row_item(a, b, h, qb);
+  int b, h, qb, part;
+  row_item(a, b, h, qb, part);
   const int len = sequence_length(a, b), hk = h / a.group;
   const int r0 = qb * kRows, row = r0 + wave_id() * 32 + (lane & 31), rr = min(row, a.Tq - 1);
   const int p = a.q_start + rr;
@@ -433,6 +607,7 @@ int setup(WindowArgs& a, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t H
   a.window = static_cast<int>(window < Tk ? window : Tk), a.sinks = static_cast<int>(sinks < Tk ? sinks : Tk);
   a.causal = causal;
   a.nqb = static_cast<int>(cdiv(Tq, kRows)), a.nkb = static_cast<int>(cdiv(Tk, kRows));
+  a.split = 1;
   a.c = scale * kLog2e, a.scale = scale;
   SOLATTN_REQUIRE(B * H * a.nqb < (1ll << 31) && B * Hkv * a.nkb < (1ll << 31), SOLATTN_EUNSUPPORTED,
                   "%s: grid too large", what);
@@ -447,9 +622,35 @@ using namespace solattn;
 // One causal row per sequence: the kernel of single tokens, which splits the keys.
 static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq == 1 && causal && !lse; }
 
-extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t H, int64_t Hkv, int64_t D,
-                                                       int64_t q_start, int64_t window, int64_t sinks, int causal) {
-  return single_token(Tq, causal, nullptr) ? paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks) : 0;
+// Rows of a workgroup and parts of their keys. 128 rows share the copies of a tile
+// among four waves; launches that would not give every CU two such workgroups take
+// 64 rows, and where these are still few their key tiles are cut into parts of at
+// least eight tiles, joined by a second launch.
+static int cut_rows(WindowArgs& a) {
+  const int64_t bh = static_cast<int64_t>(a.B) * a.H;
+  const int blk = bh * cdiv(a.Tq, 128) >= 512 ? 128 : 64;
+  a.nqb = static_cast<int>(cdiv(a.Tq, blk));
+  const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
+  const int64_t tiles = cdiv(reach < a.Tk ? reach : a.Tk, kKeys);
+  int64_t n = cdiv(512, bh * a.nqb);
+  if (n > tiles / 8) n = tiles / 8;
+  a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+  return blk;
+}
+
+static int64_t fwd_workspace(const WindowArgs& a, int64_t D) {
+  return a.split > 1 ? static_cast<int64_t>(a.B) * a.H * a.Tq * a.split * (D + 2) * 4 : 0;
+}
+
+extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
+                                                       int64_t D, int64_t q_start, int64_t window, int64_t sinks,
+                                                       int causal, int with_lse) {
+  clear_error();
+  if (Tq == 1 && causal && !with_lse) return paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks);
+  WindowArgs a{};
+  if (setup(a, B, Tq, Tk, H, Hkv, D, SOLATTN_BF16, q_start, window, sinks, causal, 1.f, "window_attn")) return 0;
+  cut_rows(a);
+  return fwd_workspace(a, D);
 }
 
 extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k,
@@ -479,10 +680,28 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   if (!rc) rc = check_mat({o, so_b, so_t, so_h}, what, "o");
   if (rc) return rc;
   const bool bf = dtype == SOLATTN_BF16;
-  const auto kern = D == 128 ? (bf ? window_fwd_kernel<Bf16, 128> : window_fwd_kernel<Fp16, 128>)
-                             : (bf ? window_fwd_kernel<Bf16, 64> : window_fwd_kernel<Fp16, 64>);
-  hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(B * H * a.nqb)), dim3(kThreads), 0,
-                     reinterpret_cast<hipStream_t>(stream), a);
+  const int blk = cut_rows(a);
+  const int64_t need = fwd_workspace(a, D);
+  SOLATTN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SOLATTN_ESIZE, "%s: workspace %lld < %lld bytes",
+                  what, (long long)workspace_bytes, (long long)need);
+  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SOLATTN_EINVAL,
+                  "%s: workspace must be 256-byte aligned", what);
+  const int64_t rows = B * H * Tq;
+  SOLATTN_REQUIRE(rows < (1ll << 31) && B * H * a.nqb * a.split < (1ll << 31), SOLATTN_EUNSUPPORTED,
+                  "%s: grid too large", what);
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = a.part + rows * a.split * D;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const auto k128 = D == 128 ? (bf ? window_fwd_kernel<Bf16, 128, 128> : window_fwd_kernel<Fp16, 128, 128>)
+                             : (bf ? window_fwd_kernel<Bf16, 128, 64> : window_fwd_kernel<Fp16, 128, 64>);
+  const auto k64 = D == 128 ? (bf ? window_fwd_kernel<Bf16, 64, 128> : window_fwd_kernel<Fp16, 64, 128>)
+                            : (bf ? window_fwd_kernel<Bf16, 64, 64> : window_fwd_kernel<Fp16, 64, 64>);
+  hipLaunchKernelGGL(blk == 128 ? k128 : k64, dim3(static_cast<uint32_t>(B * H * a.nqb * a.split)),
+                     dim3(static_cast<uint32_t>(2 * blk)), 0, s, a);
+  if ((rc = check_launch(what)) || a.split == 1) return rc;
+  const auto kj = D == 128 ? (bf ? window_join_kernel<Bf16, 128> : window_join_kernel<Fp16, 128>)
+                           : (bf ? window_join_kernel<Bf16, 64> : window_join_kernel<Fp16, 64>);
+  hipLaunchKernelGGL(kj, dim3(static_cast<uint32_t>(cdiv(rows, 4))), dim3(256), 0, s, a);
   return check_launch(what);
 }
 

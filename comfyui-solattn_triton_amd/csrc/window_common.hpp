@@ -33,8 +33,10 @@ struct WindowArgs {
   int B, H, Hkv, group, Tq, Tk, q_start;
   int window, sinks, causal; // window <= 2^30
   int nqb, nkb;              // blocks of rows and of keys
+  int split;                 // forward: parts of a block's key tiles
   int nsb, ks, kn, slots;    // backward: blocks with sinks; parts of these and of the others; cut blocks' slots a head
-  float* part;               // [B Hkv][slots][dk, dv][128][D]
+  float* part;               // backward: [B Hkv][slots][dk, dv][128][D]; forward: [B H][Tq][split][D]
+  float* part_ml;            // forward: [B H][Tq][split][max, sum]
   float c, scale;            // c = scale log2(e)
 };
 
@@ -177,6 +179,21 @@ __device__ __forceinline__ void copy_whole(uint32_t dst, const uint16_t* first, 
   const uint32_t l0 = dst + wave_id() * 64 * 16;
 #pragma unroll
   for (int u = 0; u < U; ++u) g2l16_s(first + u * R * stride, off, l0 + NTHREADS * u * 16);
+}
+
+// Half a tile (rows [32 hh, 32 hh + 32) of it) for the forward's pipeline: row i from
+// base + row_of(32 hh + i) stride, or consecutive rows from `first` on (issue_half).
+template <int NTHREADS, int D, int HOW, typename RowOf>
+__device__ __forceinline__ void copy_half(uint32_t dst, int hh, const uint16_t* base, int64_t stride, RowOf&& row_of) {
+  constexpr int C = D / 8, U = kKeys / 2 * C / NTHREADS;
+  const uint32_t l0 = dst + wave_id() * 64 * 16;
+  uint32_t tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = tid + NTHREADS * u, row = 32 * hh + e / C, pc = e % C;
+    g2l16(base + static_cast<int64_t>(row_of(row)) * stride + swz<D, HOW>(row, pc) * 8, l0 + NTHREADS * u * 16);
+  }
 }
 
 // Operands of an LDS tile (256-byte aligned): the row operand (m, cc) is rows
