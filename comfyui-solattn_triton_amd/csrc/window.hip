@@ -12,6 +12,8 @@
 // operand of the next product, whose A operand is read transposed from LDS
 // (ds_read_b64_tr_b16). P and dS are rounded to the inputs' type for the matrix
 // instruction; row sums add P as rounded, every other sum is fp32.
+#include <type_traits>
+
 #include "window_common.hpp"
 
 namespace solattn {
@@ -137,7 +139,8 @@ window_fwd_kernel(const WindowArgs a) {
   row_item(a, b, h, qb, part);
   const int len = sequence_length(a, b), hk = h / a.group;
   const int r0 = qb * BLK, row = r0 + wave_id() * 32 + (lane & 31), rr = min(row, a.Tq - 1);
-  const KeyTiles kt = key_tiles(a, a.q_start + r0, a.q_start + min(r0 + BLK, a.Tq) - 1, len);
+  const int p0 = a.q_start + r0, p1 = a.q_start + min(r0 + BLK, a.Tq) - 1;
+  const KeyTiles kt = key_tiles(a, p0, p1, len);
   const RowKeys rk = row_keys(a, a.q_start + rr, len);
   const int per = (kt.n + a.split - 1) / a.split, tile0 = min(part * per, kt.n);
   const int ntiles = __builtin_amdgcn_readfirstlane(min(per, kt.n - tile0));
@@ -216,26 +219,59 @@ window_fwd_kernel(const WindowArgs a) {
     }
     mfma_fence(st.acc);  // O's zeros are in their registers before the asm MFMAs that add to them
     land();
-    const auto odd = [&](int n) __attribute__((always_inline)) {
-      if (n + 2 <= last) issue(0, n + 2);
-      issue(1, n);
+    // (plain: copies and scores of tiles inside the run, at the pointers kn and vn)
+    const uint16_t *kn = kp, *vn = vp;
+    const int64_t k32 = 32 * a.k.t, v32 = 32 * a.v.t;
+    const auto copies = [&](int n, auto plain) __attribute__((always_inline)) {
+      if constexpr (decltype(plain)::value) {
+        issue_half<NT, D>(kb + (n & 1) * kHalf, kn, a.k.t, off.k);
+        issue_half<NT, D>(vb + (n & 1) * kHalf, vn, a.v.t, off.v);
+        kn += k32, vn += v32;
+      } else {
+        if (n + 2 <= last) issue(0, n + 2);
+        issue(1, n);
+      }
+    };
+    const auto odd = [&](int n, auto plain) __attribute__((always_inline)) {
+      copies(n, plain);
       window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, a.c);
       land();
     };
-    const auto even = [&](int n) __attribute__((always_inline)) {
-      if (n + 2 <= last) issue(0, n + 2);
-      issue(1, n);
-      mask(sa, n);
+    const auto even = [&](int n, auto plain) __attribute__((always_inline)) {
+      copies(n, plain);
+      if constexpr (!decltype(plain)::value) mask(sa, n);
       window_step<E, D>(st, sa, sb, pb, pa, kl + kHalf, vl + kHalf, q, a.c);
-      mask(sb, n + 1);
+      if constexpr (!decltype(plain)::value) mask(sb, n + 1);
       land();
     };
-    int n = 1;
-    for (; n < last; n += 2) {
-      odd(n);
-      even(n + 1);
+    // Steps 2 t + 1 and 2 t + 2 work on tiles t to t + 2 of the part. Where these lie in
+    // the run of window tiles that every row of the block sees whole, they need no
+    // masks, and their copies are 32 rows apart.
+    int t = 0, run0, run1;
+    {
+      const int lo = max(p1 - a.window + 1, 0), hi = min(a.causal ? p0 : p0 + a.window - 1, len - 1);
+      run0 = max(kt.ns, kt.ns + (lo - kt.w0 + kKeys - 1) / kKeys) - tile0;
+      run1 = p1 < len ? min(kt.ns + (hi + 1 - kt.w0) / kKeys - tile0, ntiles) - 2 : 0;
+      run0 = max(run0, 0);
     }
-    odd(n);
+    for (; t < min(run0, ntiles - 1); ++t) {
+      odd(2 * t + 1, std::false_type());
+      even(2 * t + 2, std::false_type());
+    }
+    if (t < run1) {
+      const int j0 = kt.first(tile0 + t);
+      kn += (j0 + 96) * a.k.t;
+      vn += (j0 + 32) * a.v.t;
+    }
+    for (; t < run1; ++t) {
+      odd(1, std::true_type());
+      even(2, std::true_type());
+    }
+    for (; t < ntiles - 1; ++t) {
+      odd(2 * t + 1, std::false_type());
+      even(2 * t + 2, std::false_type());
+    }
+    odd(2 * t + 1, std::false_type());
     // P.V of the last half
     mfma_fence(st.acc);
 #pragma unroll

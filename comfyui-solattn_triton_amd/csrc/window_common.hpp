@@ -93,7 +93,9 @@ __device__ __forceinline__ KeyTiles key_tiles(const WindowArgs& a, int p0, int p
     k.lo = k.hi = k.s_end = k.ns = k.n = k.w0 = 0;
     return k;
   }
-  p1 = min(p1, len - 1);
+  p0 = __builtin_amdgcn_readfirstlane(p0);  // (kept scalar: copies take scalar bases)
+  len = __builtin_amdgcn_readfirstlane(len);
+  p1 = min(__builtin_amdgcn_readfirstlane(p1), len - 1);
   k.lo = max(p0 - a.window + 1, 0);
   k.hi = min(a.causal ? p1 + 1 : max(p1 + a.window, a.sinks), len);
   k.s_end = min(a.sinks, k.lo);
