@@ -455,8 +455,10 @@ window_dkv_kernel(const WindowArgs a) {
   const int tiles = j0 < len && i0 <= i1 ? (i1 - tile0) / kKeys + 1 : 0;
   const int per = (tiles * a.group + kp.parts - 1) / kp.parts;
   const int s0 = min(kp.part * per, tiles * a.group), s1 = min(s0 + per, tiles * a.group);
-  // rows that every key of the wave is seen by
+  // rows that see every key of the wave, and those that see any (a step without is skipped)
   const int all_lo = -wave_min(-kr.pl) - a.q_start, all_hi = wave_min(kr.ph) - a.q_start;
+  const bool seen = kr.pl <= kr.ph;
+  const int any_lo = wave_min(seen ? kr.pl : a.Tk) - a.q_start, any_hi = -wave_min(seen ? -kr.ph : 0) - a.q_start;
 
   const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf), sb = lds_addr(stat);
   TileAddr<D, kBoth> qa(qb, lane), ga(gb, lane);
@@ -495,6 +497,7 @@ window_dkv_kernel(const WindowArgs a) {
     wait_tile_copies();
     __syncthreads();  // this step's tiles are in, and every wave is done with the buffers of the last
     if (st + 1 < s1) issue(buf ^ 1);
+    if (r0 > any_hi || r0 + kKeys - 1 < any_lo) continue;
     const bool masked = r0 < all_lo || r0 + kKeys - 1 > all_hi;
     const uint32_t at = buf * kBuf;
 #pragma unroll
@@ -607,7 +610,12 @@ void cut_keys(WindowArgs& a) {
   int64_t kn = cdiv(512, static_cast<int64_t>(a.B) * a.Hkv * a.nkb);
   if (kn > steps / 8) kn = steps / 8;
   if (kn < 1) kn = 1;
-  int64_t ks = cdiv(tiles_all * a.group, cdiv(steps, kn));
+  // (a block with few sinks keeps one wave busy: its parts are last and a quarter as long,
+  // unless there are many of them)
+  const int64_t whole = cdiv(tiles_all * a.group, cdiv(steps, kn));
+  const int64_t items = static_cast<int64_t>(a.B) * a.Hkv * a.nsb * whole;
+  const int64_t finer = items > 256 ? 1 : items > 128 ? 2 : 4;
+  int64_t ks = whole > 1 ? cdiv(tiles_all * a.group, cdiv(steps, finer * kn)) : whole;
   a.kn = static_cast<int>(kn);
   a.ks = static_cast<int>(ks);
   if (a.nsb == a.nkb) a.kn = a.ks;  // (only sinks' blocks)
@@ -668,7 +676,7 @@ static int cut_rows(WindowArgs& a) {
   a.nqb = static_cast<int>(cdiv(a.Tq, blk));
   const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
   const int64_t tiles = cdiv(reach < a.Tk ? reach : a.Tk, kKeys);
-  int64_t n = cdiv(512, bh * a.nqb);
+  int64_t n = cdiv(1024, bh * a.nqb);
   if (n > tiles / 8) n = tiles / 8;
   a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
   return blk;

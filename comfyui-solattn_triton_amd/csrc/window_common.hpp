@@ -122,12 +122,11 @@ __device__ __forceinline__ KeyPart key_part(const WindowArgs& a, uint32_t w) {
   const int sink_items = a.nsb * a.ks, items = sink_items + (a.nkb - a.nsb) * a.kn;
   KeyPart k;
   k.bh = static_cast<int>(w / items);
-  const int i = static_cast<int>(w % items);
-  if (i < sink_items) {
+  const int n = static_cast<int>(w % items), i = n - (items - sink_items);
+  if (i >= 0) {  // sinks' parts last: they are the shorter ones
     k.block = i / a.ks, k.part = i % a.ks, k.parts = a.ks;
     k.slot = static_cast<int64_t>(k.bh) * a.slots + i;
   } else {
-    const int n = i - sink_items;
     k.block = a.nsb + n / a.kn, k.part = n % a.kn, k.parts = a.kn;
     k.slot = static_cast<int64_t>(k.bh) * a.slots + sink_items + n;
   }
