@@ -40,6 +40,10 @@ struct Bf16 {
   static __device__ __forceinline__ void amfma_first(f32x16& d, const bf16x8& a, const bf16x8& b) {
     asm volatile("s_nop 2\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
   }
+  // (two wait states in front: b may have been written by the VALU just before)
+  static __device__ __forceinline__ void amfma_after_valu(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
   static __device__ __forceinline__ void amfma_tie(f32x16& d, const bf16x8& a, const bf16x8& b, f32x16& s) {
     asm volatile("v_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\ts_nop 3" : "+v"(d), "+v"(s) : "v"(a), "v"(b));
   }
@@ -88,6 +92,10 @@ struct Fp16 {
   }
   static __device__ __forceinline__ void amfma_first(f32x16& d, const bf16x8& a, const bf16x8& b) {
     asm volatile("s_nop 2\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  }
+  // (two wait states in front: b may have been written by the VALU just before)
+  static __device__ __forceinline__ void amfma_after_valu(f32x16& d, const bf16x8& a, const bf16x8& b) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
   }
   static __device__ __forceinline__ void amfma_tie(f32x16& d, const bf16x8& a, const bf16x8& b, f32x16& s) {
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %3, %0\n\ts_nop 3" : "+v"(d), "+v"(s) : "v"(a), "v"(b));

@@ -326,6 +326,55 @@ __global__ void __launch_bounds__(256) window_join_kernel(const WindowArgs a) {
   if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
+// The products of a half step of the backward (32 rows by 32 keys), hand-ordered: an
+// operand is read two products ahead of its own (left to itself the compiler reads it
+// right in front and waits: the matrix instructions were busy a third of the time).
+// Two scores from the tiles at x and y, rows by rows: s = X B^T, t = Y C^T.
+template <typename E, int D, typename AX, typename AY>
+__device__ __forceinline__ void two_scores(f32x16& s, f32x16& t, const AX& x, uint32_t x_at, const bf16x8 (&b)[D / 16],
+                                           const AY& y, uint32_t y_at, const bf16x8 (&c)[D / 16]) {
+  constexpr int NC = D / 16;
+  bf16x8 r[3];
+  const auto operand = [&](int i) { return i < NC ? x.by_row(0, i, x_at) : y.by_row(0, i - NC, y_at); };
+  r[0] = operand(0);
+  r[1] = operand(1);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 2 * NC; ++i) {
+    if (i + 2 < 2 * NC) {
+      r[(i + 2) % 3] = operand(i + 2);
+      asm volatile("" ::: "memory");
+    }
+    if (i == 0)
+      E::amfma0(s, r[0], b[0]);
+    else if (i < NC)
+      E::amfma(s, r[i % 3], b[i]);
+    else if (i == NC)
+      E::amfma0(t, r[i % 3], c[0]);
+    else
+      E::amfma(t, r[i % 3], c[i - NC]);
+  }
+  asm volatile("s_nop 7\n\ts_nop 7" : "+v"(s), "+v"(t));  // readers of s and t come after their wait states
+}
+
+// acc += X^T W for the 32 rows at x, read transposed; w: W's two packed operands.
+template <typename E, int D, typename AX>
+__device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, uint32_t at, const bf16x8 (&w)[2]) {
+  constexpr int ND = D / 32, N = 2 * ND;
+  bf16x8 r[3];
+  r[0] = x.transposed(0, 0, at);
+  r[1] = x.transposed(1 / ND, 1 % ND, at);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + 2 < N) {
+      r[(i + 2) % 3] = x.transposed((i + 2) / ND, (i + 2) % ND, at);
+      asm volatile("" ::: "memory");
+    }
+    E::amfma_after_valu(acc[i % ND], r[i % 3], w[i / ND]);
+  }
+}
+
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
@@ -390,16 +439,13 @@ window_dq_kernel(const WindowArgs a) {
     __syncthreads();  // this tile is in, and every wave is done with the buffers of the last
     if (t + 1 < kt.n) issue(t + 1);
     const bool masked = !((j0 >= all_lo && j0 + kKeys - 1 <= all_hi) || j0 + kKeys <= all_sk);
-    const uint32_t at = (t & 1) * kBuf;
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
       ka.remade();
       va.remade();
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(ka.by_row(m2, cc, at), q[cc], s);
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(va.by_row(m2, cc, at), g[cc], dp);
+      const uint32_t at = (t & 1) * kBuf + m2 * (64 * D);
+      f32x16 s, dp;
+      two_scores<E, D>(s, dp, ka, at, q, va, at, g);
       if (masked) mask_keys(s, rk, j0 + 32 * m2, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -409,14 +455,11 @@ window_dq_kernel(const WindowArgs a) {
       if (masked)  // (a masked dp may be anything)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 ds = pack8<E>(dp, ks);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) acc[dt] = E::mfma32(ka.transposed(2 * m2 + ks, dt, at), ds, acc[dt]);
-      }
+      const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
+      add_product<E, D>(acc, ka, at, ds);
     }
   }
+  mfma_fence(acc);
   store_row<E>(acc, a.scale, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h, row < a.Tq,
                half);
 }
@@ -461,7 +504,8 @@ window_dkv_kernel(const WindowArgs a) {
   const int any_lo = wave_min(seen ? kr.pl : a.Tk) - a.q_start, any_hi = -wave_min(seen ? -kr.ph : 0) - a.q_start;
 
   const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf), sb = lds_addr(stat);
-  TileAddr<D, kBoth> qa(qb, lane), ga(gb, lane);
+  TileAddr<D, kBoth> qa(qb, lane);  // (dO's tiles: the same, at to_g)
+  const uint32_t to_g = gb - qb;
   bf16x8 k[NC], v[NC];
   load_row<D>(k, a.k.p + b * a.k.b + static_cast<int64_t>(jj) * a.k.t + hk * a.k.h, half);
   load_row<D>(v, a.v.p + b * a.v.b + static_cast<int64_t>(jj) * a.v.t + hk * a.v.h, half);
@@ -499,16 +543,12 @@ window_dkv_kernel(const WindowArgs a) {
     if (st + 1 < s1) issue(buf ^ 1);
     if (r0 > any_hi || r0 + kKeys - 1 < any_lo) continue;
     const bool masked = r0 < all_lo || r0 + kKeys - 1 > all_hi;
-    const uint32_t at = buf * kBuf;
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
+      const uint32_t at = buf * kBuf + m2 * (64 * D);
       qa.remade();
-      ga.remade();
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) s = E::mfma32(qa.by_row(m2, cc, at), k[cc], s);
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) dp = E::mfma32(ga.by_row(m2, cc, at), v[cc], dp);
+      f32x16 s, dp;
+      two_scores<E, D>(s, dp, qa, at, k, qa, at + to_g, v);
       const float* lse = stat[buf][0] + 32 * m2 + 4 * half;
       const float* delta = stat[buf][1] + 32 * m2 + 4 * half;
 #pragma unroll
@@ -522,6 +562,7 @@ window_dkv_kernel(const WindowArgs a) {
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lx[i]));
           dp[r] = s[r] * (dp[r] - dx[i]);
         }
+        asm volatile("" ::: "memory");  // (the next four's statistics are read behind these, not held with them)
       }
       if (masked) {  // (what a key does not see may be anything up to here)
         const int off = a.q_start + r0 + 32 * m2 + 4 * half - kr.pl;
@@ -534,20 +575,14 @@ window_dkv_kernel(const WindowArgs a) {
           dp[r] = on ? dp[r] : 0.f;
         }
       }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 pb = pack8<E>(s, ks);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) dv[dt] = E::mfma32(ga.transposed(2 * m2 + ks, dt, at), pb, dv[dt]);
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 ds = pack8<E>(dp, ks);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) dk[dt] = E::mfma32(qa.transposed(2 * m2 + ks, dt, at), ds, dk[dt]);
-      }
+      const bf16x8 pb[2] = {pack8<E>(s, 0), pack8<E>(s, 1)};
+      const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
+      add_product<E, D>(dv, qa, at + to_g, pb);
+      add_product<E, D>(dk, qa, at, ds);
     }
   }
+  mfma_fence(dk);
+  mfma_fence(dv);
   if (kp.parts == 1) {
     const bool on = j < a.Tk;
     store_row<E>(dk, a.scale, a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h, on, half);
