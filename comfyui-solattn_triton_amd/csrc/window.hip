@@ -335,6 +335,7 @@ __device__ __forceinline__ void two_scores(f32x16& s, f32x16& t, const AX& x, ui
                                            const AY& y, uint32_t y_at, const bf16x8 (&c)[D / 16]) {
   constexpr int NC = D / 16;
   bf16x8 r[3];
+  __builtin_amdgcn_s_setprio(1);
   const auto operand = [&](int i) { return i < NC ? x.by_row(0, i, x_at) : y.by_row(0, i - NC, y_at); };
   r[0] = operand(0);
   r[1] = operand(1);
@@ -354,6 +355,7 @@ __device__ __forceinline__ void two_scores(f32x16& s, f32x16& t, const AX& x, ui
     else
       E::amfma(t, r[i % 3], c[i - NC]);
   }
+  __builtin_amdgcn_s_setprio(0);
   asm volatile("s_nop 7\n\ts_nop 7" : "+v"(s), "+v"(t));  // readers of s and t come after their wait states
 }
 
@@ -362,6 +364,7 @@ template <typename E, int D, typename AX>
 __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, uint32_t at, const bf16x8 (&w)[2]) {
   constexpr int ND = D / 32, N = 2 * ND;
   bf16x8 r[3];
+  __builtin_amdgcn_s_setprio(1);
   r[0] = x.transposed(0, 0, at);
   r[1] = x.transposed(1 / ND, 1 % ND, at);
   asm volatile("" ::: "memory");
@@ -373,6 +376,7 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, 
     }
     E::amfma_after_valu(acc[i % ND], r[i % 3], w[i / ND]);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
