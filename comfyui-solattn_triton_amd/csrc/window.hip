@@ -27,14 +27,16 @@ constexpr int kThreads = 2 * kRows;   // a wave for 32 of them
 constexpr float kNoMax = -1e30f;
 
 // Workgroup -> (batch, kv head, block of rows, query head, part): the query heads of
-// one kv head and block run side by side.
+// one kv head and block run side by side. Causal blocks go last first: where the
+// window is wide, the last rows have the most keys.
 __device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, int& qb, int& part) {
-  uint32_t w = xcd_run(blockIdx.x, gridDim.x);
+  uint32_t w = xcd_item(a, blockIdx.x, gridDim.x);
   part = w % a.split;
   w /= a.split;
   const int g = w % a.group;
   w /= a.group;
   qb = w % a.nqb;
+  if (a.causal) qb = a.nqb - 1 - qb;
   w /= a.nqb;
   h = (w % a.Hkv) * a.group + g;
   b = w / a.Hkv;
@@ -300,30 +302,31 @@ window_fwd_kernel(const WindowArgs a) {
   if (a.lse && on && half == 0) a.lse[at] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
 }
 
-// The parts of the rows joined: a wave per row, two channels a lane.
+// The parts of the rows joined, four channels a lane.
 template <typename E, int D>
 __global__ void __launch_bounds__(256) window_join_kernel(const WindowArgs a) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  constexpr int L = D / 4;  // lanes of a row
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
   if (at >= static_cast<int64_t>(a.B) * a.H * a.Tq) return;
-  const int lane = threadIdx.x & 63, ch = 2 * lane;
+  const int ch = 4 * (threadIdx.x % L);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.split;
-  float top = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
+  float top = kNoMax, l = 0.f, o[4] = {};
   for (int i = 0; i < a.split; ++i) top = fmaxf(top, ml[i].x);
-  const float* p = a.part + at * a.split * D + (ch < D ? ch : 0);
+  const float* p = a.part + at * a.split * D + ch;
+#pragma unroll 4
   for (int i = 0; i < a.split; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
-    const float2 x = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(i) * D);
-    l = fmaf(ml[i].y, f, l);
-    o0 = fmaf(x.x, f, o0);
-    o1 = fmaf(x.y, f, o1);
+    const float2 u = ml[i];
+    const float f = __builtin_amdgcn_exp2f(u.x - top);
+    const float4 x = *reinterpret_cast<const float4*>(p + static_cast<int64_t>(i) * D);
+    l = fmaf(u.y, f, l);
+    o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]), o[2] = fmaf(x.z, f, o[2]), o[3] = fmaf(x.w, f, o[3]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int row = static_cast<int>(at % a.Tq);
   const int64_t bh = at / a.Tq;
-  if (ch < D)
-    *reinterpret_cast<uint32_t*>(a.out + (bh / a.H) * a.out_b + static_cast<int64_t>(row) * a.out_t +
-                                 (bh % a.H) * a.out_h + ch) = E::pack(o0 * inv, o1 * inv);
-  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
+  *reinterpret_cast<uint2*>(a.out + (bh / a.H) * a.out_b + static_cast<int64_t>(row) * a.out_t + (bh % a.H) * a.out_h +
+                            ch) = make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
+  if (a.lse && ch == 0) a.lse[at] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
 // The products of a half step of the backward (32 rows by 32 keys), hand-ordered: an
@@ -488,7 +491,7 @@ window_dkv_kernel(const WindowArgs a) {
   __shared__ __align__(256) uint16_t gbuf[2 * kKeys * D];
   __shared__ __align__(16) float stat[2][2][kKeys];  // [buffer][lse, delta]
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = wave_id();
-  uint32_t w = xcd_run(blockIdx.x, gridDim.x);
+  uint32_t w = xcd_item(a, blockIdx.x, gridDim.x);
   const KeyPart kp = key_part(a, w);
   const int hk = kp.bh % a.Hkv, b = kp.bh / a.Hkv;
   const int len = sequence_length(a, b);
@@ -784,7 +787,7 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   if ((rc = check_launch(what)) || a.split == 1) return rc;
   const auto kj = D == 128 ? (bf ? window_join_kernel<Bf16, 128> : window_join_kernel<Fp16, 128>)
                            : (bf ? window_join_kernel<Bf16, 64> : window_join_kernel<Fp16, 64>);
-  hipLaunchKernelGGL(kj, dim3(static_cast<uint32_t>(cdiv(rows, 4))), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(kj, dim3(static_cast<uint32_t>(cdiv(rows, 1024 / D))), dim3(256), 0, s, a);
   return check_launch(what);
 }
 

@@ -105,9 +105,18 @@ __device__ __forceinline__ KeyTiles key_tiles(const WindowArgs& a, int p0, int p
   return k;
 }
 
-// Workgroup id -> item of the launch, so that each of the 8 XCDs (dealt round
-// robin) walks a contiguous run: neighbouring items share their keys in its L2.
-__device__ __forceinline__ uint32_t xcd_run(uint32_t w, uint32_t total) {
+// Workgroup id -> item of the launch, so that each of the 8 XCDs (dealt round robin)
+// walks contiguous runs of items: neighbours share their keys in its L2. Without
+// lengths an XCD has one run; a padded batch, whose sequences may be short or empty,
+// is dealt out in runs of 32 items (517 rows against 16000 keys, one of two sequences
+// past its end: in one run each, half of the XCDs had nothing to do).
+__device__ __forceinline__ uint32_t xcd_item(const WindowArgs& a, uint32_t w, uint32_t total) {
+  if (a.lengths) {
+    constexpr uint32_t R = 32;
+    if (w >= total / (8 * R) * (8 * R)) return w;
+    const uint32_t x = w & 7u, i = w >> 3;
+    return (i / R * 8 + x) * R + i % R;
+  }
   const uint32_t x = w & 7u, q8 = total >> 3, rem = total & 7u;
   return x * q8 + min(x, rem) + (w >> 3);
 }
