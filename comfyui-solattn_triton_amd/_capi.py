@@ -61,9 +61,9 @@ SIGNATURES = {
                                  + [_p, _l, _l, _l] * 2 + [_p, _p, _p, _l, _p], _i),
     "solattn_window_attn_workspace_bytes": ([_l] * 9 + [_i, _i], _l),
     "solattn_window_attn": ([_p, _l, _l, _l] * 3 + [_l] * 6 + [_i, _l, _p, _l, _l, _i, _f]
-                            + [_p, _l, _l, _l, _p, _p, _l, _p], _i),
+                            + [_p, _l, _l, _l, _p, _p, _p, _l, _p], _i),
     "solattn_window_attn_bwd_workspace_bytes": ([_l] * 8 + [_i], _l),
-    "solattn_window_attn_bwd": ([_p, _l, _l, _l] * 5 + [_p] + [_l] * 6 + [_i, _l, _p, _l, _l, _i, _f]
+    "solattn_window_attn_bwd": ([_p, _l, _l, _l] * 5 + [_p, _p] + [_l] * 6 + [_i, _l, _p, _l, _l, _i, _f]
                                 + [_p, _l, _l, _l] * 3 + [_p, _l, _p], _i),
     "solattn_paged_attn_workspace_bytes": ([_l] * 8, _l),
     "solattn_paged_attn": ([_p, _l, _l] + [_p, _l, _l, _l] * 2 + [_l, _l, _p, _l, _l, _p] + [_l] * 4

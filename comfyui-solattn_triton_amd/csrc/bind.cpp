@@ -341,7 +341,8 @@ struct WindowPlan {
   double scale = 1;
 };
 
-Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const WindowPlan& p, const Tensor& lse) {
+Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const WindowPlan& p, const Tensor& lse,
+                      const Tensor& o_lo) {
   const int64_t B = q.size(0), Tq = q.size(1), H = q.size(2), D = q.size(3), Tk = k.size(1), Hkv = k.size(2);
   Tensor out = at::empty({B, Tq, H, D}, q.options());
   const c10::OptionalDeviceGuard guard(q.device());
@@ -350,8 +351,8 @@ Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const W
   const Tensor ws = workspace(need, q);
   check(lib.window_attn(ptr_as<U16>(q), STRIDES(q), ptr_as<U16>(k), STRIDES(k), ptr_as<U16>(v), STRIDES(v), B, Tq, Tk,
                         H, Hkv, D, type_code(q), p.q_start, ptr_as<int32_t>(p.lengths), p.window, p.sinks, p.causal,
-                        static_cast<float>(p.scale), ptr_as<U16>(out), STRIDES(out), ptr_as<float>(lse), ptr(ws), need,
-                        stream_of(q)),
+                        static_cast<float>(p.scale), ptr_as<U16>(out), STRIDES(out), ptr_as<float>(lse),
+                        ptr_as<U16>(o_lo), ptr(ws), need, stream_of(q)),
         "solattn_window_attn");
   return out;
 }
@@ -360,8 +361,9 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const WindowPlan& p) {
     const Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    Tensor out = window_forward(q, k, v, p, lse);
-    ctx->save_for_backward({q, k, v, out, lse, p.lengths});
+    const Tensor o_lo = at::empty(q.sizes(), q.options());
+    Tensor out = window_forward(q, k, v, p, lse, o_lo);
+    ctx->save_for_backward({q, k, v, out, lse, p.lengths, o_lo});
     ctx->saved_data["window"] = p.window;
     ctx->saved_data["sinks"] = p.sinks;
     ctx->saved_data["q_start"] = p.q_start;
@@ -372,7 +374,7 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only("window_attn");
     const auto s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &lse = s[4], &lengths = s[5];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &lse = s[4], &lengths = s[5], &o_lo = s[6];
     auto& data = ctx->saved_data;
     const int64_t B = q.size(0), Tq = q.size(1), H = q.size(2), D = q.size(3), Tk = k.size(1), Hkv = k.size(2);
     const int64_t window = data["window"].toInt(), sinks = data["sinks"].toInt();
@@ -383,8 +385,8 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
     const Tensor g = as_rows(grads[0]);
     const Tensor ws = workspace(lib.window_attn_bwd_workspace_bytes(B, Tq, Tk, H, Hkv, D, window, sinks, causal), q);
     check(lib.window_attn_bwd(ptr_as<U16>(q), STRIDES(q), ptr_as<U16>(k), STRIDES(k), ptr_as<U16>(v), STRIDES(v),
-                              ptr_as<U16>(out), STRIDES(out), ptr_as<U16>(g), STRIDES(g), ptr_as<float>(lse), B, Tq, Tk,
-                              H, Hkv, D, type_code(q), data["q_start"].toInt(), ptr_as<int32_t>(lengths), window, sinks,
+                              ptr_as<U16>(out), STRIDES(out), ptr_as<U16>(g), STRIDES(g), ptr_as<float>(lse),
+                              ptr_as<U16>(o_lo), B, Tq, Tk, H, Hkv, D, type_code(q), data["q_start"].toInt(), ptr_as<int32_t>(lengths), window, sinks,
                               causal, static_cast<float>(data["scale"].toDouble()), ptr_as<U16>(dq), STRIDES(dq),
                               ptr_as<U16>(dk), STRIDES(dk), ptr_as<U16>(dv), STRIDES(dv), ptr(ws),
                               ws.defined() ? ws.numel() : 0, stream_of(q)),
@@ -419,10 +421,10 @@ Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::op
     // zero channels add exact zeros to every product; the pad's gradient is a slice
     const int64_t pad[2] = {0, (D < 64 ? 64 : 128) - D};
     const Tensor q = at::constant_pad_nd(q0, pad), k = at::constant_pad_nd(k0, pad), v = at::constant_pad_nd(v0, pad);
-    return (grad ? WindowAttn::apply(q, k, v, p) : window_forward(q, k, v, p, {})).narrow(3, 0, D).contiguous();
+    return (grad ? WindowAttn::apply(q, k, v, p) : window_forward(q, k, v, p, {}, {})).narrow(3, 0, D).contiguous();
   }
   const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0);
-  return grad ? WindowAttn::apply(q, k, v, p) : window_forward(q, k, v, p, {});
+  return grad ? WindowAttn::apply(q, k, v, p) : window_forward(q, k, v, p, {}, {});
 }
 
 // --------------------------------------------------------------------- pages

@@ -297,8 +297,12 @@ window_fwd_kernel(const WindowArgs a) {
     if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (at * a.split + part)) = make_float2(st.m, l);
     return;
   }
-  store_row<E>(st.acc, l == 0.f ? 0.f : 1.f / l, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h,
-               on, half);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store_row<E>(st.acc, inv, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h, on, half);
+  if (a.o_lo) {
+    rounded_off<E>(st.acc, inv);
+    store_row<E>(st.acc, 1.f, a.o_lo + ((static_cast<int64_t>(b) * a.Tq + row) * a.H + h) * D, on, half);
+  }
   if (a.lse && on && half == 0) a.lse[at] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
 }
 
@@ -324,8 +328,14 @@ __global__ void __launch_bounds__(256) window_join_kernel(const WindowArgs a) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int row = static_cast<int>(at % a.Tq);
   const int64_t bh = at / a.Tq;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] *= inv;
+  const uint2 w = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
   *reinterpret_cast<uint2*>(a.out + (bh / a.H) * a.out_b + static_cast<int64_t>(row) * a.out_t + (bh % a.H) * a.out_h +
-                            ch) = make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
+                            ch) = w;
+  if (a.o_lo)
+    *reinterpret_cast<uint2*>(a.o_lo + ((bh / a.H * a.Tq + row) * a.H + bh % a.H) * D + ch) =
+        make_uint2(E::pack(o[0] - E::lo(w.x), o[1] - E::hi(w.x)), E::pack(o[2] - E::lo(w.y), o[3] - E::hi(w.y)));
   if (a.lse && ch == 0) a.lse[at] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
@@ -423,17 +433,24 @@ window_dq_kernel(const WindowArgs a) {
   load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
   load_row<D>(g, a.d_o.p + b * a.d_o.b + static_cast<int64_t>(rr) * a.d_o.t + h * a.d_o.h, half);
   const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.Tq + rr;
+  // D_i from o and what its rounding took away: the rounding alone is one error for all
+  // keys of a row, and took dq and dk from 1.45 to 1.55 times the error of exact ones
+  // rounded to the type.
   float delta = 0.f;
   {
     bf16x8 o[NC];
-    load_row<D>(o, a.o.p + b * a.o.b + static_cast<int64_t>(rr) * a.o.t + h * a.o.h, half);
+    const auto add = [&](const uint16_t* row_o) __attribute__((always_inline)) {
+      load_row<D>(o, row_o, half);
 #pragma unroll
-    for (int cc = 0; cc < NC; ++cc) {
-      const uint4 x = __builtin_bit_cast(uint4, o[cc]), y = __builtin_bit_cast(uint4, g[cc]);
-      const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
+      for (int cc = 0; cc < NC; ++cc) {
+        const uint4 x = __builtin_bit_cast(uint4, o[cc]), y = __builtin_bit_cast(uint4, g[cc]);
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) delta = fmaf(E::lo(u[i]), E::lo(w[i]), fmaf(E::hi(u[i]), E::hi(w[i]), delta));
-    }
+        for (int i = 0; i < 4; ++i) delta = fmaf(E::lo(u[i]), E::lo(w[i]), fmaf(E::hi(u[i]), E::hi(w[i]), delta));
+      }
+    };
+    add(a.o.p + b * a.o.b + static_cast<int64_t>(rr) * a.o.t + h * a.o.h);
+    if (a.o_lo) add(a.o_lo + ((static_cast<int64_t>(b) * a.Tq + rr) * a.H + h) * D);
     delta = xhalf_sum(delta);
   }
   const float neg = -a.lse[at];  // -inf for a row that sees nothing
@@ -744,8 +761,8 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
                                    int64_t sv_t, int64_t sv_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
                                    int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths,
                                    int64_t window, int64_t sinks, int causal, float scale, uint16_t* o, int64_t so_b,
-                                   int64_t so_t, int64_t so_h, float* lse, void* workspace, int64_t workspace_bytes,
-                                   solattn_stream_t stream) {
+                                   int64_t so_t, int64_t so_h, float* lse, uint16_t* o_lo, void* workspace,
+                                   int64_t workspace_bytes, solattn_stream_t stream) {
   clear_error();
   const char* what = "window_attn";
   if (single_token(Tq, causal, lse)) {
@@ -758,13 +775,14 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   WindowArgs a{};
   a.q = {q, sq_b, sq_t, sq_h}, a.k = {k, sk_b, sk_t, sk_h}, a.v = {v, sv_b, sv_t, sv_h};
   a.out = o, a.out_b = so_b, a.out_t = so_t, a.out_h = so_h;
-  a.lse = lse, a.lengths = lengths;
+  a.lse = lse, a.o_lo = o_lo, a.lengths = lengths;
   int rc = setup(a, B, Tq, Tk, H, Hkv, D, dtype, q_start, window, sinks, causal, scale, what);
   if (!rc) rc = check_mat(a.q, what, "q");
   if (!rc) rc = check_mat(a.k, what, "k");
   if (!rc) rc = check_mat(a.v, what, "v");
   if (!rc) rc = check_mat({o, so_b, so_t, so_h}, what, "o");
   if (rc) return rc;
+  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(o_lo) % 16 == 0, SOLATTN_EINVAL, "%s: o_lo must be 16-byte aligned", what);
   const bool bf = dtype == SOLATTN_BF16;
   const int blk = cut_rows(a);
   const int64_t need = fwd_workspace(a, D);
@@ -809,7 +827,7 @@ extern "C" int solattn_window_attn_bwd(
     const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k, int64_t sk_b, int64_t sk_t,
     int64_t sk_h, const uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, const uint16_t* o, int64_t so_b,
     int64_t so_t, int64_t so_h, const uint16_t* d_o, int64_t sg_b, int64_t sg_t, int64_t sg_h, const float* lse,
-    int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t q_start,
+    const uint16_t* o_lo, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t q_start,
     const int32_t* lengths, int64_t window, int64_t sinks, int causal, float scale, uint16_t* dq, int64_t sdq_b,
     int64_t sdq_t, int64_t sdq_h, uint16_t* dk, int64_t sdk_b, int64_t sdk_t, int64_t sdk_h, uint16_t* dv,
     int64_t sdv_b, int64_t sdv_t, int64_t sdv_h, void* workspace, int64_t workspace_bytes, solattn_stream_t stream) {
@@ -821,14 +839,15 @@ extern "C" int solattn_window_attn_bwd(
   a.out = dq, a.out_b = sdq_b, a.out_t = sdq_t, a.out_h = sdq_h;
   a.dk = dk, a.dk_b = sdk_b, a.dk_t = sdk_t, a.dk_h = sdk_h;
   a.dv = dv, a.dv_b = sdv_b, a.dv_t = sdv_t, a.dv_h = sdv_h;
-  a.lse = const_cast<float*>(lse), a.lengths = lengths;
+  a.lse = const_cast<float*>(lse), a.o_lo = const_cast<uint16_t*>(o_lo), a.lengths = lengths;
   int rc = setup(a, B, Tq, Tk, H, Hkv, D, dtype, q_start, window, sinks, causal, scale, what);
   const Mat outs[3] = {{dq, sdq_b, sdq_t, sdq_h}, {dk, sdk_b, sdk_t, sdk_h}, {dv, sdv_b, sdv_t, sdv_h}};
   const Mat* mats[8] = {&a.q, &a.k, &a.v, &a.o, &a.d_o, &outs[0], &outs[1], &outs[2]};
   const char* names[8] = {"q", "k", "v", "o", "do", "dq", "dk", "dv"};
   for (int i = 0; i < 8 && !rc; ++i) rc = check_mat(*mats[i], what, names[i]);
   if (rc) return rc;
-  SOLATTN_REQUIRE(lse, SOLATTN_EINVAL, "%s: null lse", what);
+  SOLATTN_REQUIRE(lse && reinterpret_cast<uintptr_t>(o_lo) % 16 == 0, SOLATTN_EINVAL, "%s: null lse or unaligned o_lo",
+                  what);
   cut_keys(a);
   const int64_t need = bwd_workspace(a, D);
   SOLATTN_REQUIRE(workspace && workspace_bytes >= need, SOLATTN_ESIZE, "%s: workspace %lld < %lld bytes", what,

@@ -28,6 +28,7 @@ struct WindowArgs {
   uint16_t* dv;
   int64_t dv_b, dv_t, dv_h;
   float* lse;                // [B][H][Tq], log2 domain; +inf for a row that sees nothing
+  uint16_t* o_lo;            // [B][Tq][H][D], what rounding o took away (null: not kept)
   float* delta;              // [B][H][Tq]
   const int32_t* lengths;    // null: Tk
   int B, H, Hkv, group, Tq, Tk, q_start;
@@ -279,6 +280,20 @@ __device__ __forceinline__ void store_row(const f32x16 (&acc)[ND], float f, uint
       }
       const uint4 v = half ? make_uint4(y[0], y[1], w[1][0], w[1][1]) : make_uint4(w[0][0], w[0][1], y[0], y[1]);
       if (on) *reinterpret_cast<uint4*>(row + 32 * dt + 16 * ip + 8 * half) = v;
+    }
+}
+
+// acc f becomes what is left of it when it is rounded to the type.
+template <typename E, int ND>
+__device__ __forceinline__ void rounded_off(f32x16 (&acc)[ND], float f) {
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      const float x = acc[dt][r] * f, y = acc[dt][r + 1] * f;
+      const uint32_t w = E::pack(x, y);
+      acc[dt][r] = x - E::lo(w);
+      acc[dt][r + 1] = y - E::hi(w);
     }
 }
 

@@ -423,7 +423,9 @@ int solattn_qk_norm_rope_bwd(
  * of j < len, len = lengths[b] clamped to [0, Tk] (int32 [B]; null: Tk).
  *   o = sum_j softmax_j(scale q.k_j) v_j; rows at p >= len are zeros.
  * lse: fp32 [B][H][Tq], log2 of the row's softmax sum (+inf for a row without keys),
- * what the backward reads; null: not written. dtype bf16 or fp16, D 64 or 128
+ * what the backward reads; null: not written. o_lo: [B][Tq][H][D] of dtype, what
+ * rounding o took away, rounded itself, for a backward of full precision; null: not
+ * written. dtype bf16 or fp16, D 64 or 128
  * (D: multiples of 8 up to 128 for the call below). Keys that no row of a call sees
  * are never read; what k holds at a key reaches the rows that see it only, but a
  * NaN or infinity in v (backward: also in k, q, do) can reach rows that do not see
@@ -438,10 +440,10 @@ int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t s
                         int64_t sv_t, int64_t sv_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
                         int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths,
                         int64_t window, int64_t sinks, int causal, float scale, uint16_t* o,
-                        int64_t so_b, int64_t so_t, int64_t so_h, float* lse, void* workspace,
+                        int64_t so_b, int64_t so_t, int64_t so_h, float* lse, uint16_t* o_lo, void* workspace,
                         int64_t workspace_bytes, solattn_stream_t stream);
 
-/* Gradients of solattn_window_attn from its inputs, o, lse and do: dq like q, dk and dv
+/* Gradients of solattn_window_attn from its inputs, o, lse, o_lo (or null) and do: dq like q, dk and dv
  * like k (every row written, zeros where nothing is seen). workspace: 256-byte
  * aligned. No atomics: the same inputs give the same bits. */
 int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
@@ -450,7 +452,8 @@ int solattn_window_attn_bwd(
     const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const uint16_t* k, int64_t sk_b,
     int64_t sk_t, int64_t sk_h, const uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h,
     const uint16_t* o, int64_t so_b, int64_t so_t, int64_t so_h, const uint16_t* d_o, int64_t sg_b,
-    int64_t sg_t, int64_t sg_h, const float* lse, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+    int64_t sg_t, int64_t sg_h, const float* lse,
+    const uint16_t* o_lo, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
     int64_t Hkv, int64_t D, int dtype, int64_t q_start, const int32_t* lengths, int64_t window,
     int64_t sinks, int causal, float scale, uint16_t* dq, int64_t sdq_b, int64_t sdq_t, int64_t sdq_h,
     uint16_t* dk, int64_t sdk_b, int64_t sdk_t, int64_t sdk_h, uint16_t* dv, int64_t sdv_b,
