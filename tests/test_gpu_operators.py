@@ -236,6 +236,12 @@ WINDOW = [
     (1, 70, 90, 3, 3, 24, 33, 2, False, None, FP),
     (1, 1100, 1100, 2, 1, 128, 256, 4, True, None, FP),
     (1, 640, 640, 1, 1, 128, None, 0, False, None, BF),
+    # key tiles of the forward cut into parts; blocks of keys of the backward cut into parts
+    (1, 100, 3000, 2, 1, 128, None, 0, True, None, BF),
+    (2, 70, 2500, 4, 2, 64, 2000, 100, True, [2500, 2460], FP),
+    (1, 1100, 1100, 4, 1, 64, None, 0, True, None, BF),
+    (1, 900, 900, 2, 2, 128, 100, 300, False, None, BF),
+    (1, 1000, 1300, 2, 1, 128, 700, 1, True, None, FP),
 ]
 
 
@@ -371,6 +377,71 @@ def test_window_empty(window, dev):
     assert gq.shape == q.shape and (gk == 0).all()
 
 
+def test_window_some_gradients(window, dev):
+    """Leaves that need none get none, the others the same bits; once only."""
+    q, k, v, _, _, kw = window_case((1, 90, 90, 2, 1, 64, 30, 2, True, None, BF), dev)
+    do = randn(q.shape, 9, dev)
+    every = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(window.window_attn(*every, **kw), every, do)
+    for i in range(3):
+        x = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        got, = torch.autograd.grad(window.window_attn(*x, **kw), x[i], do)
+        assert torch.equal(got, want[i])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(window.window_attn(*every, **kw), every, do, create_graph=True)
+    with torch.no_grad():
+        assert not window.window_attn(*every, **kw).requires_grad
+
+
+def test_refusals(rope, window, paged, dev):
+    """What the Python entries refuse before any launch."""
+    x = torch.zeros(2, 8, 4, 64, device=dev, dtype=BF)
+    n = torch.ones(2, dtype=torch.int32, device=dev)
+    c = torch.zeros(3, 8, 4, 64, device=dev, dtype=BF)
+    t = torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    cos = torch.zeros(8, 32, device=dev)
+
+    def bad(match, f, *a, **kw):
+        with pytest.raises(ValueError, match=match):
+            f(*a, **kw)
+
+    bad("dtype", rope.qk_norm_rope, x, x.half())
+    bad("dtype", rope.qk_norm_rope, x.double(), x.double())
+    bad("4 dimensions", rope.qk_norm_rope, x, x[0])
+    bad("tokens", rope.qk_norm_rope, x, x[:, :3])
+    bad("head_dim", rope.qk_norm_rope, x[..., :60], x[..., :60])
+    bad("head_dim", rope.qk_norm_rope, x, x[..., :32])
+    bad("q_weight", rope.qk_norm_rope, x, x, torch.ones(32, device=dev))
+    bad("k_weight", rope.qk_norm_rope, x, x, None, torch.ones(64))
+    bad("together", rope.qk_norm_rope, x, x, None, None, cos)
+    bad("cos", rope.qk_norm_rope, x, x, None, None, cos.double(), cos.double())
+    bad("rotated", rope.qk_norm_rope, x, x, None, None, cos[:, :12].contiguous(), cos[:, :12].contiguous())
+    bad("table of 4", rope.qk_norm_rope, x, x, None, None, cos[:4], cos[:4])
+    bad("positions", rope.qk_norm_rope, x, x, None, None, cos, cos, positions=cos[:, 0])
+    bad("positions", rope.qk_norm_rope, x, x, None, None, cos, cos, positions=n)
+    bad("fp32|float16|dtype", window.window_attn, x.float(), x.float(), x.float(), window=4)
+    bad("shapes", window.window_attn, x, x, x[:, :4], window=4)
+    bad("share", window.window_attn, x, x[:, :, :3], x[:, :, :3], window=4)
+    bad("window", window.window_attn, x, x, x, window=0)
+    bad("sinks", window.window_attn, x, x, x, window=4, sinks=-1)
+    bad("scale", window.window_attn, x, x, x, window=4, scale=0.0)
+    bad("rows", window.window_attn, x, x[:, :4], x[:, :4], window=4)
+    bad("rows", window.window_attn, x, x, x, window=4, q_start=1)
+    bad("lengths", window.window_attn, x, x, x, window=4, lengths=n.long())
+    bad("lengths", window.window_attn, x, x, x, window=4, lengths=n[:1])
+    bad("tokens", paged.paged_attn, x, c, c, t, n)
+    q = x[:, :1]
+    bad("page_table", paged.paged_attn, q, c, c, t[:1], n)
+    bad("page_table", paged.paged_attn, q, c, c, t.long(), n)
+    bad("lengths", paged.paged_attn, q, c, c, t, n.cpu())
+    bad("multiple of 8", paged.paged_attn, q, c[:, :4], c[:, :4], t, n)
+    bad("cache shapes", paged.paged_attn, q, c, c[:2], t, n)
+    bad("contiguous", paged.paged_attn, q, c.transpose(1, 3).contiguous().transpose(1, 3), c, t, n)
+    bad("gradient", paged.paged_attn, q.clone().requires_grad_(True), c, c, t, n)
+    bad("gradient", rope.qk_norm_rope_append, q.clone().requires_grad_(True), q, q, c, c, t, n)
+    bad("match", rope.qk_norm_rope_append, q, q[:, :, :2], q[:, :, :2], c, c, t, n)
+
+
 # --------------------------------------------------------------------- pages
 # lengths, page, H, Hkv, D, window, sinks, dtype
 PAGED = [
@@ -429,6 +500,30 @@ def test_paged_bad_pages_and_long_lengths(paged, dev):
     neg = torch.tensor([-4, 48], dtype=torch.int32, device=dev)
     assert (paged.paged_attn(q, kc, vc, table, neg)[0] == 0).all()
     assert (paged.paged_attn(q, kc[:0], vc[:0], table, n) == 0).all()
+
+
+def test_paged_cache_views(rope, paged, dev):
+    """k and v side by side in one allocation, heads before slots, a table that is a
+    view of a wider one: the same bits as dense ones."""
+    B, H, Hkv, D, page = 3, 4, 2, 64, 16
+    kv = randn((9, 2, page, Hkv, D), 1, dev)
+    wide = torch.randint(0, 9, (B, 8), dtype=torch.int32, device=dev)
+    table, n = wide[:, 2:6], torch.tensor([60, 1, 33], dtype=torch.int32, device=dev)
+    q = randn((B, 1, H, D), 2, dev)
+    k, v = kv[:, 0], kv[:, 1]
+    want = paged.paged_attn(q, k.contiguous(), v.contiguous(), table.contiguous(), n)
+    assert torch.equal(paged.paged_attn(q, k, v, table, n), want)
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v)]
+    assert torch.equal(paged.paged_attn(q, *heads_first, table, n), want)
+    every_other = torch.stack([table, table + 100], 2).flatten(1)[:, ::2]
+    assert torch.equal(paged.paged_attn(q, k, v, every_other, n), want)
+    kn, vn = randn((B, 1, Hkv, D), 3, dev), randn((B, 1, Hkv, D), 4, dev)
+    dense = [t.clone(memory_format=torch.contiguous_format) for t in (k, v)]
+    uniq = torch.arange(9, dtype=torch.int32, device=dev).reshape(B, 3)[:, :3]
+    m = torch.tensor([48, 1, 17], dtype=torch.int32, device=dev)
+    rope.qk_norm_rope_append(q, kn, vn, k, v, uniq, m)
+    rope.qk_norm_rope_append(q, kn, vn, *dense, uniq, m)
+    assert torch.equal(k, dense[0]) and torch.equal(v, dense[1])
 
 
 # ------------------------------------------------------------------- together
@@ -514,3 +609,28 @@ def test_other_stream_and_graph(rope, window, paged, dev):
             torch.cuda.synchronize()
             for x, y in zip(out, step()):
                 assert torch.equal(x, y)
+
+
+def test_two_streams_at_once(window, paged, dev):
+    """Calls in flight on two streams, with workspaces of their own: the bits of the
+    calls one after another."""
+    sets = []
+    for i in range(2):
+        q, k, v, _, _, kw = window_case((1, 100, 3000, 2, 1, 128, None, 0, True, None, BF), dev, seed=10 * i)
+        kc, vc = randn((40, 64, 2, 128), 90 + i, dev), randn((40, 64, 2, 128), 95 + i, dev)
+        table = torch.randperm(40, generator=torch.Generator().manual_seed(i)).to(torch.int32).view(1, 40).to(dev)
+        n = torch.tensor([2500 - 700 * i], dtype=torch.int32, device=dev)
+        sets.append(lambda q=q, k=k, v=v, kw=kw, kc=kc, vc=vc, t=table, n=n: (
+            window.window_attn(q, k, v, **kw), paged.paged_attn(q[:, :1], kc, vc, t, n)))
+    want = [f() for f in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, (f, s) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(r, w))

@@ -1,0 +1,164 @@
+"""What the C entries of the operators around attention refuse, and the sizes of their
+workspaces, without a GPU: every address is a stand-in and nothing reaches a launch."""
+
+import importlib
+
+import pytest
+import torch
+
+A = 1 << 20  # aligned, never dereferenced
+EINVAL, EUNSUPPORTED, ESIZE = -1, -2, -4
+
+
+@pytest.fixture(scope="module")
+def capi(pkg):
+    return importlib.import_module(f"{pkg.__name__}._capi")
+
+
+def _rope(L, q=A, k=A, B=1, T=10, H=4, Hkv=2, D=128, dtype=0, qw=A, cos=A, sin=A, P=10, R=128, interleaved=0,
+          positions=None, qo=A, ko=A, qs=None):
+    qs = qs or (T * H * D, H * D, D)
+    ks = (T * Hkv * D, Hkv * D, D)
+    return L.solattn_qk_norm_rope(q, *qs, k, *ks, B, T, H, Hkv, D, dtype, qw, A, cos, sin, P, R, interleaved, positions, 0,
+                                  1e-6, qo, T * H * D, H * D, D, ko, *ks, None)
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(dtype=3), EINVAL, b"dtype"), (dict(B=0), EINVAL, b"sizes"), (dict(D=132), EUNSUPPORTED, b"head_dim"),
+    (dict(D=136), EUNSUPPORTED, b"head_dim"), (dict(R=24), EUNSUPPORTED, b"rotated"),
+    (dict(R=136), EUNSUPPORTED, b"rotated"), (dict(R=12, interleaved=1), EUNSUPPORTED, b"rotated"),
+    (dict(cos=None), EINVAL, b"table"), (dict(P=9), EINVAL, b"table of 9"), (dict(q=None), EINVAL, b"null q"),
+    (dict(q=A + 8), EINVAL, b"aligned"), (dict(qs=(5120, 508, 128)), EINVAL, b"aligned"), (dict(ko=None), EINVAL, b"null k"),
+    (dict(qw=A + 4), EINVAL, b"aligned"), (dict(T=1 << 31), EINVAL, b"table of"), (dict(B=1 << 31, T=2), EUNSUPPORTED, b"many"),
+])
+def test_rope_refusals(capi, kw, rc, text):
+    if kw.get("T") == 1 << 31:  # (the size is refused before the table is)
+        rc, text = EUNSUPPORTED, b"many"
+    assert _rope(capi.LIB, **kw) == rc
+    assert text in capi.LIB.solattn_last_error(), capi.LIB.solattn_last_error()
+
+
+def test_rope_backward_workspace(capi):
+    L = capi.LIB
+    assert L.solattn_qk_norm_rope_bwd_workspace_bytes(0) == 0
+    need = L.solattn_qk_norm_rope_bwd_workspace_bytes(128)
+    s = (1280, 128, 128)
+    args = [A, *s, A, *s, A, *s, A, *s, 1, 10, 1, 1, 128, 0, A, A, A, A, 10, 128, 0, None, 0, 1e-6, A, *s, A, *s]
+    assert L.solattn_qk_norm_rope_bwd(*args, A, A, A, need - 1, None) == ESIZE
+    assert L.solattn_qk_norm_rope_bwd(*args, A, A, None, need, None) == ESIZE
+    assert L.solattn_qk_norm_rope_bwd(*args, A, A, A + 16, need, None) == EINVAL
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(table=None), EINVAL, b"page table"), (dict(lengths=None), EINVAL, b"lengths"), (dict(pages=-1), EUNSUPPORTED, b"pages"),
+    (dict(page=0), EUNSUPPORTED, b"pages"), (dict(page=1 << 20, most=1 << 11), EUNSUPPORTED, b"2^31"),
+    (dict(cache=A + 2), EINVAL, b"k_cache"), (dict(cache=None), EINVAL, b"k_cache"),
+])
+def test_append_refusals(capi, kw, rc, text):
+    o = dict(table=A, lengths=A, pages=4, page=16, most=2, cache=A)
+    o.update(kw)
+    s, c = (128, 128, 128), (2048, 128, 128)
+    got = capi.LIB.solattn_qk_norm_rope_append(
+        A, *s, A, *s, A, *s, 1, 1, 1, 1, 128, 0, A, A, A, A, 10, 128, 0, 1e-6, A, *s, o["cache"], *c, A, *c, o["pages"],
+        o["page"], o["table"], o["most"], o["most"], o["lengths"], None)
+    assert got == rc and text in capi.LIB.solattn_last_error(), capi.LIB.solattn_last_error()
+
+
+def _window(L, B=1, Tq=40, Tk=100, H=4, Hkv=2, D=128, dtype=0, q_start=60, window=16, sinks=2, causal=1, scale=0.1,
+            q=A, k=A, o=A, lse=None, ws=None, ws_bytes=0, kt=None):
+    qs, ks = (Tq * H * D, H * D, D), (Tk * Hkv * D, kt or Hkv * D, D)
+    return L.solattn_window_attn(q, *qs, k, *ks, A, *ks, B, Tq, Tk, H, Hkv, D, dtype, q_start, None, window, sinks, causal,
+                                 scale, o, *qs, lse, None, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(dtype=2), EINVAL, b"dtype"), (dict(H=3), EINVAL, b"heads"), (dict(Tq=0), EINVAL, b"sizes"),
+    (dict(D=96), EUNSUPPORTED, b"head_dim"), (dict(q_start=61), EINVAL, b"rows"), (dict(q_start=-1), EINVAL, b"rows"),
+    (dict(window=0), EINVAL, b"window"), (dict(sinks=-1), EINVAL, b"sinks"), (dict(scale=0.0), EINVAL, b"scale"),
+    (dict(scale=float("nan")), EINVAL, b"scale"), (dict(q=None), EINVAL, b"null q"), (dict(o=A + 8), EINVAL, b"aligned"),
+    (dict(kt=252), EINVAL, b"aligned"), (dict(kt=1 << 24), EUNSUPPORTED, b"stride"), (dict(kt=-256), EUNSUPPORTED, b"stride"),
+    (dict(Tk=1 << 29, q_start=0), EUNSUPPORTED, b"keys"), (dict(B=1 << 24, H=128), EUNSUPPORTED, b"grid"),
+])
+def test_window_refusals(capi, kw, rc, text):
+    assert _window(capi.LIB, **kw) == rc
+    assert text in capi.LIB.solattn_last_error(), capi.LIB.solattn_last_error()
+
+
+def test_window_workspaces(capi):
+    """A short launch asks for room for its parts and refuses less; a full one for none."""
+    L = capi.LIB
+    assert L.solattn_window_attn_workspace_bytes(1, 16000, 16000, 24, 8, 128, 0, 4096, 4, 1, 0) == 0
+    need = L.solattn_window_attn_workspace_bytes(1, 64, 8192, 2, 1, 128, 8128, 8192, 0, 1, 0)
+    assert need > 0
+    kw = dict(Tq=64, Tk=8192, H=2, Hkv=1, q_start=8128, window=8192, sinks=0)
+    assert _window(L, **kw, ws=A, ws_bytes=need - 1) == ESIZE
+    assert _window(L, **kw, ws=None, ws_bytes=need) == ESIZE
+    assert _window(L, **kw, ws=A + 128, ws_bytes=need) == EINVAL
+    one = L.solattn_window_attn_workspace_bytes(1, 1, 8192, 2, 1, 128, 8191, 8192, 0, 1, 0)
+    assert one > 0 and one == L.solattn_paged_attn_workspace_bytes(1, 2, 1, 128, 1, 8192, 8192, 0)
+    assert _window(L, Tq=1, Tk=8192, H=2, Hkv=1, q_start=8191, window=8192, sinks=0, ws=A, ws_bytes=one - 1) == ESIZE
+    assert L.solattn_window_attn_workspace_bytes(1, 64, 32, 2, 1, 128, 0, 8, 0, 1, 0) == 0  # not a call that runs
+    assert L.solattn_window_attn_bwd_workspace_bytes(2, 100, 100, 4, 2, 64, 100, 0, 1) >= 2 * 100 * 4 * 4
+
+
+def test_window_backward_refusals(capi):
+    L = capi.LIB
+    s = (12800, 128, 128)
+    need = L.solattn_window_attn_bwd_workspace_bytes(1, 100, 100, 1, 1, 128, 100, 0, 1)
+
+    def call(lse=A, ws=A, ws_bytes=need, dk=A, do=A):
+        return L.solattn_window_attn_bwd(A, *s, A, *s, A, *s, A, *s, do, *s, lse, None, 1, 100, 100, 1, 1, 128, 0, 0, None,
+                                         100, 0, 1, 0.1, A, *s, dk, *s, A, *s, ws, ws_bytes, None)
+
+    assert call(lse=None) == EINVAL and call(ws_bytes=need - 1) == ESIZE and call(ws=A + 8) == EINVAL
+    assert call(dk=None) == EINVAL and b"null dk" in L.solattn_last_error()
+    assert call(do=A + 2) == EINVAL and b"do must" in L.solattn_last_error()
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(dtype=2), EINVAL, b"dtype"), (dict(H=5), EINVAL, b"heads"), (dict(D=136), EUNSUPPORTED, b"head_dim"),
+    (dict(page=12), EINVAL, b"multiple of 8"), (dict(pages=0), EINVAL, b"pages"), (dict(most=1 << 28), EUNSUPPORTED, b"2^31"),
+    (dict(scale=-1.0), EINVAL, b"scale"), (dict(window=-1), EINVAL, b"window"), (dict(table=None), EINVAL, b"table"),
+    (dict(q=A + 4), EINVAL, b"aligned"),
+])
+def test_paged_refusals(capi, kw, rc, text):
+    o = dict(dtype=0, H=4, Hkv=2, D=128, page=16, pages=9, most=4, scale=0.1, window=0, table=A, q=A)
+    o.update(kw)
+    c = (o["page"] * 256, 256, 128)
+    got = capi.LIB.solattn_paged_attn(o["q"], 512, 128, A, *c, A, *c, o["pages"], o["page"], o["table"], o["most"], o["most"],
+                                      A, 1, o["H"], o["Hkv"], o["D"], o["dtype"], o["window"], 0, o["scale"], None, 0, A, 512,
+                                      128, None)
+    assert got == rc and text in capi.LIB.solattn_last_error(), capi.LIB.solattn_last_error()
+
+
+def test_paged_workspace(capi):
+    L = capi.LIB
+    need = L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, 0, 0)
+    splits = need // (24 * 130 * 4)
+    assert need == splits * 24 * 130 * 4 and 1 < splits <= 64
+    # a window bounds what is split; enough sequences need no split
+    assert L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, 100, 4) < need
+    assert L.solattn_paged_attn_workspace_bytes(256, 24, 8, 128, 1000, 64, 0, 0) == 0
+    assert L.solattn_paged_attn_workspace_bytes(1, 24, 7, 128, 1000, 64, 0, 0) == 0
+    c = (64 * 1024, 1024, 128)
+    rc = L.solattn_paged_attn(A, 24 * 128, 128, A, *c, A, *c, 1000, 64, A, 1000, 1000, A, 1, 24, 8, 128, 0, 0, 0, 0.1, A,
+                              need - 1, A, 24 * 128, 128, None)
+    assert rc == ESIZE and b"workspace" in L.solattn_last_error()
+
+
+def test_host_tensors_are_refused(pkg):
+    """There is no CPU path: the operators say so."""
+    x = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    t = torch.zeros(1, 1, dtype=torch.int32)
+    n = torch.ones(1, dtype=torch.int32)
+    mod = lambda name: importlib.import_module(f"{pkg.__name__}.{name}")  # noqa: E731
+    with pytest.raises(ValueError, match="GPU"):
+        mod("_qk_rope").qk_norm_rope(x, x)
+    with pytest.raises(ValueError, match="GPU"):
+        mod("_window").window_attn(x, x, x, window=4)
+    with pytest.raises(ValueError, match="GPU"):
+        mod("_paged").paged_attn(x[:, :1], x, x, t, n)
+    with pytest.raises(ValueError, match="GPU"):
+        mod("_qk_rope").qk_norm_rope_append(x[:, :1], x[:, :1], x[:, :1], x, x, t, n)
+    with pytest.raises(TypeError):
+        mod("_window").window_attn(x, x, x)  # the window has no default
