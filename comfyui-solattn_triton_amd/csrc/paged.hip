@@ -129,26 +129,31 @@ paged_kernel(const PagedArgs a) {
   float m = -INFINITY, l = 0.f;  // l: this lane's keys
 
   const int vch = kFull || CH * col < a.D ? CH * col : 0;
+  const auto base_of = [&](int st) __attribute__((always_inline)) {
+    return st < vis.sink_steps ? st * kStep : vis.first + (st - vis.sink_steps) * kStep;
+  };
+  // Where the eight consecutive keys from j8 on are: they share a page (its size is a
+  // multiple of 8, or the page is a whole sequence). Page ids are read a step ahead, so
+  // that a step waits for one round of memory, not two.
+  const auto slot_of = [&](int j8, int& slot) __attribute__((always_inline)) {
+    const uint32_t j = static_cast<uint32_t>(min(j8, max(vis.len - 1, 0) & ~7));
+    const uint32_t pg = a.page_mul ? __umulhi(j, a.page_mul) >> a.page_shift : j >> a.page_shift;
+    slot = static_cast<int>(j - pg * a.page);
+    return a.table ? a.table[b * a.table_b + pg] : b;
+  };
+  int kslot = 0, vslot = 0, kid = 0, vid = 0;
+  if (step0 + wave < step1) {
+    const int base = base_of(step0 + wave);
+    kid = slot_of(base + 8 * (col >> 2), kslot);
+    vid = slot_of(base + 8 * g, vslot);
+  }
   for (int st = step0 + wave; st < step1; st += kWaves) {
     const bool sink = st < vis.sink_steps;
-    const int base = sink ? st * kStep : vis.first + (st - vis.sink_steps) * kStep;
+    const int base = base_of(st);
     const int lo = sink ? 0 : vis.low, hi = sink ? vis.sinks_end : vis.len;  // visible: lo <= j < hi
-    // Eight consecutive keys share a page (its size is a multiple of 8, or the page
-    // is a whole sequence). Keys outside the cache's pages are not visible.
-    const auto rows_of = [&](int j8, bool& ok, int64_t& page, int& slot) __attribute__((always_inline)) {
-      const uint32_t j = static_cast<uint32_t>(min(j8, max(vis.len - 1, 0) & ~7));
-      const uint32_t pg = a.page_mul ? __umulhi(j, a.page_mul) >> a.page_shift : j >> a.page_shift;
-      const int id = a.table ? a.table[b * a.table_b + pg] : b;
-      ok = id >= 0 && id < a.pages;
-      page = ok ? id : 0;
-      slot = static_cast<int>(j - pg * a.page);
-    };
-    bool kok, vok;  // (a key's score lane holds its V piece too, so vok is the one that counts)
-    int64_t kpage, vpage;
-    int kslot, vslot;
-    rows_of(base + 8 * (col >> 2), kok, kpage, kslot);
-    rows_of(base + 8 * g, vok, vpage, vslot);
-    (void)kok;
+    // Keys of page ids outside the cache are not visible (a key's score lane holds its V piece too).
+    const bool vok = vid >= 0 && vid < a.pages;
+    const int64_t kpage = kid >= 0 && kid < a.pages ? kid : 0, vpage = vok ? vid : 0;
     const int last = a.page - 1;  // a slot past the page's end (a whole-sequence page) repeats its last
     bf16x8 kr[2][NC];
 #pragma unroll
@@ -171,6 +176,11 @@ paged_kernel(const PagedArgs a) {
         const uint2 x = *reinterpret_cast<const uint2*>(vp);
         vr[i][0] = x.x, vr[i][1] = x.y;
       }
+    }
+    if (st + kWaves < step1) {
+      const int next = base_of(st + kWaves);
+      kid = slot_of(next + 8 * (col >> 2), kslot);
+      vid = slot_of(next + 8 * g, vslot);
     }
     f32x4 s[2];
 #pragma unroll
