@@ -340,54 +340,56 @@ __global__ void __launch_bounds__(256) window_join_kernel(const WindowArgs a) {
 }
 
 // The products of a half step of the backward (32 rows by 32 keys), hand-ordered: an
-// operand is read two products ahead of its own (left to itself the compiler reads it
-// right in front and waits: the matrix instructions were busy a third of the time).
+// operand is read AHEAD products before its own (left to itself the compiler reads it
+// right in front and waits: the matrix instructions were busy a third of the time). A
+// product takes 32 cycles, an LDS read beside those of seven other waves several times
+// that. Raised wave priority: the issue arbiter prefers a wave inside its products.
 // Two scores from the tiles at x and y, rows by rows: s = X B^T, t = Y C^T.
-template <typename E, int D, typename AX, typename AY>
+template <typename E, int D, int AHEAD, typename AX, typename AY>
 __device__ __forceinline__ void two_scores(f32x16& s, f32x16& t, const AX& x, uint32_t x_at, const bf16x8 (&b)[D / 16],
                                            const AY& y, uint32_t y_at, const bf16x8 (&c)[D / 16]) {
-  constexpr int NC = D / 16;
-  bf16x8 r[3];
+  constexpr int NC = D / 16, R = AHEAD + 1;
+  bf16x8 r[R];
   __builtin_amdgcn_s_setprio(1);
   const auto operand = [&](int i) { return i < NC ? x.by_row(0, i, x_at) : y.by_row(0, i - NC, y_at); };
-  r[0] = operand(0);
-  r[1] = operand(1);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) r[i] = operand(i);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 2 * NC; ++i) {
-    if (i + 2 < 2 * NC) {
-      r[(i + 2) % 3] = operand(i + 2);
+    if (i + AHEAD < 2 * NC) {
+      r[(i + AHEAD) % R] = operand(i + AHEAD);
       asm volatile("" ::: "memory");
     }
     if (i == 0)
       E::amfma0(s, r[0], b[0]);
     else if (i < NC)
-      E::amfma(s, r[i % 3], b[i]);
+      E::amfma(s, r[i % R], b[i]);
     else if (i == NC)
-      E::amfma0(t, r[i % 3], c[0]);
+      E::amfma0(t, r[i % R], c[0]);
     else
-      E::amfma(t, r[i % 3], c[i - NC]);
+      E::amfma(t, r[i % R], c[i - NC]);
   }
   __builtin_amdgcn_s_setprio(0);
   asm volatile("s_nop 7\n\ts_nop 7" : "+v"(s), "+v"(t));  // readers of s and t come after their wait states
 }
 
 // acc += X^T W for the 32 rows at x, read transposed; w: W's two packed operands.
-template <typename E, int D, typename AX>
+template <typename E, int D, int AHEAD, typename AX>
 __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, uint32_t at, const bf16x8 (&w)[2]) {
-  constexpr int ND = D / 32, N = 2 * ND;
-  bf16x8 r[3];
+  constexpr int ND = D / 32, N = 2 * ND, R = AHEAD + 1;
+  bf16x8 r[R];
   __builtin_amdgcn_s_setprio(1);
-  r[0] = x.transposed(0, 0, at);
-  r[1] = x.transposed(1 / ND, 1 % ND, at);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) r[i] = x.transposed(i / ND, i % ND, at);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (i + 2 < N) {
-      r[(i + 2) % 3] = x.transposed((i + 2) / ND, (i + 2) % ND, at);
+    if (i + AHEAD < N) {
+      r[(i + AHEAD) % R] = x.transposed((i + AHEAD) / ND, (i + AHEAD) % ND, at);
       asm volatile("" ::: "memory");
     }
-    E::amfma_after_valu(acc[i % ND], r[i % 3], w[i / ND]);
+    E::amfma_after_valu(acc[i % ND], r[i % R], w[i / ND]);
   }
   __builtin_amdgcn_s_setprio(0);
 }
@@ -426,8 +428,9 @@ window_dq_kernel(const WindowArgs a) {
       copy_tile<kThreads, D, kByRow>(vb + at, vp, a.v.t, safe);
     }
   };
-  // keys that every row of the wave sees
+  // keys that every row of the wave sees, and those that any does (a tile without is skipped)
   const int all_lo = -wave_min(-rk.jl), all_hi = wave_min(rk.jh), all_sk = wave_min(rk.sk);
+  const int any_lo = wave_min(rk.jl), any_hi = -wave_min(-rk.jh), any_sk = -wave_min(-rk.sk);
   if (kt.n) issue(0);
   bf16x8 q[NC], g[NC];
   load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
@@ -462,6 +465,7 @@ window_dq_kernel(const WindowArgs a) {
     wait_tile_copies();
     __syncthreads();  // this tile is in, and every wave is done with the buffers of the last
     if (t + 1 < kt.n) issue(t + 1);
+    if ((j0 > any_hi || j0 + kKeys - 1 < any_lo) && j0 >= any_sk) continue;
     const bool masked = !((j0 >= all_lo && j0 + kKeys - 1 <= all_hi) || j0 + kKeys <= all_sk);
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
@@ -469,7 +473,7 @@ window_dq_kernel(const WindowArgs a) {
       va.remade();
       const uint32_t at = (t & 1) * kBuf + m2 * (64 * D);
       f32x16 s, dp;
-      two_scores<E, D>(s, dp, ka, at, q, va, at, g);
+      two_scores<E, D, D == 64 ? 6 : 4>(s, dp, ka, at, q, va, at, g);
       if (masked) mask_keys(s, rk, j0 + 32 * m2, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -480,7 +484,7 @@ window_dq_kernel(const WindowArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
       const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
-      add_product<E, D>(acc, ka, at, ds);
+      add_product<E, D, 3>(acc, ka, at, ds);
     }
   }
   mfma_fence(acc);
@@ -503,6 +507,7 @@ template <typename E, int D>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dkv_kernel(const WindowArgs a) {
   constexpr int ND = D / 32, NC = D / 16;
+  constexpr int kAhead = D == 64 ? 3 : 2;  // (what the registers leave: 3 at 128 channels spills)
   constexpr uint32_t kBuf = kKeys * D * 2;  // bytes of a tile
   __shared__ __align__(256) uint16_t qbuf[2 * kKeys * D];
   __shared__ __align__(256) uint16_t gbuf[2 * kKeys * D];
@@ -572,7 +577,7 @@ window_dkv_kernel(const WindowArgs a) {
       const uint32_t at = buf * kBuf + m2 * (64 * D);
       qa.remade();
       f32x16 s, dp;
-      two_scores<E, D>(s, dp, qa, at, k, qa, at + to_g, v);
+      two_scores<E, D, kAhead>(s, dp, qa, at, k, qa, at + to_g, v);
       const float* lse = stat[buf][0] + 32 * m2 + 4 * half;
       const float* delta = stat[buf][1] + 32 * m2 + 4 * half;
 #pragma unroll
@@ -601,8 +606,8 @@ window_dkv_kernel(const WindowArgs a) {
       }
       const bf16x8 pb[2] = {pack8<E>(s, 0), pack8<E>(s, 1)};
       const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
-      add_product<E, D>(dv, qa, at + to_g, pb);
-      add_product<E, D>(dk, qa, at, ds);
+      add_product<E, D, kAhead>(dv, qa, at + to_g, pb);
+      add_product<E, D, kAhead>(dk, qa, at, ds);
     }
   }
   mfma_fence(dk);
