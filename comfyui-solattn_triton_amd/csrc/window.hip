@@ -42,11 +42,10 @@ __device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, in
   b = w / a.Hkv;
 }
 
-// Wave-wide minimum and maximum of a lane value, as scalars.
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
-  return __builtin_amdgcn_readfirstlane(x);
+// What the rows of this wave see (rows past Tq repeat the last).
+__device__ __forceinline__ RowsKeys wave_keys(const WindowArgs& a, int r0, int len) {
+  const int first = r0 + 32 * wave_id();
+  return rows_keys(a, a.q_start + min(first, a.Tq - 1), a.q_start + min(first + 31, a.Tq - 1), len);
 }
 
 template <int ND>
@@ -180,11 +179,10 @@ window_fwd_kernel(const WindowArgs a) {
       wait_tile_copies();
       __syncthreads();
     };
-    // keys that every row of the wave sees
-    const int all_lo = -wave_min(-rk.jl), all_hi = wave_min(rk.jh), all_sk = wave_min(rk.sk);
+    const RowsKeys wave = wave_keys(a, r0, len);
     const auto mask = [&](f32x16& s, int n) __attribute__((always_inline)) {
       const int j0 = kt.first(tile0 + (n >> 1)) + 32 * (n & 1);
-      if (!((j0 >= all_lo && j0 + 31 <= all_hi) || j0 + 32 <= all_sk)) mask_keys(s, rk, j0, half);
+      if (!wave.all(j0, 32)) mask_keys(s, rk, j0, half);
     };
     const int last = 2 * ntiles - 1;
 
@@ -247,31 +245,30 @@ window_fwd_kernel(const WindowArgs a) {
       land();
     };
     // Steps 2 t + 1 and 2 t + 2 work on tiles t to t + 2 of the part. Where these lie in
-    // the run of window tiles that every row of the block sees whole, they need no
-    // masks, and their copies are 32 rows apart.
-    int t = 0, run0, run1;
-    {
-      const int lo = max(p1 - a.window + 1, 0), hi = min(a.causal ? p0 : p0 + a.window - 1, len - 1);
-      run0 = max(kt.ns, kt.ns + (lo - kt.w0 + kKeys - 1) / kKeys) - tile0;
-      run1 = p1 < len ? min(kt.ns + (hi + 1 - kt.w0) / kKeys - tile0, ntiles) - 2 : 0;
-      run0 = max(run0, 0);
-    }
-    for (; t < min(run0, ntiles - 1); ++t) {
-      odd(2 * t + 1, std::false_type());
-      even(2 * t + 2, std::false_type());
-    }
-    if (t < run1) {
-      const int j0 = kt.first(tile0 + t);
-      kn += (j0 + 96) * a.k.t;
-      vn += (j0 + 32) * a.v.t;
-    }
-    for (; t < run1; ++t) {
-      odd(1, std::true_type());
-      even(2, std::true_type());
-    }
-    for (; t < ntiles - 1; ++t) {
-      odd(2 * t + 1, std::false_type());
-      even(2 * t + 2, std::false_type());
+    // a run of tiles that every row of the block sees whole, among the sinks' or the
+    // window's, they need no masks, and their copies are 32 rows apart.
+    const int lo = max(p1 - a.window + 1, 0), hi = min(a.causal ? p0 : p0 + a.window - 1, len - 1);
+    int run0 = 0, run1 = p1 < len ? min(kt.s_end / kKeys, kt.ns) : 0;
+    int t = 0;
+#pragma unroll 1
+    for (int run = 0; run < 3; ++run) {  // (the last one has no run: what is left)
+      run0 = max(min(run0 - tile0, ntiles - 1), 0);
+      run1 = min(run1 - tile0, ntiles) - 2;
+      for (; t < run0; ++t) {
+        odd(2 * t + 1, std::false_type());
+        even(2 * t + 2, std::false_type());
+      }
+      if (t < run1) {
+        const int j0 = kt.first(tile0 + t);
+        kn = kp + (j0 + 96) * a.k.t;
+        vn = vp + (j0 + 32) * a.v.t;
+      }
+      for (; t < run1; ++t) {
+        odd(1, std::true_type());
+        even(2, std::true_type());
+      }
+      run0 = run == 0 ? max(kt.ns, kt.ns + (lo - kt.w0 + kKeys - 1) / kKeys) : kt.n;
+      run1 = run == 0 && p1 < len ? kt.ns + (hi + 1 - kt.w0) / kKeys : 0;
     }
     odd(2 * t + 1, std::false_type());
     // P.V of the last half
@@ -428,9 +425,7 @@ window_dq_kernel(const WindowArgs a) {
       copy_tile<kThreads, D, kByRow>(vb + at, vp, a.v.t, safe);
     }
   };
-  // keys that every row of the wave sees, and those that any does (a tile without is skipped)
-  const int all_lo = -wave_min(-rk.jl), all_hi = wave_min(rk.jh), all_sk = wave_min(rk.sk);
-  const int any_lo = wave_min(rk.jl), any_hi = -wave_min(-rk.jh), any_sk = -wave_min(-rk.sk);
+  const RowsKeys wave = wave_keys(a, r0, len);
   if (kt.n) issue(0);
   bf16x8 q[NC], g[NC];
   load_row<D>(q, a.q.p + b * a.q.b + static_cast<int64_t>(rr) * a.q.t + h * a.q.h, half);
@@ -465,8 +460,8 @@ window_dq_kernel(const WindowArgs a) {
     wait_tile_copies();
     __syncthreads();  // this tile is in, and every wave is done with the buffers of the last
     if (t + 1 < kt.n) issue(t + 1);
-    if ((j0 > any_hi || j0 + kKeys - 1 < any_lo) && j0 >= any_sk) continue;
-    const bool masked = !((j0 >= all_lo && j0 + kKeys - 1 <= all_hi) || j0 + kKeys <= all_sk);
+    if (wave.none(j0, kKeys)) continue;
+    const bool masked = !wave.all(j0, kKeys);
 #pragma unroll
     for (int m2 = 0; m2 < 2; ++m2) {
       ka.remade();
@@ -528,9 +523,9 @@ window_dkv_kernel(const WindowArgs a) {
   const int per = (tiles * a.group + kp.parts - 1) / kp.parts;
   const int s0 = min(kp.part * per, tiles * a.group), s1 = min(s0 + per, tiles * a.group);
   // rows that see every key of the wave, and those that see any (a step without is skipped)
-  const int all_lo = -wave_min(-kr.pl) - a.q_start, all_hi = wave_min(kr.ph) - a.q_start;
-  const bool seen = kr.pl <= kr.ph;
-  const int any_lo = wave_min(seen ? kr.pl : a.Tk) - a.q_start, any_hi = -wave_min(seen ? -kr.ph : 0) - a.q_start;
+  const KeysRows kw = keys_rows(a, j0 + wave * 32, j0 + wave * 32 + 31, len);
+  const int all_lo = kw.all_lo - a.q_start, all_hi = kw.all_hi - a.q_start;
+  const int any_lo = kw.any_lo - a.q_start, any_hi = kw.any_hi - a.q_start;
 
   const uint32_t qb = lds_addr(qbuf), gb = lds_addr(gbuf), sb = lds_addr(stat);
   TileAddr<D, kBoth> qa(qb, lane);  // (dO's tiles: the same, at to_g)

@@ -74,6 +74,45 @@ __device__ __forceinline__ KeyRows key_rows(const WindowArgs& a, int j, int len)
   return r;
 }
 
+// Of consecutive rows at p0 to p1: the keys that every one of them sees, j in [all_lo,
+// all_hi] or j < all_sk, and bounds of those that any does.
+struct RowsKeys {
+  int all_lo, all_hi, all_sk, any_lo, any_hi, any_sk;
+  __device__ __forceinline__ bool all(int first, int keys) const {
+    return (first >= all_lo && first + keys - 1 <= all_hi) || first + keys <= all_sk;
+  }
+  __device__ __forceinline__ bool none(int first, int keys) const {
+    return (first > any_hi || first + keys - 1 < any_lo) && first >= any_sk;
+  }
+};
+__device__ __forceinline__ RowsKeys rows_keys(const WindowArgs& a, int p0, int p1, int len) {
+  const RowKeys lo = row_keys(a, p0, len), hi = row_keys(a, min(p1, len - 1), len);
+  RowsKeys r;
+  r.any_lo = lo.jl, r.any_hi = hi.jh, r.any_sk = hi.sk;
+  r.all_lo = hi.jl, r.all_hi = lo.jh, r.all_sk = lo.sk;
+  if (p1 >= len) r.all_hi = -1, r.all_sk = 0;  // a row that sees nothing
+  if (p0 >= len) r.any_lo = 0, r.any_hi = -1, r.any_sk = 0;
+  return r;
+}
+
+// Of consecutive keys j0 to j1: the rows that see every one of them, p in [all_lo,
+// all_hi], and bounds of those that see any.
+struct KeysRows {
+  int all_lo, all_hi, any_lo, any_hi;
+};
+__device__ __forceinline__ KeysRows keys_rows(const WindowArgs& a, int j0, int j1, int len) {
+  // intervals move up with the key, but that those of sinks end with the sequence and,
+  // symmetric, begin with it
+  const KeyRows first = key_rows(a, j0, len), last = key_rows(a, min(j1, len - 1), len);
+  const KeyRows past_sinks = key_rows(a, min(max(j0, a.sinks), j1), len);
+  KeysRows r;
+  r.any_lo = first.pl, r.any_hi = j0 < a.sinks ? first.ph : last.ph;
+  r.all_lo = last.pl, r.all_hi = past_sinks.ph;
+  if (j1 >= len) r.all_hi = -1;  // a key that no row sees
+  if (j0 >= len) r.any_lo = 1, r.any_hi = -1;
+  return r;
+}
+
 // The 64-key tiles that rows [p0, p1] see: those of the sinks below the window,
 // then the window's. Keys of a tile that none of these rows sees are not read:
 // safe(j) is a key that is.
