@@ -642,6 +642,7 @@ __global__ void __launch_bounds__(256) window_dkv_join_kernel(const WindowArgs a
   const int64_t slot = static_cast<int64_t>(bh) * a.slots + (sink ? block * a.ks : a.nsb * a.ks + (block - a.nsb) * a.kn);
   const float* p = a.part + (slot * 2 + which) * (kRows * D) + key * D + ch;
   float x[8] = {};
+#pragma unroll 8
   for (int i = 0; i < parts; ++i) {
     const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
     x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w, x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
