@@ -6,8 +6,16 @@
 //   D_i = do_i . o_i,  dS = P (do_i . v_j - D_i)
 //   dv_j = sum_i P do_i,  dq_i = scale sum_j dS k_j,  dk_j = scale sum_i dS q_i
 //
-// Bound: the matrix instructions and, beside them, the exps. Everything between
-// the products stays in registers: S^T = K Q^T puts a row on a lane column, so its
+// Bound: the LDS reads of the products' operands beside the products themselves (a
+// wave's 32 rows use an operand once, so a CU's reads take nearly as long as its matrix
+// instructions: 3770 against 4100 cycles for 64 rows of the dk, dv kernel, 1080 against
+// 1020 for the forward's 32 keys), then the exps and the power limit; short sequences
+// are bound by the latency of a step. 16001 tokens, window 4096, 24 heads of 128 over
+// 8: 657-671 us, 1050-1070 TFLOP/s; 12133 tokens, symmetric window 2401, 1333 sinks:
+// 720-730 us, 1090-1100 TFLOP/s; 8192 tokens, window 1024, with gradients: 555-600 us
+// (forward 130-145, dq 185-205, dk and dv 225-245, join 7); 2000 tokens of 16 heads of
+// 64, batch 2, window 512, with gradients: 92 us (26, 31, 34, 6).
+// Everything between the products stays in registers: S^T = K Q^T puts a row on a lane column, so its
 // statistics need one exchange (lanes 32 apart) and P converts in place into the B
 // operand of the next product, whose A operand is read transposed from LDS
 // (ds_read_b64_tr_b16). P and dS are rounded to the inputs' type for the matrix
@@ -127,7 +135,9 @@ __device__ __forceinline__ void window_step(RowState<D / 32>& st, const f32x16& 
 }
 
 // The forward. Two half buffers of 32 rows each for K and V: step n copies K(n+2)
-// over K(n) and V(n) over V(n-2), so a copy has a whole step to land.
+// over K(n) and V(n) over V(n-2), so a copy has a whole step to land. (Four half
+// buffers, copies two steps further ahead: 757 -> 773 us at 16001 tokens, 130 -> 135 for
+// 517 rows of 64 channels. Steps of 64 keys at 64 channels: 77 -> 86 us there.)
 template <typename E, int BLK, int D>
 __global__ void __launch_bounds__(2 * BLK) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
 window_fwd_kernel(const WindowArgs a) {
@@ -392,6 +402,8 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, 
 }
 
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
+// (The softmax work between the products of the next half, as the forward has it, with
+// four half buffers and a barrier for each: 191 -> 208 us at 8192 tokens.)
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dq_kernel(const WindowArgs a) {
@@ -728,8 +740,9 @@ static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq =
 
 // Rows of a workgroup and parts of their keys. 128 rows share the copies of a tile
 // among four waves; launches that would not give every CU two such workgroups take
-// 64 rows, and where these are still few their key tiles are cut into parts of at
-// least eight tiles, joined by a second launch.
+// 64 rows, and where these do not give every CU four, their key tiles are cut into parts
+// of at least eight tiles, joined by a second launch (517 rows against 16000 keys: 105
+// us with two for every CU, 77 with four, 86 with eight).
 static int cut_rows(WindowArgs& a) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
   const int blk = bh * cdiv(a.Tq, 128) >= 512 ? 128 : 64;
