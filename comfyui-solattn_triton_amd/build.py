@@ -71,7 +71,9 @@ def _native(verbose: bool) -> None:
     torch_dir = os.path.dirname(torch.__file__)
     rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
     tmp = NATIVE + ".tmp"
-    cmd = [shutil.which("g++") or "c++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall",
+    cxx = next((c for c in map(shutil.which, ("g++", "c++", "clang++")) if c),
+               os.path.join(rocm, "llvm", "bin", "clang++"))
+    cmd = [cxx, "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall",
            "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            "-isystem", os.path.join(torch_dir, "include"),

@@ -115,6 +115,12 @@ paged_kernel(const PagedArgs a) {
   const Visible vis = visible(a, b);
   const int per = (vis.steps + a.split - 1) / a.split;
   const int step0 = split * per, step1 = min(step0 + per, vis.steps);
+  if (step0 >= step1 && a.split > 1) {  // nothing here: the join passes over a sum of 0
+    if (static_cast<int>(threadIdx.x) < ncol)
+      reinterpret_cast<float2*>(a.part + a.part_ml)[(static_cast<int64_t>(b) * a.H + head0 + threadIdx.x) * a.split + split] =
+          make_float2(-INFINITY, 0.f);
+    return;
+  }
 
   bf16x8 q[NC];
   {
@@ -289,14 +295,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   const bool on = ch < a.D;
   const float* p = a.part + row * a.split * a.D + (on ? ch : 0);
   float o0 = 0.f, o1 = 0.f;
-  for (int i0 = 0; i0 < a.split; i0 += 8) {  // eight loads in flight; those past the last weigh 0 (lane split.. above)
+  // Splits behind the last that saw a key are not read (one without steps wrote no sums);
+  // eight loads in flight, those past the last read it again and weigh 0.
+  const uint64_t seen = __ballot(mine.x != -INFINITY);
+  const int used = seen ? 64 - __clzll(seen) : 0;
+  for (int i0 = 0; i0 < used; i0 += 8) {
     float2 x[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      x[u] = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(min(i0 + u, a.split - 1)) * a.D);
+      x[u] = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(min(i0 + u, used - 1)) * a.D);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const float fi = __shfl(f, i0 + u);  // (split <= 64, so i0 + u < 64)
+      const float fi = i0 + u < used ? __shfl(f, i0 + u) : 0.f;  // (split <= 64, so i0 + u < 64)
       o0 = fmaf(x[u].x, fi, o0);
       o1 = fmaf(x[u].y, fi, o1);
     }
@@ -309,11 +319,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
 // Splits of a sequence: four workgroups for every CU, so that ragged sequences even
 // out, of at least a step a wave as long as the longest sequence allows. (Two for
 // every CU: 32 ragged sequences of up to 16384 keys 83 -> 60 us, four of 131072
-// 281 -> 250; eight and sixteen: 61 and 58, 258 and 258.)
+// 281 -> 250; eight and sixteen: 61 and 58, 258 and 258.) No split is longer than 4096 keys as far
+// as there may be 64 of them: one long sequence in a large batch is not left to one
+// workgroup a head.
 int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks) {
   const int64_t keys = window && window + sinks < most ? window + sinks : most;
   const int64_t steps = cdiv(keys, kStep) + 1;
   int64_t n = cdiv(1024, B * Hkv * tiles);
+  if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);
   if (n > steps / kWaves) n = steps / kWaves;
   if (n > kMaxSplits) n = kMaxSplits;
   return n < 1 ? 1 : static_cast<int>(n);

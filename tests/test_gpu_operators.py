@@ -481,6 +481,22 @@ def test_paged(paged, dev, case):
     assert (got[n == 0] == 0).all()
 
 
+@pytest.mark.parametrize("first", [0, 4096])
+def test_paged_split_without_keys(paged, dev, first):
+    """A split whose pages all are bad, the first or one in the middle, beside others."""
+    page, Hkv, D, L = 64, 1, 64, 16384
+    kc, vc = randn((L // page, page, Hkv, D), 1, dev), randn((L // page, page, Hkv, D), 2, dev)
+    q = randn((1, 1, 2, D), 3, dev)
+    table = torch.arange(L // page, dtype=torch.int32, device=dev)[None].clone()
+    table[:, first // page:(first + 2048) // page] = -7
+    n = torch.tensor([9000], dtype=torch.int32, device=dev)
+    on = torch.arange(L, device=dev)[None, None] < 9000
+    on[..., first:first + 2048] = False
+    got = paged.paged_attn(q, kc, vc, table, n)
+    o, p, (_, _, vh) = ref.attention(q, kc.view(1, L, Hkv, D), vc.view(1, L, Hkv, D), on, D ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, BF), "o")
+
+
 def test_paged_bad_pages_and_long_lengths(paged, dev):
     """Keys on page ids that the cache lacks are not visible; a length past the table
     is the table's; a cache without pages gives zeros."""
@@ -609,6 +625,59 @@ def test_other_stream_and_graph(rope, window, paged, dev):
             torch.cuda.synchronize()
             for x, y in zip(out, step()):
                 assert torch.equal(x, y)
+
+
+def test_offsets_beyond_32_bits(rope, window, paged, dev):
+    """A cache, a key buffer and a token range of more than 2^31 values: what lies
+    behind that is read and written where it is. (Nothing else in them is touched, so
+    they stay uninitialised.)"""
+    H, Hkv, D, page = 4, 4, 128, 64
+    pages = 66000  # 2.16e9 values
+    kc, vc = (torch.empty((pages, page, Hkv, D), device=dev, dtype=BF) for _ in range(2))
+    ids = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32, device=dev)
+    q, k, v = (randn((1, 150, H, D), s, dev) for s in (1, 2, 3))
+    n = torch.tensor([150], dtype=torch.int32, device=dev)
+    qp = rope.qk_norm_rope_append(q, k, v, kc, vc, ids, n)
+    kn = rope.qk_norm_rope(q, k)[1]
+    small = [torch.stack([t[i] for i in ids[0].tolist()]) for t in (kc, vc)]
+    assert torch.equal(small[0].flatten(0, 1)[:150], kn[0]) and torch.equal(small[1].flatten(0, 1)[:150], v[0])
+    near = torch.arange(3, dtype=torch.int32, device=dev)[None]
+    assert torch.equal(paged.paged_attn(qp[:, -1:], kc, vc, ids, n), paged.paged_attn(qp[:, -1:], *small, near, n))
+    # the same memory as one long sequence, its rows at the far end
+    kf, vf = kc.view(1, pages * page, Hkv, D), vc.view(1, pages * page, Hkv, D)
+    T = kf.shape[1]
+    kf[:, T - 200:], vf[:, T - 200:] = randn((1, 200, Hkv, D), 4, dev), randn((1, 200, Hkv, D), 5, dev)
+    tail = kf[:, T - 200:].clone(), vf[:, T - 200:].clone()
+    for rows in (1, 100):  # (tiles begin at other keys than in the tail alone, so not the same bits)
+        far = window.window_attn(qp[:, :rows], kf, vf, window=90)
+        on = ref.seen(rows, 200, 200 - rows, 90, 0, True, None, 1, dev)
+        o, p, (_, _, vh) = ref.attention(qp[:, :rows], *tail, on, D ** -0.5)
+        ref.close(far, o, ref.forward_bound(o, p, vh, BF), "far rows")
+    x = kc.view(1, -1, 32, D)  # tokens of 32 heads
+    x[:, -5:] = randn((1, 5, 32, D), 6, dev)
+    at = torch.arange(x.shape[1], device=dev)
+    cos, sin = tables(8, D, dev)
+    got = rope.qk_norm_rope(x, x[:, :, :1], None, None, cos, sin, positions=at % 8)[0][:, -5:]
+    assert torch.equal(got, rope.qk_norm_rope(x[:, -5:], x[:, -5:, :1], None, None, cos, sin, positions=(at % 8)[-5:])[0])
+
+
+def test_training_keeps_no_memory(rope, window, dev):
+    q, k, v = (randn((1, 300, 4, 64), s, dev).requires_grad_(True) for s in (1, 2, 3))
+    cos, sin = tables(300, 64, dev)
+
+    def step():
+        qr, kr = rope.qk_norm_rope(q, k, None, None, cos, sin)
+        window.window_attn(qr, kr, v, window=64).float().square().sum().backward()
+        for t in (q, k, v):
+            t.grad = None
+
+    step()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
 
 
 def test_two_streams_at_once(window, paged, dev):

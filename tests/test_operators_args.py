@@ -136,9 +136,11 @@ def test_paged_workspace(capi):
     need = L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, 0, 0)
     splits = need // (24 * 130 * 4)
     assert need == splits * 24 * 130 * 4 and 1 < splits <= 64
-    # a window bounds what is split; enough sequences need no split
+    # a window bounds what is split; enough sequences need no split, but that none has
+    # more than 4096 keys where a table may hold more
     assert L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, 100, 4) < need
-    assert L.solattn_paged_attn_workspace_bytes(256, 24, 8, 128, 1000, 64, 0, 0) == 0
+    assert L.solattn_paged_attn_workspace_bytes(256, 24, 8, 128, 64, 64, 0, 0) == 0
+    assert L.solattn_paged_attn_workspace_bytes(256, 24, 8, 128, 65, 64, 0, 0) == 256 * 24 * 2 * 130 * 4
     assert L.solattn_paged_attn_workspace_bytes(1, 24, 7, 128, 1000, 64, 0, 0) == 0
     c = (64 * 1024, 1024, 128)
     rc = L.solattn_paged_attn(A, 24 * 128, 128, A, *c, A, *c, 1000, 64, A, 1000, 1000, A, 1, 24, 8, 128, 0, 0, 0, 0.1, A,
