@@ -43,9 +43,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
     ``lengths`` (int32 [B]) counts the new tokens too, as ``paged_attn`` then reads
     it: token t is at position lengths[b] - T + t, slot position % page_size of page
     ``page_table[b, position // page_size]``. k_cache, v_cache: [pages, page_size,
-    Hkv, D]. A token before position 0 (an idle slot's length 0), past the table or
-    on a page id that the cache does not have writes nothing, and its q' means
-    nothing. Has no gradient.
+    Hkv, D]. A token before position 0 (an idle slot's length 0), past the page table
+    or on a page id that the cache does not have writes nothing, and its q' means
+    nothing. Positions past the end of ``cos`` turn by its last row: it has to cover
+    the sequences. Has no gradient.
     """
     return native.qk_norm_rope_append(q, k, v, k_cache, v_cache, page_table, lengths, q_weight, k_weight, cos, sin,
                                       eps, interleaved)

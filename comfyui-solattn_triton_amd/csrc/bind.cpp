@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <utility>
 #include <vector>
@@ -89,13 +90,14 @@ int type_code(const Tensor& t) {
 
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
-// Whether the kernels read t in place: a contiguous last dim, every row 16-byte
-// aligned, token strides in their range.
-bool row_ready(const Tensor& t) {
+// A contiguous last dim and every row 16-byte aligned.
+bool rows_aligned(const Tensor& t) {
   const int64_t whole = 16 / t.element_size();
   const auto s = t.strides();
-  return (t.size(3) <= 1 || s[3] == 1) && aligned16(t) && (s[0] | s[1] | s[2]) % whole == 0 && s[1] < (1 << 24);
+  return s[3] == 1 && aligned16(t) && (s[0] | s[1] | s[2]) % whole == 0;
 }
+// Whether the kernels read t in place: aligned rows, token strides in their range.
+bool row_ready(const Tensor& t) { return rows_aligned(t) && t.stride(1) < (1 << 24); }
 Tensor as_rows(const Tensor& t) {
   // (a contiguous tensor may be misaligned, so contiguous() alone is not enough)
   return row_ready(t) ? t : t.clone(at::MemoryFormat::Contiguous);
@@ -115,14 +117,15 @@ void check_int32(const Tensor& t, const char* name, at::IntArrayRef want, const 
 void check_window(const std::optional<int64_t>& window, int64_t sinks, double scale) {
   if (window && *window < 1) refuse("window ", *window, "; at least 1, or None");
   if (sinks < 0) refuse("sinks ", sinks);
-  if (!(scale > 0.0) || !(static_cast<float>(scale) > 0.f)) refuse("scale ", scale, " is not positive");
+  if (!(static_cast<float>(scale) > 0.f) || !std::isfinite(static_cast<float>(scale)))
+    refuse("scale ", scale, " is not a positive float");
 }
 
 // A paged cache: k_cache and v_cache [pages, page_size, Hkv, D], page_table int32
 // [B, pages of a sequence], lengths int32 [B].
 void check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, const Tensor& q) {
   if (k.sizes() != v.sizes()) refuse("cache shapes differ: ", shape(k), " ", shape(v));
-  if (!row_ready(k) || !row_ready(v))  // read and written in place: a copy would not be the cache
+  if (!rows_aligned(k) || !rows_aligned(v))  // read and written in place: a copy would not be the cache
     refuse("cache rows must be contiguous and 16-byte aligned, strides ", k.strides(), " ", v.strides());
   if (k.size(1) % 8 || k.size(1) == 0) refuse("page size ", k.size(1), " is not a multiple of 8");
   const int64_t B = q.size(0);
@@ -132,10 +135,15 @@ void check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Te
   check_int32(lengths, "lengths", {B}, q.device());
 }
 
-void refuse_grad(const char* what, std::initializer_list<Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return;
+bool wants_grad(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
   for (const auto& t : ts)
-    if (t.requires_grad()) refuse(what, " has no gradient; call it under torch.no_grad()");
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+void refuse_grad(const char* what, std::initializer_list<Tensor> ts) {
+  if (wants_grad(ts)) refuse(what, " has no gradient; call it under torch.no_grad()");
 }
 
 // backward() under create_graph=True would return gradients cut off from the graph.
@@ -189,10 +197,12 @@ RopePlan rope_plan(const Tensor& q, const OptTensor& qw, const OptTensor& kw, co
   RopePlan p;
   p.qw = weight_of(qw, "q_weight", q);
   p.kw = weight_of(kw, "k_weight", q);
+  if (!(eps >= 0.0) || !std::isfinite(static_cast<float>(eps))) refuse("eps ", eps, " is not a float from 0 on");
   p.eps = eps;
   p.interleaved = interleaved;
   if (!cos && !sin) return p;
   if (!cos || !sin) refuse("cos and sin go together");
+  if (wants_grad({*cos, *sin})) refuse("cos and sin have no gradient; detach them");
   if (cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->size(0) == 0)
     refuse("cos and sin must be [positions, pairs], got ", cos->sizes(), " ", sin->sizes());
   p.P = cos->size(0);
@@ -265,13 +275,6 @@ struct NormRope : torch::autograd::Function<NormRope> {
   }
 };
 
-bool wants_grad(std::initializer_list<Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const auto& t : ts)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
-}
-
 std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, const OptTensor& qw, const OptTensor& kw,
                                        const OptTensor& cos, const OptTensor& sin, double eps,
                                        const OptTensor& positions, bool interleaved) {
@@ -306,13 +309,16 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
                            const Tensor& v_cache, const Tensor& table0, const Tensor& lengths0, const OptTensor& qw,
                            const OptTensor& kw, const OptTensor& cos, const OptTensor& sin, double eps,
                            bool interleaved) {
-  refuse_grad("qk_norm_rope_append", {q0, k0, v0});
+  refuse_grad("qk_norm_rope_append", {q0, k0, v0, k_cache, v_cache, qw.value_or(Tensor()), kw.value_or(Tensor())});
   check_rows(q0, {{"k", k0}, {"v", v0}, {"k_cache", k_cache}, {"v_cache", v_cache}}, true);
   const int64_t B = q0.size(0), T = q0.size(1), H = q0.size(2), Hkv = k0.size(2);
   if (k0.size(0) != B || k0.size(1) != T || k0.sizes() != v0.sizes() || k_cache.size(2) != Hkv)
     refuse("shapes do not match: q ", shape(q0), " k ", shape(k0), " v ", shape(v0), " cache ", shape(k_cache));
   check_kv_heads(H, Hkv);
   check_cache(k_cache, v_cache, table0, lengths0, q0);
+  for (const Tensor& c : {k_cache, v_cache})
+    for (int d = 0; d < 3; ++d)
+      if (c.stride(d) == 0 && c.size(d) > 1) refuse("a cache to write to is expanded: strides ", c.strides());
   const RopePlan p = rope_plan(q0, qw, kw, cos, sin, eps, interleaved);
   const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0);
   const Tensor table = table0.size(1) > 1 && table0.stride(1) != 1 ? table0.contiguous() : table0;
@@ -330,6 +336,9 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
             none ? 0 : k_cache.size(0), k_cache.size(1), ptr_as<int32_t>(table), table.stride(0), table.size(1),
             ptr_as<int32_t>(lengths), stream_of(q)),
         "solattn_qk_norm_rope_append");
+  // (a backward pass that has kept the cache finds it changed)
+  for (const Tensor& c : {k_cache, v_cache})
+    if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
   return qo;
 }
 
@@ -386,8 +395,8 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
     const Tensor ws = workspace(lib.window_attn_bwd_workspace_bytes(B, Tq, Tk, H, Hkv, D, window, sinks, causal), q);
     check(lib.window_attn_bwd(ptr_as<U16>(q), STRIDES(q), ptr_as<U16>(k), STRIDES(k), ptr_as<U16>(v), STRIDES(v),
                               ptr_as<U16>(out), STRIDES(out), ptr_as<U16>(g), STRIDES(g), ptr_as<float>(lse),
-                              ptr_as<U16>(o_lo), B, Tq, Tk, H, Hkv, D, type_code(q), data["q_start"].toInt(), ptr_as<int32_t>(lengths), window, sinks,
-                              causal, static_cast<float>(data["scale"].toDouble()), ptr_as<U16>(dq), STRIDES(dq),
+                              ptr_as<U16>(o_lo), B, Tq, Tk, H, Hkv, D, type_code(q), data["q_start"].toInt(),
+                              ptr_as<int32_t>(lengths), window, sinks, causal, static_cast<float>(data["scale"].toDouble()), ptr_as<U16>(dq), STRIDES(dq),
                               ptr_as<U16>(dk), STRIDES(dk), ptr_as<U16>(dv), STRIDES(dv), ptr(ws),
                               ws.defined() ? ws.numel() : 0, stream_of(q)),
           "solattn_window_attn_bwd");

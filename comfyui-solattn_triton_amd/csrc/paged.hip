@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
 // as there may be 64 of them: one long sequence in a large batch is not left to one
 // workgroup a head.
 int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks) {
-  const int64_t keys = window && window + sinks < most ? window + sinks : most;
+  const int64_t keys = window && window < most && sinks < most - window ? window + sinks : most;
   const int64_t steps = cdiv(keys, kStep) + 1;
   int64_t n = cdiv(1024, B * Hkv * tiles);
   if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);

@@ -386,6 +386,7 @@ int setup(RopeArgs& a, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, 
   SOLATTN_REQUIRE(R >= 0 && R <= D && R % (interleaved ? 8 : 16) == 0, SOLATTN_EUNSUPPORTED,
                   "%s: %lld rotated channels of %lld (multiples of %d)", what, (long long)R, (long long)D,
                   interleaved ? 8 : 16);
+  SOLATTN_REQUIRE(eps >= 0.f, SOLATTN_EINVAL, "%s: eps %g", what, static_cast<double>(eps));
   SOLATTN_REQUIRE(R == 0 || (a.cos && a.sin && P > 0), SOLATTN_EINVAL, "%s: rotation without a table", what);
   const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   SOLATTN_REQUIRE(aligned(a.qw) && aligned(a.kw) && (R == 0 || (aligned(a.cos) && aligned(a.sin))), SOLATTN_EINVAL,

@@ -782,6 +782,8 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   if (single_token(Tq, causal, lse)) {
     SOLATTN_REQUIRE(window > 0 && q_start >= 0 && q_start < Tk, SOLATTN_EINVAL, "%s: row %lld of %lld keys, window %lld",
                     what, (long long)q_start, (long long)Tk, (long long)window);
+    if (window > Tk) window = Tk;
+    if (sinks > Tk) sinks = Tk;
     return paged_attn(q, sq_b, sq_h, k, sk_b, sk_t, sk_h, v, sv_b, sv_t, sv_h, B, q_start + 1, nullptr, 0, 1, lengths,
                       q_start + 1, B, H, Hkv, D, dtype, window, sinks, scale, workspace, workspace_bytes, o, so_b, so_h,
                       reinterpret_cast<hipStream_t>(stream), what);

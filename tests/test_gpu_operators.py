@@ -442,6 +442,59 @@ def test_refusals(rope, window, paged, dev):
     bad("match", rope.qk_norm_rope_append, q, q[:, :, :2], q[:, :, :2], c, c, t, n)
 
 
+def test_refusals_of_gradients_and_numbers(rope, window, paged, dev):
+    """Tensors whose gradient would be lost, caches that cannot be written, sizes that are no numbers."""
+    c = torch.zeros(3, 8, 4, 64, device=dev, dtype=BF)
+    q = torch.zeros(2, 1, 4, 64, device=dev, dtype=BF)
+    t = torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    n = torch.ones(2, dtype=torch.int32, device=dev)
+    cos, w = torch.zeros(8, 32, device=dev), torch.ones(64, device=dev)
+    leaf = lambda x: x.clone().requires_grad_(True)  # noqa: E731
+
+    def bad(match, f, *a, **kw):
+        with pytest.raises(ValueError, match=match):
+            f(*a, **kw)
+
+    bad("gradient", rope.qk_norm_rope, q, q, None, None, leaf(cos), cos)
+    bad("gradient", rope.qk_norm_rope_append, q, q, q, c, c, t, n, leaf(w), w)
+    bad("gradient", rope.qk_norm_rope_append, q, q, q, c, c, t, n, w, leaf(w))
+    bad("gradient", rope.qk_norm_rope_append, q, q, q, c, leaf(c), t, n)
+    bad("gradient", rope.qk_norm_rope_append, q, q, q, c, c, t, n, None, None, cos, leaf(cos))
+    bad("expanded", rope.qk_norm_rope_append, q, q, q, c[:1].expand(3, 8, 4, 64), c, t, n)
+    bad("expanded", rope.qk_norm_rope_append, q, q, q, c, c[:, :, :1].expand(3, 8, 4, 64), t, n)
+    for eps in (-1e-6, float("nan"), float("inf")):
+        bad("eps", rope.qk_norm_rope, q, q, eps=eps)
+    for scale in (float("nan"), float("inf"), 1e300, 1e-300, -1.0):
+        bad("scale", window.window_attn, q, q, q, window=4, scale=scale)
+        bad("scale", paged.paged_attn, q, c, c, t, n, scale=scale)
+    with torch.no_grad():  # nothing to lose
+        rope.qk_norm_rope(q, q, None, None, leaf(cos), cos)
+        rope.qk_norm_rope_append(q, q, q, c, leaf(c), t, n, leaf(w), leaf(w))
+
+
+def test_append_is_a_change_of_the_cache(rope, window, dev):
+    """A backward pass that kept the cache refuses to run on what an append made of it."""
+    c = torch.randn(1, 16, 2, 64, device=dev, dtype=BF)
+    x = torch.randn(1, 1, 2, 64, device=dev, dtype=BF)
+    q = torch.randn(1, 16, 2, 64, device=dev, dtype=BF, requires_grad=True)
+    t, n = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.full((1,), 16, dtype=torch.int32, device=dev)
+    out = window.window_attn(q, c, c.clone(), window=4)
+    rope.qk_norm_rope_append(x, x, x, c, c.clone(), t, n)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_cache_orders(paged, dev, dim):
+    """Pages, slots or heads outermost in memory: the cache is read where it lies."""
+    c = [torch.randn(5, 16, 2, 64, device=dev, dtype=BF) for _ in "kv"]
+    q = torch.randn(2, 1, 4, 64, device=dev, dtype=BF)
+    t = torch.tensor([[4, 0], [2, 3]], dtype=torch.int32, device=dev)
+    n = torch.tensor([31, 9], dtype=torch.int32, device=dev)
+    there = [x.transpose(0, dim).contiguous().transpose(0, dim) for x in c]
+    assert torch.equal(paged.paged_attn(q, *there, t, n), paged.paged_attn(q, *c, t, n))
+
+
 # --------------------------------------------------------------------- pages
 # lengths, page, H, Hkv, D, window, sinks, dtype
 PAGED = [

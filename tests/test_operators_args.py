@@ -164,3 +164,19 @@ def test_host_tensors_are_refused(pkg):
         mod("_qk_rope").qk_norm_rope_append(x[:, :1], x[:, :1], x[:, :1], x, x, t, n)
     with pytest.raises(TypeError):
         mod("_window").window_attn(x, x, x)  # the window has no default
+
+
+def test_wide_windows_and_eps(capi):
+    """Windows past every key are no limit in each entry; eps is from 0 on."""
+    L, top = capi.LIB, (1 << 62) + (1 << 61)
+    assert L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, top, top) == \
+        L.solattn_paged_attn_workspace_bytes(1, 24, 8, 128, 1000, 64, 0, 0)
+    one = L.solattn_window_attn_workspace_bytes(1, 1, 8192, 2, 1, 128, 8191, top, top, 1, 0)
+    assert one == L.solattn_window_attn_workspace_bytes(1, 1, 8192, 2, 1, 128, 8191, 8192, 0, 1, 0) > 0
+    # (the room is what is refused, not the window)
+    assert _window(L, Tq=1, Tk=8192, H=2, Hkv=1, q_start=8191, window=top, sinks=top, ws=A, ws_bytes=one - 1) == ESIZE
+    s = (1280, 128, 128)
+    for eps in (-1e-6, float("nan")):
+        assert L.solattn_qk_norm_rope(A, *s, A, *s, 1, 10, 1, 1, 128, 0, A, A, A, A, 10, 128, 0, None, 0, eps, A, *s, A, *s,
+                                      None) == EINVAL
+        assert b"eps" in L.solattn_last_error()
