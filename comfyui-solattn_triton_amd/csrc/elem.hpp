@@ -155,4 +155,22 @@ struct Row8<Fp32> {
   }
 };
 
+// Division by a number that the host knows: exact for n < 2^31 (mul = ceil(2^(31 + log2)
+// / d), an error below 2^-31 n; mul 0: a power of two).
+struct Divisor {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return mul ? __umulhi(n, mul) >> shift : n >> shift; }
+  __device__ __forceinline__ uint32_t split(uint32_t& n) const {  // n becomes n / d; returns the remainder
+    const uint32_t q = of(n), r = n - q * d;
+    n = q;
+    return r;
+  }
+};
+inline Divisor divisor(int64_t d) {
+  uint32_t log2 = 0;
+  while ((1ll << log2) < d) ++log2;
+  if ((1ll << log2) == d) return {static_cast<uint32_t>(d), 0, log2};
+  return {static_cast<uint32_t>(d), static_cast<uint32_t>(((1ull << (31 + log2)) + d - 1) / d), log2 - 1};
+}
+
 }  // namespace solattn

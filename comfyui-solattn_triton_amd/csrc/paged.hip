@@ -42,12 +42,13 @@ struct PagedArgs {
   const int32_t* lengths;    // with a table: each sequence's. Without: one shorter than `length` holds no token
                              // here, the others `length` keys (null: all of them)
   int length, pages, page, max_pages;
-  uint32_t page_mul, page_shift;  // j / page = umulhi(j, mul) >> shift  (mul 0: j >> shift)
+  Divisor by_page;
   uint16_t* o;
   int64_t so_b, so_h;
   float* part;               // split > 1: [B][H][split][D] sums, then [B][H][split][2] max and sum
   int64_t part_ml;           // where the latter begin
   int B, H, Hkv, D, group, tiles, split;
+  Divisor by_tiles, by_hkv, by_split;
   int window, sinks;         // window 0: none
   float c;                   // scale log2(e)
 };
@@ -103,17 +104,12 @@ paged_kernel(const PagedArgs a) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   uint32_t w = blockIdx.x;
-  const int tile = w % a.tiles;
-  w /= a.tiles;
-  const int hk = w % a.Hkv;
-  w /= a.Hkv;
-  const int split = w % a.split;
-  const int b = w / a.split;
+  const int tile = a.by_tiles.split(w), hk = a.by_hkv.split(w), split = a.by_split.split(w), b = w;
   const int ncol = min(kGroups, a.group - tile * kGroups);
   const int head0 = hk * a.group + tile * kGroups;
 
   const Visible vis = visible(a, b);
-  const int per = (vis.steps + a.split - 1) / a.split;
+  const int per = a.by_split.of(vis.steps + a.split - 1);
   const int step0 = split * per, step1 = min(step0 + per, vis.steps);
   if (step0 >= step1 && a.split > 1) {  // nothing here: the join passes over a sum of 0
     if (static_cast<int>(threadIdx.x) < ncol)
@@ -147,7 +143,7 @@ paged_kernel(const PagedArgs a) {
   // that a step waits for one round of memory, not two.
   const auto slot_of = [&](int j8, int& slot) __attribute__((always_inline)) {
     const uint32_t j = static_cast<uint32_t>(min(j8, max(vis.len - 1, 0) & ~7));
-    const uint32_t pg = a.page_mul ? __umulhi(j, a.page_mul) >> a.page_shift : j >> a.page_shift;
+    const uint32_t pg = a.by_page.of(j);
     slot = static_cast<int>(j - pg * a.page);
     return a.table ? a.table[b * a.table_b + pg] : b;
   };
@@ -373,13 +369,7 @@ int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k,
   a.table = table, a.table_b = table_stride;
   a.lengths = lengths, a.length = static_cast<int>(length);
   a.pages = static_cast<int>(pages), a.page = static_cast<int>(page_size), a.max_pages = static_cast<int>(max_pages);
-  int log2 = 0;
-  while ((1ll << log2) < page_size) ++log2;
-  a.page_shift = log2;
-  if ((1ll << log2) != page_size) {  // exact for j < 2^31: mul = ceil(2^(31 + log2) / page), its error below 2^-31 j
-    a.page_mul = static_cast<uint32_t>(((1ull << (31 + log2)) + page_size - 1) / page_size);
-    a.page_shift = log2 - 1;
-  }
+  a.by_page = divisor(page_size);
   a.o = o, a.so_b = so_b, a.so_h = so_h;
   a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.Hkv = static_cast<int>(Hkv), a.D = static_cast<int>(D);
   a.group = static_cast<int>(H / Hkv);
@@ -387,6 +377,7 @@ int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k,
   a.window = static_cast<int>(window), a.sinks = static_cast<int>(sinks);
   a.c = scale * kLog2e;
   a.split = splits(B, Hkv, a.tiles, max_pages * page_size, window, sinks);
+  a.by_tiles = divisor(a.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(a.split);
   const int64_t need = part_bytes(B, H, D, a.split);
   SOLATTN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SOLATTN_ESIZE,
                   "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes, (long long)need);

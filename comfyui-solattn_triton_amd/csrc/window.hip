@@ -39,15 +39,12 @@ constexpr float kNoMax = -1e30f;
 // window is wide, the last rows have the most keys.
 __device__ __forceinline__ void row_item(const WindowArgs& a, int& b, int& h, int& qb, int& part) {
   uint32_t w = xcd_item(a, blockIdx.x, gridDim.x);
-  part = w % a.split;
-  w /= a.split;
-  const int g = w % a.group;
-  w /= a.group;
-  qb = w % a.nqb;
+  part = a.by_split.split(w);
+  const int g = a.by_group.split(w);
+  qb = a.by_nqb.split(w);
   if (a.causal) qb = a.nqb - 1 - qb;
-  w /= a.nqb;
-  h = (w % a.Hkv) * a.group + g;
-  b = w / a.Hkv;
+  h = a.by_hkv.split(w) * a.group + g;
+  b = w;
 }
 
 // What the rows of this wave see (rows past Tq repeat the last).
@@ -153,7 +150,7 @@ window_fwd_kernel(const WindowArgs a) {
   const int p0 = a.q_start + r0, p1 = a.q_start + min(r0 + BLK, a.Tq) - 1;
   const KeyTiles kt = key_tiles(a, p0, p1, len);
   const RowKeys rk = row_keys(a, a.q_start + rr, len);
-  const int per = (kt.n + a.split - 1) / a.split, tile0 = min(part * per, kt.n);
+  const int per = a.by_split.of(kt.n + a.split - 1), tile0 = min(part * per, kt.n);
   const int ntiles = __builtin_amdgcn_readfirstlane(min(per, kt.n - tile0));
   const uint16_t* kp = a.k.p + b * a.k.b + hk * a.k.h;
   const uint16_t* vp = a.v.p + b * a.v.b + hk * a.v.h;
@@ -481,15 +478,16 @@ window_dq_kernel(const WindowArgs a) {
       const uint32_t at = (t & 1) * kBuf + m2 * (64 * D);
       f32x16 s, dp;
       two_scores<E, D, D == 64 ? 6 : 4>(s, dp, ka, at, q, va, at, g);
-      if (masked) mask_keys(s, rk, j0 + 32 * m2, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, neg));
         dp[r] = pr * (dp[r] - delta);
       }
-      if (masked)  // (a masked dp may be anything)
+      if (masked) {  // (what the row does not see may be anything up to here)
+        const uint32_t bits = key_bits(rk, j0 + 32 * m2, half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
+        for (int r = 0; r < 16; ++r) dp[r] = keep(dp[r], bit_word(bits, r));
+      }
       const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
       add_product<E, D, 3>(acc, ka, at, ds);
     }
@@ -522,7 +520,8 @@ window_dkv_kernel(const WindowArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = wave_id();
   uint32_t w = xcd_item(a, blockIdx.x, gridDim.x);
   const KeyPart kp = key_part(a, w);
-  const int hk = kp.bh % a.Hkv, b = kp.bh / a.Hkv;
+  uint32_t bh = kp.bh;
+  const int hk = a.by_hkv.split(bh), b = bh;
   const int len = sequence_length(a, b);
   const int j0 = kp.block * kRows, j = j0 + wave * 32 + (lane & 31), jj = min(j, a.Tk - 1);
   const KeyRows kr = key_rows(a, j < a.Tk ? j : len, len);
@@ -532,7 +531,7 @@ window_dkv_kernel(const WindowArgs a) {
   const int i0 = k0.pl - a.q_start, i1 = (j0 < a.sinks ? k0.ph : k1.ph) - a.q_start;  // rows [i0, i1]
   const int tile0 = i0 & ~(kKeys - 1);
   const int tiles = j0 < len && i0 <= i1 ? (i1 - tile0) / kKeys + 1 : 0;
-  const int per = (tiles * a.group + kp.parts - 1) / kp.parts;
+  const int per = (kp.block < a.nsb ? a.by_ks : a.by_kn).of(tiles * a.group + kp.parts - 1);
   const int s0 = min(kp.part * per, tiles * a.group), s1 = min(s0 + per, tiles * a.group);
   // rows that see every key of the wave, and those that see any (a step without is skipped)
   const KeysRows kw = keys_rows(a, j0 + wave * 32, j0 + wave * 32 + 31, len);
@@ -548,7 +547,7 @@ window_dkv_kernel(const WindowArgs a) {
 
   const uint32_t off_q = copy_offset<kThreads, D, kBoth>(a.q.t), off_g = copy_offset<kThreads, D, kBoth>(a.d_o.t);
   // The next step to copy: head g of the group, rows from t0 on.
-  int g = tiles ? s0 / tiles : 0, t0 = tiles ? tile0 + (s0 - g * tiles) * kKeys : 0;
+  int g = tiles ? static_cast<uint32_t>(s0) / static_cast<uint32_t>(tiles) : 0, t0 = tiles ? tile0 + (s0 - g * tiles) * kKeys : 0;
   const auto issue = [&](int buf) __attribute__((always_inline)) {
     const int h = hk * a.group + g;
     const uint16_t* qp = a.q.p + b * a.q.b + h * a.q.h;
@@ -601,14 +600,12 @@ window_dkv_kernel(const WindowArgs a) {
         asm volatile("" ::: "memory");  // (the next four's statistics are read behind these, not held with them)
       }
       if (masked) {  // (what a key does not see may be anything up to here)
-        const int off = a.q_start + r0 + 32 * m2 + 4 * half - kr.pl;
-        const uint32_t span = static_cast<uint32_t>(kr.ph - kr.pl);
-        const bool none = kr.ph < kr.pl;
+        const uint32_t bits = row_bits(kr, a.q_start + r0 + 32 * m2, half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const bool on = !none && static_cast<uint32_t>(off + 8 * (r >> 2) + (r & 3)) <= span;
-          s[r] = on ? s[r] : 0.f;
-          dp[r] = on ? dp[r] : 0.f;
+          const uint32_t w = bit_word(bits, r);
+          s[r] = keep(s[r], w);
+          dp[r] = keep(dp[r], w);
         }
       }
       const bf16x8 pb[2] = {pack8<E>(s, 0), pack8<E>(s, 1)};
@@ -691,6 +688,8 @@ void cut_keys(WindowArgs& a) {
   a.kn = static_cast<int>(kn);
   a.ks = static_cast<int>(ks);
   if (a.nsb == a.nkb) a.kn = a.ks;  // (only sinks' blocks)
+  a.by_ks = divisor(a.ks), a.by_kn = divisor(a.kn);
+  a.by_items = divisor(static_cast<int64_t>(a.nsb) * a.ks + static_cast<int64_t>(a.nkb - a.nsb) * a.kn);
   a.slots = (a.ks > 1 ? a.nsb * a.ks : 0) + (a.kn > 1 ? (a.nkb - a.nsb) * a.kn : 0);
 }
 
@@ -725,6 +724,7 @@ int setup(WindowArgs& a, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t H
   a.nqb = static_cast<int>(cdiv(Tq, kRows)), a.nkb = static_cast<int>(cdiv(Tk, kRows));
   a.split = 1;
   a.c = scale * kLog2e, a.scale = scale;
+  a.by_split = divisor(1), a.by_group = divisor(a.group), a.by_nqb = divisor(a.nqb), a.by_hkv = divisor(Hkv);
   SOLATTN_REQUIRE(B * H * a.nqb < (1ll << 31) && B * Hkv * a.nkb < (1ll << 31), SOLATTN_EUNSUPPORTED,
                   "%s: grid too large", what);
   return 0;
@@ -752,6 +752,7 @@ static int cut_rows(WindowArgs& a) {
   int64_t n = cdiv(1024, bh * a.nqb);
   if (n > tiles / 8) n = tiles / 8;
   a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+  a.by_split = divisor(a.split), a.by_nqb = divisor(a.nqb);
   return blk;
 }
 

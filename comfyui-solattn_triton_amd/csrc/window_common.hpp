@@ -36,6 +36,7 @@ struct WindowArgs {
   int nqb, nkb;              // blocks of rows and of keys
   int split;                 // forward: parts of a block's key tiles
   int nsb, ks, kn, slots;    // backward: blocks with sinks; parts of these and of the others; cut blocks' slots a head
+  Divisor by_split, by_group, by_nqb, by_hkv, by_items, by_ks, by_kn;  // by_items: parts of a head in the dk, dv launch
   float* part;               // backward: [B Hkv][slots][dk, dv][128][D]; forward: [B H][Tq][split][D]
   float* part_ml;            // forward: [B H][Tq][split][max, sum]
   float c, scale;            // c = scale log2(e)
@@ -168,16 +169,18 @@ struct KeyPart {
   int64_t slot;
 };
 __device__ __forceinline__ KeyPart key_part(const WindowArgs& a, uint32_t w) {
-  const int sink_items = a.nsb * a.ks, items = sink_items + (a.nkb - a.nsb) * a.kn;
+  const int sink_items = a.nsb * a.ks;
   KeyPart k;
-  k.bh = static_cast<int>(w / items);
-  const int n = static_cast<int>(w % items), i = n - (items - sink_items);
+  uint32_t n = a.by_items.split(w);
+  k.bh = static_cast<int>(w);
+  const int i = static_cast<int>(n) - (static_cast<int>(a.by_items.d) - sink_items);
   if (i >= 0) {  // sinks' parts last: they are the shorter ones
-    k.block = i / a.ks, k.part = i % a.ks, k.parts = a.ks;
     k.slot = static_cast<int64_t>(k.bh) * a.slots + i;
+    n = i;
+    k.part = a.by_ks.split(n), k.block = n, k.parts = a.ks;
   } else {
-    k.block = a.nsb + n / a.kn, k.part = n % a.kn, k.parts = a.kn;
     k.slot = static_cast<int64_t>(k.bh) * a.slots + sink_items + n;
+    k.part = a.by_kn.split(n), k.block = a.nsb + n, k.parts = a.kn;
   }
   return k;
 }
@@ -336,17 +339,33 @@ __device__ __forceinline__ void rounded_off(f32x16 (&acc)[ND], float f) {
     }
 }
 
+// Which of the 32 x 32 tile's elements of this lane count, as bits k (element r is k =
+// 8 (r / 4) + r % 4, so below 28): those of an interval are two shifts, and an element's
+// bit drawn out to a word keeps or clears it without a compare.
+__device__ __forceinline__ uint32_t bits_from(int k) { return ~0u << min(max(k, 0), 28); }
+__device__ __forceinline__ uint32_t bit_word(uint32_t bits, int r) {
+  return static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, 8 * (r >> 2) + (r & 3), 1));
+}
+__device__ __forceinline__ float keep(float x, uint32_t word) { return __uint_as_float(__float_as_uint(x) & word); }
+
+// Bits of the keys first + 4 half + k that the row sees.
+__device__ __forceinline__ uint32_t key_bits(const RowKeys& rk, int first, int half) {
+  const int base = first + 4 * half;
+  return (bits_from(rk.jl - base) & ~bits_from(rk.jh + 1 - base)) | ~bits_from(rk.sk - base);
+}
+// Bits of the rows first + 4 half + k that see the key.
+__device__ __forceinline__ uint32_t row_bits(const KeyRows& kr, int first, int half) {
+  const int base = first + 4 * half;
+  return bits_from(kr.pl - base) & ~bits_from(kr.ph + 1 - base);
+}
+
 // Scores of 32 keys (first + the key of element r) for this lane's row: those it does not see become -inf.
 __device__ __forceinline__ void mask_keys(f32x16& s, const RowKeys& rk, int first, int half) {
-  const int base = first + 4 * half;
-  const uint32_t span = static_cast<uint32_t>(rk.jh - rk.jl);
-  const int off = base - rk.jl, sk = rk.sk - base;
-  const bool none = rk.jh < rk.jl;
+  const uint32_t bits = key_bits(rk, first, half);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int k0 = 8 * (r >> 2) + (r & 3);
-    const bool on = (!none && static_cast<uint32_t>(off + k0) <= span) || k0 < sk;
-    s[r] = on ? s[r] : -INFINITY;
+    const uint32_t w = bit_word(bits, r);
+    s[r] = __uint_as_float((__float_as_uint(s[r]) & w) | (__float_as_uint(-INFINITY) & ~w));
   }
 }
 
