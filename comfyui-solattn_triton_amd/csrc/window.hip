@@ -616,14 +616,18 @@ window_dkv_kernel(const WindowArgs a) {
   }
   mfma_fence(dk);
   mfma_fence(dv);
+  // (the lane asked for again: at 128 channels no register is left to hold it through the loop)
+  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), hf = ln >> 5;
+  const int key = wave * 32 + (ln & 31);
   if (kp.parts == 1) {
-    const bool on = j < a.Tk;
-    store_row<E>(dk, a.scale, a.dk + b * a.dk_b + static_cast<int64_t>(j) * a.dk_t + hk * a.dk_h, on, half);
-    store_row<E>(dv, 1.f, a.dv + b * a.dv_b + static_cast<int64_t>(j) * a.dv_t + hk * a.dv_h, on, half);
+    const int64_t at = j0 + key;
+    const bool on = at < a.Tk;
+    store_row<E>(dk, a.scale, a.dk + b * a.dk_b + at * a.dk_t + hk * a.dk_h, on, hf);
+    store_row<E>(dv, 1.f, a.dv + b * a.dv_b + at * a.dv_t + hk * a.dv_h, on, hf);
     return;
   }
   // [dk, dv][key][channel]: a lane has 4 consecutive channels of its key at a time
-  float* part = a.part + static_cast<int64_t>(kp.slot) * (2 * kRows * D) + (wave * 32 + (lane & 31)) * D + 4 * half;
+  float* part = a.part + static_cast<int64_t>(kp.slot) * (2 * kRows * D) + key * D + 4 * hf;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -739,13 +743,15 @@ using namespace solattn;
 static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq == 1 && causal && !lse; }
 
 // Rows of a workgroup and parts of their keys. 128 rows share the copies of a tile
-// among four waves; launches that would not give every CU two such workgroups take
-// 64 rows, and where these do not give every CU four, their key tiles are cut into parts
-// of at least eight tiles, joined by a second launch (517 rows against 16000 keys: 105
-// us with two for every CU, 77 with four, 86 with eight).
+// among four waves (16000 tokens: 668 us against 710 with 64 rows). Launches that would
+// not give every CU four such workgroups take 64 rows, which leave fewer CUs idle at
+// the end (3900 tokens of 32 heads, 992 workgroups: 173 -> 132 us; 1128 of them: 199
+// against 211), and where these do not give every CU four, their key tiles are cut into
+// parts of at least eight tiles, joined by a second launch (517 rows against 16000
+// keys: 105 us with two for every CU, 77 with four, 86 with eight).
 static int cut_rows(WindowArgs& a) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
-  const int blk = bh * cdiv(a.Tq, 128) >= 512 ? 128 : 64;
+  const int blk = bh * cdiv(a.Tq, 128) >= 1024 ? 128 : 64;
   a.nqb = static_cast<int>(cdiv(a.Tq, blk));
   const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
   const int64_t tiles = cdiv(reach < a.Tk ? reach : a.Tk, kKeys);

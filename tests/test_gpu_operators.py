@@ -287,6 +287,24 @@ def test_window_gradients(window, dev, case):
         assert torch.equal(x, y)
 
 
+# As WINDOW, enough heads for the forward's workgroups of 128 rows.
+MANY_HEADS = [
+    (8, 257, 320, 48, 8, 64, 90, 70, True, [320, 0, 63, 64, 200, 319, 190, 256], BF),
+    (4, 600, 600, 60, 20, 128, 200, 5, False, None, FP),
+    (2, 1400, 1400, 52, 4, 64, 300, 130, True, None, FP),
+    (16, 130, 500, 40, 8, 128, None, 0, True, [500] * 15 + [431], BF),
+    (3, 500, 500, 96, 8, 64, 64, 200, False, [500, 301, 12], BF),
+    (1, 1030, 1030, 128, 4, 128, 450, 64, True, None, BF),
+]
+
+
+@pytest.mark.parametrize("case", MANY_HEADS, ids=[str(i) for i in range(len(MANY_HEADS))])
+def test_window_many_heads(window, dev, case):
+    assert case[0] * case[3] * -(-case[1] // 128) >= 1024
+    test_window(window, dev, case)
+    test_window_gradients(window, dev, case)
+
+
 def test_window_gradients_against_differences(window, dev):
     """Along a direction, the float64 form's differences against the kernels' gradients."""
     c = (1, 150, 150, 4, 2, 64, 60, 3, True, None, FP)
