@@ -155,6 +155,17 @@ struct Row8<Fp32> {
   }
 };
 
+// Asks for every 64-byte line of a kernel's arguments at once: left to their first uses,
+// they come one after the other, each a round trip to memory that the host has just written.
+template <typename A>
+__device__ __forceinline__ void fetch_arguments(const A& a) {
+  constexpr int N = sizeof(A) / 4;
+  uint32_t w[N];
+  __builtin_memcpy(w, &a, N * 4);
+#pragma unroll
+  for (int i = 0; i < N; i += 16) asm volatile("" ::"s"(w[i]));
+}
+
 // Division by a number that the host knows: exact for n < 2^31 (mul = ceil(2^(31 + log2)
 // / d), an error below 2^-31 n; mul 0: a power of two).
 struct Divisor {

@@ -101,6 +101,7 @@ paged_kernel(const PagedArgs a) {
   __shared__ float lds_o[kWaves][kGroups][DP + 4];
   __shared__ float lds_m[kWaves][kGroups], lds_l[kWaves][kGroups];
 
+  fetch_arguments(a);
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   uint32_t w = blockIdx.x;
@@ -312,16 +313,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     *reinterpret_cast<uint32_t*>(a.o + (row / a.H) * a.so_b + (row % a.H) * a.so_h + ch) = E::pack(o0 * inv, o1 * inv);
 }
 
-// Splits of a sequence: four workgroups for every CU, so that ragged sequences even
-// out, of at least a step a wave as long as the longest sequence allows. (Two for
-// every CU: 32 ragged sequences of up to 16384 keys 83 -> 60 us, four of 131072
-// 281 -> 250; eight and sixteen: 61 and 58, 258 and 258.) No split is longer than 4096 keys as far
-// as there may be 64 of them: one long sequence in a large batch is not left to one
-// workgroup a head.
+// Splits of a sequence: as many as leave the launch within four workgroups a CU, eight
+// in a batch of sixteen or more, whose sequences are rarely of one length; of at least a
+// step a wave as long as the longest sequence allows. (Within four against one more
+// split: three sequences of 32768 keys 84 -> 81 us, five 138 -> 127. Within eight against four: 32
+// ragged sequences of up to 16384 keys 61 -> 56, 72 of up to 4096 156 -> 134; 96 of
+// 4096 each 275 -> 284. Four of 32768 to 131072: within two 281, four 250, eight 258.)
+// No split is longer than 4096 keys as far as there may be 64 of them: one long sequence
+// in a large batch is not left to one workgroup a head.
 int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks) {
   const int64_t keys = window && window < most && sinks < most - window ? window + sinks : most;
   const int64_t steps = cdiv(keys, kStep) + 1;
-  int64_t n = cdiv(1024, B * Hkv * tiles);
+  int64_t n = (B < 16 ? 1024 : 2048) / (B * Hkv * tiles);
   if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);
   if (n > steps / kWaves) n = steps / kWaves;
   if (n > kMaxSplits) n = kMaxSplits;

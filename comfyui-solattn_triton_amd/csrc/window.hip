@@ -142,6 +142,7 @@ window_fwd_kernel(const WindowArgs a) {
   constexpr uint32_t kHalf = kKeys * D;  // bytes of half a tile
   __shared__ __align__(256) uint16_t kbuf[kKeys * D];
   __shared__ __align__(256) uint16_t vbuf[kKeys * D];
+  fetch_arguments(a);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   int b, h, qb, part;
   row_item(a, b, h, qb, part);
@@ -408,6 +409,7 @@ window_dq_kernel(const WindowArgs a) {
   constexpr uint32_t kBuf = kKeys * D * 2;  // bytes of a tile
   __shared__ __align__(256) uint16_t kbuf[2 * kKeys * D];
   __shared__ __align__(256) uint16_t vbuf[2 * kKeys * D];
+  fetch_arguments(a);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   int b, h, qb, part;
   row_item(a, b, h, qb, part);
@@ -517,6 +519,7 @@ window_dkv_kernel(const WindowArgs a) {
   __shared__ __align__(256) uint16_t qbuf[2 * kKeys * D];
   __shared__ __align__(256) uint16_t gbuf[2 * kKeys * D];
   __shared__ __align__(16) float stat[2][2][kKeys];  // [buffer][lse, delta]
+  fetch_arguments(a);
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = wave_id();
   uint32_t w = xcd_item(a, blockIdx.x, gridDim.x);
   const KeyPart kp = key_part(a, w);
@@ -671,16 +674,17 @@ __global__ void __launch_bounds__(256) window_dkv_join_kernel(const WindowArgs a
 }
 
 // How the key blocks of the backward are cut (WindowArgs::nsb, ks, kn, slots): the
-// sinks' blocks into parts no longer than another block, and every block further
-// where the launch would leave the CUs' two workgroups each empty, as long as a
-// part keeps eight steps.
+// sinks' blocks into parts no longer than another block, and every block into as many
+// as leave the launch within the CUs' two workgroups each (one more, and the last wait
+// for a second round: 6000 tokens of 8 heads, backward: 183 us as it is, 209 with one
+// more), as long as a part keeps eight steps.
 void cut_keys(WindowArgs& a) {
   const int64_t tiles_all = cdiv(a.Tq, kKeys) + 1;
   int64_t tiles = cdiv(static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + kRows, kKeys) + 1;
   if (tiles > tiles_all) tiles = tiles_all;
   const int64_t steps = tiles * a.group;
   a.nsb = static_cast<int>(cdiv(a.sinks, kRows));
-  int64_t kn = cdiv(512, static_cast<int64_t>(a.B) * a.Hkv * a.nkb);
+  int64_t kn = 512 / (static_cast<int64_t>(a.B) * a.Hkv * a.nkb);
   if (kn > steps / 8) kn = steps / 8;
   if (kn < 1) kn = 1;
   // (a block with few sinks keeps one wave busy: its parts are last and a quarter as long,
@@ -746,16 +750,19 @@ static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq =
 // among four waves (16000 tokens: 668 us against 710 with 64 rows). Launches that would
 // not give every CU four such workgroups take 64 rows, which leave fewer CUs idle at
 // the end (3900 tokens of 32 heads, 992 workgroups: 173 -> 132 us; 1128 of them: 199
-// against 211), and where these do not give every CU four, their key tiles are cut into
-// parts of at least eight tiles, joined by a second launch (517 rows against 16000
-// keys: 105 us with two for every CU, 77 with four, 86 with eight).
-static int cut_rows(WindowArgs& a) {
+// against 211). Their key tiles are cut into as many parts, of at least eight tiles and
+// joined by a second launch, as leave the launch within four workgroups a CU (256 rows
+// of 24 heads against 32000 keys: ten parts 113 us, eleven, which take a second round,
+// 143). In a padded batch, whose sequences may be short or empty, within eight (517
+// rows against 16000 keys, one of two sequences past its end: 44 us; within four 54).
+// padded: for a workspace, which has to do with lengths and without.
+static int cut_rows(WindowArgs& a, bool padded) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
   const int blk = bh * cdiv(a.Tq, 128) >= 1024 ? 128 : 64;
   a.nqb = static_cast<int>(cdiv(a.Tq, blk));
   const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
   const int64_t tiles = cdiv(reach < a.Tk ? reach : a.Tk, kKeys);
-  int64_t n = cdiv(1024, bh * a.nqb);
+  int64_t n = (padded ? 2048 : 1024) / (bh * a.nqb);
   if (n > tiles / 8) n = tiles / 8;
   a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
   a.by_split = divisor(a.split), a.by_nqb = divisor(a.nqb);
@@ -773,7 +780,7 @@ extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, in
   if (Tq == 1 && causal && !with_lse) return paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks);
   WindowArgs a{};
   if (setup(a, B, Tq, Tk, H, Hkv, D, SOLATTN_BF16, q_start, window, sinks, causal, 1.f, "window_attn")) return 0;
-  cut_rows(a);
+  cut_rows(a, true);
   return fwd_workspace(a, D);
 }
 
@@ -807,7 +814,7 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   if (rc) return rc;
   SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(o_lo) % 16 == 0, SOLATTN_EINVAL, "%s: o_lo must be 16-byte aligned", what);
   const bool bf = dtype == SOLATTN_BF16;
-  const int blk = cut_rows(a);
+  const int blk = cut_rows(a, lengths != nullptr);
   const int64_t need = fwd_workspace(a, D);
   SOLATTN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SOLATTN_ESIZE, "%s: workspace %lld < %lld bytes",
                   what, (long long)workspace_bytes, (long long)need);

@@ -430,8 +430,9 @@ int solattn_qk_norm_rope_bwd(
  * are never read; what k holds at a key reaches the rows that see it only, but a
  * NaN or infinity in v (backward: also in k, q, do) can reach rows that do not see
  * it within the same 128 rows.
- * workspace: 256-byte aligned, of the size below (0: may be null): short launches run
- * split over the keys, one causal row per sequence without lse as solattn_paged_attn. */
+ * workspace: 256-byte aligned, of the size below (0: may be null; enough with and
+ * without lengths): short launches run split over the keys, one causal row per sequence
+ * without lse as solattn_paged_attn. */
 int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
                                             int64_t D, int64_t q_start, int64_t window, int64_t sinks,
                                             int causal, int with_lse);
