@@ -344,7 +344,9 @@ __device__ __forceinline__ void rounded_off(f32x16 (&acc)[ND], float f) {
 // bit drawn out to a word keeps or clears it without a compare.
 __device__ __forceinline__ uint32_t bits_from(int k) { return ~0u << min(max(k, 0), 28); }
 __device__ __forceinline__ uint32_t bit_word(uint32_t bits, int r) {
-  return static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, 8 * (r >> 2) + (r & 3), 1));
+  uint32_t w;  // (hidden from the optimiser, which would go back to compares)
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(w) : "v"(bits), "i"(8 * (r >> 2) + (r & 3)));
+  return w;
 }
 __device__ __forceinline__ float keep(float x, uint32_t word) { return __uint_as_float(__float_as_uint(x) & word); }
 
