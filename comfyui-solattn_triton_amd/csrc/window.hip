@@ -379,9 +379,11 @@ __device__ __forceinline__ void two_scores(f32x16& s, f32x16& t, const AX& x, ui
   asm volatile("s_nop 7\n\ts_nop 7" : "+v"(s), "+v"(t));  // readers of s and t come after their wait states
 }
 
-// acc += X^T W for the 32 rows at x, read transposed; w: W's two packed operands.
-template <typename E, int D, int AHEAD, typename AX>
-__device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, uint32_t at, const bf16x8 (&w)[2]) {
+// acc += X^T W for the 32 rows at x, read transposed; w: W's packed operands, in one
+// rounding or the two of pack_all, which share the reads.
+template <typename E, int D, int AHEAD, int NW, typename AX>
+__device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, uint32_t at,
+                                            const bf16x8 (&w)[NW][2]) {
   constexpr int ND = D / 32, N = 2 * ND, R = AHEAD + 1;
   bf16x8 r[R];
   __builtin_amdgcn_s_setprio(1);
@@ -394,7 +396,8 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, 
       r[(i + AHEAD) % R] = x.transposed((i + AHEAD) / ND, (i + AHEAD) % ND, at);
       asm volatile("" ::: "memory");
     }
-    E::amfma_after_valu(acc[i % ND], r[i % R], w[i / ND]);
+#pragma unroll
+    for (int n = 0; n < NW; ++n) E::amfma_after_valu(acc[i % ND], r[i % R], w[n][i / ND]);
   }
   __builtin_amdgcn_s_setprio(0);
 }
@@ -402,7 +405,7 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[D / 32], const AX& x, 
 // dq, a block of rows at a time as the forward; D_i on the way, for the other kernel.
 // (The softmax work between the products of the next half, as the forward has it, with
 // four half buffers and a barrier for each: 191 -> 208 us at 8192 tokens.)
-template <typename E, int D>
+template <typename E, int D, int NW>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dq_kernel(const WindowArgs a) {
   constexpr int ND = D / 32, NC = D / 16;
@@ -490,7 +493,8 @@ window_dq_kernel(const WindowArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = keep(dp[r], bit_word(bits, r));
       }
-      const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
+      bf16x8 ds[NW][2];
+      pack_all<E>(ds, dp);
       add_product<E, D, 3>(acc, ka, at, ds);
     }
   }
@@ -510,11 +514,11 @@ window_dq_kernel(const WindowArgs a) {
 // the sinks, and few or short heads leave CUs without a block. A part's sums go to
 // the workspace in fp32 and window_dkv_join_kernel adds them up in order; a block
 // of one part is stored straight.
-template <typename E, int D>
+template <typename E, int D, int NW>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 window_dkv_kernel(const WindowArgs a) {
   constexpr int ND = D / 32, NC = D / 16;
-  constexpr int kAhead = D == 64 ? 3 : 2;  // (what the registers leave: 3 at 128 channels spills)
+  constexpr int kAhead = D == 64 ? 3 : NW == 1 ? 2 : 1;  // (what the registers leave: one more at 128 channels spills)
   constexpr uint32_t kBuf = kKeys * D * 2;  // bytes of a tile
   __shared__ __align__(256) uint16_t qbuf[2 * kKeys * D];
   __shared__ __align__(256) uint16_t gbuf[2 * kKeys * D];
@@ -527,7 +531,13 @@ window_dkv_kernel(const WindowArgs a) {
   const int hk = a.by_hkv.split(bh), b = bh;
   const int len = sequence_length(a, b);
   const int j0 = kp.block * kRows, j = j0 + wave * 32 + (lane & 31), jj = min(j, a.Tk - 1);
-  const KeyRows kr = key_rows(a, j < a.Tk ? j : len, len);
+  // (the lane asked for again where it is needed: at 128 channels no register is left to
+  // hold it or what follows from it through the loop)
+  const auto lane_again = []() __attribute__((always_inline)) {
+    int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(ln));
+    return ln;
+  };
   // rows that see a key of the block: a key's interval moves up with it, but that a sink's has no end
   const int jlast = min(min(j0 + kRows, a.Tk), len) - 1;
   const KeyRows k0 = key_rows(a, j0, len), k1 = key_rows(a, max(jlast, j0), len);
@@ -603,7 +613,8 @@ window_dkv_kernel(const WindowArgs a) {
         asm volatile("" ::: "memory");  // (the next four's statistics are read behind these, not held with them)
       }
       if (masked) {  // (what a key does not see may be anything up to here)
-        const uint32_t bits = row_bits(kr, a.q_start + r0 + 32 * m2, half);
+        const int ln = lane_again();  // (a key past the last is past the sequence)
+        const uint32_t bits = row_bits(key_rows(a, j0 + wave * 32 + (ln & 31), len), a.q_start + r0 + 32 * m2, ln >> 5);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const uint32_t w = bit_word(bits, r);
@@ -611,16 +622,17 @@ window_dkv_kernel(const WindowArgs a) {
           dp[r] = keep(dp[r], w);
         }
       }
-      const bf16x8 pb[2] = {pack8<E>(s, 0), pack8<E>(s, 1)};
-      const bf16x8 ds[2] = {pack8<E>(dp, 0), pack8<E>(dp, 1)};
+      bf16x8 pb[NW][2], ds[NW][2];
+      pack_all<E>(pb, s);
+      if constexpr (NW == 1) pack_all<E>(ds, dp);
       add_product<E, D, kAhead>(dv, qa, at + to_g, pb);
+      if constexpr (NW == 2) pack_all<E>(ds, dp);  // (not held through the other product)
       add_product<E, D, kAhead>(dk, qa, at, ds);
     }
   }
   mfma_fence(dk);
   mfma_fence(dv);
-  // (the lane asked for again: at 128 channels no register is left to hold it through the loop)
-  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), hf = ln >> 5;
+  const int ln = lane_again(), hf = ln >> 5;
   const int key = wave * 32 + (ln & 31);
   if (kp.parts == 1) {
     const int64_t at = j0 + key;
@@ -892,12 +904,22 @@ extern "C" int solattn_window_attn_bwd(
   SOLATTN_REQUIRE(items < (1ll << 31) && join < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf = dtype == SOLATTN_BF16;
-  const auto kq = D == 128 ? (bf ? window_dq_kernel<Bf16, 128> : window_dq_kernel<Fp16, 128>)
-                           : (bf ? window_dq_kernel<Bf16, 64> : window_dq_kernel<Fp16, 64>);
+  // P and dS in two roundings where rows see few keys: the fewer, the more of dq and dk
+  // cancels, but not of the errors of one rounding (up to 512 keys these took dq to 1.45 to
+  // 1.65 times the error of exact values rounded once, two to 1.02 to 1.2). From 512 keys on 1.42
+  // to 1.49, and the products of the second rounding would take 8192 tokens 540 -> 607 us.
+  const int64_t seen = (causal ? a.window : 2 * static_cast<int64_t>(a.window) - 1) + a.sinks;
+  const bool two = (seen < Tk ? seen : Tk) < 512;
+  const auto kq = D == 128 ? (bf ? (two ? window_dq_kernel<Bf16, 128, 2> : window_dq_kernel<Bf16, 128, 1>)
+                                 : (two ? window_dq_kernel<Fp16, 128, 2> : window_dq_kernel<Fp16, 128, 1>))
+                           : (bf ? (two ? window_dq_kernel<Bf16, 64, 2> : window_dq_kernel<Bf16, 64, 1>)
+                                 : (two ? window_dq_kernel<Fp16, 64, 2> : window_dq_kernel<Fp16, 64, 1>));
   hipLaunchKernelGGL(kq, dim3(static_cast<uint32_t>(B * H * a.nqb)), dim3(kThreads), 0, s, a);
   if ((rc = check_launch(what))) return rc;
-  const auto kk = D == 128 ? (bf ? window_dkv_kernel<Bf16, 128> : window_dkv_kernel<Fp16, 128>)
-                           : (bf ? window_dkv_kernel<Bf16, 64> : window_dkv_kernel<Fp16, 64>);
+  const auto kk = D == 128 ? (bf ? (two ? window_dkv_kernel<Bf16, 128, 2> : window_dkv_kernel<Bf16, 128, 1>)
+                                 : (two ? window_dkv_kernel<Fp16, 128, 2> : window_dkv_kernel<Fp16, 128, 1>))
+                           : (bf ? (two ? window_dkv_kernel<Bf16, 64, 2> : window_dkv_kernel<Bf16, 64, 1>)
+                                 : (two ? window_dkv_kernel<Fp16, 64, 2> : window_dkv_kernel<Fp16, 64, 1>));
   hipLaunchKernelGGL(kk, dim3(static_cast<uint32_t>(items)), dim3(kThreads), 0, s, a);
   if ((rc = check_launch(what)) || cut == 0) return rc;
   const auto kj = D == 128 ? (bf ? window_dkv_join_kernel<Bf16, 128> : window_dkv_join_kernel<Fp16, 128>)

@@ -299,6 +299,29 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& s, int ks) {
   return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
+// Elements of an accumulator as B operands: in one rounding, or in two that add up to
+// the value but for some 2^-17 of it (bf16; fp16: 2^-22).
+template <typename E, int NW>
+__device__ __forceinline__ void pack_all(bf16x8 (&w)[NW][2], const f32x16& s) {
+  if constexpr (NW == 1) {
+    w[0][0] = pack8<E>(s, 0);
+    w[0][1] = pack8<E>(s, 1);
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      uint32_t u[4], v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = s[8 * ks + 2 * i], y = s[8 * ks + 2 * i + 1];
+        u[i] = E::pack(x, y);
+        v[i] = E::pack(x - E::lo(u[i]), y - E::hi(u[i]));
+      }
+      w[0][ks] = __builtin_bit_cast(bf16x8, make_uint4(u[0], u[1], u[2], u[3]));
+      w[1][ks] = __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3]));
+    }
+  }
+}
+
 // acc^T (channel 32 dt + 8 (r / 4) + 4 half + r % 4 of row `lane % 32`) times f into a row of D values.
 template <typename E, int ND>
 __device__ __forceinline__ void store_row(const f32x16 (&acc)[ND], float f, uint16_t* row, bool on, int half) {

@@ -287,6 +287,25 @@ def test_window_gradients(window, dev, case):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D,T,w,sinks,causal", [(64, 700, 22, 1, False), (128, 900, 36, 4, True), (80, 300, 250, 0, True)])
+def test_window_gradients_of_few_keys(window, dev, D, T, w, sinks, causal, dtype):
+    """Where rows see few keys, P and dS keep what their rounding takes away: what is left
+    is D_i (its o in two roundings), fp32 sums and the outputs' own rounding, whose error
+    alone is 1 here. Independent errors add up in squares: 1.25 leaves 0.75 of it for
+    the others; one rounding of dS as large as the outputs' would give 1.41 or more."""
+    c = (1, T, T, 4, 2, D, w, sinks, causal, None, dtype)
+    q, k, v, n, on, kw = window_case(c, dev, seed=120)
+    do = randn(q.shape, 130, dev, dtype)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    got = torch.autograd.grad(window.window_attn(q, k, v, scale=0.11, **kw), (q, k, v), do)
+    want, _ = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.11, do, dtype)
+    for name, g, x in zip(("dq", "dk", "dv"), got, want):
+        ideal = (x.to(dtype).double() - x).norm()
+        assert (g.double() - x).norm() <= 1.25 * ideal, (name, ((g.double() - x).norm() / ideal).item())
+
+
 # As WINDOW, enough heads for the forward's workgroups of 128 rows.
 MANY_HEADS = [
     (8, 257, 320, 48, 8, 64, 90, 70, True, [320, 0, 63, 64, 200, 319, 190, 256], BF),
