@@ -11,14 +11,15 @@
 // instructions: 3770 against 4100 cycles for 64 rows of the dk, dv kernel, 1080 against
 // 1020 for the forward's 32 keys), then the exps and the power limit; short sequences
 // are bound by the latency of a step. 16001 tokens, window 4096, 24 heads of 128 over
-// 8: 657-671 us, 1050-1070 TFLOP/s; 12133 tokens, symmetric window 2401, 1333 sinks:
-// 720-730 us, 1090-1100 TFLOP/s; 8192 tokens, window 1024, with gradients: 555-600 us
-// (forward 130-145, dq 185-205, dk and dv 225-245, join 7); 2000 tokens of 16 heads of
-// 64, batch 2, window 512, with gradients: 92 us (26, 31, 34, 6).
+// 8: 663-704 us, 1000-1060 TFLOP/s; 12133 tokens, symmetric window 2401, 1333 sinks:
+// 724-765 us, 1040-1100 TFLOP/s; 8192 tokens, window 1024, with gradients: 534-574 us
+// (forward 133-143, dq 179-196, dk and dv 221-240, join 8); 2000 tokens of 16 heads of
+// 64, batch 2, window 512, with gradients: 82-84 us (23, 29, 33, 6).
 // Everything between the products stays in registers: S^T = K Q^T puts a row on a lane column, so its
 // statistics need one exchange (lanes 32 apart) and P converts in place into the B
 // operand of the next product, whose A operand is read transposed from LDS
-// (ds_read_b64_tr_b16). P and dS are rounded to the inputs' type for the matrix
+// (ds_read_b64_tr_b16). P and dS are rounded to the inputs' type (in the
+// gradients of short windows twice: the value and what that left) for the matrix
 // instruction; row sums add P as rounded, every other sum is fp32.
 #include <type_traits>
 
@@ -904,12 +905,14 @@ extern "C" int solattn_window_attn_bwd(
   SOLATTN_REQUIRE(items < (1ll << 31) && join < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf = dtype == SOLATTN_BF16;
-  // P and dS in two roundings where rows see few keys: the fewer, the more of dq and dk
-  // cancels, but not of the errors of one rounding (up to 512 keys these took dq to 1.45 to
-  // 1.65 times the error of exact values rounded once, two to 1.02 to 1.2). From 512 keys on 1.42
-  // to 1.49, and the products of the second rounding would take 8192 tokens 540 -> 607 us.
+  // P and dS in two roundings where rows see few keys or few rows see a key: the fewer, the
+  // more of dq and dk cancels, but not of the errors of one rounding (these took dq to
+  // 1.45 to 1.65 times the error of exact values rounded once, two to 1.02 to 1.2). From
+  // windows of 512 keys, 1024 keys and 128 rows on it is 1.42 to 1.49, and the products
+  // of the second rounding would take 8192 tokens 540 -> 607 us, 2000 of 64 channels
+  // 83 -> 93.
   const int64_t seen = (causal ? a.window : 2 * static_cast<int64_t>(a.window) - 1) + a.sinks;
-  const bool two = (seen < Tk ? seen : Tk) < 512;
+  const bool two = seen < 512 || Tk < 1024 || Tq < 128;
   const auto kq = D == 128 ? (bf ? (two ? window_dq_kernel<Bf16, 128, 2> : window_dq_kernel<Bf16, 128, 1>)
                                  : (two ? window_dq_kernel<Fp16, 128, 2> : window_dq_kernel<Fp16, 128, 1>))
                            : (bf ? (two ? window_dq_kernel<Bf16, 64, 2> : window_dq_kernel<Bf16, 64, 1>)
