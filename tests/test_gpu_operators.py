@@ -287,6 +287,22 @@ def test_window_gradients(window, dev, case):
         assert torch.equal(x, y)
 
 
+# As WINDOW, windows and sequences whose gradients round P and dS once.
+LONG = [
+    (2, 1300, 1300, 4, 2, 64, 400, 30, False, [1300, 700], FP),
+    (2, 1500, 1500, 4, 2, 128, 600, 4, True, [1500, 1], BF),
+    (1, 1029, 2051, 6, 1, 64, 900, 200, True, None, BF),
+    (1, 1111, 1111, 2, 2, 128, 300, 513, False, None, FP),
+    (2, 128, 1024, 3, 3, 96, 511, 1, True, [1024, 960], BF),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=[str(i) for i in range(len(LONG))])
+def test_window_long(window, dev, case):
+    test_window(window, dev, case)
+    test_window_gradients(window, dev, case)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("D,T,w,sinks,causal", [(64, 700, 22, 1, False), (128, 900, 36, 4, True), (80, 300, 250, 0, True)])
 def test_window_gradients_of_few_keys(window, dev, D, T, w, sinks, causal, dtype):
