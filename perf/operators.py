@@ -27,17 +27,11 @@ own = False
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
-_modules = {}
-
-
 def _mod(name):
-    """A module of the package, imported once as a program does."""
-    if name not in _modules:
-        import importlib
-        entry = importlib.import_module("__graft_entry__")
-        entry.load_package()
-        _modules[name] = importlib.import_module(f"{entry.PKG_NAME}.{name}")
-    return _modules[name]
+    import importlib
+    entry = importlib.import_module("__graft_entry__")
+    entry.load_package()
+    return importlib.import_module(f"{entry.PKG_NAME}.{name}")
 
 
 # ------------------------------------------------------------------- cases
