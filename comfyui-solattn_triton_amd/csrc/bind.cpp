@@ -11,7 +11,9 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/util/StringUtil.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -61,6 +63,16 @@ template <typename... A>
 std::string shape(const Tensor& t) { return c10::str(t.sizes()); }
 
 constexpr int64_t kMaxHeadDim = 128;
+
+// A recorder of torch operators sees the outputs' allocation and nothing of the kernels,
+// so what it records would return memory that nobody wrote.
+void refuse_recording(const char* what) {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  bool on = torch::jit::tracer::isTracing();
+  for (const Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+    on = on || c10::impl::TorchDispatchModeTLS::get_mode(m).has_value();
+  if (on) refuse(what, " cannot be traced: its kernels are no torch operators");
+}
 
 // Inputs of one call: 4-dimensional, of one type and device, one head dim.
 struct Named {
@@ -278,6 +290,7 @@ struct NormRope : torch::autograd::Function<NormRope> {
 std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, const OptTensor& qw, const OptTensor& kw,
                                        const OptTensor& cos, const OptTensor& sin, double eps,
                                        const OptTensor& positions, bool interleaved) {
+  refuse_recording("qk_norm_rope");
   check_rows(q0, {{"k", k0}}, true);
   const int64_t B = q0.size(0), T = q0.size(1);
   if (k0.size(0) != B || k0.size(1) != T) refuse("q and k hold different tokens: ", shape(q0), " ", shape(k0));
@@ -309,6 +322,7 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
                            const Tensor& v_cache, const Tensor& table0, const Tensor& lengths0, const OptTensor& qw,
                            const OptTensor& kw, const OptTensor& cos, const OptTensor& sin, double eps,
                            bool interleaved) {
+  refuse_recording("qk_norm_rope_append");
   refuse_grad("qk_norm_rope_append", {q0, k0, v0, k_cache, v_cache, qw.value_or(Tensor()), kw.value_or(Tensor())});
   check_rows(q0, {{"k", k0}, {"v", v0}, {"k_cache", k_cache}, {"v_cache", v_cache}}, true);
   const int64_t B = q0.size(0), T = q0.size(1), H = q0.size(2), Hkv = k0.size(2);
@@ -406,6 +420,7 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
 
 Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::optional<int64_t> window, int64_t sinks,
                    bool causal, std::optional<double> scale, const OptTensor& lengths, std::optional<int64_t> q_start) {
+  refuse_recording("window_attn");
   check_rows(q0, {{"k", k0}, {"v", v0}}, false);
   const int64_t B = q0.size(0), Tq = q0.size(1), H = q0.size(2), D = q0.size(3), Tk = k0.size(1);
   WindowPlan p;
@@ -439,6 +454,7 @@ Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::op
 // --------------------------------------------------------------------- pages
 Tensor paged_attn(const Tensor& q0, const Tensor& k, const Tensor& v, const Tensor& table0, const Tensor& lengths0,
                   std::optional<int64_t> window, int64_t sinks, std::optional<double> scale0) {
+  refuse_recording("paged_attn");
   refuse_grad("paged_attn", {q0, k, v});
   check_rows(q0, {{"k_cache", k}, {"v_cache", v}}, false);
   const int64_t B = q0.size(0), H = q0.size(2), D = q0.size(3), Hkv = k.size(2), pages = k.size(0), page = k.size(1);

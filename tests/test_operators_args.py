@@ -180,3 +180,37 @@ def test_wide_windows_and_eps(capi):
         assert L.solattn_qk_norm_rope(A, *s, A, *s, 1, 10, 1, 1, 128, 0, A, A, A, A, 10, 128, 0, None, 0, eps, A, *s, A, *s,
                                       None) == EINVAL
         assert b"eps" in L.solattn_last_error()
+
+
+def _calls(pkg):
+    """Every operator as a function of its float tensors: (name, function, arguments on the host)."""
+    mod = lambda name: importlib.import_module(f"{pkg.__name__}.{name}")  # noqa: E731
+    x = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    one = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    w, cos = torch.ones(64), torch.ones(8, 32)
+    t, n = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    rope, window, paged = mod("_qk_rope"), mod("_window"), mod("_paged")
+    return [
+        ("qk_norm_rope", lambda *a: rope.qk_norm_rope(*a), [x, x, w, w, cos, cos]),
+        ("qk_norm_rope_append", lambda q, k, v, kc, vc, qw, kw, c, s: rope.qk_norm_rope_append(
+            q, k, v, kc, vc, t, n, qw, kw, c, s), [one, one, one, x, x, w, w, cos, cos]),
+        ("window_attn", lambda q, k, v: window.window_attn(q, k, v, window=4), [x, x, x]),
+        ("paged_attn", lambda q, kc, vc: paged.paged_attn(q, kc, vc, t, n), [one, x, x]),
+    ]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_recorders_are_refused(pkg, i):
+    """A trace would hold the outputs' allocation and no kernel: the calls refuse to be recorded."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    name, f, args = _calls(pkg)[i]
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        torch.jit.trace(f, tuple(args))
+    with pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        make_fx(f)(*args)
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(ValueError, match=f"{name} cannot be traced"):
+        f(*args)
+    with pytest.raises(ValueError, match="GPU"):  # (and only while they are)
+        f(*args)
