@@ -9,9 +9,10 @@
 // binding has loaded, so both always call the same library.
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/util/StringUtil.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/util/StringUtil.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -147,6 +148,8 @@ void check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Te
   check_int32(lengths, "lengths", {B}, q.device());
 }
 
+Tensor tensor(const OptTensor& t) { return t.value_or(Tensor()); }
+
 bool wants_grad(std::initializer_list<Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const auto& t : ts)
@@ -156,6 +159,14 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
 
 void refuse_grad(const char* what, std::initializer_list<Tensor> ts) {
   if (wants_grad(ts)) refuse(what, " has no gradient; call it under torch.no_grad()");
+}
+
+// Forward-mode derivatives: the nodes below have backward passes only, and without a
+// node a tangent would be dropped.
+void refuse_tangents(const char* what, std::initializer_list<Tensor> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const auto& t : ts)
+    if (t.defined() && t._fw_grad(0).defined()) refuse(what, " has no forward-mode derivative");
 }
 
 // backward() under create_graph=True would return gradients cut off from the graph.
@@ -241,7 +252,7 @@ std::pair<Tensor, Tensor> rope_forward(const Tensor& q, const Tensor& k, const R
 struct NormRope : torch::autograd::Function<NormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& q_weight,
                                const OptTensor& k_weight, const RopePlan& plan) {
-    const Tensor qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor());
+    const Tensor qw = tensor(q_weight), kw = tensor(k_weight);
     ctx->save_for_backward({q, k, qw, kw, plan.cos, plan.sin, plan.positions});
     ctx->saved_data["P"] = plan.P;
     ctx->saved_data["R"] = plan.R;
@@ -291,6 +302,7 @@ std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, const
                                        const OptTensor& cos, const OptTensor& sin, double eps,
                                        const OptTensor& positions, bool interleaved) {
   refuse_recording("qk_norm_rope");
+  refuse_tangents("qk_norm_rope", {q0, k0, tensor(qw), tensor(kw), tensor(cos), tensor(sin)});
   check_rows(q0, {{"k", k0}}, true);
   const int64_t B = q0.size(0), T = q0.size(1);
   if (k0.size(0) != B || k0.size(1) != T) refuse("q and k hold different tokens: ", shape(q0), " ", shape(k0));
@@ -323,7 +335,9 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
                            const OptTensor& kw, const OptTensor& cos, const OptTensor& sin, double eps,
                            bool interleaved) {
   refuse_recording("qk_norm_rope_append");
-  refuse_grad("qk_norm_rope_append", {q0, k0, v0, k_cache, v_cache, qw.value_or(Tensor()), kw.value_or(Tensor())});
+  refuse_tangents("qk_norm_rope_append",
+                  {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw), tensor(cos), tensor(sin)});
+  refuse_grad("qk_norm_rope_append", {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw)});
   check_rows(q0, {{"k", k0}, {"v", v0}, {"k_cache", k_cache}, {"v_cache", v_cache}}, true);
   const int64_t B = q0.size(0), T = q0.size(1), H = q0.size(2), Hkv = k0.size(2);
   if (k0.size(0) != B || k0.size(1) != T || k0.sizes() != v0.sizes() || k_cache.size(2) != Hkv)
@@ -421,6 +435,7 @@ struct WindowAttn : torch::autograd::Function<WindowAttn> {
 Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::optional<int64_t> window, int64_t sinks,
                    bool causal, std::optional<double> scale, const OptTensor& lengths, std::optional<int64_t> q_start) {
   refuse_recording("window_attn");
+  refuse_tangents("window_attn", {q0, k0, v0});
   check_rows(q0, {{"k", k0}, {"v", v0}}, false);
   const int64_t B = q0.size(0), Tq = q0.size(1), H = q0.size(2), D = q0.size(3), Tk = k0.size(1);
   WindowPlan p;
@@ -455,6 +470,7 @@ Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::op
 Tensor paged_attn(const Tensor& q0, const Tensor& k, const Tensor& v, const Tensor& table0, const Tensor& lengths0,
                   std::optional<int64_t> window, int64_t sinks, std::optional<double> scale0) {
   refuse_recording("paged_attn");
+  refuse_tangents("paged_attn", {q0, k, v});
   refuse_grad("paged_attn", {q0, k, v});
   check_rows(q0, {{"k_cache", k}, {"v_cache", v}}, false);
   const int64_t B = q0.size(0), H = q0.size(2), D = q0.size(3), Hkv = k.size(2), pages = k.size(0), page = k.size(1);

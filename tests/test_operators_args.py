@@ -214,3 +214,23 @@ def test_recorders_are_refused(pkg, i):
         f(*args)
     with pytest.raises(ValueError, match="GPU"):  # (and only while they are)
         f(*args)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_tangents_are_refused(pkg, i):
+    """A forward-mode derivative would be dropped: the calls refuse tensors that carry a tangent, whether
+    or not these require a gradient, and take them where forward mode is off."""
+    from torch.autograd import forward_ad
+
+    name, f, args = _calls(pkg)[i]
+    for j in range(len(args)):
+        for leaf in (False, True):
+            with forward_ad.dual_level():
+                x = list(args)
+                x[j] = forward_ad.make_dual(args[j].clone().requires_grad_(leaf), torch.ones_like(args[j]))
+                with pytest.raises(ValueError, match=f"{name} has no forward-mode derivative"):
+                    f(*x)
+                with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                    f(*x)
+                with torch.no_grad(), forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="GPU"):
+                    f(*x)
