@@ -54,6 +54,28 @@ __device__ __forceinline__ RowsKeys wave_keys(const WindowArgs& a, int r0, int l
   return rows_keys(a, a.q_start + min(first, a.Tq - 1), a.q_start + min(first + 31, a.Tq - 1), len);
 }
 
+// P and dS of fp16 are rounded as multiples of themselves by powers of two. As they are,
+// those of many keys and of small gradients lie among or below fp16's subnormals (8192
+// keys: dq and dk 4.5 to 15 times as far from exact values as these are when rounded,
+// for do of 1e-2 and 1e-3), and those of large gradients above its largest number.
+//   dk, dv: P by 2^kPScale, and dS by what takes a bound of it, max |v_j| max |do_i| +
+//     max |D_i| over a wave's keys and the rows that see its block, to 2^14;
+//   dq: dS of row i by 2^13 / |do_i|, less where that passes 2^15 in a tile (its sums are
+//     then made smaller too, as those of a softmax whose maximum grows).
+// The sums are multiplied back in fp32. bf16 has the range and needs none of it. 8192
+// tokens, window 1024, with gradients: 565 -> 579 us.
+constexpr int kPScale = 12;
+template <typename E>
+constexpr bool kScaled = std::is_same_v<E, Fp16>;
+__device__ __forceinline__ float pow2(int x) { return __uint_as_float(static_cast<uint32_t>(127 + x) << 23); }
+__device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.f; }
+// The largest over the 32 lanes of a wave's half.
+__device__ __forceinline__ float max32(float x) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+
 template <int ND>
 struct RowState {
   float m, l;      // running max (log2 domain) and this lane's row sum
@@ -449,7 +471,7 @@ window_dq_kernel(const WindowArgs a) {
   // D_i from o and what its rounding took away: the rounding alone is one error for all
   // keys of a row, and took dq and dk from 1.45 to 1.55 times the error of exact ones
   // rounded to the type.
-  float delta = 0.f;
+  float delta = 0.f, size = 0.f;  // size: |do_i|^2
   {
     bf16x8 o[NC];
     const auto add = [&](const uint16_t* row_o) __attribute__((always_inline)) {
@@ -465,9 +487,29 @@ window_dq_kernel(const WindowArgs a) {
     add(a.o.p + b * a.o.b + static_cast<int64_t>(rr) * a.o.t + h * a.o.h);
     if (a.o_lo) add(a.o_lo + ((static_cast<int64_t>(b) * a.Tq + rr) * a.H + h) * D);
     delta = xhalf_sum(delta);
+    if constexpr (kScaled<E>) {
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) {
+        const uint4 y = __builtin_bit_cast(uint4, g[cc]);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) size = fmaf(E::lo(w[i]), E::lo(w[i]), fmaf(E::hi(w[i]), E::hi(w[i]), size));
+      }
+      size = xhalf_sum(size);
+    }
   }
-  const float neg = -a.lse[at];  // -inf for a row that sees nothing
+  const float lse = a.lse[at];
+  float neg = -lse;  // -inf for a row that sees nothing
   if (row < a.Tq && half == 0) a.delta[at] = delta;
+  int up = 0;  // dS is held as 2^up of itself
+  if constexpr (kScaled<E>) {
+    if (row < a.Tq && half == 0) a.lse_p[at] = lse - kPScale;
+    const bool on = row < a.Tq && lse < INFINITY;
+    const float big = max32(on ? sqrtf(finite_or_0(size)) : 0.f), big_d = max32(on ? fabsf(finite_or_0(delta)) : 0.f);
+    if (lane == 0) a.mag[(static_cast<int64_t>(b) * a.H + h) * (4 * a.nqb) + 4 * qb + wave_id()] = make_float2(big, big_d);
+    up = 13 - ((__builtin_amdgcn_frexp_expf(size) + 1) >> 1);
+    neg += static_cast<float>(up);
+  }
 
   f32x16 acc[ND] = {};
   for (int t = 0; t < kt.n; ++t) {
@@ -494,14 +536,31 @@ window_dq_kernel(const WindowArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = keep(dp[r], bit_word(bits, r));
       }
+      if constexpr (kScaled<E>) {
+        float top = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+        if (__any(top > 32768.f)) {
+          top = xhalf_max(top);
+          const int down = top > 32768.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 13 : 0;
+          const float f = __builtin_amdgcn_ldexpf(1.f, -down);
+          up -= down;
+          neg -= static_cast<float>(down);
+          mfma_fence(acc);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) acc[dt] *= f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= f;
+        }
+      }
       bf16x8 ds[NW][2];
       pack_all<E>(ds, dp);
       add_product<E, D, 3>(acc, ka, at, ds);
     }
   }
   mfma_fence(acc);
-  store_row<E>(acc, a.scale, a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h, row < a.Tq,
-               half);
+  store_row<E>(acc, kScaled<E> ? __builtin_amdgcn_ldexpf(a.scale, -up) : a.scale,
+               a.out + b * a.out_b + static_cast<int64_t>(row) * a.out_t + h * a.out_h, row < a.Tq, half);
 }
 
 // dk and dv: a workgroup owns 128 keys of a kv head and walks, head by head of the
@@ -558,6 +617,32 @@ window_dkv_kernel(const WindowArgs a) {
   bf16x8 k[NC], v[NC];
   load_row<D>(k, a.k.p + b * a.k.b + static_cast<int64_t>(jj) * a.k.t + hk * a.k.h, half);
   load_row<D>(v, a.v.p + b * a.v.b + static_cast<int64_t>(jj) * a.v.t + hk * a.v.h, half);
+  int down = 0;  // |dS| < 2^down
+  if constexpr (kScaled<E>) {
+    if (tiles) {
+      float size = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) {
+        const uint4 y = __builtin_bit_cast(uint4, v[cc]);
+        const uint32_t x[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) size = fmaf(E::lo(x[i]), E::lo(x[i]), fmaf(E::hi(x[i]), E::hi(x[i]), size));
+      }
+      const KeyRows kr = key_rows(a, j, len);
+      size = max32(kr.pl <= kr.ph ? finite_or_0(xhalf_sum(size)) : 0.f);
+      float big = 0.f, big_d = 0.f;
+      const uint32_t c0 = static_cast<uint32_t>(i0) >> 5, cells = (static_cast<uint32_t>(i1) >> 5) - c0 + 1;
+      const float2* mag = a.mag + (static_cast<int64_t>(b) * a.H + hk * a.group) * (4 * a.nqb) + c0;
+      for (int g = 0; g < a.group; ++g, mag += 4 * a.nqb)
+        for (uint32_t c = lane; c < cells; c += 64) {
+          big = fmaxf(big, mag[c].x);
+          big_d = fmaxf(big_d, mag[c].y);
+        }
+      big = xhalf_max(max32(big)), big_d = xhalf_max(max32(big_d));
+      down = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(fmaf(sqrtf(size), big, big_d)));
+    }
+  }
+  const float to_ds = pow2(2 - down);
 
   const uint32_t off_q = copy_offset<kThreads, D, kBoth>(a.q.t), off_g = copy_offset<kThreads, D, kBoth>(a.d_o.t);
   // The next step to copy: head g of the group, rows from t0 on.
@@ -574,7 +659,7 @@ window_dkv_kernel(const WindowArgs a) {
       copy_tile<kThreads, D, kBoth>(qb + buf * kBuf, qp, a.q.t, safe);
       copy_tile<kThreads, D, kBoth>(gb + buf * kBuf, gp, a.d_o.t, safe);
     }
-    const float* st = wave == 0 ? a.lse : a.delta;
+    const float* st = wave ? a.delta : kScaled<E> ? a.lse_p : a.lse;
     if (wave < 2)
       g2l4(st + (static_cast<int64_t>(b) * a.H + h) * a.Tq + safe(lane), sb + (2 * buf + wave) * kKeys * 4);
     t0 += kKeys;
@@ -609,7 +694,7 @@ window_dkv_kernel(const WindowArgs a) {
         for (int i = 0; i < 4; ++i) {
           const int r = 4 * r4 + i;
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lx[i]));
-          dp[r] = s[r] * (dp[r] - dx[i]);
+          dp[r] = s[r] * (kScaled<E> ? (dp[r] - dx[i]) * to_ds : dp[r] - dx[i]);
         }
         asm volatile("" ::: "memory");  // (the next four's statistics are read behind these, not held with them)
       }
@@ -635,11 +720,12 @@ window_dkv_kernel(const WindowArgs a) {
   mfma_fence(dv);
   const int ln = lane_again(), hf = ln >> 5;
   const int key = wave * 32 + (ln & 31);
+  const float from_p = kScaled<E> ? pow2(-kPScale) : 1.f, from_ds = kScaled<E> ? pow2(down - 2 - kPScale) : 1.f;
   if (kp.parts == 1) {
     const int64_t at = j0 + key;
     const bool on = at < a.Tk;
-    store_row<E>(dk, a.scale, a.dk + b * a.dk_b + at * a.dk_t + hk * a.dk_h, on, hf);
-    store_row<E>(dv, 1.f, a.dv + b * a.dv_b + at * a.dv_t + hk * a.dv_h, on, hf);
+    store_row<E>(dk, a.scale * from_ds, a.dk + b * a.dk_b + at * a.dk_t + hk * a.dk_h, on, hf);
+    store_row<E>(dv, from_p, a.dv + b * a.dv_b + at * a.dv_t + hk * a.dv_h, on, hf);
     return;
   }
   // [dk, dv][key][channel]: a lane has 4 consecutive channels of its key at a time
@@ -648,7 +734,7 @@ window_dkv_kernel(const WindowArgs a) {
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x16 &x = dk[dt], &y = dv[dt];
+      const f32x16 x = dk[dt] * from_ds, y = dv[dt] * from_p;
       *reinterpret_cast<float4*>(part + 32 * dt + 8 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
       *reinterpret_cast<float4*>(part + kRows * D + 32 * dt + 8 * i) =
           make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
@@ -852,9 +938,11 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   return check_launch(what);
 }
 
+// D_i and lse_p, the 32-row blocks' magnitudes, the parts of dk and dv.
+static int64_t stat_bytes(const WindowArgs& a) { return cdiv(static_cast<int64_t>(a.B) * a.H * a.Tq * 4, 256) * 256; }
+static int64_t mag_bytes(const WindowArgs& a) { return cdiv(static_cast<int64_t>(a.B) * a.H * a.nqb * 32, 256) * 256; }
 static int64_t bwd_workspace(const WindowArgs& a, int64_t D) {
-  return cdiv(static_cast<int64_t>(a.B) * a.H * a.Tq * 4, 256) * 256 +
-         static_cast<int64_t>(a.B) * a.Hkv * a.slots * 2 * kRows * D * 4;
+  return 2 * stat_bytes(a) + mag_bytes(a) + static_cast<int64_t>(a.B) * a.Hkv * a.slots * 2 * kRows * D * 4;
 }
 
 extern "C" int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
@@ -898,7 +986,9 @@ extern "C" int solattn_window_attn_bwd(
   SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SOLATTN_EINVAL,
                   "%s: workspace must be 256-byte aligned", what);
   a.delta = static_cast<float*>(workspace);
-  a.part = a.delta + cdiv(B * H * Tq * 4, 256) * 64;
+  a.lse_p = a.delta + stat_bytes(a) / 4;
+  a.mag = reinterpret_cast<float2*>(a.lse_p + stat_bytes(a) / 4);
+  a.part = reinterpret_cast<float*>(a.mag) + mag_bytes(a) / 4;
   const int64_t items = B * Hkv * (static_cast<int64_t>(a.nsb) * a.ks + static_cast<int64_t>(a.nkb - a.nsb) * a.kn);
   const int64_t cut = a.kn > 1 ? a.nkb : a.ks > 1 ? a.nsb : 0;  // blocks of keys to join
   const int64_t join = cdiv(B * Hkv * cut * 2 * kRows * (D / 8), 256);

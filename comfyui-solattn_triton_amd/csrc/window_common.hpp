@@ -30,6 +30,8 @@ struct WindowArgs {
   float* lse;                // [B][H][Tq], log2 domain; +inf for a row that sees nothing
   uint16_t* o_lo;            // [B][Tq][H][D], what rounding o took away (null: not kept)
   float* delta;              // [B][H][Tq]
+  float* lse_p;              // fp16's backward: [B][H][Tq], lse less kPScale
+  float2* mag;               // fp16's backward: [B][H][4 nqb], of 32 rows: the largest |do_i| and |D_i|
   const int32_t* lengths;    // null: Tk
   int B, H, Hkv, group, Tq, Tk, q_start;
   int window, sinks, causal; // window <= 2^30

@@ -809,3 +809,63 @@ def test_two_streams_at_once(window, paged, dev):
     for w, runs in zip(want, got):
         for r in runs:
             assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+# fp16: T, D, window, sinks, causal, do's size and whether it varies from row to row, v's size
+SMALL_FP16 = [
+    (8192, 64, None, 0, False, 1e-2, False, 1.0),
+    (8192, 128, None, 0, False, 1e-3, False, 1.0),
+    (4096, 128, None, 0, False, 1e-5, False, 1.0),
+    (4100, 64, 1500, 70, True, 1e-3, True, 0.01),
+    (8192, 64, None, 0, False, 30.0, False, 1.0),
+    (700, 128, 20, 4, True, 1e-3, False, 1.0),
+]
+
+
+@pytest.mark.parametrize("case", SMALL_FP16, ids=[str(i) for i in range(len(SMALL_FP16))])
+def test_window_fp16_gradients_of_any_size(window, dev, case):
+    """P and dS of many keys, and of small gradients of the output, lie below fp16's normal numbers
+    (dS of 8192 keys and gradients of 1e-3: below its smallest one), and of large ones above its
+    largest; the gradients do not show it. Independent errors add up in squares: the outputs' own
+    rounding counts 1, that of P or dS as a normal number 1, everything else 0.75 of that (as above)."""
+    T, D, w, sinks, causal, size, varies, vsize = case
+    q, k, v = randn((1, T, 2, D), 140, dev, FP, 2.0), randn((1, T, 1, D), 141, dev, FP), randn((1, T, 1, D), 142, dev, FP, vsize)
+    do = randn((1, T, 2, D), 143, dev, F32, size)
+    if varies:  # rows 2^0 to 2^-9 as large
+        do = do * 2.0 ** -(torch.arange(T, device=dev) % 10)[None, :, None, None]
+    do = do.to(FP)
+    on = ref.seen(T, T, 0, w, sinks, causal, None, 1, dev)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    got = torch.autograd.grad(window.window_attn(q, k, v, window=w, sinks=sinks, causal=causal, scale=0.06), (q, k, v), do)
+    want, _ = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.06, do, FP)
+    worst = {}
+    for name, g, x in zip(("dq", "dk", "dv"), got, want):
+        ideal = (x.to(FP).double() - x).norm()
+        worst[name] = ((g.double() - x).norm() / ideal).item()
+    print("[fp16]", case, worst, flush=True)
+    assert all(x <= 1.6 for x in worst.values()), worst
+
+
+def test_window_fp16_gradients_beyond_ds(window, dev):
+    """dS past fp16's largest number where dq, dk and dv are well inside it: few keys of small k,
+    q and large do; a row with an infinite do takes its own keys' gradients with it and no others'."""
+    T, D = 300, 64
+    q, k = randn((1, T, 2, D), 150, dev, FP, 0.01), randn((1, T, 2, D), 151, dev, FP, 0.01)
+    v, do = randn((1, T, 2, D), 152, dev, FP, 8.0), randn((1, T, 2, D), 153, dev, FP, 3000.0)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    for scale in (0.125, 0.01):
+        on = ref.seen(T, T, 0, 3, 0, True, None, 1, dev)
+        got = torch.autograd.grad(window.window_attn(q, k, v, window=3, scale=scale), (q, k, v), do)
+        want, bound = ref.gradients(q.detach(), k.detach(), v.detach(), on, scale, do, FP)
+        for name, g, x, b in zip(("dq", "dk", "dv"), got, want, bound):
+            assert x.abs().max() < 60000
+            ref.close(g, x, b, name)
+    bad = do.clone()
+    bad[:, 200] = float("inf")
+    hurt = torch.autograd.grad(window.window_attn(q, k, v, window=3, scale=scale), (q, k, v), bad)
+    far = torch.ones(T, dtype=torch.bool, device=dev)
+    far[128:256] = False  # (the rows and keys that share a workgroup with it may be reached by 0 times it)
+    for g, x in zip(hurt, got):
+        assert torch.equal(g[:, far], x[:, far]) and not torch.isfinite(g[:, 200]).all()
