@@ -772,29 +772,37 @@ __global__ void __launch_bounds__(256) window_dkv_join_kernel(const WindowArgs a
   Row8<E>::store(out + ch, x);
 }
 
-// How the key blocks of the backward are cut (WindowArgs::nsb, ks, kn, slots): the
-// sinks' blocks into parts no longer than another block, and every block into as many
-// as leave the launch within the CUs' two workgroups each (one more, and the last wait
-// for a second round: 6000 tokens of 8 heads, backward: 183 us as it is, 209 with one
-// more), as long as a part keeps eight steps.
+// How the key blocks of the backward are cut (WindowArgs::nsb, ks, kn, slots): every
+// block into as many parts as leave the launch within the CUs' two workgroups each (one
+// more, and the last wait for a second round: 6000 tokens of 8 heads, backward: 183 us as
+// it is, 209 with one more), as long as a part keeps eight steps; the sinks' blocks, which
+// every row behind them sees, into parts no longer than another block, but no more than
+// 1024 of them, four a CU (a part writes its keys' dk and dv in fp32: 12133 tokens of 24
+// heads, window 64, 1333 sinks in 792 parts 1190 us, in 10296 parts of 1.35 GB 1610), and
+// where there are several such blocks also of eight steps at least.
 void cut_keys(WindowArgs& a) {
   const int64_t tiles_all = cdiv(a.Tq, kKeys) + 1;
   int64_t tiles = cdiv(static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + kRows, kKeys) + 1;
   if (tiles > tiles_all) tiles = tiles_all;
-  const int64_t steps = tiles * a.group;
+  const int64_t steps = tiles * a.group, heads = static_cast<int64_t>(a.B) * a.Hkv;
   a.nsb = static_cast<int>(cdiv(a.sinks, kRows));
-  int64_t kn = 512 / (static_cast<int64_t>(a.B) * a.Hkv * a.nkb);
+  int64_t kn = 512 / (heads * a.nkb);
   if (kn > steps / 8) kn = steps / 8;
   if (kn < 1) kn = 1;
   // (a block with few sinks keeps one wave busy: its parts are last and a quarter as long,
   // unless there are many of them)
   const int64_t whole = cdiv(tiles_all * a.group, cdiv(steps, kn));
-  const int64_t items = static_cast<int64_t>(a.B) * a.Hkv * a.nsb * whole;
+  const int64_t items = heads * a.nsb * whole;
   const int64_t finer = items > 256 ? 1 : items > 128 ? 2 : 4;
   int64_t ks = whole > 1 ? cdiv(tiles_all * a.group, cdiv(steps, finer * kn)) : whole;
+  if (a.nsb > 0 && ks > 1024 / (heads * a.nsb)) ks = 1024 / (heads * a.nsb);
+  if (a.nsb > 1 && ks > tiles_all * a.group / 8) ks = tiles_all * a.group / 8;
+  if (ks < 1) ks = 1;
   a.kn = static_cast<int>(kn);
   a.ks = static_cast<int>(ks);
   if (a.nsb == a.nkb) a.kn = a.ks;  // (only sinks' blocks)
+  // (kn above 1 leaves ks above 1: then heads nkb <= 256 and steps >= 16. So the slots are
+  // those of both kinds of blocks or of the sinks' alone)
   a.by_ks = divisor(a.ks), a.by_kn = divisor(a.kn);
   a.by_items = divisor(static_cast<int64_t>(a.nsb) * a.ks + static_cast<int64_t>(a.nkb - a.nsb) * a.kn);
   a.slots = (a.ks > 1 ? a.nsb * a.ks : 0) + (a.kn > 1 ? (a.nkb - a.nsb) * a.kn : 0);
@@ -827,6 +835,9 @@ int setup(WindowArgs& a, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t H
   a.Tq = static_cast<int>(Tq), a.Tk = static_cast<int>(Tk), a.q_start = static_cast<int>(q_start);
   // wider than the sequence is the same as wide as it
   a.window = static_cast<int>(window < Tk ? window : Tk), a.sinks = static_cast<int>(sinks < Tk ? sinks : Tk);
+  // and sinks that reach every key, alone or (causal) with the window, are no window
+  if (a.window == Tk || a.sinks == Tk || (causal && static_cast<int64_t>(a.window) + a.sinks >= Tk))
+    a.window = static_cast<int>(Tk), a.sinks = 0;
   a.causal = causal;
   a.nqb = static_cast<int>(cdiv(Tq, kRows)), a.nkb = static_cast<int>(cdiv(Tk, kRows));
   a.split = 1;

@@ -176,7 +176,7 @@ __device__ __forceinline__ KeyPart key_part(const WindowArgs& a, uint32_t w) {
   uint32_t n = a.by_items.split(w);
   k.bh = static_cast<int>(w);
   const int i = static_cast<int>(n) - (static_cast<int>(a.by_items.d) - sink_items);
-  if (i >= 0) {  // sinks' parts last: they are the shorter ones
+  if (i >= 0) {  // sinks' parts last: the shorter ones, unless there are very many sinks
     k.slot = static_cast<int64_t>(k.bh) * a.slots + i;
     n = i;
     k.part = a.by_ks.split(n), k.block = n, k.parts = a.ks;

@@ -869,3 +869,33 @@ def test_window_fp16_gradients_beyond_ds(window, dev):
     far[128:256] = False  # (the rows and keys that share a workgroup with it may be reached by 0 times it)
     for g, x in zip(hurt, got):
         assert torch.equal(g[:, far], x[:, far]) and not torch.isfinite(g[:, 200]).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_window_sinks_that_are_all_keys(window, dev, causal):
+    """Sinks that reach every key, alone or with the window: the bits of a call without a window."""
+    q, k, v = (randn((1, 700, h, 64), s, dev).requires_grad_(True) for s, h in enumerate((4, 2, 2)))
+    do = randn((1, 700, 4, 64), 3, dev)
+
+    def run(w, s):
+        o = window.window_attn(q, k, v, window=w, sinks=s, causal=causal)
+        return [o, *torch.autograd.grad(o, (q, k, v), do)]
+
+    want = run(None, 0)
+    for w, s in ((64, 700), (1, 10 ** 9), (700, 30)) + (((100, 600), (599, 101)) if causal else ()):
+        assert all(torch.equal(x, y) for x, y in zip(run(w, s), want)), (w, s)
+
+
+# As WINDOW: many sinks and narrow windows, whose blocks' parts are long
+MANY_SINKS = [
+    (1, 3000, 3000, 2, 1, 128, 33, 700, True, None, BF),
+    (2, 2100, 2300, 8, 8, 64, 16, 1000, False, [2300, 1500], FP),
+    (1, 1700, 1700, 40, 40, 128, 10, 600, True, None, FP),
+    (1, 1500, 1500, 6, 2, 64, 64, 1500, False, None, BF),
+]
+
+
+@pytest.mark.parametrize("case", MANY_SINKS, ids=[str(i) for i in range(len(MANY_SINKS))])
+def test_window_many_sinks(window, dev, case):
+    test_window(window, dev, case)
+    test_window_gradients(window, dev, case)

@@ -234,3 +234,31 @@ def test_tangents_are_refused(pkg, i):
                     f(*x)
                 with torch.no_grad(), forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="GPU"):
                     f(*x)
+
+
+@pytest.mark.parametrize("T,H,Hkv,window,sinks,causal", [
+    (32760, 24, 24, 64, 1333, 0), (32760, 24, 24, 64, 4096, 0), (32760, 24, 24, 256, 300, 0), (65536, 24, 24, 128, 4000, 1),
+    (12133, 24, 24, 64, 1333, 0), (32768, 24, 8, 64, 2000, 1), (32768, 1, 1, 64, 1000, 0), (100000, 2, 1, 16, 5000, 1),
+])
+def test_window_backward_workspace_of_many_sinks(capi, T, H, Hkv, window, sinks, causal):
+    """The parts of sinks' blocks are bounded by what fills the CUs (1024 of a block's dk and dv in fp32,
+    beside 512 of other blocks), and not by the length over the window: no more than twice q where q is long."""
+    need = capi.LIB.solattn_window_attn_bwd_workspace_bytes(1, T, T, H, Hkv, 128, window, sinks, causal)
+    rows = 2 * 4 * T * H + T * H + 1024  # two numbers a row, two for 32 rows, rounding up
+    assert 0 < need <= rows + 1536 * 2 * 128 * 128 * 4
+    if H == 24:
+        assert need <= 2 * (T * H * 128 * 2)
+
+
+@pytest.mark.parametrize("T,B,H", [(32768, 1, 24), (65536, 1, 24), (4096, 1, 1), (1000, 2, 3)])
+def test_window_workspaces_of_sinks_that_are_all_keys(capi, T, B, H):
+    """Sinks that reach every key are no window: the same call, the same workspace."""
+    L = capi.LIB
+    for causal in (0, 1):
+        full = L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 0, causal)
+        assert L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, 64, T, causal) == full
+        assert L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 77, causal) == full
+    assert L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, 64, T - 64, 1) == \
+        L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 0, 1)
+    rows = 2 * 4 * B * T * H + B * T * H + 1024
+    assert L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 0, 1) <= rows + 1024 * 2 * 128 * 128 * 4
