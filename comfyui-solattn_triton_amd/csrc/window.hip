@@ -1009,11 +1009,14 @@ extern "C" int solattn_window_attn_bwd(
   // P and dS in two roundings where rows see few keys or few rows see a key: the fewer, the
   // more of dq and dk cancels, but not of the errors of one rounding (these took dq to
   // 1.45 to 1.65 times the error of exact values rounded once, two to 1.02 to 1.2). From
-  // windows of 512 keys, 1024 keys and 128 rows on it is 1.42 to 1.49, and the products
-  // of the second rounding would take 8192 tokens 540 -> 607 us, 2000 of 64 channels
-  // 83 -> 93.
-  const int64_t seen = (causal ? a.window : 2 * static_cast<int64_t>(a.window) - 1) + a.sinks;
-  const bool two = seen < 512 || Tk < 1024 || Tq < 128;
+  // windows of 512 keys, 1024 keys and 128 rows on it is 1.42 to 1.49 in one, and two
+  // would take 8192 tokens 540 -> 607 us, 2000 of 64 channels 83 -> 93: where the line
+  // is drawn is a choice between the two, the errors do not jump there. The rule is on
+  // what the call as a whole can see, up to its last position; what `lengths` hold and the
+  // first rows of a long causal call are not looked at.
+  const int64_t reach = causal ? q_start + Tq : Tk;
+  const int64_t wide = (causal ? a.window : 2 * static_cast<int64_t>(a.window) - 1) + a.sinks;
+  const bool two = wide < 512 || reach < 1024 || Tq < 128;
   const auto kq = D == 128 ? (bf ? (two ? window_dq_kernel<Bf16, 128, 2> : window_dq_kernel<Bf16, 128, 1>)
                                  : (two ? window_dq_kernel<Fp16, 128, 2> : window_dq_kernel<Fp16, 128, 1>))
                            : (bf ? (two ? window_dq_kernel<Bf16, 64, 2> : window_dq_kernel<Bf16, 64, 1>)

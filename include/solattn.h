@@ -445,8 +445,10 @@ int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t s
                         int64_t workspace_bytes, solattn_stream_t stream);
 
 /* Gradients of solattn_window_attn from its inputs, o, lse, o_lo (or null) and do: dq like q, dk and dv
- * like k (every row written, zeros where nothing is seen). workspace: 256-byte
- * aligned. No atomics: the same inputs give the same bits. */
+ * like k (every row written, zeros where nothing is seen). P and dS are rounded to
+ * dtype, in two parts where the call's rows see fewer than 512 keys, all of them fewer
+ * than 1024, or there are fewer than 128 rows (lengths are not looked at). workspace:
+ * 256-byte aligned. No atomics: the same inputs give the same bits. */
 int64_t solattn_window_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hkv,
                                                 int64_t D, int64_t window, int64_t sinks, int causal);
 int solattn_window_attn_bwd(

@@ -899,3 +899,22 @@ MANY_SINKS = [
 def test_window_many_sinks(window, dev, case):
     test_window(window, dev, case)
     test_window_gradients(window, dev, case)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D,T,Tk,start,w,sinks", [(128, 200, 8000, 0, None, 0), (64, 300, 3000, 60, 2900, 4), (128, 900, 5000, 0, None, 0)])
+def test_window_gradients_of_few_keys_by_position(window, dev, D, T, Tk, start, w, sinks, dtype):
+    """A prompt at the beginning of a long buffer of keys: its rows see few of them whatever the window
+    is, and the bound is that of few keys above."""
+    q, k, v = randn((1, T, 4, D), 160, dev, dtype, 2.0), randn((1, Tk, 2, D), 161, dev, dtype), randn((1, Tk, 2, D), 162, dev, dtype)
+    do = randn(q.shape, 163, dev, dtype)
+    on = ref.seen(T, Tk, start, w, sinks, True, None, 1, dev)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    got = torch.autograd.grad(window.window_attn(q, k, v, window=w, sinks=sinks, q_start=start, scale=0.11), (q, k, v), do)
+    want, _ = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.11, do, dtype)
+    ratios = {}
+    for name, g, x in zip(("dq", "dk", "dv"), got, want):
+        ratios[name] = ((g.double() - x).norm() / (x.to(dtype).double() - x).norm()).item()
+    print("[few keys]", D, T, Tk, start, ratios, flush=True)
+    assert all(x <= 1.25 for x in ratios.values()), ratios
