@@ -871,7 +871,8 @@ static int cut_rows(WindowArgs& a, bool padded) {
   const int blk = bh * cdiv(a.Tq, 128) >= 1024 ? 128 : 64;
   a.nqb = static_cast<int>(cdiv(a.Tq, blk));
   const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
-  const int64_t tiles = cdiv(reach < a.Tk ? reach : a.Tk, kKeys);
+  const int64_t keys = a.causal ? a.q_start + a.Tq : a.Tk;  // (none behind the last row)
+  const int64_t tiles = cdiv(reach < keys ? reach : keys, kKeys);
   int64_t n = (padded ? 2048 : 1024) / (bh * a.nqb);
   if (n > tiles / 8) n = tiles / 8;
   a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);

@@ -262,3 +262,18 @@ def test_window_workspaces_of_sinks_that_are_all_keys(capi, T, B, H):
         L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 0, 1)
     rows = 2 * 4 * B * T * H + B * T * H + 1024
     assert L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, H, 128, T, 0, 1) <= rows + 1024 * 2 * 128 * 128 * 4
+
+
+def test_window_parts_follow_what_rows_see(capi):
+    """A causal call is cut by the keys up to its last position, not by those behind it."""
+    need = capi.LIB.solattn_window_attn_workspace_bytes
+    assert need(1, 64, 131072, 32, 32, 128, 0, 131072, 0, 1, 0) == 0  # one tile of 64 keys
+    far = need(1, 256, 32000, 24, 8, 128, 31744, 32000, 0, 1, 0)
+    assert need(1, 256, 32000, 24, 8, 128, 0, 32000, 0, 1, 0) == 0 < far
+    row = 24 * 256 * 130 * 4
+    for start in (500, 2000, 4000, 8000, 16000):
+        parts = need(1, 256, 32000, 24, 8, 128, start, 32000, 0, 1, 0) // row
+        assert parts <= max(1, (start + 256) // 64 // 8 + 1) and parts * row <= far
+        # the keys behind the last row make no difference
+        assert need(1, 256, start + 256, 24, 8, 128, start, 32000, 0, 1, 0) // row == parts
+    assert need(1, 256, 32000, 24, 8, 128, 0, 32000, 0, 0, 0) == far  # (symmetric: every key is seen)
