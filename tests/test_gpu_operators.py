@@ -918,3 +918,120 @@ def test_window_gradients_of_few_keys_by_position(window, dev, D, T, Tk, start, 
         ratios[name] = ((g.double() - x).norm() / (x.to(dtype).double() - x).norm()).item()
     print("[few keys]", D, T, Tk, start, ratios, flush=True)
     assert all(x <= 1.25 for x in ratios.values()), ratios
+
+
+# As WINDOW, and q_start: rows at the beginning or in the middle of the keys
+PLACED = [
+    (1, 300, 900, 2, 1, 128, 100, 4, True, None, BF, 0),
+    (2, 257, 1500, 4, 2, 64, 200, 30, True, [1500, 700], FP, 600),
+    (1, 200, 1000, 2, 2, 128, 50, 700, True, None, BF, 100),   # sinks above the rows
+    (1, 300, 1200, 2, 2, 128, 64, 200, False, None, BF, 500),  # and below them
+    (1, 190, 800, 2, 1, 64, 50, 400, False, None, FP, 0),
+    (3, 150, 700, 3, 1, 64, 33, 0, False, [700, 0, 301], BF, 250),
+    (1, 2000, 2600, 1, 1, 64, None, 0, True, None, BF, 300),   # blocks of keys cut into parts
+    (1, 2000, 2500, 2, 1, 128, 40, 100, True, None, FP, 200),  # sinks' blocks cut into parts
+    (1, 70, 6000, 2, 1, 128, None, 0, True, None, FP, 3000),   # key tiles of the forward cut into parts
+    (1, 200, 700, 3, 3, 80, 60, 5, True, None, BF, 250),
+    (2, 1, 500, 4, 2, 64, 90, 3, True, None, FP, 77),
+]
+
+
+@pytest.mark.parametrize("case", PLACED, ids=[str(i) for i in range(len(PLACED))])
+def test_window_placed_rows(window, dev, case):
+    """Forward and gradients where q_start is not Tk - Tq; keys that no row sees may hold anything and
+    have gradients of exact zeros."""
+    B, Tq, Tk, H, Hkv, D, w, sinks, causal, lengths, dtype, start = case
+    q, do = randn((B, Tq, H, D), 170, dev, dtype, 2.0), randn((B, Tq, H, D), 171, dev, dtype)
+    k, v = randn((B, Tk, Hkv, D), 172, dev, dtype), randn((B, Tk, Hkv, D), 173, dev, dtype)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev)
+    on = ref.seen(Tq, Tk, start, w, sinks, causal, n, B, dev)
+    dead_rows, dead_keys = ~on.any(2), ~on.any(1)
+    q[dead_rows], do[dead_rows] = float("nan"), float("nan")
+    k[dead_keys], v[dead_keys] = float("nan"), float("inf")
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    kw = dict(window=w, sinks=sinks, causal=causal, lengths=n, q_start=start, scale=0.11)
+    print("[placed]", case, flush=True)
+    o, p, (_, _, vh) = ref.attention(q.detach(), k.detach(), v.detach(), on, 0.11)
+    bound = ref.forward_bound(o, p, vh, dtype)
+    with torch.no_grad():
+        ref.close(window.window_attn(q, k, v, **kw), o, bound, "o")
+    out = window.window_attn(q, k, v, **kw)
+    ref.close(out.detach(), o, bound, "o of training")
+    got = torch.autograd.grad(out, (q, k, v), do)
+    want, bounds = ref.gradients(q.detach(), k.detach(), v.detach(), on, 0.11, do, dtype)
+    for name, g, x, b in zip(("dq", "dk", "dv"), got, want, bounds):
+        ref.close(g, x, b, name)
+    assert (got[0][dead_rows] == 0).all() and (got[1][dead_keys] == 0).all() and (got[2][dead_keys] == 0).all()
+
+
+# -------------------------------------------------- promises of the C entries
+@pytest.fixture(scope="module")
+def lib(pkg):
+    return importlib.import_module(f"{pkg.__name__}._capi")
+
+
+def _at(t):
+    return [t.data_ptr(), *t.stride()[:3]]
+
+
+@pytest.mark.parametrize("dtype,code", [(BF, 0), (FP, 1), (F32, 2)])
+@pytest.mark.parametrize("Hkv,interleaved", [(2, 0), (0, 1)])
+def test_c_norm_rope_in_place(rope, lib, dev, dtype, code, Hkv, interleaved):
+    """Outputs that are the inputs, and q alone (no kv heads, null k)."""
+    B, T, H, D = 2, 37, 6, 96
+    q, k = randn((B, T, H, D), 1, dev, dtype), randn((B, T, 2, D), 2, dev, dtype)
+    w = 1 + 0.1 * randn((D,), 3, dev, F32)
+    cos, sin = tables(T, D, dev)
+    want = rope.qk_norm_rope(q, k, w, w, cos, sin, interleaved=bool(interleaved))
+    k0, none = k.clone(), [None, 0, 0, 0]
+    rc = lib.LIB.solattn_qk_norm_rope(
+        *_at(q), *(_at(k) if Hkv else none), B, T, H, Hkv, D, code, w.data_ptr(), w.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        T, D, interleaved, None, 0, 1e-6, *_at(q), *(_at(k) if Hkv else none), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.LIB.solattn_last_error()
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1] if Hkv else k0)
+
+
+def test_c_norm_rope_backward_of_q_alone(rope, lib, dev):
+    """No kv heads in the backward pass, one weight's gradient or the other's left out."""
+    B, T, H, D = 1, 50, 5, 64
+    q, g = randn((B, T, H, D), 1, dev), randn((B, T, H, D), 2, dev)
+    w = (1 + 0.1 * randn((D,), 3, dev, F32)).requires_grad_(True)
+    cos, sin = tables(T, D, dev)
+    leaf = q.clone().requires_grad_(True)
+    want = torch.autograd.grad(rope.qk_norm_rope(leaf, q, w, None, cos, sin)[0], (leaf, w), g)
+    need = lib.LIB.solattn_qk_norm_rope_bwd_workspace_bytes(D)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    none, dq, dw = [None, 0, 0, 0], torch.empty_like(q), torch.empty(D, device=dev)
+    for with_w in (True, False):
+        rc = lib.LIB.solattn_qk_norm_rope_bwd(
+            *_at(q), *none, *_at(g), *none, B, T, H, 0, D, 0, w.data_ptr(), None, cos.data_ptr(), sin.data_ptr(), T, D, 0, None,
+            0, 1e-6, *_at(dq), *none, dw.data_ptr() if with_w else None, None, ws.data_ptr() if with_w else None,
+            need if with_w else 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, lib.LIB.solattn_last_error()
+        assert torch.equal(dq, want[0]) and torch.equal(dw, want[1])
+        dq.fill_(0)
+
+
+@pytest.mark.parametrize("dtype,code", [(BF, 0), (FP, 1)])
+def test_c_window_backward_without_o_lo(lib, dev, dtype, code):
+    """The forward's o_lo left out of both calls: o alone gives D_i, within the bounds of o as rounded."""
+    B, T, H, Hkv, D, w = 1, 333, 4, 2, 128, 90
+    q, do = randn((B, T, H, D), 1, dev, dtype, 2.0), randn((B, T, H, D), 4, dev, dtype)
+    k, v = randn((B, T, Hkv, D), 2, dev, dtype), randn((B, T, Hkv, D), 3, dev, dtype)
+    L, stream = lib.LIB, torch.cuda.current_stream().cuda_stream
+    o, lse = torch.empty_like(q), torch.empty(B, H, T, device=dev)
+    need = L.solattn_window_attn_workspace_bytes(B, T, T, H, Hkv, D, 0, w, 3, 1, 1)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+    sizes = [B, T, T, H, Hkv, D, code, 0, None, w, 3, 1, 0.11]
+    assert L.solattn_window_attn(*_at(q), *_at(k), *_at(v), *sizes, *_at(o), lse.data_ptr(), None, ws.data_ptr(), need,
+                                 stream) == 0, L.solattn_last_error()
+    need = L.solattn_window_attn_bwd_workspace_bytes(B, T, T, H, Hkv, D, w, 3, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    assert L.solattn_window_attn_bwd(*_at(q), *_at(k), *_at(v), *_at(o), *_at(do), lse.data_ptr(), None, *sizes, *_at(dq),
+                                     *_at(dk), *_at(dv), ws.data_ptr(), need, stream) == 0, L.solattn_last_error()
+    on = ref.seen(T, T, 0, w, 3, True, None, B, dev)
+    want, bound = ref.gradients(q, k, v, on, 0.11, do, dtype)
+    for name, g, x, b in zip(("dq", "dk", "dv"), (dq, dk, dv), want, bound):
+        ref.close(g, x, b, name)
