@@ -445,7 +445,7 @@ Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::op
     refuse("q/k/v shapes do not match: ", shape(q0), " ", shape(k0), " ", shape(v0));
   check_kv_heads(H, k0.size(2));
   p.q_start = q_start ? *q_start : Tk - Tq;
-  if (p.q_start < 0 || p.q_start + Tq > Tk) refuse("rows ", p.q_start, " to ", p.q_start + Tq, " of ", Tk, " keys");
+  if (Tq > Tk || p.q_start < 0 || p.q_start > Tk - Tq) refuse(Tq, " rows from ", p.q_start, " on of ", Tk, " keys");
   if (lengths) {
     check_int32(*lengths, "lengths", {B}, q0.device());
     p.lengths = lengths->contiguous();

@@ -347,6 +347,8 @@ int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k,
   SOLATTN_REQUIRE(dtype == SOLATTN_BF16 || dtype == SOLATTN_FP16, SOLATTN_EINVAL, "%s: dtype %d", what, dtype);
   SOLATTN_REQUIRE(B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0, SOLATTN_EINVAL,
                   "%s: %lld query heads over %lld kv heads", what, (long long)H, (long long)Hkv);
+  SOLATTN_REQUIRE(B < (1ll << 31) && H < (1ll << 31) && B * H < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large",
+                  what);
   SOLATTN_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, SOLATTN_EUNSUPPORTED,
                   "%s: head_dim %lld (multiples of 8 up to 128)", what, (long long)D);
   SOLATTN_REQUIRE(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), SOLATTN_EINVAL,
@@ -389,7 +391,7 @@ int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k,
   a.part = static_cast<float*>(workspace);
   a.part_ml = B * H * a.split * D;
   const int64_t grid = B * Hkv * a.tiles * a.split;
-  SOLATTN_REQUIRE(grid < (1ll << 31) && B * H < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
+  SOLATTN_REQUIRE(grid < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   const bool bf = dtype == SOLATTN_BF16;
   const auto kern = D == 128 ? (bf ? paged_kernel<Bf16, 128, true> : paged_kernel<Fp16, 128, true>)
                     : D == 64 ? (bf ? paged_kernel<Bf16, 64, true> : paged_kernel<Fp16, 64, true>)
@@ -405,7 +407,9 @@ int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k,
 
 int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
                              int64_t sinks) {
+  constexpr int64_t top = 1ll << 31;  // (what the call takes: nothing passes 64 bits)
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || keys < 0 || window < 0 || sinks < 0) return 0;
+  if (B >= top || H >= top || B * H >= top || D > 128 || keys >= top) return 0;
   return part_bytes(B, H, D, splits(B, Hkv, cdiv(H / Hkv, kGroups), keys, window, sinks));
 }
 
@@ -415,8 +419,8 @@ using namespace solattn;
 
 extern "C" int64_t solattn_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
                                                       int64_t page_size, int64_t window, int64_t sinks) {
-  return max_pages < 0 || page_size < 0 ? 0
-                                        : paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks);
+  const bool fit = max_pages >= 0 && page_size >= 0 && max_pages < (1ll << 31) && page_size < (1ll << 31);
+  return fit ? paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks) : 0;
 }
 
 extern "C" int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k_cache,

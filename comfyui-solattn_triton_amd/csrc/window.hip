@@ -823,9 +823,11 @@ int setup(WindowArgs& a, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t H
   SOLATTN_REQUIRE(dtype == SOLATTN_BF16 || dtype == SOLATTN_FP16, SOLATTN_EINVAL, "%s: dtype %d", what, dtype);
   SOLATTN_REQUIRE(B > 0 && Tq > 0 && Tk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0, SOLATTN_EINVAL,
                   "%s: bad sizes (%lld query heads over %lld kv heads)", what, (long long)H, (long long)Hkv);
+  SOLATTN_REQUIRE(B < (1ll << 31) && H < (1ll << 31) && B * H < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large",
+                  what);  // (nothing below passes 64 bits)
   SOLATTN_REQUIRE(D == 64 || D == 128, SOLATTN_EUNSUPPORTED, "%s: head_dim %lld not in {64, 128}", what, (long long)D);
   SOLATTN_REQUIRE(Tk < (1ll << 29), SOLATTN_EUNSUPPORTED, "%s: %lld keys", what, (long long)Tk);
-  SOLATTN_REQUIRE(q_start >= 0 && q_start + Tq <= Tk, SOLATTN_EINVAL, "%s: rows %lld + %lld past %lld keys", what,
+  SOLATTN_REQUIRE(Tq <= Tk && q_start >= 0 && q_start <= Tk - Tq, SOLATTN_EINVAL, "%s: rows %lld + %lld past %lld keys", what,
                   (long long)q_start, (long long)Tq, (long long)Tk);
   SOLATTN_REQUIRE(window > 0 && sinks >= 0, SOLATTN_EINVAL, "%s: window %lld, sinks %lld", what, (long long)window,
                   (long long)sinks);
@@ -888,7 +890,8 @@ extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, in
                                                        int64_t D, int64_t q_start, int64_t window, int64_t sinks,
                                                        int causal, int with_lse) {
   clear_error();
-  if (Tq == 1 && causal && !with_lse) return paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks);
+  if (Tq == 1 && causal && !with_lse)
+    return q_start < 0 || q_start >= Tk ? 0 : paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks);
   WindowArgs a{};
   if (setup(a, B, Tq, Tk, H, Hkv, D, SOLATTN_BF16, q_start, window, sinks, causal, 1.f, "window_attn")) return 0;
   cut_rows(a, true);

@@ -1035,3 +1035,11 @@ def test_c_window_backward_without_o_lo(lib, dev, dtype, code):
     want, bound = ref.gradients(q, k, v, on, 0.11, do, dtype)
     for name, g, x, b in zip(("dq", "dk", "dv"), (dq, dk, dv), want, bound):
         ref.close(g, x, b, name)
+
+
+def test_window_refuses_wrapped_positions(window, dev):
+    x = torch.zeros(1, 8, 2, 64, device=dev, dtype=BF)
+    for start in (2 ** 63 - 1, 2 ** 63 - 8, 2 ** 62, -2 ** 63):
+        for rows in (x, x[:, :1]):
+            with pytest.raises(ValueError, match="rows"):
+                window.window_attn(rows, x, x, window=4, q_start=start)

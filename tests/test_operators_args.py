@@ -277,3 +277,27 @@ def test_window_parts_follow_what_rows_see(capi):
         # the keys behind the last row make no difference
         assert need(1, 256, start + 256, 24, 8, 128, start, 32000, 0, 1, 0) // row == parts
     assert need(1, 256, 32000, 24, 8, 128, 0, 32000, 0, 0, 0) == far  # (symmetric: every key is seen)
+
+
+TOP = (1 << 63) - 1
+
+
+def test_sizes_beyond_64_bits(capi):
+    """Sizes whose sums and products pass 64 bits are refused like any that are too large: no wrapped
+    position reaches a launch, no workspace's size divides by a product that became zero."""
+    L = capi.LIB
+    for start in (TOP, TOP - 1, TOP - 39, 1 << 62):
+        assert _window(L, q_start=start) == EINVAL and b"rows" in L.solattn_last_error()
+        assert _window(L, q_start=start, Tq=1) == EINVAL and b"row" in L.solattn_last_error()
+        assert L.solattn_window_attn_workspace_bytes(1, 1, 100, 4, 2, 128, start, 16, 2, 1, 0) == 0
+        assert L.solattn_window_attn_workspace_bytes(1, 40, 100, 4, 2, 128, start, 16, 2, 1, 0) == 0
+    assert _window(L, Tq=TOP, q_start=1) == EINVAL and b"rows" in L.solattn_last_error()
+    for B, H in ((1 << 62, 4), (1 << 40, 1 << 24), (1 << 31, 1), (1, 1 << 31), (1 << 16, 1 << 15), (TOP, 2)):
+        assert _window(L, B=B, H=H, Hkv=1) == EUNSUPPORTED and b"grid" in L.solattn_last_error()
+        assert _window(L, B=B, H=H, Hkv=1, Tq=1, q_start=9) == EUNSUPPORTED and b"grid" in L.solattn_last_error()
+        assert L.solattn_window_attn_workspace_bytes(B, 64, 64, H, 1, 128, 0, 64, 0, 1, 0) == 0
+        assert L.solattn_window_attn_workspace_bytes(B, 1, 64, H, 1, 128, 0, 64, 0, 1, 0) == 0
+        assert L.solattn_window_attn_bwd_workspace_bytes(B, 64, 64, H, 1, 128, 64, 0, 1) == 0
+        assert L.solattn_paged_attn_workspace_bytes(B, H, 1, 128, 4, 64, 0, 0) == 0
+    assert L.solattn_paged_attn_workspace_bytes(1, 4, 4, 128, 1 << 40, 1 << 40, 0, 0) == 0
+    assert L.solattn_paged_attn_workspace_bytes(1, 4, 4, TOP, 1000, 64, 0, 0) == 0
