@@ -348,6 +348,7 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
     for (int d = 0; d < 3; ++d)
       if (c.stride(d) == 0 && c.size(d) > 1) refuse("a cache to write to is expanded: strides ", c.strides());
   const RopePlan p = rope_plan(q0, qw, kw, cos, sin, eps, interleaved);
+  if (k_cache.numel() && k_cache.data_ptr() == v_cache.data_ptr()) refuse("k_cache and v_cache are the same memory");
   const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0);
   const Tensor table = table0.size(1) > 1 && table0.stride(1) != 1 ? table0.contiguous() : table0;
   const Tensor lengths = lengths0.contiguous();

@@ -1043,3 +1043,16 @@ def test_window_refuses_wrapped_positions(window, dev):
         for rows in (x, x[:, :1]):
             with pytest.raises(ValueError, match="rows"):
                 window.window_attn(rows, x, x, window=4, q_start=start)
+
+
+def test_append_refuses_one_cache_for_both(rope, dev):
+    """k and v of a token would race for the same slot."""
+    kv = torch.zeros(3, 2, 8, 2, 64, device=dev, dtype=BF)
+    x = torch.ones(1, 1, 2, 64, device=dev, dtype=BF)
+    t, n = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    for k, v in ((kv[:, 0], kv[:, 0]), (kv[0], kv.flatten(0, 1)[:2])):
+        with pytest.raises(ValueError, match="same memory"):
+            rope.qk_norm_rope_append(x, x, x, k, v, t, n)
+    assert (kv == 0).all()
+    rope.qk_norm_rope_append(x, x, x, kv[:, 0], kv[:, 1], t, n)  # side by side is fine
+    assert (kv[0, :, 0] == 1).all() and (kv[1:] == 0).all()
