@@ -865,17 +865,19 @@ static bool single_token(int64_t Tq, int causal, const float* lse) { return Tq =
 // against 211). Their key tiles are cut into as many parts, of at least eight tiles and
 // joined by a second launch, as leave the launch within four workgroups a CU (256 rows
 // of 24 heads against 32000 keys: ten parts 113 us, eleven, which take a second round,
-// 143). In a padded batch, whose sequences may be short or empty, within eight (517
-// rows against 16000 keys, one of two sequences past its end: 44 us; within four 54).
-// padded: for a workspace, which has to do with lengths and without.
-static int cut_rows(WindowArgs& a, bool padded) {
+// 143). Padded batches too: within eight, short and empty sequences leave more of the CUs
+// to the others, but whole ones share less of their keys in the L2 (517 rows against 16000
+// keys, two sequences, one of them past its end: 46.6 us against 53.6, neither: 70.5
+// against 62; 128 rows of eight sequences of 32000 keys 206 against 139, half of these
+// past their end 101 against 95; prompts of 2000 that no launch needs to cut 86 against 55).
+static int cut_rows(WindowArgs& a) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
   const int blk = bh * cdiv(a.Tq, 128) >= 1024 ? 128 : 64;
   a.nqb = static_cast<int>(cdiv(a.Tq, blk));
   const int64_t reach = static_cast<int64_t>(a.causal ? a.window : 2 * static_cast<int64_t>(a.window)) + blk + a.sinks;
   const int64_t keys = a.causal ? a.q_start + a.Tq : a.Tk;  // (none behind the last row)
   const int64_t tiles = cdiv(reach < keys ? reach : keys, kKeys);
-  int64_t n = (padded ? 2048 : 1024) / (bh * a.nqb);
+  int64_t n = 1024 / (bh * a.nqb);
   if (n > tiles / 8) n = tiles / 8;
   a.split = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
   a.by_split = divisor(a.split), a.by_nqb = divisor(a.nqb);
@@ -894,7 +896,7 @@ extern "C" int64_t solattn_window_attn_workspace_bytes(int64_t B, int64_t Tq, in
     return q_start < 0 || q_start >= Tk ? 0 : paged_attn_workspace(B, H, Hkv, D, q_start + 1, window, sinks);
   WindowArgs a{};
   if (setup(a, B, Tq, Tk, H, Hkv, D, SOLATTN_BF16, q_start, window, sinks, causal, 1.f, "window_attn")) return 0;
-  cut_rows(a, true);
+  cut_rows(a);
   return fwd_workspace(a, D);
 }
 
@@ -928,7 +930,7 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
   if (rc) return rc;
   SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(o_lo) % 16 == 0, SOLATTN_EINVAL, "%s: o_lo must be 16-byte aligned", what);
   const bool bf = dtype == SOLATTN_BF16;
-  const int blk = cut_rows(a, lengths != nullptr);
+  const int blk = cut_rows(a);
   const int64_t need = fwd_workspace(a, D);
   SOLATTN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SOLATTN_ESIZE, "%s: workspace %lld < %lld bytes",
                   what, (long long)workspace_bytes, (long long)need);

@@ -301,3 +301,14 @@ def test_sizes_beyond_64_bits(capi):
         assert L.solattn_paged_attn_workspace_bytes(B, H, 1, 128, 4, 64, 0, 0) == 0
     assert L.solattn_paged_attn_workspace_bytes(1, 4, 4, 128, 1 << 40, 1 << 40, 0, 0) == 0
     assert L.solattn_paged_attn_workspace_bytes(1, 4, 4, TOP, 1000, 64, 0, 0) == 0
+
+
+def test_window_forward_parts_fill_one_round(capi):
+    """Parts stay within four workgroups a CU, and a launch that fills these is not cut (a batch with
+    lengths has the same workspace as one without: the size does not know)."""
+    need = capi.LIB.solattn_window_attn_workspace_bytes
+    for B, Tq, Tk, H, Hkv, D in ((4, 2000, 2000, 16, 4, 128), (4, 1024, 4096, 16, 4, 128), (2, 4000, 4000, 8, 8, 128),
+                                 (2, 517, 16000, 16, 4, 64), (8, 128, 32000, 8, 1, 128), (4, 256, 8000, 24, 8, 128)):
+        parts = max(1, need(B, Tq, Tk, H, Hkv, D, Tk - Tq, Tk, 0, 1, 0) // (B * H * Tq * (D + 2) * 4))
+        blocks = B * H * -(-Tq // 64)
+        assert parts == 1 or parts * blocks <= 1024, (B, Tq, Tk, parts)
