@@ -1,5 +1,6 @@
 """Norms of queries and keys per head with the position rotation, in one pass
-(``solattn_qk_norm_rope``): what runs in front of every attention call.
+(``solattn_qk_norm_rope``): what runs in front of the attention of models that norm each
+head's queries and keys.
 
 ``qk_norm_rope`` is differentiable in q, k and the weights;
 ``qk_norm_rope_append`` is its form for new tokens, writing k and v into the pages
@@ -20,9 +21,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
                  sin: torch.Tensor | None = None, *, eps: float = 1e-6,
                  positions: torch.Tensor | None = None, interleaved: bool = False):
     """(q', k'): every head's row of q [B, T, H, D] and k [B, T, Hkv, D] divided by
-    its root mean square, times the weight [D] (None: 1), its first channels turned
-    by the token's angles; fresh BTHD tensors of the inputs' type (bf16, fp16 or
-    fp32).
+    its root mean square, times the weight [D] (None: 1; the row is divided all the
+    same), its first channels turned by the token's angles; fresh BTHD tensors of the
+    inputs' type (bf16, fp16 or fp32).
 
     ``cos``, ``sin``: float32 [positions, pairs] (both None: no rotation); the pairs
     are channels (i, i + pairs), or (2i, 2i + 1) with ``interleaved``. Token t is at

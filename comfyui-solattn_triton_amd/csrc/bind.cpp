@@ -1,9 +1,9 @@
 // Host side of the operators around attention: argument checks, outputs and
 // workspaces from torch's allocator, autograd nodes and the calls into libsolattn,
-// as a Python extension (_native.so). A call takes 5-7 us of host time, what one of
-// torch's own elementwise kernels takes, where the same steps in Python and ctypes
-// took 25-33; a forward and backward pass 45-80 us, most of it torch's engine, where
-// Python nodes took 95-175.
+// as a Python extension (_native.so). A call of one launch takes 5.5-6.5 us of host time,
+// what one of torch's own elementwise kernels takes, of two 9-10, where the same steps in
+// Python and ctypes took 25-33; a forward and backward pass 45-95 us, most of it torch's
+// engine, where Python nodes took 95-175.
 //
 // Nothing here links against libsolattn: init() takes the addresses that the ctypes
 // binding has loaded, so both always call the same library.

@@ -11,7 +11,7 @@
 // sequences of 32768 to 131072 tokens, 24 heads over 8, bf16: 232-251 us, 5.3-5.8
 // TB/s (a large copy reaches 5.0); 32 of 512 to 16384, 16 heads of 64 over 4, pages of
 // 16: 65-68 us, 4.1 TB/s, of it the kernel 54 and the join and its launch the rest; one
-// sequence with a window of 4096: 10.5 us, two latency-bound launches (5.8 and 4.3).
+// sequence with a window of 4096: 10.2 us, two launches of the host's (kernels 5.9 and 4.7).
 // A wave takes 32 keys at a time straight from HBM into operand registers, no LDS:
 //   S^T = K Q^T (v_mfma_f32_16x16x32): row r of tile t is key 8 (r/4) + 4 t + r%4
 //     of the 32, so lane (q, g) = (lane % 16, lane / 16) gets the scores of the

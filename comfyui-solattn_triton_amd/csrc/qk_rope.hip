@@ -12,8 +12,8 @@
 //
 // Bound: HBM; for a few tokens the launch. 32760 tokens of 24 + 24 heads of 128
 // channels, bf16: 156 us, 5.25 TB/s (a large copy reaches 5.0); one token of each of
-// four sequences into its pages: 5.4 us a call, the kernel 4.6; gradients of 8200
-// tokens of 16 + 4 heads of 64, fp16: 17 us and 4.6 for the weights' join, 3.7 TB/s.
+// four sequences into its pages: 7 us a call (the host's), the kernel 4.9; gradients of 8200
+// tokens of 16 + 4 heads of 64, fp16: 17 us and 4.9 for the weights' join, 3.7 TB/s.
 // A lane holds 8 channels, so a row is LPR = 16 lanes (8 up to 64
 // channels) and a wave works on G = 64 / LPR rows at a time, all of the same
 // token: the token's cos and sin and the weights stay in registers while the
