@@ -59,8 +59,8 @@ def listed():
         # One decode step of four sequences: the newest token's norms, rotation and
         # codes, and the short sequences read back. Launches and latency only.
         _case("append_step_4", "append", 100, B=4, T=1),
-        # A 16K-token prompt into an empty cache, codes of 8 bits with scales that are
-        # no powers of two, and back as its attention reads it.
+        # A 16K-token prompt into an empty cache of whole numbers, and back as its
+        # attention reads it.
         _case("append_prompt_16k", "append", 16001, T=16001, interleaved=True, cache="int8"),
         # One chunk of two ragged prompts, no norms, heads of 64 channels, small pages.
         _case("write_chunk_1000", "write", 4100, B=2, T=1000, H=16, Hkv=4, D=64, page=16, dtype="fp16", cache="int8",
@@ -153,18 +153,20 @@ def _tables(case, dev):
 
 
 def _encode(x, kind):
-    """(codes, scales) of the rows of x (fp32): the last dim's largest value over 127, or the
-    power of two that keeps it within 448; rows of next to nothing are zeros."""
+    """(codes, scales) of the rows of x (fp32): the power of two that keeps the last dim's largest
+    value within 127 or 448, as its exponent's byte; rows of next to nothing are zeros."""
     top = x.abs().amax(-1, keepdim=True)
     none = top < 2.0 ** -110
-    if kind == "int8":
-        scale = top / 127.0
-        codes = (x * (127.0 / top)).round_().masked_fill_(none, 0.0).to(torch.int8)
-    else:
-        m, e = torch.frexp(top / 448.0)
-        scale = torch.ldexp(torch.ones_like(top), e - (m == 0.5).to(e.dtype))
-        codes = (x / scale).masked_fill_(none, 0.0).to(torch.float8_e4m3fn)
-    return codes, scale.masked_fill(none, 0.0)[..., 0]
+    m, e = torch.frexp(top / (127.0 if kind == "int8" else 448.0))
+    e = (e - (m == 0.5).to(e.dtype)).masked_fill_(none, 0)
+    codes = torch.ldexp(x, -e).masked_fill_(none, 0.0)
+    codes = codes.round_().to(torch.int8) if kind == "int8" else codes.to(torch.float8_e4m3fn)
+    return codes, (e + 127).masked_fill_(none, 0).to(torch.uint8)[..., 0].view(torch.float8_e8m0fnu)
+
+
+def _power(scale):
+    """The powers of two that exponent bytes stand for, in 32 bits."""
+    return (scale.view(torch.uint8).to(torch.int32) << 23).view(torch.float32)
 
 
 def prepare(case, seed):
@@ -202,7 +204,7 @@ def prepare(case, seed):
         if case["cache"] == "same":
             return x.to(dt), None
         codes, scale = _encode(x.to(dt).float(), case["cache"])
-        return codes, scale.transpose(1, 2).contiguous()
+        return codes, scale.view(torch.uint8).transpose(1, 2).contiguous().view(scale.dtype)
 
     if op in ("append", "write"):
         T = case["T"]
@@ -248,7 +250,7 @@ def _put(s, x, name):
     page, slot = s["table"].long().gather(1, at // c["page"]), at % c["page"]
     codes, scale = _encode(x, c["cache"])
     s[name + "_cache"].view(torch.uint8)[page, slot] = codes.view(torch.uint8)
-    s[name + "_scale"].transpose(1, 2)[page, slot] = scale
+    s[name + "_scale"].view(torch.uint8).transpose(1, 2)[page, slot] = scale.view(torch.uint8)
 
 
 def _get(s, name):
@@ -260,7 +262,7 @@ def _get(s, name):
     page = s["table"].long().gather(1, torch.where(on, at // c["page"], torch.zeros_like(at))).clamp_min(0)
     slot = at % c["page"]
     codes = s[name + "_cache"].view(torch.uint8)[page, slot].view(CODES[c["cache"]]).float()
-    x = codes * s[name + "_scale"].transpose(1, 2)[page, slot][..., None]
+    x = codes * _power(s[name + "_scale"]).transpose(1, 2)[page, slot][..., None]
     return x.masked_fill_(~on[:, :, None, None], 0.0).to(TYPES[c["dtype"]])
 
 
@@ -289,7 +291,7 @@ def _values(s, name, at):
     x = s[name]
     x = x.view(torch.uint8)[at].view(x.dtype).float() if s[name + "_scale"] is not None else x[at].float()
     x = x.flatten(1, 2).transpose(1, 2)
-    return x if s[name + "_scale"] is None else x * s[name + "_scale"][at].transpose(1, 2).flatten(2)[..., None]
+    return x if s[name + "_scale"] is None else x * _power(s[name + "_scale"].view(torch.uint8)[at]).transpose(1, 2).flatten(2)[..., None]
 
 
 def _softmax(x):
@@ -383,7 +385,7 @@ def run(state):
 # -------------------------------------------------------------------- work
 def work(case):
     op, B, H, Hkv, D = (case[n] for n in ("op", "B", "H", "Hkv", "D"))
-    row = 2 * D if case["cache"] == "same" else D + 4  # bytes of a row in the cache
+    row = 2 * D if case["cache"] == "same" else D + 1  # bytes of a row in the cache
     n = np.array(_lengths(case), dtype=np.int64)
     if op in ("append", "write", "read"):
         tokens = case["tokens"] if op == "read" else case["length"]
@@ -416,12 +418,11 @@ def _exact_rows(x, kind):
     """What the cache keeps of the rows x [..., D] (64 bits)."""
     top = x.abs().max(-1, keepdim=True).values
     safe = top.clamp_min(2.0 ** -110)
+    s = torch.exp2(torch.ceil(torch.log2(safe / (127 if kind == "int8" else 448))))
+    y = x / s
     if kind == "int8":
-        kept = torch.round(x / safe * 127) * (safe / 127)
-    else:
-        s = torch.exp2(torch.ceil(torch.log2(safe / 448)))
-        y = x / s
-        # three bits behind the leading one, none below 2^-9
+        kept = torch.round(y) * s
+    else:  # three bits behind the leading one, none below 2^-9
         step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -30))).clamp_min(-6) - 3)
         kept = torch.round(y / step) * step * s
     return torch.where(top < 2.0 ** -110, torch.zeros_like(kept), kept)
@@ -432,7 +433,7 @@ def _exact_old(s, name, ids):
     x = s[name][ids].double().flatten(0, 1) if s[name].element_size() > 1 else \
         s[name].view(torch.uint8)[ids].view(s[name].dtype).float().double().flatten(0, 1)
     scale = s[name.split("_")[0] + "_scale"]
-    return x if scale is None else x * scale[ids].double().transpose(1, 2).flatten(0, 1)[..., None]
+    return x if scale is None else x * scale.view(torch.uint8)[ids].double().sub(127).exp2().transpose(1, 2).flatten(0, 1)[..., None]
 
 
 def _exact_turn(x, w, cos, sin, interleaved):
