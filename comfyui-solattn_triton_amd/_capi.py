@@ -68,6 +68,16 @@ SIGNATURES = {
     "solattn_paged_attn_workspace_bytes": ([_l] * 8, _l),
     "solattn_paged_attn": ([_p, _l, _l] + [_p, _l, _l, _l] * 2 + [_l, _l, _p, _l, _l, _p] + [_l] * 4
                            + [_i, _l, _l, _f, _p, _l, _p, _l, _l, _p], _i),
+    "solattn_qk_norm_rope_append8": ([_p, _l, _l, _l] * 3 + [_l] * 5 + [_i] + [_p] * 4 + [_l, _l, _i, _f]
+                                     + [_p, _l, _l, _l] * 3 + [_l, _l, _i] + [_p, _l, _l] * 2 + [_p, _l, _l, _p, _p],
+                                     _i),
+    "solattn_cache_append": ([_p, _l, _l, _l] * 2 + [_l] * 4 + [_i] + [_p, _l, _l, _l] * 2 + [_l, _l, _i]
+                             + [_p, _l, _l] * 2 + [_p, _l, _l, _p, _p], _i),
+    "solattn_cache_read": ([_p, _l, _l, _l] * 2 + [_l, _l, _i] + [_p, _l, _l] * 2 + [_p, _l, _l, _p, _p] + [_l] * 4
+                           + [_i] + [_p, _l, _l, _l] * 2 + [_p], _i),
+    "solattn_paged_attn_shared_workspace_bytes": ([_l] * 8 + [_i, _l, _l], _l),
+    "solattn_paged_attn_shared": ([_p, _l, _l] + [_p, _l, _l, _l] * 2 + [_l, _l, _i] + [_p, _l, _l] * 2
+                                  + [_p, _l, _l, _p] + [_l] * 4 + [_i] + [_l] * 4 + [_f, _p, _l, _p, _l, _l, _p], _i),
 }
 
 # Size of the per-device scratch array behind solattn_sol_attn_noalloc

@@ -37,7 +37,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
                         v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                         q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                         cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, *,
-                        eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+                        eps: float = 1e-6, interleaved: bool = False, k_scale: torch.Tensor | None = None,
+                        v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """``qk_norm_rope`` of the newest T tokens of B sequences: returns q', and writes
     k' and v to the tokens' places in the cache.
 
@@ -48,6 +49,9 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
     or on a page id that the cache does not have writes nothing, and its q' means
     nothing. Positions past the end of ``cos`` turn by its last row: it has to cover
     the sequences. Has no gradient.
+
+    With ``k_scale`` and ``v_scale`` the caches are of 8 bits (``_cache``): k' and v are
+    rounded to codes, k' once, from 32 bits.
     """
     return native.qk_norm_rope_append(q, k, v, k_cache, v_cache, page_table, lengths, q_weight, k_weight, cos, sin,
-                                      eps, interleaved)
+                                      eps, interleaved, k_scale, v_scale)

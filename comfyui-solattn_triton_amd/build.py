@@ -25,7 +25,7 @@ NATIVE = os.path.join(HERE, "_native.so")
 ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "reorder.hip", "prep.hip", "quant.hip", "fwd_bf16.hip", "fwd_int8.hip",
-           "qk_rope.hip", "window.hip", "paged.hip"]
+           "qk_rope.hip", "window.hip", "paged.hip", "cache.hip"]
 STRICT_FP = {"prep.hip", "quant.hip"}
 # clang 22 (ROCm 7.2) segfaults in SimplifyCFG's common-code sinking on the
 # INT8 forward; switching that one transform off builds it.

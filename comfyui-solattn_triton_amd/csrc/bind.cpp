@@ -43,8 +43,11 @@ struct Library {
   decltype(&solattn_window_attn_workspace_bytes) window_attn_workspace_bytes = nullptr;
   decltype(&solattn_window_attn_bwd) window_attn_bwd = nullptr;
   decltype(&solattn_window_attn_bwd_workspace_bytes) window_attn_bwd_workspace_bytes = nullptr;
-  decltype(&solattn_paged_attn) paged_attn = nullptr;
-  decltype(&solattn_paged_attn_workspace_bytes) paged_attn_workspace_bytes = nullptr;
+  decltype(&solattn_paged_attn_shared) paged_attn_shared = nullptr;
+  decltype(&solattn_paged_attn_shared_workspace_bytes) paged_attn_shared_workspace_bytes = nullptr;
+  decltype(&solattn_qk_norm_rope_append8) qk_norm_rope_append8 = nullptr;
+  decltype(&solattn_cache_append) cache_append = nullptr;
+  decltype(&solattn_cache_read) cache_read = nullptr;
 } lib;
 
 // A libsolattn call that returned a status; raised as _capi.SolAttnError.
@@ -80,18 +83,18 @@ struct Named {
   const char* name;
   const Tensor& t;
 };
-void check_rows(const Tensor& q, std::initializer_list<Named> others, bool fp32) {
-  if (!q.is_cuda()) refuse("q is not a GPU tensor");
+void check_rows(const Tensor& q, std::initializer_list<Named> others, bool fp32, const char* name = "q") {
+  if (!q.is_cuda()) refuse(name, " is not a GPU tensor");
   const auto type = q.scalar_type();
   if (type != at::kBFloat16 && type != at::kHalf && !(fp32 && type == at::kFloat))
-    refuse("q dtype ", type, "; bfloat16", fp32 ? ", float16 or float32" : " or float16");
-  if (q.dim() != 4) refuse("q must have 4 dimensions, got shape ", shape(q));
+    refuse(name, " dtype ", type, "; bfloat16", fp32 ? ", float16 or float32" : " or float16");
+  if (q.dim() != 4) refuse(name, " must have 4 dimensions, got shape ", shape(q));
   const int64_t D = q.size(3);
   for (const auto& o : others) {
     if (o.t.dim() != 4) refuse(o.name, " must have 4 dimensions, got shape ", shape(o.t));
-    if (o.t.scalar_type() != type) refuse(o.name, " dtype ", o.t.scalar_type(), " differs from q's ", type);
-    if (o.t.device() != q.device()) refuse(o.name, " is on ", o.t.device(), ", q on ", q.device());
-    if (o.t.size(3) != D) refuse(o.name, " has head_dim ", o.t.size(3), ", q ", D);
+    if (o.t.scalar_type() != type) refuse(o.name, " dtype ", o.t.scalar_type(), " differs from ", name, "'s ", type);
+    if (o.t.device() != q.device()) refuse(o.name, " is on ", o.t.device(), ", ", name, " on ", q.device());
+    if (o.t.size(3) != D) refuse(o.name, " has head_dim ", o.t.size(3), ", ", name, " ", D);
   }
   if (D < 8 || D > kMaxHeadDim || D % 8)
     refuse("head_dim ", D, " not supported (multiples of 8 up to ", kMaxHeadDim, ")");
@@ -136,16 +139,66 @@ void check_window(const std::optional<int64_t>& window, int64_t sinks, double sc
 
 // A paged cache: k_cache and v_cache [pages, page_size, Hkv, D], page_table int32
 // [B, pages of a sequence], lengths int32 [B].
-void check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, const Tensor& q) {
+void check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, int64_t B,
+                 const at::Device& device) {
   if (k.sizes() != v.sizes()) refuse("cache shapes differ: ", shape(k), " ", shape(v));
   if (!rows_aligned(k) || !rows_aligned(v))  // read and written in place: a copy would not be the cache
     refuse("cache rows must be contiguous and 16-byte aligned, strides ", k.strides(), " ", v.strides());
   if (k.size(1) % 8 || k.size(1) == 0) refuse("page size ", k.size(1), " is not a multiple of 8");
-  const int64_t B = q.size(0);
   if (table.dim() != 2 || table.size(0) != B)
     refuse("page_table must be [", B, ", pages of a sequence], got ", shape(table));
-  check_int32(table, "page_table", table.sizes(), q.device());
-  check_int32(lengths, "lengths", {B}, q.device());
+  check_int32(table, "page_table", table.sizes(), device);
+  check_int32(lengths, "lengths", {B}, device);
+}
+
+// (the stride of a dim of one says nothing)
+int64_t scale_stride(const Tensor& t, int d) { return t.defined() && t.size(d) > 1 ? t.stride(d) : 0; }
+
+// A cache of codes: k_cache and v_cache of int8 or float8_e4m3fn, each with the rows'
+// powers of two, float8_e8m0fnu [pages, Hkv, page_size]. Returns the library's cache_type.
+int check_codes(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, int64_t D,
+                const at::Device& device) {
+  if (!ks || !vs) refuse("k_scale and v_scale go together");
+  const auto type = k.scalar_type();
+  if (type != at::kChar && type != at::kFloat8_e4m3fn)
+    refuse("k_cache dtype ", type, " with scales; int8 or float8_e4m3fn");
+  if (v.scalar_type() != type) refuse("v_cache dtype ", v.scalar_type(), " differs from k_cache's ", type);
+  if (k.dim() != 4 || v.dim() != 4) refuse("caches must have 4 dimensions, got ", shape(k), " ", shape(v));
+  if (k.device() != device || v.device() != device)
+    refuse("caches are on ", k.device(), " and ", v.device(), ", the call on ", device);
+  if (k.size(3) != D) refuse("k_cache has head_dim ", k.size(3), ", the call ", D);
+  if (D < 16 || D > kMaxHeadDim || D % 16)
+    refuse("head_dim ", D, " of an 8-bit cache (multiples of 16 up to ", kMaxHeadDim, ")");
+  for (const Tensor& t : {*ks, *vs}) {
+    const int64_t want[3] = {k.size(0), k.size(2), k.size(1)};
+    if (t.scalar_type() != at::kFloat8_e8m0fnu || t.sizes() != at::IntArrayRef(want, 3) || t.device() != device)
+      refuse("scales must be float8_e8m0fnu of shape ", at::IntArrayRef(want, 3), " on ", device, ", got ",
+             t.scalar_type(), " ", t.sizes(), " on ", t.device());
+    if (t.stride(2) != 1 || (scale_stride(t, 0) | scale_stride(t, 1)) % 8 ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % 8)
+      refuse("a page's scales of a head must be contiguous and 8-byte aligned, strides ", t.strides());
+  }
+  return type == at::kChar ? SOLATTN_INT8 : SOLATTN_E4M3;
+}
+
+// k's and v's tensors that a call writes to in place.
+void check_written(const Tensor& k, const Tensor& v) {
+  for (const Tensor& c : {k, v})
+    for (int64_t d = 0; d + 1 < c.dim(); ++d)
+      if (c.stride(d) == 0 && c.size(d) > 1) refuse("a cache to write to is expanded: strides ", c.strides());
+}
+void check_apart(const Tensor& k, const Tensor& v) {
+  if (k.numel() && k.data_ptr() == v.data_ptr()) refuse("k_cache and v_cache are the same memory");
+}
+void written(std::initializer_list<Tensor> ts) {  // (a backward pass that has kept the cache finds it changed)
+  for (const Tensor& c : ts)
+    if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
+}
+
+// (a table without pages is never read, but its address must not be null)
+Tensor page_rows(const Tensor& table, const Tensor& lengths) {
+  if (table.size(1) == 0) return lengths;
+  return table.size(1) > 1 && table.stride(1) != 1 ? table.contiguous() : table;
 }
 
 Tensor tensor(const OptTensor& t) { return t.value_or(Tensor()); }
@@ -330,45 +383,126 @@ std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, const
   return rope_forward(q, k, p);
 }
 
+#define SCALES(t) ptr_as<uint8_t>(t), scale_stride(t, 0), scale_stride(t, 1)
+
 Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& k_cache,
                            const Tensor& v_cache, const Tensor& table0, const Tensor& lengths0, const OptTensor& qw,
                            const OptTensor& kw, const OptTensor& cos, const OptTensor& sin, double eps,
-                           bool interleaved) {
-  refuse_recording("qk_norm_rope_append");
-  refuse_tangents("qk_norm_rope_append",
-                  {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw), tensor(cos), tensor(sin)});
-  refuse_grad("qk_norm_rope_append", {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw)});
-  check_rows(q0, {{"k", k0}, {"v", v0}, {"k_cache", k_cache}, {"v_cache", v_cache}}, true);
+                           bool interleaved, const OptTensor& k_scale, const OptTensor& v_scale) {
+  const char* what = "qk_norm_rope_append";
+  refuse_recording(what);
+  refuse_tangents(what, {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw), tensor(cos), tensor(sin)});
+  refuse_grad(what, {q0, k0, v0, k_cache, v_cache, tensor(qw), tensor(kw)});
+  const bool codes = k_scale || v_scale;
+  int cache_type = 0;
+  if (codes) {
+    check_rows(q0, {{"k", k0}, {"v", v0}}, true);
+    cache_type = check_codes(k_cache, v_cache, k_scale, v_scale, q0.size(3), q0.device());
+  } else {
+    check_rows(q0, {{"k", k0}, {"v", v0}, {"k_cache", k_cache}, {"v_cache", v_cache}}, true);
+  }
   const int64_t B = q0.size(0), T = q0.size(1), H = q0.size(2), Hkv = k0.size(2);
   if (k0.size(0) != B || k0.size(1) != T || k0.sizes() != v0.sizes() || k_cache.size(2) != Hkv)
     refuse("shapes do not match: q ", shape(q0), " k ", shape(k0), " v ", shape(v0), " cache ", shape(k_cache));
   check_kv_heads(H, Hkv);
-  check_cache(k_cache, v_cache, table0, lengths0, q0);
-  for (const Tensor& c : {k_cache, v_cache})
-    for (int d = 0; d < 3; ++d)
-      if (c.stride(d) == 0 && c.size(d) > 1) refuse("a cache to write to is expanded: strides ", c.strides());
+  check_cache(k_cache, v_cache, table0, lengths0, B, q0.device());
+  check_written(k_cache, v_cache);
+  if (codes) check_written(*k_scale, *v_scale);
   const RopePlan p = rope_plan(q0, qw, kw, cos, sin, eps, interleaved);
-  if (k_cache.numel() && k_cache.data_ptr() == v_cache.data_ptr()) refuse("k_cache and v_cache are the same memory");
+  check_apart(k_cache, v_cache);
+  if (codes) check_apart(*k_scale, *v_scale);
   const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0);
-  const Tensor table = table0.size(1) > 1 && table0.stride(1) != 1 ? table0.contiguous() : table0;
-  const Tensor lengths = lengths0.contiguous();
+  const Tensor lengths = lengths0.contiguous(), table = page_rows(table0, lengths);
   Tensor qo = at::empty(q.sizes(), q.options());
   if (q.numel() == 0) return qo;
   // a cache without pages is never written, but its address must not be null
   const bool none = k_cache.numel() == 0;
   const Tensor &kc = none ? k : k_cache, &vc = none ? v : v_cache;
+  const int64_t pages = none ? 0 : k_cache.size(0), page = k_cache.size(1);
   const c10::OptionalDeviceGuard guard(q.device());
+  if (codes) {
+    const Tensor &ks = none ? table : *k_scale, &vs = none ? table : *v_scale;
+    const auto stride = [none](const Tensor& t, int d) { return none ? 0 : t.stride(d); };
+    check(lib.qk_norm_rope_append8(
+              ptr(q), STRIDES(q), ptr(k), STRIDES(k), ptr(v), STRIDES(v), B, T, H, Hkv, q.size(3), type_code(q),
+              ptr_as<float>(p.qw), ptr_as<float>(p.kw), ptr_as<float>(p.cos), ptr_as<float>(p.sin), p.P, p.R,
+              interleaved, static_cast<float>(eps), ptr(qo), STRIDES(qo), ptr(kc), stride(kc, 0), stride(kc, 1),
+              stride(kc, 2), ptr(vc), stride(vc, 0), stride(vc, 1), stride(vc, 2), pages, page, cache_type,
+              SCALES(ks), SCALES(vs),
+              ptr_as<int32_t>(table), table.stride(0), table0.size(1), ptr_as<int32_t>(lengths), stream_of(q)),
+          "solattn_qk_norm_rope_append8");
+    written({k_cache, v_cache, *k_scale, *v_scale});
+    return qo;
+  }
   check(lib.qk_norm_rope_append(
             ptr(q), STRIDES(q), ptr(k), STRIDES(k), ptr(v), STRIDES(v), B, T, H, Hkv, q.size(3), type_code(q),
             ptr_as<float>(p.qw), ptr_as<float>(p.kw), ptr_as<float>(p.cos), ptr_as<float>(p.sin), p.P, p.R, interleaved,
-            static_cast<float>(eps), ptr(qo), STRIDES(qo), ptr(kc), STRIDES(kc), ptr(vc), STRIDES(vc),
-            none ? 0 : k_cache.size(0), k_cache.size(1), ptr_as<int32_t>(table), table.stride(0), table.size(1),
-            ptr_as<int32_t>(lengths), stream_of(q)),
+            static_cast<float>(eps), ptr(qo), STRIDES(qo), ptr(kc), STRIDES(kc), ptr(vc), STRIDES(vc), pages, page,
+            ptr_as<int32_t>(table), table.stride(0), table0.size(1), ptr_as<int32_t>(lengths), stream_of(q)),
         "solattn_qk_norm_rope_append");
-  // (a backward pass that has kept the cache finds it changed)
-  for (const Tensor& c : {k_cache, v_cache})
-    if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
+  written({k_cache, v_cache});
   return qo;
+}
+
+// -------------------------------------------------------------- 8-bit caches
+void cache_append(const Tensor& k0, const Tensor& v0, const Tensor& k_cache, const Tensor& v_cache,
+                  const Tensor& table0, const Tensor& lengths0, const OptTensor& k_scale, const OptTensor& v_scale) {
+  const char* what = "cache_append";
+  refuse_recording(what);
+  refuse_tangents(what, {k0, v0, k_cache, v_cache});
+  refuse_grad(what, {k0, v0, k_cache, v_cache});
+  check_rows(k0, {{"v", v0}}, true, "k");
+  const int64_t B = k0.size(0), T = k0.size(1), Hkv = k0.size(2), D = k0.size(3);
+  const int cache_type = check_codes(k_cache, v_cache, k_scale, v_scale, D, k0.device());
+  if (k0.sizes() != v0.sizes() || k_cache.size(2) != Hkv)
+    refuse("shapes do not match: k ", shape(k0), " v ", shape(v0), " cache ", shape(k_cache));
+  check_cache(k_cache, v_cache, table0, lengths0, B, k0.device());
+  check_written(k_cache, v_cache);
+  check_written(*k_scale, *v_scale);
+  check_apart(k_cache, v_cache);
+  check_apart(*k_scale, *v_scale);
+  if (k0.numel() == 0 || k_cache.numel() == 0) return;
+  const Tensor k = as_rows(k0), v = as_rows(v0), lengths = lengths0.contiguous(), table = page_rows(table0, lengths);
+  const c10::OptionalDeviceGuard guard(k.device());
+  check(lib.cache_append(ptr(k), STRIDES(k), ptr(v), STRIDES(v), B, T, Hkv, D, type_code(k), ptr(k_cache),
+                         STRIDES(k_cache), ptr(v_cache), STRIDES(v_cache), k_cache.size(0), k_cache.size(1), cache_type,
+                         SCALES(*k_scale), SCALES(*v_scale), ptr_as<int32_t>(table), table.stride(0), table0.size(1),
+                         ptr_as<int32_t>(lengths), stream_of(k)),
+        "solattn_cache_append");
+  written({k_cache, v_cache, *k_scale, *v_scale});
+}
+
+std::pair<Tensor, Tensor> cache_read(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table0,
+                                     const Tensor& lengths0, const OptTensor& k_scale, const OptTensor& v_scale,
+                                     int64_t tokens, const OptTensor& start0, at::ScalarType dtype) {
+  const char* what = "cache_read";
+  refuse_recording(what);
+  refuse_tangents(what, {k_cache, v_cache});
+  refuse_grad(what, {k_cache, v_cache});
+  if (!k_cache.is_cuda()) refuse("k_cache is not a GPU tensor");
+  if (k_cache.dim() != 4) refuse("k_cache must have 4 dimensions, got shape ", shape(k_cache));
+  const auto device = k_cache.device();
+  const int64_t D = k_cache.size(3), Hkv = k_cache.size(2);
+  const int cache_type = check_codes(k_cache, v_cache, k_scale, v_scale, D, device);
+  if (dtype != at::kBFloat16 && dtype != at::kHalf) refuse("dtype ", dtype, "; bfloat16 or float16");
+  if (tokens < 0) refuse(tokens, " tokens");
+  if (table0.dim() != 2) refuse("page_table must be [sequences, pages of a sequence], got ", shape(table0));
+  const int64_t B = table0.size(0);
+  check_cache(k_cache, v_cache, table0, lengths0, B, device);
+  if (start0) check_int32(*start0, "start", {B}, device);
+  const auto options = k_cache.options().dtype(dtype);
+  Tensor k = at::empty({B, tokens, Hkv, D}, options), v = at::empty({B, tokens, Hkv, D}, options);
+  if (k.numel() == 0) return {k, v};
+  if (k_cache.numel() == 0) return {k.zero_(), v.zero_()};
+  const Tensor lengths = lengths0.contiguous(), table = page_rows(table0, lengths);
+  const Tensor start = start0 ? start0->contiguous() : Tensor();
+  const c10::OptionalDeviceGuard guard(device);
+  check(lib.cache_read(ptr(k_cache), STRIDES(k_cache), ptr(v_cache), STRIDES(v_cache), k_cache.size(0), k_cache.size(1),
+                       cache_type, SCALES(*k_scale), SCALES(*v_scale), ptr_as<int32_t>(table), table.stride(0),
+                       table0.size(1), ptr_as<int32_t>(lengths), ptr_as<int32_t>(start), B, tokens, Hkv, D, type_code(k),
+                       ptr_as<U16>(k), STRIDES(k), ptr_as<U16>(v), STRIDES(v), stream_of(k)),
+        "solattn_cache_read");
+  return {k, v};
 }
 
 // ------------------------------------------------------------------- windows
@@ -469,33 +603,45 @@ Tensor window_attn(const Tensor& q0, const Tensor& k0, const Tensor& v0, std::op
 
 // --------------------------------------------------------------------- pages
 Tensor paged_attn(const Tensor& q0, const Tensor& k, const Tensor& v, const Tensor& table0, const Tensor& lengths0,
-                  std::optional<int64_t> window, int64_t sinks, std::optional<double> scale0) {
+                  std::optional<int64_t> window, int64_t sinks, std::optional<double> scale0, const OptTensor& k_scale,
+                  const OptTensor& v_scale, int64_t shared, int64_t groups) {
   refuse_recording("paged_attn");
   refuse_tangents("paged_attn", {q0, k, v});
   refuse_grad("paged_attn", {q0, k, v});
-  check_rows(q0, {{"k_cache", k}, {"v_cache", v}}, false);
+  int cache_type = 0;
+  if (k_scale || v_scale) {
+    check_rows(q0, {}, false);
+    cache_type = check_codes(k, v, k_scale, v_scale, q0.size(3), q0.device());
+  } else {
+    check_rows(q0, {{"k_cache", k}, {"v_cache", v}}, false);
+  }
   const int64_t B = q0.size(0), H = q0.size(2), D = q0.size(3), Hkv = k.size(2), pages = k.size(0), page = k.size(1);
   const double scale = scale0 ? *scale0 : 1.0 / std::sqrt(static_cast<double>(D));
   check_window(window, sinks, scale);
   if (q0.size(1) != 1) refuse("q holds ", q0.size(1), " tokens of a sequence; one");
   check_kv_heads(H, Hkv);
-  check_cache(k, v, table0, lengths0, q0);
+  check_cache(k, v, table0, lengths0, B, q0.device());
+  if (shared < 0) refuse("shared ", shared);
+  if (groups < 1 || B % groups) refuse(B, " sequences in ", groups, " groups");
+  if (shared && (window || sinks)) refuse("shared keys and a window: what windows leave of them differs");
   Tensor out = at::empty({B, 1, H, D}, q0.options());
   if (B == 0) return out;
   const int64_t max_pages = table0.size(1);
   if (pages == 0 || max_pages == 0) return out.zero_();
   const Tensor q = as_rows(q0);
-  const Tensor table = max_pages > 1 && table0.stride(1) != 1 ? table0.contiguous() : table0;
-  const Tensor lengths = lengths0.contiguous();
+  const Tensor lengths = lengths0.contiguous(), table = page_rows(table0, lengths);
   const int64_t top = (1ll << 31) - 1, w = window ? std::min(*window, top) : 0;
   sinks = std::min(sinks, top);
+  shared = std::min(shared, top);
   const c10::OptionalDeviceGuard guard(q.device());
-  const int64_t need = lib.paged_attn_workspace_bytes(B, H, Hkv, D, max_pages, page, w, sinks);
+  const int64_t need =
+      lib.paged_attn_shared_workspace_bytes(B, H, Hkv, D, max_pages, page, w, sinks, cache_type, shared, groups);
   const Tensor ws = workspace(need, q);
-  check(lib.paged_attn(ptr_as<U16>(q), q.stride(0), q.stride(2), ptr_as<U16>(k), STRIDES(k), ptr_as<U16>(v), STRIDES(v),
-                       pages, page, ptr_as<int32_t>(table), table.stride(0), max_pages, ptr_as<int32_t>(lengths), B, H,
-                       Hkv, D, type_code(q), w, sinks, static_cast<float>(scale), ptr(ws), need, ptr_as<U16>(out),
-                       out.stride(0), out.stride(2), stream_of(q)),
+  const Tensor ks = tensor(k_scale), vs = tensor(v_scale);
+  check(lib.paged_attn_shared(
+            ptr_as<U16>(q), q.stride(0), q.stride(2), ptr(k), STRIDES(k), ptr(v), STRIDES(v), pages, page, cache_type,
+            SCALES(ks), SCALES(vs), ptr_as<int32_t>(table), table.stride(0), max_pages, ptr_as<int32_t>(lengths), B, H, Hkv, D, type_code(q), w, sinks, shared, groups,
+            static_cast<float>(scale), ptr(ws), need, ptr_as<U16>(out), out.stride(0), out.stride(2), stream_of(q)),
         "solattn_paged_attn");
   return out;
 }
@@ -520,8 +666,11 @@ PYBIND11_MODULE(_native, m) {
     take(lib.window_attn_workspace_bytes, at, "solattn_window_attn_workspace_bytes");
     take(lib.window_attn_bwd, at, "solattn_window_attn_bwd");
     take(lib.window_attn_bwd_workspace_bytes, at, "solattn_window_attn_bwd_workspace_bytes");
-    take(lib.paged_attn, at, "solattn_paged_attn");
-    take(lib.paged_attn_workspace_bytes, at, "solattn_paged_attn_workspace_bytes");
+    take(lib.paged_attn_shared, at, "solattn_paged_attn_shared");
+    take(lib.paged_attn_shared_workspace_bytes, at, "solattn_paged_attn_shared_workspace_bytes");
+    take(lib.qk_norm_rope_append8, at, "solattn_qk_norm_rope_append8");
+    take(lib.cache_append, at, "solattn_cache_append");
+    take(lib.cache_read, at, "solattn_cache_read");
   });
   py::register_local_exception_translator([](std::exception_ptr p) {
     try {
@@ -534,4 +683,6 @@ PYBIND11_MODULE(_native, m) {
   m.def("qk_norm_rope_append", &qk_norm_rope_append);
   m.def("window_attn", &window_attn);
   m.def("paged_attn", &paged_attn);
+  m.def("cache_append", &cache_append);
+  m.def("cache_read", &cache_read);
 }

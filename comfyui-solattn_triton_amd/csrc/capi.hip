@@ -116,7 +116,7 @@ using namespace solattn;
 
 extern "C" const char* solattn_last_error(void) { return g_error; }
 
-extern "C" int solattn_abi_version(void) { return (2 << 16) | 3; }
+extern "C" int solattn_abi_version(void) { return (2 << 16) | 4; }
 
 extern "C" int solattn_morton_perm(int64_t frames, int64_t height, int64_t width, int curve,
                                    int64_t roll, int64_t* perm, int64_t* inverse) {

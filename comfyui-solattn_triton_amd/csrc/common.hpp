@@ -186,13 +186,34 @@ int fwd_int8(const uint16_t* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const 
 // Attention of one token per sequence over a cache, split over its length (paged.hip).
 // table null: sequence b is page b, and the token sits at position length - 1 of the
 // sequences that lengths (if any) says are that long.
-int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k, int64_t sk_p, int64_t sk_s,
-               int64_t sk_h, const uint16_t* v, int64_t sv_p, int64_t sv_s, int64_t sv_h, int64_t pages,
-               int64_t page_size, const int32_t* table, int64_t table_stride, int64_t max_pages,
-               const int32_t* lengths, int64_t length, int64_t B, int64_t H, int64_t Hkv, int64_t D, int dtype,
-               int64_t window, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, uint16_t* o,
-               int64_t so_b, int64_t so_h, hipStream_t s, const char* what);
+struct PagedCall {
+  const uint16_t* q;
+  int64_t sq_b, sq_h;
+  const void* k;  // strides in elements, as all others
+  int64_t sk_p, sk_s, sk_h;
+  const void* v;
+  int64_t sv_p, sv_s, sv_h;
+  const uint8_t* ks;  // cache_type not 0: exponent bytes
+  int64_t ks_p, ks_h;
+  const uint8_t* vs;
+  int64_t vs_p, vs_h;
+  int cache_type;
+  int64_t pages, page_size;
+  const int32_t* table;
+  int64_t table_stride, max_pages;
+  const int32_t* lengths;
+  int64_t length;
+  int64_t B, H, Hkv, D;
+  int dtype;
+  int64_t window, sinks, shared, groups;
+  float scale;
+  void* workspace;
+  int64_t workspace_bytes;
+  uint16_t* o;
+  int64_t so_b, so_h;
+};
+int paged_attn(const PagedCall& call, hipStream_t s, const char* what);
 int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
-                             int64_t sinks);
+                             int64_t sinks, int64_t shared = 0, int64_t groups = 1);
 
 }  // namespace solattn

@@ -20,23 +20,38 @@
 //     and transposes them in registers (v_perm_b32), one A operand per channel of
 //     the D / 16: row i of operand j is channel (D / 16) i + j.
 // The row's statistics need an exchange between the lanes g only.
-#include "elem.hpp"
+#include "cache8.hpp"
 
 namespace solattn {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kStep = 32;       // keys of a wave's step
-constexpr int kMaxSplits = 64;
+constexpr int kBlock = 32;      // keys of a block of products
+constexpr int kMaxSplits = 64;  // parts of a row
+constexpr int kMaxShared = 48;  // of these over shared keys
 constexpr int kGroups = 16;     // query columns of a tile
+
+// What the cache holds: 16-bit values of the queries' type, or codes (cache8.hpp).
+struct SameType {};
+template <typename C>
+constexpr bool kCodes = !__is_same(C, SameType);
+// Keys of a wave's step: 16 KiB of 128 channels are in flight either way.
+template <typename C>
+constexpr int kBlocks = kCodes<C> ? 2 : 1;
+template <typename C>
+constexpr int kStep = kBlock * kBlocks<C>;
 
 struct PagedArgs {
   const uint16_t* q;
   int64_t sq_b, sq_h;
-  const uint16_t* k;
+  const uint8_t* k;          // strides in bytes
   int64_t sk_p, sk_s, sk_h;
-  const uint16_t* v;
+  const uint8_t* v;
   int64_t sv_p, sv_s, sv_h;
+  const uint8_t* ks;         // codes: exponent bytes
+  int64_t ks_p, ks_h;
+  const uint8_t* vs;
+  int64_t vs_p, vs_h;
   const int32_t* table;      // null: sequence b is page b
   int64_t table_b;
   const int32_t* lengths;    // with a table: each sequence's. Without: one shorter than `length` holds no token
@@ -45,12 +60,16 @@ struct PagedArgs {
   Divisor by_page;
   uint16_t* o;
   int64_t so_b, so_h;
-  float* part;               // split > 1: [B][H][split][D] sums, then [B][H][split][2] max and sum
+  float* part;               // parts > 1: [B][H][parts][D] sums, then [B][H][parts][2] max and sum
   int64_t part_ml;           // where the latter begin
   int B, H, Hkv, D, group, tiles, split;
   Divisor by_tiles, by_hkv, by_split;
   int window, sinks;         // window 0: none
   float c;                   // scale log2(e)
+  // Keys in common: of `per` sequences each the first `shared`, cut into psplit parts, for
+  // ptiles tiles of columns; the launch's first pitems workgroups. parts: psplit + split.
+  int shared, per, psplit, ptiles, pitems, parts;
+  Divisor by_ptiles, by_psplit, by_group;
 };
 
 __device__ __forceinline__ float over_groups_max(float x) {
@@ -71,73 +90,106 @@ __device__ __forceinline__ float weight_of(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
 }
 
-// The visible keys as steps of 32: first those of the sinks below the window, then the window's.
+__device__ __forceinline__ int sequence_length(const PagedArgs& a, int b) {
+  const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
+  int n = a.lengths ? a.lengths[b] : a.length;
+  if (!a.table) n = n < a.length ? 0 : a.length;
+  return static_cast<int>(min(static_cast<int64_t>(max(n, 0)), cap));
+}
+
+// The visible keys as steps: first those of the sinks below the window, then the window's.
 struct Visible {
   int len, low;        // keys [low, len) and [0, sinks_end)
   int sinks_end;       // <= low
   int sink_steps, first, steps;  // the window's steps begin at key `first`
 };
-__device__ __forceinline__ Visible visible(const PagedArgs& a, int b) {
+template <typename C>
+__device__ __forceinline__ Visible visible(int len, int low, int sinks) {
+  constexpr int S = kStep<C>;
   Visible s;
-  const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
-  int n = a.lengths ? a.lengths[b] : a.length;
-  if (!a.table) n = n < a.length ? 0 : a.length;
-  s.len = static_cast<int>(min(static_cast<int64_t>(max(n, 0)), cap));
-  s.low = a.window ? max(s.len - a.window, 0) : 0;
-  s.sinks_end = min(a.sinks, s.low);
-  s.sink_steps = (s.sinks_end + kStep - 1) / kStep;
-  s.first = s.low & ~(kStep - 1);
-  s.steps = s.sink_steps + (s.len - s.first + kStep - 1) / kStep;
+  s.len = len, s.low = min(low, len);
+  s.sinks_end = min(sinks, s.low);
+  s.sink_steps = (s.sinks_end + S - 1) / S;
+  s.first = s.low & ~(S - 1);
+  s.steps = s.sink_steps + (len - s.first + S - 1) / S;
   return s;
 }
 
-// DP: the head dim that the registers hold; D < DP (kFull false) leaves the rest zero.
-template <typename E, int DP, bool kFull>
-__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
-paged_kernel(const PagedArgs a) {
-  constexpr int NC = DP / 32;   // 32-channel pieces of a score
-  constexpr int CH = DP / 16;   // channels of a lane's V piece = operands of the second product
-  constexpr int VW = CH / 2;    // their registers
-  __shared__ float lds_o[kWaves][kGroups][DP + 4];
-  __shared__ float lds_m[kWaves][kGroups], lds_l[kWaves][kGroups];
+// A workgroup's keys and columns. The columns of own keys are the heads of one sequence
+// that share a kv head, those of shared keys the heads of all its sequences.
+struct Work {
+  Visible vis;
+  int step0, step1, part;
+  int b, seq;          // whose pages; the first column's sequence
+  int hk, col0, ncol;  // columns col0 .. col0 + ncol - 1 of the kv head
+  __device__ __forceinline__ void row(const PagedArgs& a, int c, bool many, int& b, int& h) const {
+    uint32_t n = col0 + min(c, ncol - 1);
+    const uint32_t g = many ? a.by_group.split(n) : n;
+    b = many ? seq + static_cast<int>(n) : seq;
+    h = hk * a.group + static_cast<int>(g);
+  }
+};
 
-  fetch_arguments(a);
+template <int DP>
+struct PagedLds {
+  float o[kWaves][kGroups][DP + 4];
+  float m[kWaves][kGroups], l[kWaves][kGroups];
+};
+
+// DP: the head dim that the registers hold; D < DP (kFull false) leaves the rest zero.
+// NT: tiles of 16 columns. MANY: the columns are of several sequences.
+template <typename E, typename C, int DP, bool kFull, int NT, bool MANY>
+__device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, const Work& w) {
+  constexpr bool Q8 = kCodes<C>;
+  constexpr int KB = kBlocks<C>, S = kStep<C>;
+  constexpr int NC = DP / 32;           // products of a score tile
+  constexpr int KL = Q8 ? NC / 2 : NC;  // 16-byte pieces of a key that a lane reads
+  constexpr int CH = DP / 16;           // channels of a lane's V piece = operands of the second product
+  constexpr int VW = Q8 ? CH / 4 : CH / 2;  // their registers
+  constexpr int ES = Q8 ? 1 : 2;        // bytes of a value
+  constexpr int NP = Q8 ? 2 : 1;        // roundings of P (below)
+
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  uint32_t w = blockIdx.x;
-  const int tile = a.by_tiles.split(w), hk = a.by_hkv.split(w), split = a.by_split.split(w), b = w;
-  const int ncol = min(kGroups, a.group - tile * kGroups);
-  const int head0 = hk * a.group + tile * kGroups;
+  const Visible& vis = w.vis;
+  const int hk = w.hk;
 
-  const Visible vis = visible(a, b);
-  const int per = a.by_split.of(vis.steps + a.split - 1);
-  const int step0 = split * per, step1 = min(step0 + per, vis.steps);
-  if (step0 >= step1 && a.split > 1) {  // nothing here: the join passes over a sum of 0
-    if (static_cast<int>(threadIdx.x) < ncol)
-      reinterpret_cast<float2*>(a.part + a.part_ml)[(static_cast<int64_t>(b) * a.H + head0 + threadIdx.x) * a.split + split] =
-          make_float2(-INFINITY, 0.f);
-    return;
-  }
-
-  bf16x8 q[NC];
-  {
-    const uint16_t* qp = a.q + b * a.sq_b + (head0 + min(col, ncol - 1)) * a.sq_h;
+  // Channels of product cc that this lane holds of q and of a key: eight from
+  // 32 cc + 8 g on, of codes, read 16 bytes at a time, from 64 (cc / 2) + 16 g + 8 (cc % 2).
+  bf16x8 q[NT][NC];
+  int hi[NT], safe = vis.len;  // MANY: keys that a column sees; that every one does
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    int b, h;
+    w.row(a, 16 * t + col, MANY, b, h);
+    const uint16_t* qp = a.q + b * a.sq_b + h * a.sq_h;
+    hi[t] = MANY ? min(sequence_length(a, b), vis.len) : vis.len;
+    safe = min(safe, hi[t]);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-      const int ch = 32 * cc + 8 * g;
+      const int ch = Q8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (kFull || ch < a.D) x = *reinterpret_cast<const uint4*>(qp + ch);
-      q[cc] = __builtin_bit_cast(bf16x8, x);
+      q[t][cc] = __builtin_bit_cast(bf16x8, x);
     }
   }
-  f32x4 acc[CH];
+  if constexpr (MANY) {
 #pragma unroll
-  for (int j = 0; j < CH; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // l: this lane's keys
+    for (int o = 1; o < 16; o <<= 1) safe = min(safe, __shfl_xor(safe, o));
+    safe = __builtin_amdgcn_readfirstlane(safe);
+  }
+  f32x4 acc[NT][CH];
+  float m[NT], l[NT];  // l: this lane's keys
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[t] = -INFINITY, l[t] = 0.f;
+  }
 
   const int vch = kFull || CH * col < a.D ? CH * col : 0;
   const auto base_of = [&](int st) __attribute__((always_inline)) {
-    return st < vis.sink_steps ? st * kStep : vis.first + (st - vis.sink_steps) * kStep;
+    return st < vis.sink_steps ? st * S : vis.first + (st - vis.sink_steps) * S;
   };
   // Where the eight consecutive keys from j8 on are: they share a page (its size is a
   // multiple of 8, or the page is a whole sequence). Page ids are read a step ahead, so
@@ -146,132 +198,295 @@ paged_kernel(const PagedArgs a) {
     const uint32_t j = static_cast<uint32_t>(min(j8, max(vis.len - 1, 0) & ~7));
     const uint32_t pg = a.by_page.of(j);
     slot = static_cast<int>(j - pg * a.page);
-    return a.table ? a.table[b * a.table_b + pg] : b;
+    return a.table ? a.table[w.b * a.table_b + pg] : w.b;
   };
-  int kslot = 0, vslot = 0, kid = 0, vid = 0;
-  if (step0 + wave < step1) {
-    const int base = base_of(step0 + wave);
-    kid = slot_of(base + 8 * (col >> 2), kslot);
-    vid = slot_of(base + 8 * g, vslot);
-  }
-  for (int st = step0 + wave; st < step1; st += kWaves) {
+  int kslot[KB], vslot[KB], kid[KB], vid[KB];
+  const auto find = [&](int st) __attribute__((always_inline)) {
+    const int base = base_of(st);
+#pragma unroll
+    for (int u = 0; u < KB; ++u) {
+      kid[u] = slot_of(base + kBlock * u + 8 * (col >> 2), kslot[u]);
+      vid[u] = slot_of(base + kBlock * u + 8 * g, vslot[u]);
+    }
+  };
+  if (w.step0 + wave < w.step1) find(w.step0 + wave);
+  for (int st = w.step0 + wave; st < w.step1; st += kWaves) {
     const bool sink = st < vis.sink_steps;
     const int base = base_of(st);
-    const int lo = sink ? 0 : vis.low, hi = sink ? vis.sinks_end : vis.len;  // visible: lo <= j < hi
+    const int lo = sink ? 0 : vis.low, end = sink ? vis.sinks_end : vis.len;  // visible: lo <= j < end
     // Keys of page ids outside the cache are not visible (a key's score lane holds its V piece too).
-    const bool vok = vid >= 0 && vid < a.pages;
-    const int64_t kpage = kid >= 0 && kid < a.pages ? kid : 0, vpage = vok ? vid : 0;
+    bool vok[KB];
+    uint4 kr[KB][2][KL];
+    uint32_t vr[KB][8][VW];
+    uint2 ke[KB], ve[KB];  // exponents of the keys 8 g + 0..7
     const int last = a.page - 1;  // a slot past the page's end (a whole-sequence page) repeats its last
-    bf16x8 kr[2][NC];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t* kp = a.k + kpage * a.sk_p + static_cast<int64_t>(min(kslot + 4 * t + (col & 3), last)) * a.sk_s + hk * a.sk_h;
+    for (int u = 0; u < KB; ++u) {
+      vok[u] = vid[u] >= 0 && vid[u] < a.pages;
+      const int64_t kpage = kid[u] >= 0 && kid[u] < a.pages ? kid[u] : 0, vpage = vok[u] ? vid[u] : 0;
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) {
-        const int ch = 32 * cc + 8 * g;
-        kr[t][cc] = *reinterpret_cast<const bf16x8*>(kp + (kFull || ch < a.D ? ch : 0));
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t* kp = a.k + kpage * a.sk_p + static_cast<int64_t>(min(kslot[u] + 4 * t + (col & 3), last)) * a.sk_s + hk * a.sk_h;
+#pragma unroll
+        for (int cc = 0; cc < KL; ++cc) {
+          const int ch = Q8 ? 64 * cc + 16 * g : 32 * cc + 8 * g;
+          kr[u][t][cc] = *reinterpret_cast<const uint4*>(kp + (kFull || ch < a.D ? ES * ch : 0));
+        }
       }
-    }
-    uint32_t vr[8][VW];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t* vp = a.v + vpage * a.sv_p + static_cast<int64_t>(min(vslot + i, last)) * a.sv_s + hk * a.sv_h + vch;
-      if constexpr (VW == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(vp);
-        vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(vp);
-        vr[i][0] = x.x, vr[i][1] = x.y;
-      }
-    }
-    if (st + kWaves < step1) {
-      const int next = base_of(st + kWaves);
-      kid = slot_of(next + 8 * (col >> 2), kslot);
-      vid = slot_of(next + 8 * g, vslot);
-    }
-    f32x4 s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int cc = 0; cc < NC; ++cc) s[t] = E::mfma16(kr[t][cc], q[cc], s[t]);
-    }
-    // keys of this lane: base + 8 g + 4 t + i, i.e. those of its V piece
-    if (base < lo || base + kStep > hi || __any(!vok)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int j = base + 8 * g + i;
-        const bool on = vok && j >= lo && j < hi;
-        s[i >> 2][i & 3] = on ? s[i >> 2][i & 3] : -INFINITY;
-#pragma unroll
-        for (int r = 0; r < VW; ++r) vr[i][r] = on ? vr[i][r] : 0u;  // 0 P of a value that may be anything
+        const uint8_t* vp = a.v + vpage * a.sv_p + static_cast<int64_t>(min(vslot[u] + i, last)) * a.sv_s + hk * a.sv_h + ES * vch;
+        if constexpr (VW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vp);
+          vr[u][i][0] = x.x, vr[u][i][1] = x.y, vr[u][i][2] = x.z, vr[u][i][3] = x.w;
+        } else if constexpr (VW == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(vp);
+          vr[u][i][0] = x.x, vr[u][i][1] = x.y;
+        } else {
+          vr[u][i][0] = *reinterpret_cast<const uint32_t*>(vp);
+        }
+      }
+      if constexpr (Q8) {
+        ke[u] = *reinterpret_cast<const uint2*>(a.ks + vpage * a.ks_p + hk * a.ks_h + vslot[u]);
+        ve[u] = *reinterpret_cast<const uint2*>(a.vs + vpage * a.vs_p + hk * a.vs_h + vslot[u]);
       }
     }
-    float mx = -INFINITY;
+    if (st + kWaves < w.step1) find(st + kWaves);
+    // scores of this lane: key base + 32 u + 8 g + i in element i % 4 of tile i / 4
+    f32x4 s[NT][KB][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
-    const float m_new = fmaxf(m, over_groups_max(mx) * a.c);
-    if (__any(m_new != m)) {
-      const float alpha = weight_of(m, m_new);
-      l *= alpha;
+    for (int u = 0; u < KB; ++u)
 #pragma unroll
-      for (int j = 0; j < CH; ++j) acc[j] *= alpha;
-      m = m_new;
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc) {
+          bf16x8 kop;
+          if constexpr (Q8) {
+            const uint4 x = kr[u][i][cc >> 1];
+            const uint32_t lo2 = cc & 1 ? x.z : x.x, hi2 = cc & 1 ? x.w : x.y;
+            kop = __builtin_bit_cast(bf16x8, make_uint4(C::template pair<E>(lo2, 0), C::template pair<E>(lo2, 2),
+                                                        C::template pair<E>(hi2, 0), C::template pair<E>(hi2, 2)));
+          } else {
+            kop = __builtin_bit_cast(bf16x8, kr[u][i][cc]);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (cc == 0) s[t][u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            s[t][u][i] = E::mfma16(kop, q[t][cc], s[t][u][i]);
+          }
+        }
+    const float c = Q8 ? 1.f : a.c;  // codes: the factor is the key's
+    if constexpr (Q8) {
+#pragma unroll
+      for (int u = 0; u < KB; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = power_at(i < 4 ? ke[u].x : ke[u].y, i & 3) * a.c;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][u][i >> 2][i & 3] *= f;
+        }
     }
-    const float neg = m == -INFINITY ? 0.f : -m;
-    float p[8];
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], a.c, neg));
-      l += p[i];
+    for (int u = 0; u < KB; ++u) bad = bad || !vok[u];
+    if (base < lo || base + S > (MANY ? safe : end) || __any(bad)) {
+#pragma unroll
+      for (int u = 0; u < KB; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = base + kBlock * u + 8 * g + i;
+          const bool on = vok[u] && j >= lo && j < end;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            s[t][u][i >> 2][i & 3] = on && (!MANY || j < hi[t]) ? s[t][u][i >> 2][i & 3] : -INFINITY;
+#pragma unroll
+          for (int r = 0; r < VW; ++r) vr[u][i][r] = on ? vr[u][i][r] : 0u;  // 0 P of a value that may be anything
+          if constexpr (Q8) {
+            uint32_t& e = i < 4 ? ve[u].x : ve[u].y;
+            e = on ? e : e & ~(0xFFu << (8 * (i & 3)));
+          }
+        }
     }
-    const bf16x8 pb = __builtin_bit_cast(
-        bf16x8, make_uint4(E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])));
+    float neg[NT];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {  // channel j of the lane's piece, its eight keys
-      const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
-      uint32_t x[4];
+    for (int t = 0; t < NT; ++t) {
+      float mx = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_perm(vr[2 * r + 1][j >> 1], vr[2 * r][j >> 1], sel);
-      acc[j] = E::mfma16(__builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3])), pb, acc[j]);
+      for (int u = 0; u < KB; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[t][u][i >> 2][i & 3]);
+      const float m_new = fmaxf(m[t], over_groups_max(mx) * c);
+      if (__any(m_new != m[t])) {
+        const float alpha = weight_of(m[t], m_new);
+        l[t] *= alpha;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) acc[t][j] *= alpha;
+        m[t] = m_new;
+      }
+      neg[t] = m[t] == -INFINITY ? 0.f : -m[t];
+    }
+#pragma unroll
+    for (int u = 0; u < KB; ++u) {
+      // P, of codes times V's powers in two bf16 parts: fp16 does not have their range, and
+      // the sums are as near as in fp16.
+      bf16x8 pb[NT][NP];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u][i >> 2][i & 3], c, neg[t]));
+          l[t] += p[i];
+          if constexpr (Q8) p[i] *= power_at(i < 4 ? ve[u].x : ve[u].y, i & 3);
+        }
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = Q8 ? Bf16::pack(p[2 * r], p[2 * r + 1]) : E::pack(p[2 * r], p[2 * r + 1]);
+          if constexpr (NP == 2) y[r] = Bf16::pack(p[2 * r] - Bf16::lo(x[r]), p[2 * r + 1] - Bf16::hi(x[r]));
+        }
+        pb[t][0] = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+        if constexpr (NP == 2) pb[t][1] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+      }
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {  // channel j of the lane's piece, its eight keys
+        uint32_t x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (Q8)
+            x[r] = C::across(vr[u][2 * r][j >> 2], vr[u][2 * r + 1][j >> 2], j & 3);
+          else
+            x[r] = __builtin_amdgcn_perm(vr[u][2 * r + 1][j >> 1], vr[u][2 * r][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+        }
+        const bf16x8 vop = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+            acc[t][j] = Q8 ? Bf16::mfma16(vop, pb[t][n], acc[t][j]) : E::mfma16(vop, pb[t][n], acc[t][j]);
+      }
     }
   }
-  l = over_groups_sum(l);
 
-  // Join the waves: O[q][channel], channel CH (4 g + i) + j in acc[j][i].
+  // Join the waves, a tile of columns at a time: O[q][channel], channel CH (4 g + i) + j in acc[j][i].
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int t = 0; t < NT; ++t) {
+    if (t) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < CH; ++j) lds_o[wave][col][CH * (4 * g + i) + j] = acc[j][i];
-  if (g == 0) {
-    lds_m[wave][col] = m;
-    lds_l[wave][col] = l;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < ncol * (DP / 2); e += kWaves * 64) {
-    const int qc = e / (DP / 2), ch = 2 * (e % (DP / 2));
-    if (!kFull && ch >= a.D) continue;
-    float top = lds_m[0][qc];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds_m[i][qc]);
-    float o0 = 0.f, o1 = 0.f, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float f = weight_of(lds_m[i][qc], top);
-      o0 = fmaf(lds_o[i][qc][ch], f, o0);
-      o1 = fmaf(lds_o[i][qc][ch + 1], f, o1);
-      sum = fmaf(lds_l[i][qc], f, sum);
+      for (int j = 0; j < CH; ++j) lds.o[wave][col][CH * (4 * g + i) + j] = acc[t][j][i];
+    const float sum_l = over_groups_sum(l[t]);
+    if (g == 0) {
+      lds.m[wave][col] = m[t];
+      lds.l[wave][col] = sum_l;
     }
-    const int64_t row = static_cast<int64_t>(b) * a.H + head0 + qc;
-    if (a.split > 1) {
-      const int64_t at = row * a.split + split;
-      *reinterpret_cast<float2*>(a.part + at * a.D + ch) = make_float2(o0, o1);
-      if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
-    } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
-      *reinterpret_cast<uint32_t*>(a.o + b * a.so_b + (head0 + qc) * a.so_h + ch) = E::pack(o0 * inv, o1 * inv);
+    __syncthreads();
+    const int ncol = min(kGroups, w.ncol - 16 * t);
+    for (int e = threadIdx.x; e < ncol * (DP / 2); e += kWaves * 64) {
+      const int qc = e / (DP / 2), ch = 2 * (e % (DP / 2));
+      if (!kFull && ch >= a.D) continue;
+      float top = lds.m[0][qc];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds.m[i][qc]);
+      float o0 = 0.f, o1 = 0.f, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float f = weight_of(lds.m[i][qc], top);
+        o0 = fmaf(lds.o[i][qc][ch], f, o0);
+        o1 = fmaf(lds.o[i][qc][ch + 1], f, o1);
+        sum = fmaf(lds.l[i][qc], f, sum);
+      }
+      int b, h;
+      w.row(a, 16 * t + qc, MANY, b, h);
+      if (a.parts > 1) {
+        const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
+        *reinterpret_cast<float2*>(a.part + at * a.D + ch) = make_float2(o0, o1);
+        if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
+        *reinterpret_cast<uint32_t*>(a.o + b * a.so_b + h * a.so_h + ch) = E::pack(o0 * inv, o1 * inv);
+      }
     }
   }
+}
+
+// Nothing in this part: the join passes over a sum of 0.
+template <bool MANY>
+__device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
+  for (int c = threadIdx.x; c < w.ncol; c += kWaves * 64) {
+    int b, h;
+    w.row(a, c, MANY, b, h);
+    reinterpret_cast<float2*>(a.part + a.part_ml)[(static_cast<int64_t>(b) * a.H + h) * a.parts + w.part] =
+        make_float2(-INFINITY, 0.f);
+  }
+}
+
+// The longest sequence of a run of `per` (the first of these), and its length.
+__device__ __forceinline__ void longest(const PagedArgs& a, int first, int& b, int& len) {
+  const int lane = threadIdx.x & 63;
+  int n = -1, at = 0;
+  for (int i = lane; i < a.per; i += 64) {
+    const int x = sequence_length(a, first + i);
+    if (x > n) n = x, at = i;
+  }
+  int top = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o));
+  int best = n == top ? at : 0x7fffffff;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) best = min(best, __shfl_xor(best, o));
+  b = first + __builtin_amdgcn_readfirstlane(best);
+  len = __builtin_amdgcn_readfirstlane(top);
+}
+
+// PT: tiles of 16 columns over shared keys (0: a launch without any).
+template <typename E, typename C, int DP, bool kFull, int PT>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+paged_kernel(const PagedArgs a) {
+  __shared__ PagedLds<DP> lds;
+  fetch_arguments(a);
+  uint32_t n = blockIdx.x;
+  Work w;
+  if constexpr (PT > 0) {
+    if (n < static_cast<uint32_t>(a.pitems)) {
+      // an XCD (they are dealt round robin) takes a run of items: the tiles over the same keys side by side
+      const uint32_t x = n & 7u, q8 = a.pitems >> 3, rem = a.pitems & 7u;
+      n = x * q8 + min(x, rem) + (n >> 3);
+      const int tile = a.by_ptiles.split(n);
+      w.hk = a.by_hkv.split(n);
+      w.part = a.by_psplit.split(n);
+      w.seq = static_cast<int>(n) * a.per;
+      w.col0 = tile * 16 * PT;
+      w.ncol = min(16 * PT, a.per * a.group - w.col0);
+      int len;
+      longest(a, w.seq, w.b, len);
+      w.vis = visible<C>(min(len, a.shared), 0, 0);
+      const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
+      w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
+      if (w.step0 >= w.step1)
+        no_keys<true>(a, w);
+      else
+        attend<E, C, DP, kFull, PT, true>(a, lds, w);
+      return;
+    }
+    n -= a.pitems;
+  }
+  const int tile = a.by_tiles.split(n);
+  w.hk = a.by_hkv.split(n);
+  const int split = a.by_split.split(n);
+  w.part = a.psplit + split;
+  w.b = w.seq = n;
+  w.col0 = tile * kGroups;
+  w.ncol = min(kGroups, a.group - w.col0);
+  const int len = sequence_length(a, w.b);
+  w.vis = visible<C>(len, PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0, PT > 0 ? 0 : a.sinks);
+  const int per = a.by_split.of(w.vis.steps + a.split - 1);
+  w.step0 = split * per, w.step1 = min(w.step0 + per, w.vis.steps);
+  if (w.step0 >= w.step1 && a.parts > 1)
+    no_keys<false>(a, w);
+  else
+    attend<E, C, DP, kFull, 1, false>(a, lds, w);
 }
 
 // Joins the splits of a row: a wave per (b, head), two channels a lane.
@@ -280,8 +495,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= static_cast<int64_t>(a.B) * a.H) return;
   const int lane = threadIdx.x & 63, ch = 2 * lane;
-  const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_ml) + row * a.split;
-  const float2 mine = lane < a.split ? ml[lane] : make_float2(-INFINITY, 0.f);  // (split <= 64)
+  const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_ml) + row * a.parts;
+  const float2 mine = lane < a.parts ? ml[lane] : make_float2(-INFINITY, 0.f);  // (parts <= 64)
   float top = mine.x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -290,7 +505,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
   const bool on = ch < a.D;
-  const float* p = a.part + row * a.split * a.D + (on ? ch : 0);
+  const float* p = a.part + row * a.parts * a.D + (on ? ch : 0);
   float o0 = 0.f, o1 = 0.f;
   // Splits behind the last that saw a key are not read (one without steps wrote no sums);
   // eight loads in flight, those past the last read it again and weigh 0.
@@ -303,9 +518,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
       x[u] = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(min(i0 + u, used - 1)) * a.D);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const float fi = i0 + u < used ? __shfl(f, i0 + u) : 0.f;  // (split <= 64, so i0 + u < 64)
-      o0 = fmaf(x[u].x, fi, o0);
-      o1 = fmaf(x[u].y, fi, o1);
+      const float fi = i0 + u < used ? __shfl(f, i0 + u) : 0.f;  // (parts <= 64, so i0 + u < 64)
+      // (a part without keys of this row is not looked at: it may hold none, or others' NaN)
+      o0 = fi == 0.f ? o0 : fmaf(x[u].x, fi, o0);
+      o1 = fi == 0.f ? o1 : fmaf(x[u].y, fi, o1);
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -321,106 +537,196 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
 // 4096 each 275 -> 284. Four of 32768 to 131072: within two 281, four 250, eight 258.)
 // No split is longer than 4096 keys as far as there may be 64 of them: one long sequence
 // in a large batch is not left to one workgroup a head.
-int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks) {
+int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks, int64_t limit) {
   const int64_t keys = window && window < most && sinks < most - window ? window + sinks : most;
-  const int64_t steps = cdiv(keys, kStep) + 1;
+  const int64_t steps = cdiv(keys, kBlock) + 1;
   int64_t n = (B < 16 ? 1024 : 2048) / (B * Hkv * tiles);
   if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);
   if (n > steps / kWaves) n = steps / kWaves;
-  if (n > kMaxSplits) n = kMaxSplits;
+  if (n > limit) n = limit;
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
-int64_t part_bytes(int64_t B, int64_t H, int64_t D, int64_t split) {
-  return split > 1 ? B * H * split * (D + 2) * 4 : 0;
+// How a call is cut.
+struct Cut {
+  int64_t tiles, split;
+  int64_t ctiles, ptiles, psplit;  // shared keys: tiles of 16 columns in a workgroup, tiles of columns, splits
+  int64_t parts() const { return psplit + split; }
+  int64_t part_bytes(int64_t B, int64_t H, int64_t D) const { return parts() > 1 ? B * H * parts() * (D + 2) * 4 : 0; }
+};
+Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups) {
+  Cut c{};
+  c.tiles = cdiv(H / Hkv, kGroups);
+  if (shared > 0) {
+    const int64_t cols = B / groups * (H / Hkv);
+    c.ctiles = cols > kGroups ? 2 : 1;
+    c.ptiles = cdiv(cols, kGroups * c.ctiles);
+    int64_t n = 1024 / (groups * Hkv * c.ptiles);
+    const int64_t steps = cdiv(shared, 2 * kBlock) / kWaves;
+    if (n > steps) n = steps;
+    if (n > kMaxShared) n = kMaxShared;
+    c.psplit = n < 1 ? 1 : n;
+    keys = keys > shared ? keys - shared : 0;
+  }
+  c.split = splits(B, Hkv, c.tiles, keys, window, sinks, kMaxSplits - c.psplit);
+  return c;
+}
+
+// The kernel of a head dim: <channels of the registers, all of them used>.
+template <typename E, typename C, int PT>
+auto kernel_of(int64_t D) {
+  return D == 128 ? paged_kernel<E, C, 128, true, PT>
+         : D == 64 ? paged_kernel<E, C, 64, true, PT>
+         : D > 64  ? paged_kernel<E, C, 128, false, PT>
+                   : paged_kernel<E, C, 64, false, PT>;
+}
+template <typename E, typename C>
+auto kernel_of(int64_t D, int64_t ctiles) {
+  return ctiles == 0 ? kernel_of<E, C, 0>(D) : ctiles == 1 ? kernel_of<E, C, 1>(D) : kernel_of<E, C, 2>(D);
+}
+template <typename E>
+auto kernel_of(int64_t D, int64_t ctiles, int cache_type) {
+  return cache_type == 0              ? kernel_of<E, SameType>(D, ctiles)
+         : cache_type == SOLATTN_INT8 ? kernel_of<E, Int8Codes>(D, ctiles)
+                                      : kernel_of<E, Fp8Codes>(D, ctiles);
 }
 
 }  // namespace
 
-// Checked arguments of both entries; keys: the longest sequence that the cache can hold.
-int paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k, int64_t sk_p, int64_t sk_s,
-               int64_t sk_h, const uint16_t* v, int64_t sv_p, int64_t sv_s, int64_t sv_h, int64_t pages,
-               int64_t page_size, const int32_t* table, int64_t table_stride, int64_t max_pages,
-               const int32_t* lengths, int64_t length, int64_t B, int64_t H, int64_t Hkv, int64_t D, int dtype,
-               int64_t window, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, uint16_t* o,
-               int64_t so_b, int64_t so_h, hipStream_t s, const char* what) {
-  SOLATTN_REQUIRE(dtype == SOLATTN_BF16 || dtype == SOLATTN_FP16, SOLATTN_EINVAL, "%s: dtype %d", what, dtype);
+int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
+  const int64_t B = p.B, H = p.H, Hkv = p.Hkv, D = p.D;
+  SOLATTN_REQUIRE(p.dtype == SOLATTN_BF16 || p.dtype == SOLATTN_FP16, SOLATTN_EINVAL, "%s: dtype %d", what, p.dtype);
+  SOLATTN_REQUIRE(p.cache_type == 0 || p.cache_type == SOLATTN_INT8 || p.cache_type == SOLATTN_E4M3, SOLATTN_EINVAL,
+                  "%s: cache type %d", what, p.cache_type);
   SOLATTN_REQUIRE(B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0, SOLATTN_EINVAL,
                   "%s: %lld query heads over %lld kv heads", what, (long long)H, (long long)Hkv);
   SOLATTN_REQUIRE(B < (1ll << 31) && H < (1ll << 31) && B * H < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large",
                   what);
-  SOLATTN_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, SOLATTN_EUNSUPPORTED,
-                  "%s: head_dim %lld (multiples of 8 up to 128)", what, (long long)D);
-  SOLATTN_REQUIRE(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), SOLATTN_EINVAL,
-                  "%s: window %lld, sinks %lld", what, (long long)window, (long long)sinks);
-  SOLATTN_REQUIRE(pages > 0 && pages < (1ll << 31) && page_size > 0 && max_pages >= 0 &&
-                      (!table || page_size % 8 == 0),
-                  SOLATTN_EINVAL, "%s: %lld pages of %lld (a multiple of 8)", what, (long long)pages,
-                  (long long)page_size);
-  SOLATTN_REQUIRE(page_size < (1ll << 31) && max_pages < (1ll << 31) && max_pages * page_size < (1ll << 31) - kStep,
+  const int64_t whole = p.cache_type ? 16 : 8;
+  SOLATTN_REQUIRE(D >= whole && D <= 128 && D % whole == 0, SOLATTN_EUNSUPPORTED,
+                  "%s: head_dim %lld (multiples of %lld up to 128)", what, (long long)D, (long long)whole);
+  SOLATTN_REQUIRE(p.window >= 0 && p.sinks >= 0 && p.window < (1ll << 31) && p.sinks < (1ll << 31), SOLATTN_EINVAL,
+                  "%s: window %lld, sinks %lld", what, (long long)p.window, (long long)p.sinks);
+  SOLATTN_REQUIRE(p.pages > 0 && p.pages < (1ll << 31) && p.page_size > 0 && p.max_pages >= 0 &&
+                      (!p.table || p.page_size % 8 == 0),
+                  SOLATTN_EINVAL, "%s: %lld pages of %lld (a multiple of 8)", what, (long long)p.pages,
+                  (long long)p.page_size);
+  SOLATTN_REQUIRE(p.page_size < (1ll << 31) && p.max_pages < (1ll << 31) && p.max_pages * p.page_size < (1ll << 31) - (p.cache_type ? 2 : 1) * kBlock,
                   SOLATTN_EUNSUPPORTED, "%s: sequences beyond 2^31 keys", what);
-  SOLATTN_REQUIRE(scale > 0.f, SOLATTN_EINVAL, "%s: scale %g", what, static_cast<double>(scale));
-  SOLATTN_REQUIRE(q && k && v && o, SOLATTN_EINVAL, "%s: null pointer", what);
-  const auto rows = [](const void* p, int64_t x, int64_t y, int64_t z) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && x % 8 == 0 && y % 8 == 0 && z % 8 == 0;
+  SOLATTN_REQUIRE(p.shared >= 0 && p.shared < (1ll << 31), SOLATTN_EINVAL, "%s: %lld shared keys", what, (long long)p.shared);
+  SOLATTN_REQUIRE(p.shared == 0 || (p.window == 0 && p.sinks == 0), SOLATTN_EINVAL, "%s: shared keys and a window", what);
+  SOLATTN_REQUIRE(p.shared == 0 || (p.groups > 0 && B % p.groups == 0), SOLATTN_EINVAL,
+                  "%s: %lld sequences in %lld groups", what, (long long)B, (long long)p.groups);
+  SOLATTN_REQUIRE(p.scale > 0.f, SOLATTN_EINVAL, "%s: scale %g", what, static_cast<double>(p.scale));
+  SOLATTN_REQUIRE(p.q && p.k && p.v && p.o, SOLATTN_EINVAL, "%s: null pointer", what);
+  const auto rows = [](const void* at, int64_t x, int64_t y, int64_t z, int64_t m) {
+    return reinterpret_cast<uintptr_t>(at) % 16 == 0 && x % m == 0 && y % m == 0 && z % m == 0;
   };
-  SOLATTN_REQUIRE(rows(q, sq_b, sq_h, 0) && rows(k, sk_p, sk_s, sk_h) && rows(v, sv_p, sv_s, sv_h) &&
-                      rows(o, so_b, so_h, 0),
-                  SOLATTN_EINVAL, "%s: rows must be 16-byte aligned with strides multiple of 8", what);
+  SOLATTN_REQUIRE(rows(p.q, p.sq_b, p.sq_h, 0, 8) && rows(p.k, p.sk_p, p.sk_s, p.sk_h, whole) &&
+                      rows(p.v, p.sv_p, p.sv_s, p.sv_h, whole) && rows(p.o, p.so_b, p.so_h, 0, 8),
+                  SOLATTN_EINVAL, "%s: rows must be 16-byte aligned with strides multiple of %lld", what, (long long)whole);
+  const auto scales = [](const void* at, int64_t x, int64_t y) {
+    return at && reinterpret_cast<uintptr_t>(at) % 8 == 0 && x % 8 == 0 && y % 8 == 0;
+  };
+  SOLATTN_REQUIRE(!p.cache_type || (scales(p.ks, p.ks_p, p.ks_h) && scales(p.vs, p.vs_p, p.vs_h)), SOLATTN_EINVAL,
+                  "%s: scales must be 8-byte aligned with strides multiple of 8", what);
   PagedArgs a{};
-  a.q = q, a.sq_b = sq_b, a.sq_h = sq_h;
-  a.k = k, a.sk_p = sk_p, a.sk_s = sk_s, a.sk_h = sk_h;
-  a.v = v, a.sv_p = sv_p, a.sv_s = sv_s, a.sv_h = sv_h;
-  a.table = table, a.table_b = table_stride;
-  a.lengths = lengths, a.length = static_cast<int>(length);
-  a.pages = static_cast<int>(pages), a.page = static_cast<int>(page_size), a.max_pages = static_cast<int>(max_pages);
-  a.by_page = divisor(page_size);
-  a.o = o, a.so_b = so_b, a.so_h = so_h;
+  const int64_t es = p.cache_type ? 1 : 2;
+  a.q = p.q, a.sq_b = p.sq_b, a.sq_h = p.sq_h;
+  a.k = static_cast<const uint8_t*>(p.k), a.sk_p = es * p.sk_p, a.sk_s = es * p.sk_s, a.sk_h = es * p.sk_h;
+  a.v = static_cast<const uint8_t*>(p.v), a.sv_p = es * p.sv_p, a.sv_s = es * p.sv_s, a.sv_h = es * p.sv_h;
+  a.ks = p.ks, a.ks_p = p.ks_p, a.ks_h = p.ks_h;
+  a.vs = p.vs, a.vs_p = p.vs_p, a.vs_h = p.vs_h;
+  a.table = p.table, a.table_b = p.table_stride;
+  a.lengths = p.lengths, a.length = static_cast<int>(p.length);
+  a.pages = static_cast<int>(p.pages), a.page = static_cast<int>(p.page_size), a.max_pages = static_cast<int>(p.max_pages);
+  a.by_page = divisor(p.page_size);
+  a.o = p.o, a.so_b = p.so_b, a.so_h = p.so_h;
   a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.Hkv = static_cast<int>(Hkv), a.D = static_cast<int>(D);
   a.group = static_cast<int>(H / Hkv);
-  a.tiles = static_cast<int>(cdiv(a.group, kGroups));
-  a.window = static_cast<int>(window), a.sinks = static_cast<int>(sinks);
-  a.c = scale * kLog2e;
-  a.split = splits(B, Hkv, a.tiles, max_pages * page_size, window, sinks);
-  a.by_tiles = divisor(a.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(a.split);
-  const int64_t need = part_bytes(B, H, D, a.split);
-  SOLATTN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SOLATTN_ESIZE,
-                  "%s: workspace %lld < %lld bytes", what, (long long)workspace_bytes, (long long)need);
-  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, SOLATTN_EINVAL,
+  a.window = static_cast<int>(p.window), a.sinks = static_cast<int>(p.sinks);
+  a.c = p.scale * kLog2e;
+  const Cut c = cut(B, H, Hkv, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups);
+  a.tiles = static_cast<int>(c.tiles), a.split = static_cast<int>(c.split);
+  a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split);
+  a.parts = static_cast<int>(c.parts());
+  const int64_t need = c.part_bytes(B, H, D);
+  SOLATTN_REQUIRE(need == 0 || (p.workspace && p.workspace_bytes >= need), SOLATTN_ESIZE,
+                  "%s: workspace %lld < %lld bytes", what, (long long)p.workspace_bytes, (long long)need);
+  SOLATTN_REQUIRE(reinterpret_cast<uintptr_t>(p.workspace) % 256 == 0, SOLATTN_EINVAL,
                   "%s: workspace must be 256-byte aligned", what);
-  a.part = static_cast<float*>(workspace);
-  a.part_ml = B * H * a.split * D;
-  const int64_t grid = B * Hkv * a.tiles * a.split;
+  a.part = static_cast<float*>(p.workspace);
+  a.part_ml = B * H * c.parts() * D;
+  int64_t grid = B * Hkv * c.tiles * c.split;
+  if (p.shared > 0) {
+    const int64_t items = p.groups * Hkv * c.ptiles * c.psplit;
+    grid += items;
+    SOLATTN_REQUIRE(grid < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
+    a.shared = static_cast<int>(p.shared), a.per = static_cast<int>(B / p.groups);
+    a.psplit = static_cast<int>(c.psplit), a.ptiles = static_cast<int>(c.ptiles), a.pitems = static_cast<int>(items);
+    a.by_ptiles = divisor(c.ptiles), a.by_psplit = divisor(c.psplit), a.by_group = divisor(a.group);
+  }
   SOLATTN_REQUIRE(grid < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
-  const bool bf = dtype == SOLATTN_BF16;
-  const auto kern = D == 128 ? (bf ? paged_kernel<Bf16, 128, true> : paged_kernel<Fp16, 128, true>)
-                    : D == 64 ? (bf ? paged_kernel<Bf16, 64, true> : paged_kernel<Fp16, 64, true>)
-                    : D > 64  ? (bf ? paged_kernel<Bf16, 128, false> : paged_kernel<Fp16, 128, false>)
-                              : (bf ? paged_kernel<Bf16, 64, false> : paged_kernel<Fp16, 64, false>);
+  const bool bf = p.dtype == SOLATTN_BF16;
+  const auto kern = bf ? kernel_of<Bf16>(D, c.ctiles, p.cache_type) : kernel_of<Fp16>(D, c.ctiles, p.cache_type);
   hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(grid)), dim3(kWaves * 64), 0, s, a);
   if (int rc = check_launch(what)) return rc;
-  if (a.split == 1) return SOLATTN_OK;
+  if (a.parts == 1) return SOLATTN_OK;
   hipLaunchKernelGGL(bf ? paged_join_kernel<Bf16> : paged_join_kernel<Fp16>,
                      dim3(static_cast<uint32_t>(cdiv(B * H, 4))), dim3(256), 0, s, a);
   return check_launch(what);
 }
 
 int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
-                             int64_t sinks) {
+                             int64_t sinks, int64_t shared, int64_t groups) {
   constexpr int64_t top = 1ll << 31;  // (what the call takes: nothing passes 64 bits)
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || keys < 0 || window < 0 || sinks < 0) return 0;
   if (B >= top || H >= top || B * H >= top || D > 128 || keys >= top) return 0;
-  return part_bytes(B, H, D, splits(B, Hkv, cdiv(H / Hkv, kGroups), keys, window, sinks));
+  if (shared < 0 || shared >= top || (shared && (groups <= 0 || B % groups))) return 0;
+  return cut(B, H, Hkv, keys, window, sinks, shared, groups).part_bytes(B, H, D);
 }
 
 }  // namespace solattn
 
 using namespace solattn;
 
+extern "C" int64_t solattn_paged_attn_shared_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                                             int64_t max_pages, int64_t page_size, int64_t window,
+                                                             int64_t sinks, int cache_type, int64_t shared,
+                                                             int64_t groups) {
+  (void)cache_type;
+  const bool fit = max_pages >= 0 && page_size >= 0 && max_pages < (1ll << 31) && page_size < (1ll << 31);
+  return fit ? paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks, shared, groups) : 0;
+}
+
 extern "C" int64_t solattn_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
                                                       int64_t page_size, int64_t window, int64_t sinks) {
-  const bool fit = max_pages >= 0 && page_size >= 0 && max_pages < (1ll << 31) && page_size < (1ll << 31);
-  return fit ? paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks) : 0;
+  return solattn_paged_attn_shared_workspace_bytes(B, H, Hkv, D, max_pages, page_size, window, sinks, 0, 0, 1);
+}
+
+extern "C" int solattn_paged_attn_shared(const uint16_t* q, int64_t sq_b, int64_t sq_h, const void* k_cache, int64_t sk_p,
+                                         int64_t sk_s, int64_t sk_h, const void* v_cache, int64_t sv_p, int64_t sv_s,
+                                         int64_t sv_h, int64_t pages, int64_t page_size, int cache_type,
+                                         const uint8_t* k_scale, int64_t sks_p, int64_t sks_h, const uint8_t* v_scale,
+                                         int64_t svs_p, int64_t svs_h, const int32_t* page_table, int64_t table_stride,
+                                         int64_t max_pages, const int32_t* lengths, int64_t B, int64_t H, int64_t Hkv,
+                                         int64_t D, int dtype, int64_t window, int64_t sinks, int64_t shared,
+                                         int64_t groups, float scale, void* workspace, int64_t workspace_bytes,
+                                         uint16_t* o, int64_t so_b, int64_t so_h, solattn_stream_t stream) {
+  clear_error();
+  const char* what = "paged_attn";
+  SOLATTN_REQUIRE(page_table && lengths, SOLATTN_EINVAL, "%s: null page table or lengths", what);
+  PagedCall p{};
+  p.q = q, p.sq_b = sq_b, p.sq_h = sq_h;
+  p.k = k_cache, p.sk_p = sk_p, p.sk_s = sk_s, p.sk_h = sk_h;
+  p.v = v_cache, p.sv_p = sv_p, p.sv_s = sv_s, p.sv_h = sv_h;
+  p.ks = k_scale, p.ks_p = sks_p, p.ks_h = sks_h, p.vs = v_scale, p.vs_p = svs_p, p.vs_h = svs_h;
+  p.cache_type = cache_type, p.pages = pages, p.page_size = page_size;
+  p.table = page_table, p.table_stride = table_stride, p.max_pages = max_pages, p.lengths = lengths;
+  p.B = B, p.H = H, p.Hkv = Hkv, p.D = D, p.dtype = dtype;
+  p.window = window, p.sinks = sinks, p.shared = shared, p.groups = groups, p.scale = scale;
+  p.workspace = workspace, p.workspace_bytes = workspace_bytes, p.o = o, p.so_b = so_b, p.so_h = so_h;
+  return paged_attn(p, reinterpret_cast<hipStream_t>(stream), what);
 }
 
 extern "C" int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint16_t* k_cache,
@@ -431,9 +737,8 @@ extern "C" int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h,
                                   int64_t window, int64_t sinks, float scale, void* workspace,
                                   int64_t workspace_bytes, uint16_t* o, int64_t so_b, int64_t so_h,
                                   solattn_stream_t stream) {
-  clear_error();
-  SOLATTN_REQUIRE(page_table && lengths, SOLATTN_EINVAL, "paged_attn: null page table or lengths");
-  return paged_attn(q, sq_b, sq_h, k_cache, sk_p, sk_s, sk_h, v_cache, sv_p, sv_s, sv_h, pages, page_size, page_table,
-                    table_stride, max_pages, lengths, 0, B, H, Hkv, D, dtype, window, sinks, scale, workspace,
-                    workspace_bytes, o, so_b, so_h, reinterpret_cast<hipStream_t>(stream), "paged_attn");
+  return solattn_paged_attn_shared(q, sq_b, sq_h, k_cache, sk_p, sk_s, sk_h, v_cache, sv_p, sv_s, sv_h, pages, page_size,
+                                   0, nullptr, 0, 0, nullptr, 0, 0, page_table, table_stride, max_pages, lengths, B, H,
+                                   Hkv, D, dtype, window, sinks, 0, 1, scale, workspace, workspace_bytes, o, so_b, so_h,
+                                   stream);
 }

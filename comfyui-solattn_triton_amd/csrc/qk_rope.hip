@@ -20,7 +20,7 @@
 // wave walks the heads (a table entry is 8 bytes a pair, as much as two rows'
 // values). Few tokens: their heads are dealt over S waves, so that one decode
 // step is one or two rounds of loads.
-#include "elem.hpp"
+#include "cache8.hpp"
 
 namespace solattn {
 namespace {
@@ -40,6 +40,7 @@ struct Cache {
   void* k;
   void* v;
   int64_t kp, ks, kh, vp, vs, vh;  // page, slot and head strides
+  CodePages kq, vq;                // the same of a cache of codes
   const int32_t* table;
   int64_t table_b;
   const int32_t* lengths;
@@ -178,13 +179,13 @@ __device__ __forceinline__ typename E::Raw* row_of(const Rows& r, int64_t b, int
   return static_cast<typename E::Raw*>(r.p) + b * r.b + t * r.t + h * r.h;
 }
 
-// One tensor's heads of this lane's token: norm, rotation, store at dst(h).
+// One tensor's heads of this lane's token: norm, rotation, put(head, values, stored).
 // Every lane of a wave makes the same passes (its rows' sums and exchanges are
 // wave operations); heads past `heads` read the last one and are not stored.
-template <typename E, int LPR, typename Dst>
+template <typename E, int LPR, typename Put>
 __device__ __forceinline__ void norm_turn_rows(const RopeArgs& a, const Rows& src, const Place& p, int heads,
                                                const float* weight, const Turn& tr, int l, bool active, bool store,
-                                               Dst&& dst) {
+                                               Put&& put) {
   float w[8];
   load_weight(w, weight, l, active);
   const int n = (heads + p.step - 1) / p.step;
@@ -206,17 +207,24 @@ __device__ __forceinline__ void norm_turn_rows(const RopeArgs& a, const Rows& sr
       for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
       if (a.R) turn(x, tr, a.interleaved, 1.f);
       const int h = p.first + (i0 + u) * p.step;
-      if (store && active && h < heads) Row8<E>::store(dst(h) + chan, x);
+      put(h, x, store && h < heads);
     }
   }
 }
 
-template <typename E, int LPR, bool APPEND>
+// What the newest tokens' k and v are kept as: no cache (positions instead), one of the
+// inputs' type, or codes (cache8.hpp), which k' is rounded to from fp32.
+struct NoCache {};
+struct SameType {};
+
+template <typename E, int LPR, typename KEPT>
 __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const RopeArgs a) {
+  constexpr bool APPEND = !__is_same(KEPT, NoCache);
   const int lane = threadIdx.x & 63, l = lane & (LPR - 1), group = lane / LPR;
   const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kRopeThreads / 64) + (threadIdx.x >> 6);
   const Place p = place<LPR>(a, wave, group);
   const bool active = 8 * l < a.D;
+  const int chan = active ? 8 * l : 0;
   int pos = p.t;
   bool keep = p.on;  // the token has a position (append: the sequence holds it)
   if constexpr (APPEND) {
@@ -229,30 +237,49 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const RopeArgs a)
   }
   Turn tr;
   if (a.R) load_turn<LPR>(tr, a, min(max(pos, 0), a.P - 1), l, lane);
+  const auto to = [&](const Rows& out) {
+    return [&, out](int h, const float (&x)[8], bool on) {
+      if (on && active) Row8<E>::store(row_of<E>(out, p.b, p.t, h) + chan, x);
+    };
+  };
+  // (append: q rows of tokens without a position are written too: they are finite and no
+  // attention call reads them as anything but an empty row)
+  norm_turn_rows<E, LPR>(a, a.q, p, a.H, a.qw, tr, l, active, p.on, to(a.qo));
   if constexpr (!APPEND) {
-    norm_turn_rows<E, LPR>(a, a.q, p, a.H, a.qw, tr, l, active, p.on,
-                           [&](int h) { return row_of<E>(a.qo, p.b, p.t, h); });
-    norm_turn_rows<E, LPR>(a, a.k, p, a.Hkv, a.kw, tr, l, active, p.on,
-                           [&](int h) { return row_of<E>(a.ko, p.b, p.t, h); });
+    norm_turn_rows<E, LPR>(a, a.k, p, a.Hkv, a.kw, tr, l, active, p.on, to(a.ko));
   } else {
-    // q rows of tokens without a position are written too: they are finite and no
-    // attention call reads them as anything but an empty row
-    norm_turn_rows<E, LPR>(a, a.q, p, a.H, a.qw, tr, l, active, p.on,
-                           [&](int h) { return row_of<E>(a.qo, p.b, p.t, h); });
     const Cache& c = a.cache;
     const int page = c.max_pages ? c.table[p.b * c.table_b + pos / c.page] : -1;
+    const int slot = pos % c.page;
     const bool put = keep && page >= 0 && page < c.npages;
-    const int64_t kat = put ? static_cast<int64_t>(page) * c.kp + static_cast<int64_t>(pos % c.page) * c.ks : 0;
-    const int64_t vat = put ? static_cast<int64_t>(page) * c.vp + static_cast<int64_t>(pos % c.page) * c.vs : 0;
-    typename E::Raw* kc = static_cast<typename E::Raw*>(c.k) + kat;
-    typename E::Raw* vc = static_cast<typename E::Raw*>(c.v) + vat;
-    norm_turn_rows<E, LPR>(a, a.k, p, a.Hkv, a.kw, tr, l, active, put, [&](int h) { return kc + h * c.kh; });
-    if (put && active)
-      for (int h = p.first; h < a.Hkv; h += p.step) {
+    if constexpr (__is_same(KEPT, SameType)) {
+      const int64_t kat = put ? static_cast<int64_t>(page) * c.kp + static_cast<int64_t>(slot) * c.ks : 0;
+      const int64_t vat = put ? static_cast<int64_t>(page) * c.vp + static_cast<int64_t>(slot) * c.vs : 0;
+      typename E::Raw* kc = static_cast<typename E::Raw*>(c.k) + kat;
+      typename E::Raw* vc = static_cast<typename E::Raw*>(c.v) + vat;
+      norm_turn_rows<E, LPR>(a, a.k, p, a.Hkv, a.kw, tr, l, active, put, [&](int h, const float (&x)[8], bool on) {
+        if (on && active) Row8<E>::store(kc + h * c.kh + chan, x);
+      });
+      if (put && active)
+        for (int h = p.first; h < a.Hkv; h += p.step) {
+          Row8<E> in;
+          in.load(row_of<E>(a.v, p.b, p.t, h) + 8 * l);
+          *reinterpret_cast<Row8<E>*>(vc + h * c.vh + 8 * l) = in;
+        }
+    } else {
+      norm_turn_rows<E, LPR>(a, a.k, p, a.Hkv, a.kw, tr, l, active, put, [&](int h, const float (&x)[8], bool on) {
+        put_codes<KEPT, LPR>(x, c.kq, page, slot, h, l, active, on);
+      });
+      const int n = (a.Hkv + p.step - 1) / p.step;
+      for (int i = 0; i < n; ++i) {
+        const int h = p.first + i * p.step;
         Row8<E> in;
-        in.load(row_of<E>(a.v, p.b, p.t, h) + 8 * l);
-        *reinterpret_cast<Row8<E>*>(vc + h * c.vh + 8 * l) = in;
+        float x[8];
+        in.load(row_of<E>(a.v, p.b, p.t, min(h, a.Hkv - 1)) + chan);
+        in.get(x);
+        put_codes<KEPT, LPR>(x, c.vq, page, slot, h, l, active, put && h < a.Hkv);
       }
+    }
   }
 }
 
@@ -415,15 +442,15 @@ int setup(RopeArgs& a, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, 
 
 int64_t wave_count(const RopeArgs& a) { return (a.tokens * a.split + a.tpw - 1) / a.tpw; }
 
-template <bool APPEND>
+template <typename KEPT>
 int launch(const RopeArgs& a, int dtype, hipStream_t s, const char* what) {
   const int64_t blocks = cdiv(wave_count(a), kRopeThreads / 64);
   SOLATTN_REQUIRE(blocks < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   const dim3 grid(static_cast<uint32_t>(blocks)), block(kRopeThreads);
   const bool wide = a.D > 64;
-  const auto kern = dtype == SOLATTN_BF16   ? (wide ? qk_rope_kernel<Bf16, 16, APPEND> : qk_rope_kernel<Bf16, 8, APPEND>)
-                    : dtype == SOLATTN_FP16 ? (wide ? qk_rope_kernel<Fp16, 16, APPEND> : qk_rope_kernel<Fp16, 8, APPEND>)
-                                            : (wide ? qk_rope_kernel<Fp32, 16, APPEND> : qk_rope_kernel<Fp32, 8, APPEND>);
+  const auto kern = dtype == SOLATTN_BF16   ? (wide ? qk_rope_kernel<Bf16, 16, KEPT> : qk_rope_kernel<Bf16, 8, KEPT>)
+                    : dtype == SOLATTN_FP16 ? (wide ? qk_rope_kernel<Fp16, 16, KEPT> : qk_rope_kernel<Fp16, 8, KEPT>)
+                                            : (wide ? qk_rope_kernel<Fp32, 16, KEPT> : qk_rope_kernel<Fp32, 8, KEPT>);
   hipLaunchKernelGGL(kern, grid, block, 0, s, a);
   return check_launch(what);
 }
@@ -466,7 +493,40 @@ extern "C" int solattn_qk_norm_rope(const void* q, int64_t sq_b, int64_t sq_t, i
   if (!rc && Hkv) rc = check_rows(a.k, e, "qk_norm_rope", "k");
   if (!rc && Hkv) rc = check_rows(a.ko, e, "qk_norm_rope", "k output");
   if (rc) return rc;
-  return launch<false>(a, dtype, reinterpret_cast<hipStream_t>(stream), "qk_norm_rope");
+  return launch<NoCache>(a, dtype, reinterpret_cast<hipStream_t>(stream), "qk_norm_rope");
+}
+
+static int append(RopeArgs& a, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t P, int64_t R,
+                  int interleaved, float eps, Cache c, int64_t pages, int64_t page_size, int64_t max_pages,
+                  int cache_type, hipStream_t s, const char* what) {
+  if (int rc = setup(a, B, T, H, Hkv, D, dtype, P, R, interleaved, eps, what)) return rc;
+  SOLATTN_REQUIRE(Hkv > 0 && c.table && c.lengths, SOLATTN_EINVAL, "%s: null page table or lengths", what);
+  SOLATTN_REQUIRE(pages >= 0 && pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31) && max_pages >= 0 &&
+                      max_pages < (1ll << 31) && max_pages * page_size < (1ll << 31),
+                  SOLATTN_EUNSUPPORTED, "%s: pages beyond 2^31 tokens", what);
+  const bool codes = cache_type >= 0;
+  const int e = esize(dtype);
+  int rc = check_rows(a.q, e, what, "q");
+  if (!rc) rc = check_rows(a.k, e, what, "k");
+  if (!rc) rc = check_rows(a.v, e, what, "v");
+  if (!rc) rc = check_rows(a.qo, e, what, "q output");
+  if (!rc) rc = check_rows(Rows{c.k, c.kp, c.ks, c.kh}, codes ? 1 : e, what, "k_cache");
+  if (!rc) rc = check_rows(Rows{c.v, c.vp, c.vs, c.vh}, codes ? 1 : e, what, "v_cache");
+  if (rc) return rc;
+  c.npages = static_cast<int>(pages), c.page = static_cast<int>(page_size), c.max_pages = static_cast<int>(max_pages);
+  if (codes) {
+    SOLATTN_REQUIRE(cache_type == SOLATTN_INT8 || cache_type == SOLATTN_E4M3, SOLATTN_EINVAL, "%s: cache type %d", what,
+                    cache_type);
+    SOLATTN_REQUIRE(D % 16 == 0, SOLATTN_EUNSUPPORTED, "%s: head_dim %lld of an 8-bit cache (multiples of 16)", what,
+                    (long long)D);
+    SOLATTN_REQUIRE(c.kq.exps && c.vq.exps, SOLATTN_EINVAL, "%s: null scales", what);
+    c.kq.codes = static_cast<uint8_t*>(c.k), c.kq.p = c.kp, c.kq.s = c.ks, c.kq.h = c.kh;
+    c.vq.codes = static_cast<uint8_t*>(c.v), c.vq.p = c.vp, c.vq.s = c.vs, c.vq.h = c.vh;
+  }
+  a.cache = c;
+  return !codes                      ? launch<SameType>(a, dtype, s, what)
+         : cache_type == SOLATTN_INT8 ? launch<Int8Codes>(a, dtype, s, what)
+                                      : launch<Fp8Codes>(a, dtype, s, what);
 }
 
 extern "C" int solattn_qk_norm_rope_append(
@@ -478,33 +538,38 @@ extern "C" int solattn_qk_norm_rope_append(
     int64_t page_size, const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
     solattn_stream_t stream) {
   clear_error();
-  const char* what = "qk_norm_rope_append";
   RopeArgs a{};
   a.q = {const_cast<void*>(q), sq_b, sq_t, sq_h};
   a.k = {const_cast<void*>(k), sk_b, sk_t, sk_h};
   a.v = {const_cast<void*>(v), sv_b, sv_t, sv_h};
   a.qo = {qo, sqo_b, sqo_t, sqo_h};
-  a.qw = q_weight;
-  a.kw = k_weight;
-  a.cos = cos;
-  a.sin = sin;
-  if (int rc = setup(a, B, T, H, Hkv, D, dtype, P, R, interleaved, eps, what)) return rc;
-  SOLATTN_REQUIRE(Hkv > 0 && page_table && lengths, SOLATTN_EINVAL, "%s: null page table or lengths", what);
-  SOLATTN_REQUIRE(pages >= 0 && pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31) && max_pages >= 0 &&
-                      max_pages < (1ll << 31) && max_pages * page_size < (1ll << 31),
-                  SOLATTN_EUNSUPPORTED, "%s: pages beyond 2^31 tokens", what);
-  const int e = esize(dtype);
-  const Rows kc{k_cache, skc_p, skc_s, skc_h}, vc{v_cache, svc_p, svc_s, svc_h};
-  int rc = check_rows(a.q, e, what, "q");
-  if (!rc) rc = check_rows(a.k, e, what, "k");
-  if (!rc) rc = check_rows(a.v, e, what, "v");
-  if (!rc) rc = check_rows(a.qo, e, what, "q output");
-  if (!rc) rc = check_rows(kc, e, what, "k_cache");
-  if (!rc) rc = check_rows(vc, e, what, "v_cache");
-  if (rc) return rc;
-  a.cache = {k_cache, v_cache, skc_p, skc_s, skc_h, svc_p, svc_s, svc_h, page_table, table_stride, lengths,
-             static_cast<int>(pages), static_cast<int>(page_size), static_cast<int>(max_pages)};
-  return launch<true>(a, dtype, reinterpret_cast<hipStream_t>(stream), what);
+  a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin;
+  const Cache c{k_cache, v_cache, skc_p, skc_s, skc_h, svc_p, svc_s, svc_h, {}, {}, page_table, table_stride, lengths};
+  return append(a, B, T, H, Hkv, D, dtype, P, R, interleaved, eps, c, pages, page_size, max_pages, -1,
+                reinterpret_cast<hipStream_t>(stream), "qk_norm_rope_append");
+}
+
+extern "C" int solattn_qk_norm_rope_append8(
+    const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h,
+    const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+    int dtype, const float* q_weight, const float* k_weight, const float* cos, const float* sin, int64_t P, int64_t R,
+    int interleaved, float eps, void* qo, int64_t sqo_b, int64_t sqo_t, int64_t sqo_h, void* k_cache, int64_t skc_p,
+    int64_t skc_s, int64_t skc_h, void* v_cache, int64_t svc_p, int64_t svc_s, int64_t svc_h, int64_t pages,
+    int64_t page_size, int cache_type, uint8_t* k_scale, int64_t sks_p, int64_t sks_h, uint8_t* v_scale, int64_t svs_p,
+    int64_t svs_h, const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+    solattn_stream_t stream) {
+  clear_error();
+  RopeArgs a{};
+  a.q = {const_cast<void*>(q), sq_b, sq_t, sq_h};
+  a.k = {const_cast<void*>(k), sk_b, sk_t, sk_h};
+  a.v = {const_cast<void*>(v), sv_b, sv_t, sv_h};
+  a.qo = {qo, sqo_b, sqo_t, sqo_h};
+  a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin;
+  Cache c{k_cache, v_cache, skc_p, skc_s, skc_h, svc_p, svc_s, svc_h, {}, {}, page_table, table_stride, lengths};
+  c.kq.exps = k_scale, c.kq.ep = sks_p, c.kq.eh = sks_h;
+  c.vq.exps = v_scale, c.vq.ep = svs_p, c.vq.eh = svs_h;
+  return append(a, B, T, H, Hkv, D, dtype, P, R, interleaved, eps, c, pages, page_size, max_pages,
+                cache_type < 0 ? 0 : cache_type, reinterpret_cast<hipStream_t>(stream), "qk_norm_rope_append");
 }
 
 extern "C" int64_t solattn_qk_norm_rope_bwd_workspace_bytes(int64_t D) {

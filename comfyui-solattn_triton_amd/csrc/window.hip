@@ -915,9 +915,15 @@ extern "C" int solattn_window_attn(const uint16_t* q, int64_t sq_b, int64_t sq_t
                     what, (long long)q_start, (long long)Tk, (long long)window);
     if (window > Tk) window = Tk;
     if (sinks > Tk) sinks = Tk;
-    return paged_attn(q, sq_b, sq_h, k, sk_b, sk_t, sk_h, v, sv_b, sv_t, sv_h, B, q_start + 1, nullptr, 0, 1, lengths,
-                      q_start + 1, B, H, Hkv, D, dtype, window, sinks, scale, workspace, workspace_bytes, o, so_b, so_h,
-                      reinterpret_cast<hipStream_t>(stream), what);
+    PagedCall p{};
+    p.q = q, p.sq_b = sq_b, p.sq_h = sq_h;
+    p.k = k, p.sk_p = sk_b, p.sk_s = sk_t, p.sk_h = sk_h;
+    p.v = v, p.sv_p = sv_b, p.sv_s = sv_t, p.sv_h = sv_h;
+    p.pages = B, p.page_size = q_start + 1, p.max_pages = 1, p.lengths = lengths, p.length = q_start + 1;
+    p.B = B, p.H = H, p.Hkv = Hkv, p.D = D, p.dtype = dtype;
+    p.window = window, p.sinks = sinks, p.groups = 1, p.scale = scale;
+    p.workspace = workspace, p.workspace_bytes = workspace_bytes, p.o = o, p.so_b = so_b, p.so_h = so_h;
+    return paged_attn(p, reinterpret_cast<hipStream_t>(stream), what);
   }
   WindowArgs a{};
   a.q = {q, sq_b, sq_t, sq_h}, a.k = {k, sk_b, sk_t, sk_h}, a.v = {v, sv_b, sv_t, sv_h};

@@ -368,6 +368,7 @@ int solattn_sol_attn_noalloc(const uint16_t* q, int64_t sq_b, int64_t sq_t, int6
  * so; strides may be 0 for inputs, token strides below 2^24 elements. Sums, softmax statistics and
  * accumulators are fp32; outputs are rounded once. */
 enum { SOLATTN_BF16 = 0, SOLATTN_FP16 = 1, SOLATTN_FP32 = 2 }; /* dtype arguments */
+enum { SOLATTN_INT8 = 1, SOLATTN_E4M3 = 2 };                   /* cache_type arguments */
 
 /* Per (batch, token, head) row x of q and k, D channels (a multiple of 8 up to 128):
  *   n = x / sqrt(mean(x^2) + eps) * weight        (weight null: 1)
@@ -479,6 +480,73 @@ int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint
                        int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t window, int64_t sinks,
                        float scale, void* workspace, int64_t workspace_bytes, uint16_t* o, int64_t so_b,
                        int64_t so_h, solattn_stream_t stream);
+
+/* ------------------------------------------------------- caches of 8 bits --
+ * A cache k_cache, v_cache [pages][page_size][Hkv][D] of codes (cache_type SOLATTN_INT8:
+ * two's complement; SOLATTN_E4M3: four bits of exponent, three of mantissa, no
+ * infinities) with k_scale, v_scale [pages][Hkv][page_size], an exponent byte b for each
+ * row: a value is code 2^(b - 127). Codes' rows are 16-byte aligned and every stride
+ * keeps them so (D a multiple of 16 up to 128); scales' last dim is contiguous, their
+ * strides are those of pages and heads.
+ * Written rows: the smallest power of two that keeps the row's largest magnitude within
+ * 127 or 448 (below 2^-110: a row of zeros), codes rounded to nearest even. A row that
+ * holds a NaN or an infinity reads as NaN in every channel.
+ *
+ * solattn_qk_norm_rope_append with such a cache; k' is rounded once, from fp32. */
+int solattn_qk_norm_rope_append8(
+    const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_b,
+    int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int64_t B,
+    int64_t T, int64_t H, int64_t Hkv, int64_t D, int dtype, const float* q_weight,
+    const float* k_weight, const float* cos, const float* sin, int64_t P, int64_t R, int interleaved,
+    float eps, void* qo, int64_t sqo_b, int64_t sqo_t, int64_t sqo_h, void* k_cache, int64_t skc_p,
+    int64_t skc_s, int64_t skc_h, void* v_cache, int64_t svc_p, int64_t svc_s, int64_t svc_h,
+    int64_t pages, int64_t page_size, int cache_type, uint8_t* k_scale, int64_t sks_p, int64_t sks_h,
+    uint8_t* v_scale, int64_t svs_p, int64_t svs_h, const int32_t* page_table, int64_t table_stride,
+    int64_t max_pages, const int32_t* lengths, solattn_stream_t stream);
+
+/* k and v [B][T][Hkv][D] (any dtype), the newest T tokens of sequences of lengths[b]
+ * tokens, as they are: what solattn_qk_norm_rope_append8 does of k' and v, with its rule
+ * of the places. */
+int solattn_cache_append(const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v,
+                         int64_t sv_b, int64_t sv_t, int64_t sv_h, int64_t B, int64_t T, int64_t Hkv,
+                         int64_t D, int dtype, void* k_cache, int64_t skc_p, int64_t skc_s,
+                         int64_t skc_h, void* v_cache, int64_t svc_p, int64_t svc_s, int64_t svc_h,
+                         int64_t pages, int64_t page_size, int cache_type, uint8_t* k_scale,
+                         int64_t sks_p, int64_t sks_h, uint8_t* v_scale, int64_t svs_p, int64_t svs_h,
+                         const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                         const int32_t* lengths, solattn_stream_t stream);
+
+/* Row t of k and v [B][T][Hkv][D] (bf16 or fp16) becomes key start[b] + t of sequence b
+ * (start null: t); zeros where that is not in [0, lengths[b]), past the table, or on a
+ * page id outside [0, pages). */
+int solattn_cache_read(const void* k_cache, int64_t skc_p, int64_t skc_s, int64_t skc_h,
+                       const void* v_cache, int64_t svc_p, int64_t svc_s, int64_t svc_h, int64_t pages,
+                       int64_t page_size, int cache_type, const uint8_t* k_scale, int64_t sks_p,
+                       int64_t sks_h, const uint8_t* v_scale, int64_t svs_p, int64_t svs_h,
+                       const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                       const int32_t* lengths, const int32_t* start, int64_t B, int64_t T, int64_t Hkv,
+                       int64_t D, int dtype, uint16_t* k, int64_t sk_b, int64_t sk_t, int64_t sk_h,
+                       uint16_t* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, solattn_stream_t stream);
+
+/* solattn_paged_attn with a cache of codes (cache_type 0: of dtype, scales null;
+ * page_size and scales' strides multiples of 8, scales 8-byte aligned), and for batches
+ * whose sequences have keys in common: of each of `groups` runs of B / groups sequences
+ * the first `shared` keys are the same, and are read once, from the pages of the run's
+ * longest sequence (the first of these); the other sequences' pages for them are not
+ * looked at. With shared > 0: no window. A NaN or infinity in v at a key behind the end
+ * of a sequence that is shorter than `shared` (but not empty) can reach it. */
+int64_t solattn_paged_attn_shared_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
+                                            int64_t page_size, int64_t window, int64_t sinks,
+                                            int cache_type, int64_t shared, int64_t groups);
+int solattn_paged_attn_shared(const uint16_t* q, int64_t sq_b, int64_t sq_h, const void* k_cache, int64_t sk_p,
+                        int64_t sk_s, int64_t sk_h, const void* v_cache, int64_t sv_p, int64_t sv_s,
+                        int64_t sv_h, int64_t pages, int64_t page_size, int cache_type,
+                        const uint8_t* k_scale, int64_t sks_p, int64_t sks_h, const uint8_t* v_scale,
+                        int64_t svs_p, int64_t svs_h, const int32_t* page_table, int64_t table_stride,
+                        int64_t max_pages, const int32_t* lengths, int64_t B, int64_t H, int64_t Hkv,
+                        int64_t D, int dtype, int64_t window, int64_t sinks, int64_t shared,
+                        int64_t groups, float scale, void* workspace, int64_t workspace_bytes, uint16_t* o,
+                        int64_t so_b, int64_t so_h, solattn_stream_t stream);
 
 #ifdef __cplusplus
 }
