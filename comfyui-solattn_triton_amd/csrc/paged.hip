@@ -20,7 +20,7 @@
 //     and transposes them in registers (v_perm_b32), one A operand per channel of
 //     the D / 16: row i of operand j is channel (D / 16) i + j.
 // The row's statistics need an exchange between the lanes g only.
-#include "cache8.hpp"
+#include "paged_tiles.hpp"
 
 namespace solattn {
 namespace {
@@ -411,6 +411,46 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
   }
 }
 
+// The same for 128 columns of several sequences, by tiles in LDS: steps of 64 keys.
+constexpr int kTiled = kTileRows / kGroups;  // its tiles of columns
+template <typename E, typename C, int D>
+__device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, const Work& w) {
+  static_assert(kWaves * 64 == kTileThreads, "a wave for 32 rows");
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = 32 * wave_id() + (lane & 31);
+  int b, h;
+  w.row(a, row, true, b, h);
+  const int hi = min(sequence_length(a, b), w.vis.len);
+  int safe = hi;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) safe = min(safe, __shfl_xor(safe, o));
+  safe = __builtin_amdgcn_readfirstlane(safe);
+  const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p};
+  const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p};
+  const TilePages pg{a.table + w.b * a.table_b, a.by_page, a.pages, w.vis.len};
+  const uint32_t kb = lds_addr(lds), vb = kb + 2 * kKeys * D;
+  RowState<D / 32> st;
+  const uint16_t* q = a.q + b * a.sq_b + h * a.sq_h;
+  if constexpr (kCodes<C>)
+    attend_tiles<E, D, HalfDecode<E, C, D, kByRow>, HalfDecode<E, C, D, kTransposed>>(st, q, kb, vb, ks, vs, pg, w.step0,
+                                                                                     w.step1 - w.step0, hi, safe, a.c);
+  else
+    attend_tiles<E, D, HalfCopy<D, kByRow>, HalfCopy<D, kTransposed>>(st, q, kb, vb, ks, vs, pg, w.step0,
+                                                                     w.step1 - w.step0, hi, safe, a.c);
+  const float l = xhalf_sum(st.l);
+  if (row >= w.ncol) return;
+  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
+  float* p = a.part + at * D + 4 * half;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x16& x = st.acc[dt];
+      *reinterpret_cast<float4*>(p + 32 * dt + 8 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    }
+  if (half == 0)
+    *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(l == 0.f ? -INFINITY : st.m, l);
+}
+
 // Nothing in this part: the join passes over a sum of 0.
 template <bool MANY>
 __device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
@@ -440,11 +480,14 @@ __device__ __forceinline__ void longest(const PagedArgs& a, int first, int& b, i
   len = __builtin_amdgcn_readfirstlane(top);
 }
 
-// PT: tiles of 16 columns over shared keys (0: a launch without any).
+// PT: tiles of 16 columns over shared keys (0: a launch without any; kTiled: by tiles in LDS).
 template <typename E, typename C, int DP, bool kFull, int PT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 paged_kernel(const PagedArgs a) {
-  __shared__ PagedLds<DP> lds;
+  constexpr bool TILED = PT == kTiled;
+  constexpr size_t kLds = TILED && 4 * kKeys * DP > sizeof(PagedLds<DP>) ? 4 * kKeys * DP : sizeof(PagedLds<DP>);
+  __shared__ __align__(256) uint8_t lds_bytes[kLds];
+  PagedLds<DP>& lds = *reinterpret_cast<PagedLds<DP>*>(lds_bytes);
   fetch_arguments(a);
   uint32_t n = blockIdx.x;
   Work w;
@@ -462,10 +505,13 @@ paged_kernel(const PagedArgs a) {
       int len;
       longest(a, w.seq, w.b, len);
       w.vis = visible<C>(min(len, a.shared), 0, 0);
+      if constexpr (TILED) w.vis.steps = (w.vis.len + kKeys - 1) / kKeys;
       const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
       w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
       if (w.step0 >= w.step1)
         no_keys<true>(a, w);
+      else if constexpr (TILED)
+        attend_many<E, C, DP>(a, lds_bytes, w);
       else
         attend<E, C, DP, kFull, PT, true>(a, lds, w);
       return;
@@ -547,6 +593,9 @@ int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, 
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
+#ifndef TILED_FROM
+#define TILED_FROM 64
+#endif
 // How a call is cut.
 struct Cut {
   int64_t tiles, split;
@@ -554,12 +603,12 @@ struct Cut {
   int64_t parts() const { return psplit + split; }
   int64_t part_bytes(int64_t B, int64_t H, int64_t D) const { return parts() > 1 ? B * H * parts() * (D + 2) * 4 : 0; }
 };
-Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups) {
+Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups) {
   Cut c{};
   c.tiles = cdiv(H / Hkv, kGroups);
   if (shared > 0) {
     const int64_t cols = B / groups * (H / Hkv);
-    c.ctiles = cols > kGroups ? 2 : 1;
+    c.ctiles = cols > kGroups ? cols > TILED_FROM && (D == 64 || D == 128) ? kTiled : 2 : 1;
     c.ptiles = cdiv(cols, kGroups * c.ctiles);
     int64_t n = 1024 / (groups * Hkv * c.ptiles);
     const int64_t steps = cdiv(shared, 2 * kBlock) / kWaves;
@@ -575,6 +624,9 @@ Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t keys, int64_t window, int64_t
 // The kernel of a head dim: <channels of the registers, all of them used>.
 template <typename E, typename C, int PT>
 auto kernel_of(int64_t D) {
+  if constexpr (PT == kTiled)
+    return D == 128 ? paged_kernel<E, C, 128, true, PT> : paged_kernel<E, C, 64, true, PT>;
+  else
   return D == 128 ? paged_kernel<E, C, 128, true, PT>
          : D == 64 ? paged_kernel<E, C, 64, true, PT>
          : D > 64  ? paged_kernel<E, C, 128, false, PT>
@@ -582,7 +634,10 @@ auto kernel_of(int64_t D) {
 }
 template <typename E, typename C>
 auto kernel_of(int64_t D, int64_t ctiles) {
-  return ctiles == 0 ? kernel_of<E, C, 0>(D) : ctiles == 1 ? kernel_of<E, C, 1>(D) : kernel_of<E, C, 2>(D);
+  return ctiles == 0   ? kernel_of<E, C, 0>(D)
+         : ctiles == 1 ? kernel_of<E, C, 1>(D)
+         : ctiles == 2 ? kernel_of<E, C, 2>(D)
+                       : kernel_of<E, C, kTiled>(D);
 }
 template <typename E>
 auto kernel_of(int64_t D, int64_t ctiles, int cache_type) {
@@ -646,7 +701,9 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.group = static_cast<int>(H / Hkv);
   a.window = static_cast<int>(p.window), a.sinks = static_cast<int>(p.sinks);
   a.c = p.scale * kLog2e;
-  const Cut c = cut(B, H, Hkv, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups);
+  const Cut c = cut(B, H, Hkv, D, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups);
+  SOLATTN_REQUIRE(c.ctiles != kTiled || (es * p.sk_s < (1ll << 28) && es * p.sv_s < (1ll << 28) && p.sk_s >= 0 && p.sv_s >= 0),
+                  SOLATTN_EUNSUPPORTED, "%s: slots of a cache 2^28 bytes apart, shared keys", what);
   a.tiles = static_cast<int>(c.tiles), a.split = static_cast<int>(c.split);
   a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split);
   a.parts = static_cast<int>(c.parts());
@@ -683,7 +740,7 @@ int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || keys < 0 || window < 0 || sinks < 0) return 0;
   if (B >= top || H >= top || B * H >= top || D > 128 || keys >= top) return 0;
   if (shared < 0 || shared >= top || (shared && (groups <= 0 || B % groups))) return 0;
-  return cut(B, H, Hkv, keys, window, sinks, shared, groups).part_bytes(B, H, D);
+  return cut(B, H, Hkv, D, keys, window, sinks, shared, groups).part_bytes(B, H, D);
 }
 
 }  // namespace solattn

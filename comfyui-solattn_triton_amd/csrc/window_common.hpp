@@ -398,4 +398,87 @@ __device__ __forceinline__ void mask_keys(f32x16& s, const RowKeys& rk, int firs
   }
 }
 
+// ------------------------------------------------------------ the forwards' step
+// Running maximum before any visible key: finite, so that exp2 of a masked score
+// stays 0, and below every score that counts.
+constexpr float kNoMax = -1e30f;
+
+template <int ND>
+struct RowState {
+  float m, l;      // running max (log2 domain) and this lane's row sum
+  f32x16 acc[ND];  // O^T
+};
+
+// One step of the forward's pipeline over half tiles of 32 keys, in one hand-ordered
+// stream: S(n+1) = K(n+1) Q^T, O += P(n-1) V(n-1) and the softmax of S(n). Slot i
+// issues a score MFMA, two exps and a P.V MFMA; the operands of slot i + 2 are read
+// at its top (the empty asm keeps them there). The running max stays as it is unless
+// a lane's sum of P passes 255 (no sum above 255: no score more than 8 above it), in
+// which case P is made again and O rescaled, behind the products with P(n-1).
+template <typename E, int D>
+__device__ __forceinline__ void window_step(RowState<D / 32>& st, const f32x16& sc, f32x16& sn, const bf16x8 (&pp)[2],
+                                            bf16x8 (&pn)[2], uint32_t kl, uint32_t vl, const bf16x8 (&q)[D / 16],
+                                            float c) {
+  constexpr int ND = D / 32, NM = D / 16, SLOTS = 8 / NM;
+  bf16x8 ka[3], va[3];
+  uint32_t pw[2][4];
+  float psum = 0.f;
+  const float neg = -st.m;
+  ka[0] = k_op_x<D>(kl, 0, 0);
+  ka[1] = k_op_x<D>(kl, 0, 1);
+  va[0] = v_op_x<D>(vl, 0, 0);
+  va[1] = v_op_x<D>(vl, 0, 1);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int j = i / SLOTS;
+    if (i % SLOTS == 0) {
+      if (j + 2 < NM) {
+        ka[(j + 2) % 3] = k_op_x<D>(kl, 0, j + 2);
+        va[(j + 2) % 3] = v_op_x<D>(vl, (j + 2) / ND, (j + 2) % ND);
+        asm volatile("" ::: "memory");
+      }
+      if (j == 0)
+        E::amfma0(sn, ka[0], q[0]);
+      else
+        E::amfma(sn, ka[j % 3], q[j]);
+    }
+    pw[i >> 2][i & 3] = E::exp_pair(sc[2 * i], sc[2 * i + 1], c, neg, psum);
+    if (i % SLOTS == SLOTS - 1) {
+      if (j == 0)
+        E::amfma_first(st.acc[0], va[0], pp[0]);
+      else if (j == NM - 1)
+        E::amfma_tie(st.acc[ND - 1], va[j % 3], pp[1], sn);
+      else
+        E::amfma(st.acc[j % ND], va[j % 3], pp[j / ND]);
+    }
+    if (i == 0) __builtin_amdgcn_s_setprio(1);
+  }
+  __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+    pn[ks] = __builtin_bit_cast(bf16x8, make_uint4(pw[ks][0], pw[ks][1], pw[ks][2], pw[ks][3]));
+  if (__any(!(psum <= 255.f))) {  // (also infinities and NaN)
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+    float alpha;
+    const float m_new = new_max(st.m, xhalf_max(mx) * c, alpha);
+    if (__any(m_new != st.m)) {  // lanes whose max stays make the same P
+      st.m = m_new;
+      st.l *= alpha;
+      psum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pw[i >> 2][i & 3] = E::exp_pair(sc[2 * i], sc[2 * i + 1], c, -m_new, psum);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        pn[ks] = __builtin_bit_cast(bf16x8, make_uint4(pw[ks][0], pw[ks][1], pw[ks][2], pw[ks][3]));
+      mfma_fence(st.acc);  // the rescale reads O
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) st.acc[dt] *= alpha;
+    }
+  }
+  st.l += psum;
+}
+
 }  // namespace solattn
