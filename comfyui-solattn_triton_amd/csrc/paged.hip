@@ -424,8 +424,9 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, co
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) safe = min(safe, __shfl_xor(safe, o));
   safe = __builtin_amdgcn_readfirstlane(safe);
-  const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p};
-  const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p};
+  const auto near = [](int64_t slot) { return slot >= 0 && slot < (1 << 28); };
+  const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p, near(a.sk_s)};
+  const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p, near(a.sv_s)};
   const TilePages pg{a.table + w.b * a.table_b, a.by_page, a.pages, w.vis.len};
   const uint32_t kb = lds_addr(lds), vb = kb + 2 * kKeys * D;
   RowState<D / 32> st;
@@ -702,8 +703,6 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.window = static_cast<int>(p.window), a.sinks = static_cast<int>(p.sinks);
   a.c = p.scale * kLog2e;
   const Cut c = cut(B, H, Hkv, D, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups);
-  SOLATTN_REQUIRE(c.ctiles != kTiled || (es * p.sk_s < (1ll << 28) && es * p.sv_s < (1ll << 28) && p.sk_s >= 0 && p.sv_s >= 0),
-                  SOLATTN_EUNSUPPORTED, "%s: slots of a cache 2^28 bytes apart, shared keys", what);
   a.tiles = static_cast<int>(c.tiles), a.split = static_cast<int>(c.split);
   a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split);
   a.parts = static_cast<int>(c.parts());

@@ -3,11 +3,13 @@
 // windowed forward has (window_common.hpp). A row is a head of one of the sequences that
 // share the keys.
 //
-// What differs is where a half comes from: a wave copies rows of eight consecutive keys at
-// most, so of one page, whose id a lane has read two halves ahead; the copy's base is
-// scalar. Keys past the end or on pages that are none of the cache's come from a row of
-// zeros and are masked. Codes go through registers and become 16-bit values there, once
-// for all the rows that read the tile.
+// What differs is where keys come from: a lane finds the place of one key of a tile of 64
+// well ahead of its copy, and the copies of a half (rows of eight consecutive keys a wave
+// at most, so of one page) take their scalar bases from these lanes. (Bases found by each
+// copy in scalar arithmetic: some 40 scalar instructions a copy, 160 a step of 16 matrix
+// instructions.) Keys past the end or on pages that are none of the cache's are rows of
+// zeros, and masked. Codes go through registers and become 16-bit values there, once for
+// all the rows that read the tile.
 #pragma once
 
 #include "cache8.hpp"
@@ -19,59 +21,85 @@ constexpr int kTileRows = 128, kTileThreads = 2 * kTileRows;
 
 static __device__ uint4 zero_row[16];  // (never written)
 
-// The cache as the tiles read it; strides in bytes, slots' below 2^28.
+// The cache as the tiles read it; strides in bytes.
 struct TileSource {
   const uint8_t* p;  // this kv head
   int64_t page, slot;
   const uint8_t* e;  // codes: exponents
   int64_t e_page;
+  bool near;         // a few slots are within 32 bits
 };
 
-// The pages' ids of the 32 keys of a half, a lane each (twice); -1: not visible.
+// Where a tile's keys are, a lane each: rows' addresses and, of codes, their powers of two.
+struct TileRows {
+  uint32_t lo, hi;
+  float power;
+  __device__ __forceinline__ const uint8_t* of_lane(int lane) const {  // (another for every lane)
+    const uint64_t x = static_cast<uint32_t>(__shfl(lo, lane)) | static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, lane))) << 32;
+    return reinterpret_cast<const uint8_t*>(x);
+  }
+  __device__ __forceinline__ const uint8_t* of_group(int lane) const {  // (the same for all)
+    const uint64_t x = static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, lane)) |
+                       static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, lane))) << 32;
+    return reinterpret_cast<const uint8_t*>(x);
+  }
+};
+
 struct TilePages {
   const int32_t* table;  // the sequence's row
   Divisor by_page;
   int pages, end;        // keys [0, end) are visible
+  // The page of this lane's key of the 64 from j0 on; -1: not visible.
   __device__ __forceinline__ int ids(int j0) const {
-    const int j = j0 + (static_cast<int>(threadIdx.x) & 31);
+    const int j = j0 + (static_cast<int>(threadIdx.x) & 63);
     const int id = table[by_page.of(static_cast<uint32_t>(min(j, end - 1)))];
     return j < end && id >= 0 && id < pages ? id : -1;
   }
-  __device__ __forceinline__ int slot(int j) const {
-    const uint32_t n = static_cast<uint32_t>(j);
-    return static_cast<int>(n - by_page.of(n) * by_page.d);
+  template <bool CODES>
+  __device__ __forceinline__ TileRows rows(int id, int j0, const TileSource& s) const {
+    const uint32_t j = static_cast<uint32_t>(j0 + (static_cast<int>(threadIdx.x) & 63));
+    const uint32_t slot = j - by_page.of(j) * by_page.d;
+    const uint8_t* at = id >= 0 ? s.p + id * s.page + slot * s.slot : reinterpret_cast<const uint8_t*>(zero_row);
+    TileRows r;
+    r.lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at));
+    r.hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at) >> 32);
+    r.power = 0.f;
+    if constexpr (CODES)
+      if (id >= 0) r.power = power_of(s.e[id * s.e_page + slot]);
+    return r;
   }
 };
 
-// Copies of one half (keys j0 .. j0 + 31) into the half buffer at dst.
+// Copies of half `hf` of a tile into the half buffer at dst: start() asks for the rows,
+// finish() has them in LDS, or on their way there.
 template <int D, int HOW>
 struct HalfCopy {  // 16-bit values, straight into LDS
+  static constexpr bool kCodes = false;
   static constexpr int C = D / 8, R = 64 / C, U = 32 / (kTileThreads / C);  // pieces of a row; rows of a wave's copy; copies
   uint32_t off;
   __device__ __forceinline__ void init(const TileSource& s) {
-    const int lane = threadIdx.x & 63, row = R * wave_id() + lane / C;
-    off = static_cast<uint32_t>(lane / C * s.slot + swz<D, HOW>(row, lane % C) * 16);
+    off = static_cast<uint32_t>((threadIdx.x & 63) / C * s.slot) + piece();
   }
-  __device__ __forceinline__ void start(uint32_t dst, int j0, int ids, const TileSource& s, const TilePages& pg) const {
+  __device__ __forceinline__ uint32_t piece() const {
     const int lane = threadIdx.x & 63;
+    return swz<D, HOW>(R * wave_id() + lane / C, lane % C) * 16;
+  }
+  __device__ __forceinline__ void start(uint32_t dst, int hf, uint64_t seen, const TileRows& rows, const TileSource& s) {
+    const bool plain = static_cast<uint32_t>(seen >> (32 * hf)) == ~0u && s.near;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int g0 = u * (kTileThreads / C) + R * wave_id(), j = j0 + g0;
-      const uint32_t to = dst + g0 * 2 * D;
-      const int id = __builtin_amdgcn_readlane(ids, g0);
-      const uint8_t* base = s.p + max(id, 0) * s.page + pg.slot(j) * s.slot;
-      if (id >= 0 && j + R <= pg.end) {
-        g2l16_s(base, off, to);
-      } else {
-        const bool on = id >= 0 && j + lane / C < pg.end;
-        g2l16(on ? base + off : reinterpret_cast<const uint8_t*>(zero_row) + lane % C * 16, to);
-      }
+      const int g0 = u * (kTileThreads / C) + R * wave_id();
+      if (plain)
+        g2l16_s(rows.of_group(32 * hf + g0), off, dst + g0 * 2 * D);
+      else
+        g2l16(rows.of_lane(32 * hf + g0 + (threadIdx.x & 63) / C) + piece(), dst + g0 * 2 * D);
     }
   }
   __device__ __forceinline__ void finish(uint32_t) const {}
 };
 template <typename E, typename CODES, int D, int HOW>
 struct HalfDecode {  // codes, 16 of a row a thread, through registers
+  static constexpr bool kCodes = true;
   static constexpr int C = D / 16;
   uint4 w;
   float power;
@@ -83,15 +111,11 @@ struct HalfDecode {  // codes, 16 of a row a thread, through registers
     to0 = row * 2 * D + swz<D, HOW>(row, 2 * pc) * 16;
     to1 = row * 2 * D + swz<D, HOW>(row, 2 * pc + 1) * 16;
   }
-  __device__ __forceinline__ void start(uint32_t, int j0, int ids, const TileSource& s, const TilePages& pg) {
-    const int e = threadIdx.x, row = e / C % 32, pc = e % C;
-    const int id = __shfl(ids, row), slot = pg.slot(j0 + row);
-    w = make_uint4(0, 0, 0, 0);
-    power = 0.f;
-    if (id >= 0 && mine) {
-      w = *reinterpret_cast<const uint4*>(s.p + id * s.page + slot * s.slot + pc * 16);
-      power = power_of(s.e[id * s.e_page + slot]);
-    }
+  __device__ __forceinline__ void start(uint32_t, int hf, uint64_t, const TileRows& rows, const TileSource&) {
+    const int e = threadIdx.x, row = 32 * hf + e / C % 32;
+    power = __shfl(rows.power, row);
+    const uint8_t* at = rows.of_lane(row);
+    if (mine) w = *reinterpret_cast<const uint4*>(at + e % C * 16);
   }
   __device__ __forceinline__ void finish(uint32_t dst) const {
     if (!mine) return;
@@ -120,7 +144,8 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_
   constexpr uint32_t kHalf = kKeys * D;  // bytes of half a tile
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const uint32_t kl = k_lane<D>(kb, lane & 31, half), vl = v_lane<D>(vb, lane);
-  const int first = tile0 * kKeys, last = 2 * ntiles - 1;
+  constexpr bool Q8 = KCopy::kCodes;
+  const int first = tile0 * kKeys;
   KCopy kc;
   VCopy vc;
   kc.init(ks);
@@ -129,17 +154,20 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_
   st.l = 0.f;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt) st.acc[dt] = f32x16{};
-  const auto ids_of = [&](int n) __attribute__((always_inline)) { return pg.ids(first + 32 * min(n, last)); };
+  const auto key0 = [&](int t) __attribute__((always_inline)) { return first + kKeys * min(t, ntiles - 1); };
+  const auto ids_of = [&](int t) __attribute__((always_inline)) { return pg.ids(key0(t)); };
+  const auto krows = [&](int id, int t) __attribute__((always_inline)) { return pg.template rows<Q8>(id, key0(t), ks); };
+  const auto vrows = [&](int id, int t) __attribute__((always_inline)) { return pg.template rows<Q8>(id, key0(t), vs); };
   const auto land = [&]() __attribute__((always_inline)) {
     wait_tile_copies();
     __syncthreads();
   };
-  // Scores of half n: keys that are not visible become -inf.
-  const auto mask = [&](f32x16& s, int n, int ids) __attribute__((always_inline)) {
-    const uint32_t seen = static_cast<uint32_t>(__ballot(ids >= 0));
-    const int j0 = first + 32 * n;
-    if (seen != ~0u || j0 + 32 > safe) {
-      const uint32_t bits = (seen >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
+  // Scores of half hf of the tile from j0 on: keys that are not visible become -inf.
+  const auto mask = [&](f32x16& s, int j0, int hf, uint64_t seen) __attribute__((always_inline)) {
+    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * hf));
+    j0 += 32 * hf;
+    if (mine != ~0u || j0 + 32 > safe) {
+      const uint32_t bits = (mine >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const uint32_t w = bit_word(bits, r);
@@ -147,77 +175,83 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_
       }
     }
   };
-  // ids of the halves n to n + 3 in step n
-  int i0 = ids_of(0), i1 = ids_of(1), i2 = ids_of(2), i3 = ids_of(3);
-  kc.start(kb, first, i0, ks, pg);
-  kc.finish(kb);
-  kc.start(kb + kHalf, first + 32, i1, ks, pg);
-  kc.finish(kb + kHalf);
-  vc.start(vb, first, i0, vs, pg);
-  vc.finish(vb);
+  // In round t: K's rows of the tiles t + 1 and t + 2, V's of t and t + 1; those of a tile
+  // further on are found here, the ids of t + 4 asked for.
+  int i2, i3, i4;
+  uint64_t s0w, s1w, s2w, s3w;  // which keys of the tiles t, t + 1, t + 2, t + 3 are visible
+  TileRows k1, k2, v0, v1;
+  {
+    const int i0 = ids_of(0), i1 = ids_of(1);
+    i2 = ids_of(2), i3 = ids_of(3);
+    const TileRows k0 = krows(i0, 0);
+    v0 = vrows(i0, 0);
+    s0w = __ballot(i0 >= 0), s1w = __ballot(i1 >= 0), s2w = __ballot(i2 >= 0), s3w = __ballot(i3 >= 0);
+    kc.start(kb, 0, s0w, k0, ks);
+    kc.finish(kb);
+    kc.start(kb + kHalf, 1, s0w, k0, ks);
+    kc.finish(kb + kHalf);
+    vc.start(vb, 0, s0w, v0, vs);
+    vc.finish(vb);
+    k1 = krows(i1, 1), v1 = vrows(i1, 1), k2 = krows(i2, 2);
+  }
   bf16x8 q[NC];
   load_row<D>(q, qrow, half);
   f32x16 sa, sb;  // scores of even and odd halves
   bf16x8 pa[2], pb[2];
   land();
   {  // step 0, without a stream: both halves are scored, the running max is the whole tile's
-    f32x16 s0 = {}, s1 = {};
+    f32x16 x0 = {}, x1 = {};
 #pragma unroll
-    for (int cc = 0; cc < NC; ++cc) s0 = E::mfma32(k_op_x<D>(kl, 0, cc), q[cc], s0);
+    for (int cc = 0; cc < NC; ++cc) x0 = E::mfma32(k_op_x<D>(kl, 0, cc), q[cc], x0);
     __syncthreads();  // every wave is done with K(0)
-    if (last > 1) kc.start(kb, first + 64, i2, ks, pg);
+    if (ntiles > 1) kc.start(kb, 0, s1w, k1, ks);
 #pragma unroll
-    for (int cc = 0; cc < NC; ++cc) s1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], s1);
-    mask(s0, 0, i0);
-    mask(s1, 1, i1);
+    for (int cc = 0; cc < NC; ++cc) x1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], x1);
+    mask(x0, first, 0, s0w);
+    mask(x1, first, 1, s0w);
     float mx = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(s0[r], s1[r]));
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(x0[r], x1[r]));
     st.m = fmaxf(kNoMax, xhalf_max(mx) * c);
     uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = E::exp_pair(s0[2 * i], s0[2 * i + 1], c, -st.m, st.l);
+    for (int i = 0; i < 8; ++i) w[i] = E::exp_pair(x0[2 * i], x0[2 * i + 1], c, -st.m, st.l);
     pa[0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
     pa[1] = __builtin_bit_cast(bf16x8, make_uint4(w[4], w[5], w[6], w[7]));
-    sb = s1;
-    if (last > 1) kc.finish(kb);
+    sb = x1;
+    if (ntiles > 1) kc.finish(kb);
   }
   mfma_fence(st.acc);  // O's zeros are in their registers before the asm MFMAs that add to them
   land();
-  const auto next_ids = [&](int n) __attribute__((always_inline)) {
-    i0 = i1, i1 = i2, i2 = i3;
-    i3 = ids_of(n + 3);
-  };
-  const auto copies = [&](int n) __attribute__((always_inline)) {
-    if (n + 2 <= last) kc.start(kb + (n & 1) * kHalf, first + 32 * (n + 2), i2, ks, pg);
-    vc.start(vb + (n & 1) * kHalf, first + 32 * n, i0, vs, pg);
-  };
-  const auto landed = [&](int n) __attribute__((always_inline)) {
-    if (n + 2 <= last) kc.finish(kb + (n & 1) * kHalf);
-    vc.finish(vb + (n & 1) * kHalf);
-    land();
-  };
-  const auto odd = [&](int n) __attribute__((always_inline)) {
-    next_ids(n);
-    copies(n);
-    window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, c);
-    landed(n);
-  };
-  const auto even = [&](int n) __attribute__((always_inline)) {
-    next_ids(n);
-    copies(n);
-    mask(sa, n, i0);
-    window_step<E, D>(st, sa, sb, pb, pa, kl + kHalf, vl + kHalf, q, c);
-    mask(sb, n + 1, i1);
-    landed(n);
-  };
-  int n = 1;
+  int t = 0;
 #pragma unroll 1
-  for (; n < last; n += 2) {
-    odd(n);
-    even(n + 1);
+  for (; t < ntiles - 1; ++t) {
+    i4 = ids_of(t + 4);
+    const TileRows k3 = krows(i3, t + 3), v2 = vrows(i2, t + 2);
+    // step 2 t + 1: K of half 2 t + 3, V of 2 t + 1
+    kc.start(kb + kHalf, 1, s1w, k1, ks);
+    vc.start(vb + kHalf, 1, s0w, v0, vs);
+    window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, c);
+    kc.finish(kb + kHalf);
+    vc.finish(vb + kHalf);
+    land();
+    // step 2 t + 2: K of half 2 t + 4, V of 2 t + 2
+    if (t + 2 < ntiles) kc.start(kb, 0, s2w, k2, ks);
+    vc.start(vb, 0, s1w, v1, vs);
+    mask(sa, first + kKeys * (t + 1), 0, s1w);
+    window_step<E, D>(st, sa, sb, pb, pa, kl + kHalf, vl + kHalf, q, c);
+    mask(sb, first + kKeys * (t + 1), 1, s1w);
+    if (t + 2 < ntiles) kc.finish(kb);
+    vc.finish(vb);
+    land();
+    i2 = i3, i3 = i4;
+    k1 = k2, k2 = k3, v0 = v1, v1 = v2;
+    s0w = s1w, s1w = s2w, s2w = s3w, s3w = __ballot(i4 >= 0);
   }
-  odd(n);
+  vc.start(vb + kHalf, 1, s0w, v0, vs);
+  window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, c);
+  vc.finish(vb + kHalf);
+  land();
   mfma_fence(st.acc);
 #pragma unroll
   for (int i = 0; i < NC; ++i)  // P.V of the last half
