@@ -214,6 +214,7 @@ struct PagedCall {
 };
 int paged_attn(const PagedCall& call, hipStream_t s, const char* what);
 int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
-                             int64_t sinks, int64_t shared = 0, int64_t groups = 1);
+                             int64_t sinks, int64_t shared = 0, int64_t groups = 1,
+                             int cache_type = 0);
 
 }  // namespace solattn

@@ -27,8 +27,8 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kBlock = 32;      // keys of a block of products
-constexpr int kMaxSplits = 64;  // parts of a row
-constexpr int kMaxShared = 48;  // of these over shared keys
+constexpr int kMaxSplits = 64;  // parts of a row over its own keys
+constexpr int kMaxShared = 64;  // and over shared ones
 constexpr int kGroups = 16;     // query columns of a tile
 
 // What the cache holds: 16-bit values of the queries' type, or codes (cache8.hpp).
@@ -85,6 +85,37 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The same over all 64 lanes; within 16 by lane moves, in the order of a butterfly.
+template <typename F>
+__device__ __forceinline__ uint32_t over_row16(uint32_t x, F&& f) {
+#define SOLATTN_DPP(ctrl) \
+  x = f(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), ctrl, 0xf, 0xf, false)))
+  SOLATTN_DPP(0xB1);   // quad_perm 1 0 3 2
+  SOLATTN_DPP(0x4E);   // quad_perm 2 3 0 1
+  SOLATTN_DPP(0x141);  // row_half_mirror
+  SOLATTN_DPP(0x140);  // row_mirror
+#undef SOLATTN_DPP
+  return x;
+}
+template <typename F>
+__device__ __forceinline__ uint32_t over_wave(uint32_t x, F&& f) {
+  x = over_row16(x, f);
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(r[0], r[1]);
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __uint_as_float(over_wave(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return __uint_as_float(over_wave(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
 // exp2 of the distance to a maximum; a row without keys has the maximum -inf and weight 0.
 __device__ __forceinline__ float weight_of(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
@@ -115,6 +146,24 @@ __device__ __forceinline__ Visible visible(int len, int low, int sinks) {
   return s;
 }
 
+// The longest sequence of a run of `per` (the first of these), its length, and the lengths
+// of the first 64 sequences, a lane each.
+__device__ __forceinline__ int longest(const PagedArgs& a, int first, int& b, int& len) {
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < a.per ? sequence_length(a, first + lane) : -1;
+  int n = mine, at = lane;
+  for (int i = lane + 64; i < a.per; i += 64) {
+    const int x = sequence_length(a, first + i);
+    if (x > n) n = x, at = i;
+  }
+  const auto larger = [](uint32_t x, uint32_t y) { return static_cast<uint32_t>(max(static_cast<int>(x), static_cast<int>(y))); };
+  const int top = static_cast<int>(over_wave(static_cast<uint32_t>(n), larger));
+  const uint32_t best = over_wave(n == top ? static_cast<uint32_t>(at) : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
+  b = first + __builtin_amdgcn_readfirstlane(static_cast<int>(best));
+  len = __builtin_amdgcn_readfirstlane(top);
+  return mine;
+}
+
 // A workgroup's keys and columns. The columns of own keys are the heads of one sequence
 // that share a kv head, those of shared keys the heads of all its sequences.
 struct Work {
@@ -122,6 +171,12 @@ struct Work {
   int step0, step1, part;
   int b, seq;          // whose pages; the first column's sequence
   int hk, col0, ncol;  // columns col0 .. col0 + ncol - 1 of the kv head
+  int lengths;         // of several sequences: of the first 64, a lane each
+  // How many of the shared keys sequence b (another a lane) sees.
+  __device__ __forceinline__ int sees(const PagedArgs& a, int b) const {
+    const int n = a.per <= 64 ? __shfl(lengths, b - seq) : sequence_length(a, b);
+    return min(n, vis.len);
+  }
   __device__ __forceinline__ void row(const PagedArgs& a, int c, bool many, int& b, int& h) const {
     uint32_t n = col0 + min(c, ncol - 1);
     const uint32_t g = many ? a.by_group.split(n) : n;
@@ -131,7 +186,7 @@ struct Work {
 };
 
 template <int DP>
-struct PagedLds {
+struct __align__(16) PagedLds {
   float o[kWaves][kGroups][DP + 4];
   float m[kWaves][kGroups], l[kWaves][kGroups];
 };
@@ -163,7 +218,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
     int b, h;
     w.row(a, 16 * t + col, MANY, b, h);
     const uint16_t* qp = a.q + b * a.sq_b + h * a.sq_h;
-    hi[t] = MANY ? min(sequence_length(a, b), vis.len) : vis.len;
+    hi[t] = MANY ? w.sees(a, b) : vis.len;
     safe = min(safe, hi[t]);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
@@ -174,9 +229,8 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
     }
   }
   if constexpr (MANY) {
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) safe = min(safe, __shfl_xor(safe, o));
-    safe = __builtin_amdgcn_readfirstlane(safe);
+    safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
+        over_row16(static_cast<uint32_t>(safe), [](uint32_t x, uint32_t y) { return min(x, y); })));
   }
   f32x4 acc[NT][CH];
   float m[NT], l[NT];  // l: this lane's keys
@@ -368,45 +422,53 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
     }
   }
 
-  // Join the waves, a tile of columns at a time: O[q][channel], channel CH (4 g + i) + j in acc[j][i].
+  // Join the waves, a tile of columns at a time: O[q][channel], channel CH (4 g + i) + j in
+  // acc[j][i]. A thread takes eight channels of a column.
+  constexpr int L = DP / 8;
+  const int qc = threadIdx.x / L, ch = 8 * (threadIdx.x % L);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t) __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < CH; ++j) lds.o[wave][col][CH * (4 * g + i) + j] = acc[t][j][i];
+      for (int j = 0; j < CH; j += 4)
+        *reinterpret_cast<float4*>(&lds.o[wave][col][CH * (4 * g + i) + j]) =
+            make_float4(acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]);
     const float sum_l = over_groups_sum(l[t]);
     if (g == 0) {
       lds.m[wave][col] = m[t];
       lds.l[wave][col] = sum_l;
     }
     __syncthreads();
-    const int ncol = min(kGroups, w.ncol - 16 * t);
-    for (int e = threadIdx.x; e < ncol * (DP / 2); e += kWaves * 64) {
-      const int qc = e / (DP / 2), ch = 2 * (e % (DP / 2));
-      if (!kFull && ch >= a.D) continue;
-      float top = lds.m[0][qc];
+    if (qc >= min(kGroups, w.ncol - 16 * t) || (!kFull && ch >= a.D)) continue;
+    float top = lds.m[0][qc];
 #pragma unroll
-      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds.m[i][qc]);
-      float o0 = 0.f, o1 = 0.f, sum = 0.f;
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds.m[i][qc]);
+    float o[8] = {}, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        const float f = weight_of(lds.m[i][qc], top);
-        o0 = fmaf(lds.o[i][qc][ch], f, o0);
-        o1 = fmaf(lds.o[i][qc][ch + 1], f, o1);
-        sum = fmaf(lds.l[i][qc], f, sum);
-      }
-      int b, h;
-      w.row(a, 16 * t + qc, MANY, b, h);
-      if (a.parts > 1) {
-        const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
-        *reinterpret_cast<float2*>(a.part + at * a.D + ch) = make_float2(o0, o1);
-        if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
-      } else {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
-        *reinterpret_cast<uint32_t*>(a.o + b * a.so_b + h * a.so_h + ch) = E::pack(o0 * inv, o1 * inv);
-      }
+    for (int i = 0; i < kWaves; ++i) {
+      const float f = weight_of(lds.m[i][qc], top);
+      const float4 x = *reinterpret_cast<const float4*>(&lds.o[i][qc][ch]);
+      const float4 y = *reinterpret_cast<const float4*>(&lds.o[i][qc][ch + 4]);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
+      sum = fmaf(lds.l[i][qc], f, sum);
+    }
+    int b, h;
+    w.row(a, 16 * t + qc, MANY, b, h);
+    if (a.parts > 1) {
+      const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
+      float4* to = reinterpret_cast<float4*>(a.part + at * a.D + ch);
+      to[0] = make_float4(o[0], o[1], o[2], o[3]);
+      to[1] = make_float4(o[4], o[5], o[6], o[7]);
+      if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
+      *reinterpret_cast<uint4*>(a.o + b * a.so_b + h * a.so_h + ch) =
+          make_uint4(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv), E::pack(o[4] * inv, o[5] * inv),
+                     E::pack(o[6] * inv, o[7] * inv));
     }
   }
 }
@@ -419,11 +481,9 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, co
   const int lane = threadIdx.x & 63, half = lane >> 5, row = 32 * wave_id() + (lane & 31);
   int b, h;
   w.row(a, row, true, b, h);
-  const int hi = min(sequence_length(a, b), w.vis.len);
-  int safe = hi;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) safe = min(safe, __shfl_xor(safe, o));
-  safe = __builtin_amdgcn_readfirstlane(safe);
+  const int hi = w.sees(a, b);
+  const int safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
+      over_wave(static_cast<uint32_t>(hi), [](uint32_t x, uint32_t y) { return min(x, y); })));
   const auto near = [](int64_t slot) { return slot >= 0 && slot < (1 << 28); };
   const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p, near(a.sk_s)};
   const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p, near(a.sv_s)};
@@ -463,24 +523,6 @@ __device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
   }
 }
 
-// The longest sequence of a run of `per` (the first of these), and its length.
-__device__ __forceinline__ void longest(const PagedArgs& a, int first, int& b, int& len) {
-  const int lane = threadIdx.x & 63;
-  int n = -1, at = 0;
-  for (int i = lane; i < a.per; i += 64) {
-    const int x = sequence_length(a, first + i);
-    if (x > n) n = x, at = i;
-  }
-  int top = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o));
-  int best = n == top ? at : 0x7fffffff;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) best = min(best, __shfl_xor(best, o));
-  b = first + __builtin_amdgcn_readfirstlane(best);
-  len = __builtin_amdgcn_readfirstlane(top);
-}
-
 // PT: tiles of 16 columns over shared keys (0: a launch without any; kTiled: by tiles in LDS).
 template <typename E, typename C, int DP, bool kFull, int PT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
@@ -504,7 +546,7 @@ paged_kernel(const PagedArgs a) {
       w.col0 = tile * 16 * PT;
       w.ncol = min(16 * PT, a.per * a.group - w.col0);
       int len;
-      longest(a, w.seq, w.b, len);
+      w.lengths = longest(a, w.seq, w.b, len);
       w.vis = visible<C>(min(len, a.shared), 0, 0);
       if constexpr (TILED) w.vis.steps = (w.vis.len + kKeys - 1) / kKeys;
       const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
@@ -536,7 +578,7 @@ paged_kernel(const PagedArgs a) {
     attend<E, C, DP, kFull, 1, false>(a, lds, w);
 }
 
-// Joins the splits of a row: a wave per (b, head), two channels a lane.
+// Joins the parts of a row: a wave per (b, head), two channels a lane.
 template <typename E>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -544,13 +586,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   const int lane = threadIdx.x & 63, ch = 2 * lane;
   const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_ml) + row * a.parts;
   const float2 mine = lane < a.parts ? ml[lane] : make_float2(-INFINITY, 0.f);  // (parts <= 64)
-  float top = mine.x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float f = weight_of(mine.x, top);
-  float sum = mine.y * f;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  const float top = wave_max(mine.x), f = weight_of(mine.x, top), sum = wave_sum(mine.y * f);
   const bool on = ch < a.D;
   const float* p = a.part + row * a.parts * a.D + (on ? ch : 0);
   float o0 = 0.f, o1 = 0.f;
@@ -566,14 +602,55 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const float fi = i0 + u < used ? __shfl(f, i0 + u) : 0.f;  // (parts <= 64, so i0 + u < 64)
-      // (a part without keys of this row is not looked at: it may hold none, or others' NaN)
-      o0 = fi == 0.f ? o0 : fmaf(x[u].x, fi, o0);
-      o1 = fi == 0.f ? o1 : fmaf(x[u].y, fi, o1);
+      o0 = fmaf(x[u].x, fi, o0);
+      o1 = fmaf(x[u].y, fi, o1);
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (on)
     *reinterpret_cast<uint32_t*>(a.o + (row / a.H) * a.so_b + (row % a.H) * a.so_h + ch) = E::pack(o0 * inv, o1 * inv);
+}
+
+// The same in one round of memory: a workgroup per row, a thread asks for every
+// kJoinThreads / (D / 4)-th part at once, four channels of each, and LDS adds them up.
+constexpr int kMaxParts = kMaxSplits + kMaxShared, kJoinThreads = 256;
+template <typename E, int L, int N>  // L: threads of a part; N: parts of a thread
+__global__ void __launch_bounds__(kJoinThreads) paged_wide_join_kernel(const PagedArgs a) {
+  constexpr int G = kJoinThreads / L;
+  __shared__ float f[kMaxParts];
+  __shared__ __align__(16) float sums[G][4 * L];
+  const uint32_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, g = threadIdx.x / L, ch = 4 * (threadIdx.x % L);
+  const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_ml) + static_cast<int64_t>(row) * a.parts;
+  const float* p = a.part + static_cast<int64_t>(row) * a.parts * a.D + min(ch, a.D - 4);
+  const float2 m0 = lane < a.parts ? ml[lane] : make_float2(-INFINITY, 0.f);
+  const float2 m1 = lane + 64 < a.parts ? ml[lane + 64] : make_float2(-INFINITY, 0.f);  // (parts <= 128)
+  float4 x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    x[n] = *reinterpret_cast<const float4*>(p + static_cast<int64_t>(min(g + G * n, a.parts - 1)) * a.D);
+  const float top = wave_max(fmaxf(m0.x, m1.x)), f0 = weight_of(m0.x, top), f1 = weight_of(m1.x, top);
+  const float sum = wave_sum(fmaf(m0.y, f0, m1.y * f1));
+  if (threadIdx.x < 64) f[lane] = f0, f[lane + 64] = f1;
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float fi = g + G * n < a.parts ? f[g + G * n] : 0.f;
+    // (a part without keys of this row is passed over: it may hold anything)
+    if (fi != 0.f) o.x = fmaf(x[n].x, fi, o.x), o.y = fmaf(x[n].y, fi, o.y), o.z = fmaf(x[n].z, fi, o.z), o.w = fmaf(x[n].w, fi, o.w);
+  }
+  *reinterpret_cast<float4*>(&sums[g][ch]) = o;
+  __syncthreads();
+  if (g || ch >= a.D) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    const float4 y = *reinterpret_cast<const float4*>(&sums[i][ch]);
+    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(a.o + static_cast<int64_t>(row / a.H) * a.so_b + (row % a.H) * a.so_h + ch) =
+      make_uint2(E::pack(o.x * inv, o.y * inv), E::pack(o.z * inv, o.w * inv));
 }
 
 // Splits of a sequence: as many as leave the launch within four workgroups a CU, eight
@@ -594,6 +671,9 @@ int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, 
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
+#ifndef PS
+#define PS 512
+#endif
 #ifndef TILED_FROM
 #define TILED_FROM 64
 #endif
@@ -604,21 +684,22 @@ struct Cut {
   int64_t parts() const { return psplit + split; }
   int64_t part_bytes(int64_t B, int64_t H, int64_t D) const { return parts() > 1 ? B * H * parts() * (D + 2) * 4 : 0; }
 };
-Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups) {
+Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups, int cache_type) {
   Cut c{};
   c.tiles = cdiv(H / Hkv, kGroups);
   if (shared > 0) {
     const int64_t cols = B / groups * (H / Hkv);
     c.ctiles = cols > kGroups ? cols > TILED_FROM && (D == 64 || D == 128) ? kTiled : 2 : 1;
     c.ptiles = cdiv(cols, kGroups * c.ctiles);
-    int64_t n = 1024 / (groups * Hkv * c.ptiles);
-    const int64_t steps = cdiv(shared, 2 * kBlock) / kWaves;
-    if (n > steps) n = steps;
-    if (n > kMaxShared) n = kMaxShared;
-    c.psplit = n < 1 ? 1 : n;
+    // whole rounds of a workgroup's steps: a wave with a step more than the others is waited for
+    const int64_t steps = cdiv(shared, c.ctiles == kTiled ? kKeys : cache_type ? 2 * kBlock : kBlock);
+    const int64_t round = c.ctiles == kTiled ? 1 : kWaves;
+    int64_t n = PS / (groups * Hkv * c.ptiles);
+    n = n < 1 ? 1 : n > kMaxShared ? kMaxShared : n;
+    c.psplit = cdiv(steps, round * cdiv(steps, round * n));
     keys = keys > shared ? keys - shared : 0;
   }
-  c.split = splits(B, Hkv, c.tiles, keys, window, sinks, kMaxSplits - c.psplit);
+  c.split = splits(B, Hkv, c.tiles, keys, window, sinks, kMaxSplits);
   return c;
 }
 
@@ -639,6 +720,11 @@ auto kernel_of(int64_t D, int64_t ctiles) {
          : ctiles == 1 ? kernel_of<E, C, 1>(D)
          : ctiles == 2 ? kernel_of<E, C, 2>(D)
                        : kernel_of<E, C, kTiled>(D);
+}
+template <typename E>
+auto wide_join_of(int64_t D, int64_t parts) {
+  return D > 64 ? (parts <= 32 ? paged_wide_join_kernel<E, 32, 4> : paged_wide_join_kernel<E, 32, 16>)
+                : (parts <= 64 ? paged_wide_join_kernel<E, 16, 4> : paged_wide_join_kernel<E, 16, 8>);
 }
 template <typename E>
 auto kernel_of(int64_t D, int64_t ctiles, int cache_type) {
@@ -702,7 +788,7 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.group = static_cast<int>(H / Hkv);
   a.window = static_cast<int>(p.window), a.sinks = static_cast<int>(p.sinks);
   a.c = p.scale * kLog2e;
-  const Cut c = cut(B, H, Hkv, D, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups);
+  const Cut c = cut(B, H, Hkv, D, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups, p.cache_type);
   a.tiles = static_cast<int>(c.tiles), a.split = static_cast<int>(c.split);
   a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split);
   a.parts = static_cast<int>(c.parts());
@@ -728,18 +814,23 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(grid)), dim3(kWaves * 64), 0, s, a);
   if (int rc = check_launch(what)) return rc;
   if (a.parts == 1) return SOLATTN_OK;
-  hipLaunchKernelGGL(bf ? paged_join_kernel<Bf16> : paged_join_kernel<Fp16>,
-                     dim3(static_cast<uint32_t>(cdiv(B * H, 4))), dim3(256), 0, s, a);
+  if (p.cache_type == 0 && p.shared == 0) {  // (the order of sums of the calls without codes and shared keys)
+    hipLaunchKernelGGL(bf ? paged_join_kernel<Bf16> : paged_join_kernel<Fp16>,
+                       dim3(static_cast<uint32_t>(cdiv(B * H, 4))), dim3(256), 0, s, a);
+    return check_launch(what);
+  }
+  const auto join = bf ? wide_join_of<Bf16>(D, a.parts) : wide_join_of<Fp16>(D, a.parts);
+  hipLaunchKernelGGL(join, dim3(static_cast<uint32_t>(B * H)), dim3(kJoinThreads), 0, s, a);
   return check_launch(what);
 }
 
 int64_t paged_attn_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window,
-                             int64_t sinks, int64_t shared, int64_t groups) {
+                             int64_t sinks, int64_t shared, int64_t groups, int cache_type) {
   constexpr int64_t top = 1ll << 31;  // (what the call takes: nothing passes 64 bits)
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || keys < 0 || window < 0 || sinks < 0) return 0;
   if (B >= top || H >= top || B * H >= top || D > 128 || keys >= top) return 0;
   if (shared < 0 || shared >= top || (shared && (groups <= 0 || B % groups))) return 0;
-  return cut(B, H, Hkv, D, keys, window, sinks, shared, groups).part_bytes(B, H, D);
+  return cut(B, H, Hkv, D, keys, window, sinks, shared, groups, cache_type).part_bytes(B, H, D);
 }
 
 }  // namespace solattn
@@ -750,9 +841,8 @@ extern "C" int64_t solattn_paged_attn_shared_workspace_bytes(int64_t B, int64_t 
                                                              int64_t max_pages, int64_t page_size, int64_t window,
                                                              int64_t sinks, int cache_type, int64_t shared,
                                                              int64_t groups) {
-  (void)cache_type;
   const bool fit = max_pages >= 0 && page_size >= 0 && max_pages < (1ll << 31) && page_size < (1ll << 31);
-  return fit ? paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks, shared, groups) : 0;
+  return fit ? paged_attn_workspace(B, H, Hkv, D, max_pages * page_size, window, sinks, shared, groups, cache_type) : 0;
 }
 
 extern "C" int64_t solattn_paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
