@@ -146,13 +146,11 @@ __device__ __forceinline__ Visible visible(int len, int low, int sinks) {
   return s;
 }
 
-// The longest sequence of a run of `per` (the first of these), its length, and the lengths
-// of the first 64 sequences, a lane each.
-__device__ __forceinline__ int longest(const PagedArgs& a, int first, int& b, int& len) {
+// The longest sequence of a run of `per` (the first of these) and its length.
+__device__ __forceinline__ void longest(const PagedArgs& a, int first, int& b, int& len) {
   const int lane = threadIdx.x & 63;
-  const int mine = lane < a.per ? sequence_length(a, first + lane) : -1;
-  int n = mine, at = lane;
-  for (int i = lane + 64; i < a.per; i += 64) {
+  int n = -1, at = 0;
+  for (int i = lane; i < a.per; i += 64) {
     const int x = sequence_length(a, first + i);
     if (x > n) n = x, at = i;
   }
@@ -161,7 +159,6 @@ __device__ __forceinline__ int longest(const PagedArgs& a, int first, int& b, in
   const uint32_t best = over_wave(n == top ? static_cast<uint32_t>(at) : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
   b = first + __builtin_amdgcn_readfirstlane(static_cast<int>(best));
   len = __builtin_amdgcn_readfirstlane(top);
-  return mine;
 }
 
 // A workgroup's keys and columns. The columns of own keys are the heads of one sequence
@@ -171,12 +168,6 @@ struct Work {
   int step0, step1, part;
   int b, seq;          // whose pages; the first column's sequence
   int hk, col0, ncol;  // columns col0 .. col0 + ncol - 1 of the kv head
-  int lengths;         // of several sequences: of the first 64, a lane each
-  // How many of the shared keys sequence b (another a lane) sees.
-  __device__ __forceinline__ int sees(const PagedArgs& a, int b) const {
-    const int n = a.per <= 64 ? __shfl(lengths, b - seq) : sequence_length(a, b);
-    return min(n, vis.len);
-  }
   __device__ __forceinline__ void row(const PagedArgs& a, int c, bool many, int& b, int& h) const {
     uint32_t n = col0 + min(c, ncol - 1);
     const uint32_t g = many ? a.by_group.split(n) : n;
@@ -185,16 +176,42 @@ struct Work {
   }
 };
 
+// The part's steps of `keys` shared ones, on sequence b's pages.
+template <typename C, bool TILED>
+__device__ __forceinline__ void shared_steps(const PagedArgs& a, Work& w, int b, int keys) {
+  w.b = b;
+  w.vis = visible<C>(keys, 0, 0);
+  if constexpr (TILED) w.vis.steps = (keys + kKeys - 1) / kKeys;
+  const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
+  w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
+}
+// What shared keys mostly are: all of them, on the first sequence's pages. The first page
+// ids are asked for as if they were, beside the lengths that tell.
+__device__ __forceinline__ int all_shared(const PagedArgs& a) {
+  return static_cast<int>(min(static_cast<int64_t>(a.shared), static_cast<int64_t>(a.max_pages) * a.page));
+}
+
 template <int DP>
 struct __align__(16) PagedLds {
   float o[kWaves][kGroups][DP + 4];
   float m[kWaves][kGroups], l[kWaves][kGroups];
 };
 
+// Nothing in this part: the join passes over a sum of 0.
+template <bool MANY>
+__device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
+  for (int c = threadIdx.x; c < w.ncol; c += kWaves * 64) {
+    int b, h;
+    w.row(a, c, MANY, b, h);
+    reinterpret_cast<float2*>(a.part + a.part_ml)[(static_cast<int64_t>(b) * a.H + h) * a.parts + w.part] =
+        make_float2(-INFINITY, 0.f);
+  }
+}
+
 // DP: the head dim that the registers hold; D < DP (kFull false) leaves the rest zero.
 // NT: tiles of 16 columns. MANY: the columns are of several sequences.
 template <typename E, typename C, int DP, bool kFull, int NT, bool MANY>
-__device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, const Work& w) {
+__device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Work& w) {
   constexpr bool Q8 = kCodes<C>;
   constexpr int KB = kBlocks<C>, S = kStep<C>;
   constexpr int NC = DP / 32;           // products of a score tile
@@ -212,14 +229,13 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
   // Channels of product cc that this lane holds of q and of a key: eight from
   // 32 cc + 8 g on, of codes, read 16 bytes at a time, from 64 (cc / 2) + 16 g + 8 (cc % 2).
   bf16x8 q[NT][NC];
-  int hi[NT], safe = vis.len;  // MANY: keys that a column sees; that every one does
+  int hi[NT];  // MANY: keys that a column sees
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     int b, h;
     w.row(a, 16 * t + col, MANY, b, h);
     const uint16_t* qp = a.q + b * a.sq_b + h * a.sq_h;
-    hi[t] = MANY ? w.sees(a, b) : vis.len;
-    safe = min(safe, hi[t]);
+    hi[t] = MANY ? sequence_length(a, b) : 0;
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       const int ch = Q8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g;
@@ -227,10 +243,6 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
       if (kFull || ch < a.D) x = *reinterpret_cast<const uint4*>(qp + ch);
       q[t][cc] = __builtin_bit_cast(bf16x8, x);
     }
-  }
-  if constexpr (MANY) {
-    safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
-        over_row16(static_cast<uint32_t>(safe), [](uint32_t x, uint32_t y) { return min(x, y); })));
   }
   f32x4 acc[NT][CH];
   float m[NT], l[NT];  // l: this lane's keys
@@ -264,6 +276,24 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
     }
   };
   if (w.step0 + wave < w.step1) find(w.step0 + wave);
+  int safe = 0;  // MANY: keys that every column sees
+  if constexpr (MANY) {
+    int b, len;
+    longest(a, w.seq, b, len);
+    if (b != w.seq || len < vis.len) {
+      shared_steps<C, false>(a, w, b, min(len, vis.len));
+      if (w.step0 >= w.step1) return no_keys<true>(a, w);
+      if (w.step0 + wave < w.step1) find(w.step0 + wave);
+    }
+    safe = vis.len;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      hi[t] = min(hi[t], vis.len);
+      safe = min(safe, hi[t]);
+    }
+    safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
+        over_row16(static_cast<uint32_t>(safe), [](uint32_t x, uint32_t y) { return min(x, y); })));
+  }
   for (int st = w.step0 + wave; st < w.step1; st += kWaves) {
     const bool sink = st < vis.sink_steps;
     const int base = base_of(st);
@@ -476,27 +506,41 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, co
 // The same for 128 columns of several sequences, by tiles in LDS: steps of 64 keys.
 constexpr int kTiled = kTileRows / kGroups;  // its tiles of columns
 template <typename E, typename C, int D>
-__device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, const Work& w) {
+__device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Work& w) {
   static_assert(kWaves * 64 == kTileThreads, "a wave for 32 rows");
   const int lane = threadIdx.x & 63, half = lane >> 5, row = 32 * wave_id() + (lane & 31);
   int b, h;
   w.row(a, row, true, b, h);
-  const int hi = w.sees(a, b);
-  const int safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
-      over_wave(static_cast<uint32_t>(hi), [](uint32_t x, uint32_t y) { return min(x, y); })));
+  bf16x8 q[D / 16];
+  load_row<D>(q, a.q + b * a.sq_b + h * a.sq_h, half);
+  int hi = sequence_length(a, b);
   const auto near = [](int64_t slot) { return slot >= 0 && slot < (1 << 28); };
   const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p, near(a.sk_s)};
   const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p, near(a.sv_s)};
-  const TilePages pg{a.table + w.b * a.table_b, a.by_page, a.pages, w.vis.len};
-  const uint32_t kb = lds_addr(lds), vb = kb + 2 * kKeys * D;
+  TilePages pg{a.table + w.b * a.table_b, a.by_page, a.pages, w.vis.len};
+  TileLds<D>& ring = *reinterpret_cast<TileLds<D>*>(lds);
+  if constexpr (!kCodes<C>) pg.fetch_ids(ring.ids, w.step0 * kKeys, 0);
+  {
+    int best, len;
+    longest(a, w.seq, best, len);
+    if (best != w.seq || len < w.vis.len) {
+      shared_steps<C, true>(a, w, best, min(len, w.vis.len));
+      if (w.step0 >= w.step1) return no_keys<true>(a, w);
+      pg.table = a.table + w.b * a.table_b, pg.end = w.vis.len;
+      if constexpr (!kCodes<C>) pg.fetch_ids(ring.ids, w.step0 * kKeys, 0);
+    }
+  }
+  hi = min(hi, w.vis.len);
+  const int safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
+      over_wave(static_cast<uint32_t>(hi), [](uint32_t x, uint32_t y) { return min(x, y); })));
   RowState<D / 32> st;
-  const uint16_t* q = a.q + b * a.sq_b + h * a.sq_h;
-  if constexpr (kCodes<C>)
+  if constexpr (kCodes<C>) {
+    const uint32_t kb = lds_addr(lds), vb = kb + 2 * kKeys * D;
     attend_tiles<E, D, HalfDecode<E, C, D, kByRow>, HalfDecode<E, C, D, kTransposed>>(st, q, kb, vb, ks, vs, pg, w.step0,
                                                                                      w.step1 - w.step0, hi, safe, a.c);
-  else
-    attend_tiles<E, D, HalfCopy<D, kByRow>, HalfCopy<D, kTransposed>>(st, q, kb, vb, ks, vs, pg, w.step0,
-                                                                     w.step1 - w.step0, hi, safe, a.c);
+  } else {
+    attend_ring<E, D>(st, q, ring, ks, vs, pg, w.step0, w.step1 - w.step0, hi, safe, a.c);
+  }
   const float l = xhalf_sum(st.l);
   if (row >= w.ncol) return;
   const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
@@ -512,23 +556,13 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, co
     *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(l == 0.f ? -INFINITY : st.m, l);
 }
 
-// Nothing in this part: the join passes over a sum of 0.
-template <bool MANY>
-__device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
-  for (int c = threadIdx.x; c < w.ncol; c += kWaves * 64) {
-    int b, h;
-    w.row(a, c, MANY, b, h);
-    reinterpret_cast<float2*>(a.part + a.part_ml)[(static_cast<int64_t>(b) * a.H + h) * a.parts + w.part] =
-        make_float2(-INFINITY, 0.f);
-  }
-}
-
 // PT: tiles of 16 columns over shared keys (0: a launch without any; kTiled: by tiles in LDS).
 template <typename E, typename C, int DP, bool kFull, int PT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 paged_kernel(const PagedArgs a) {
   constexpr bool TILED = PT == kTiled;
-  constexpr size_t kLds = TILED && 4 * kKeys * DP > sizeof(PagedLds<DP>) ? 4 * kKeys * DP : sizeof(PagedLds<DP>);
+  constexpr size_t kTileLds = !TILED ? 0 : kCodes<C> ? 4 * kKeys * DP : sizeof(TileLds<DP>);
+  constexpr size_t kLds = kTileLds > sizeof(PagedLds<DP>) ? kTileLds : sizeof(PagedLds<DP>);
   __shared__ __align__(256) uint8_t lds_bytes[kLds];
   PagedLds<DP>& lds = *reinterpret_cast<PagedLds<DP>*>(lds_bytes);
   fetch_arguments(a);
@@ -545,12 +579,8 @@ paged_kernel(const PagedArgs a) {
       w.seq = static_cast<int>(n) * a.per;
       w.col0 = tile * 16 * PT;
       w.ncol = min(16 * PT, a.per * a.group - w.col0);
-      int len;
-      w.lengths = longest(a, w.seq, w.b, len);
-      w.vis = visible<C>(min(len, a.shared), 0, 0);
-      if constexpr (TILED) w.vis.steps = (w.vis.len + kKeys - 1) / kKeys;
-      const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
-      w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
+      // (a part that the longest sequence may have keys for; whether it does is found out there)
+      shared_steps<C, TILED>(a, w, w.seq, all_shared(a));
       if (w.step0 >= w.step1)
         no_keys<true>(a, w);
       else if constexpr (TILED)

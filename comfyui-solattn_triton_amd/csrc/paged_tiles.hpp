@@ -45,6 +45,9 @@ struct TileRows {
   }
 };
 
+// Page ids that are kept in LDS: of 64 tiles, twice.
+constexpr int kIdTiles = 64, kIds = kIdTiles * kKeys / 8 + 1;  // (pages have 8 slots at least)
+
 struct TilePages {
   const int32_t* table;  // the sequence's row
   Divisor by_page;
@@ -54,6 +57,17 @@ struct TilePages {
     const int j = j0 + (static_cast<int>(threadIdx.x) & 63);
     const int id = table[by_page.of(static_cast<uint32_t>(min(j, end - 1)))];
     return j < end && id >= 0 && id < pages ? id : -1;
+  }
+  // The ids of segment s (64 tiles) of the keys from `first` on, into LDS.
+  __device__ __forceinline__ int page0(int first, int s) const {
+    return static_cast<int>(by_page.of(static_cast<uint32_t>(first + s * kIdTiles * kKeys)));
+  }
+  __device__ __forceinline__ void fetch_ids(int32_t (&to)[2][kIds + 3], int first, int s) const {
+    const int p0 = page0(first, s), n = static_cast<int>(by_page.of(static_cast<uint32_t>(end - 1))) - p0 + 1;
+    for (int i = threadIdx.x; i < min(n, kIds); i += kTileThreads) {
+      const int id = table[p0 + i];
+      to[s & 1][i] = id >= 0 && id < pages ? id : -1;
+    }
   }
   template <bool CODES>
   __device__ __forceinline__ TileRows rows(int id, int j0, const TileSource& s) const {
@@ -137,7 +151,7 @@ struct HalfDecode {  // codes, 16 of a row a thread, through registers
 // lane's row (32 wave + lane % 32 of the workgroup's), which sees those below `hi`; every
 // row of the workgroup sees those below `safe`. st: the row's O^T, maximum and sum.
 template <typename E, int D, typename KCopy, typename VCopy>
-__device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_t* qrow, uint32_t kb, uint32_t vb,
+__device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const bf16x8 (&q)[D / 16], uint32_t kb, uint32_t vb,
                                              const TileSource& ks, const TileSource& vs, const TilePages& pg,
                                              int tile0, int ntiles, int hi, int safe, float c) {
   constexpr int ND = D / 32, NC = D / 16;
@@ -194,8 +208,6 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_
     vc.finish(vb);
     k1 = krows(i1, 1), v1 = vrows(i1, 1), k2 = krows(i2, 2);
   }
-  bf16x8 q[NC];
-  load_row<D>(q, qrow, half);
   f32x16 sa, sb;  // scores of even and odd halves
   bf16x8 pa[2], pb[2];
   land();
@@ -256,6 +268,149 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const uint16_
 #pragma unroll
   for (int i = 0; i < NC; ++i)  // P.V of the last half
     st.acc[i % ND] = E::mfma32(v_op_x<D>(vl + kHalf, i / ND, i % ND), pb[i / ND], st.acc[i % ND]);
+}
+
+// The same with 16-bit values, copied four halves ahead into rings of four: a copy has two
+// steps to land, and the wait at a step's end leaves the newest two steps' copies in flight.
+// Page ids are kept in LDS, so that no load of the loop but the copies counts.
+template <int D>
+struct TileLds {
+  uint16_t k[4][32 * D], v[4][32 * D];
+  int32_t ids[2][kIds + 3];
+};
+
+// Leaves N copies in flight.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+}
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+template <typename E, int D>
+__device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (&q)[D / 16], TileLds<D>& lds,
+                                            const TileSource& ks, const TileSource& vs, const TilePages& pg, int tile0,
+                                            int ntiles, int hi, int safe, float c) {
+  constexpr int ND = D / 32, NC = D / 16;
+  constexpr uint32_t kHalf = kKeys * D;  // bytes of half a tile
+  using KCopy = HalfCopy<D, kByRow>;
+  using VCopy = HalfCopy<D, kTransposed>;
+  constexpr int STEP = KCopy::U + VCopy::U;  // copies of a step
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const uint32_t kb = lds_addr(lds.k), vb = lds_addr(lds.v);
+  const uint32_t kl = k_lane<D>(kb, lane & 31, half), vl = v_lane<D>(vb, lane);
+  const int first = tile0 * kKeys;
+  KCopy kc;
+  VCopy vc;
+  kc.init(ks);
+  vc.init(vs);
+  st.m = kNoMax;
+  st.l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) st.acc[dt] = f32x16{};
+  const auto rows = [&](int t, const TileSource& s, uint64_t& seen) __attribute__((always_inline)) {
+    t = min(t, ntiles - 1);
+    const int j = first + kKeys * t + lane;
+    const uint32_t page = pg.by_page.of(static_cast<uint32_t>(j));
+    const int slot = static_cast<int>(static_cast<uint32_t>(j) - page * pg.by_page.d);
+    const int sg = t / kIdTiles;
+    int id = lds.ids[sg & 1][min(static_cast<int>(page) - pg.page0(first, sg), kIds - 1)];
+    id = j < pg.end ? id : -1;
+    seen = __ballot(id >= 0);
+    const uint8_t* at = id >= 0 ? s.p + id * s.page + slot * s.slot : reinterpret_cast<const uint8_t*>(zero_row);
+    TileRows r;
+    r.lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at));
+    r.hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at) >> 32);
+    return r;
+  };
+  const auto mask = [&](f32x16& s, int j0, int hf, uint64_t seen) __attribute__((always_inline)) {
+    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * hf));
+    j0 += 32 * hf;
+    if (mine != ~0u || j0 + 32 > safe) {
+      const uint32_t bits = (mine >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t w = bit_word(bits, r);
+        s[r] = __uint_as_float((__float_as_uint(s[r]) & w) | (__float_as_uint(-INFINITY) & ~w));
+      }
+    }
+  };
+  wait_copies<0>();
+  tile_barrier();
+  // Round t copies the second half of tile t + 2 and the first of t + 3 for K, of t + 1 and
+  // t + 2 for V.
+  uint64_t s0w, s1w, s2w, s3w, unused;  // visible keys of the tiles t, t + 1, t + 2, t + 3
+  TileRows k2, k3, v1, v2;
+  {
+    const TileRows k0 = rows(0, ks, s0w), k1 = rows(1, ks, s1w), v0 = rows(0, vs, unused);
+    kc.start(kb, 0, s0w, k0, ks);
+    kc.start(kb + kHalf, 1, s0w, k0, ks);
+    if (ntiles > 1) kc.start(kb + 2 * kHalf, 0, s1w, k1, ks);
+    vc.start(vb, 0, s0w, v0, vs);
+    if (ntiles > 1) kc.start(kb + 3 * kHalf, 1, s1w, k1, ks);
+    vc.start(vb + kHalf, 1, s0w, v0, vs);
+    k2 = rows(2, ks, s2w), v1 = rows(1, vs, unused);
+  }
+  // All but the newest two steps' copies are there; near the end, where steps ask for
+  // fewer, all are.
+  const auto land = [&](int t) __attribute__((always_inline)) {
+    if (t + 3 < ntiles)
+      wait_copies<2 * STEP>();
+    else
+      wait_copies<0>();
+    tile_barrier();
+  };
+  f32x16 sa, sb;  // scores of even and odd halves
+  bf16x8 pa[2], pb[2];
+  land(-1);
+  {  // step 0, without a stream: both halves are scored, the running max is the whole tile's
+    f32x16 x0 = {}, x1 = {};
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) x0 = E::mfma32(k_op_x<D>(kl, 0, cc), q[cc], x0);
+    tile_barrier();  // every wave is done with K(0)
+    if (ntiles > 2) kc.start(kb, 0, s2w, k2, ks);
+    if (ntiles > 1) vc.start(vb + 2 * kHalf, 0, s1w, v1, vs);
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) x1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], x1);
+    mask(x0, first, 0, s0w);
+    mask(x1, first, 1, s0w);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(x0[r], x1[r]));
+    st.m = fmaxf(kNoMax, xhalf_max(mx) * c);
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = E::exp_pair(x0[2 * i], x0[2 * i + 1], c, -st.m, st.l);
+    pa[0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+    pa[1] = __builtin_bit_cast(bf16x8, make_uint4(w[4], w[5], w[6], w[7]));
+    sb = x1;
+  }
+  mfma_fence(st.acc);  // O's zeros are in their registers before the asm MFMAs that add to them
+  land(-1);
+  int t = 0;
+#pragma unroll 1
+  for (; t < ntiles - 1; ++t) {
+    if (t % kIdTiles == kIdTiles / 2 && (t / kIdTiles + 1) * kIdTiles < ntiles) pg.fetch_ids(lds.ids, first, t / kIdTiles + 1);
+    const uint32_t a0 = (t & 1) * 2 * kHalf, b0 = 2 * kHalf - a0;  // halves 2 t and 2 t + 2 of the rings
+    k3 = rows(t + 3, ks, s3w), v2 = rows(t + 2, vs, unused);
+    if (t + 2 < ntiles) kc.start(kb + a0 + kHalf, 1, s2w, k2, ks);  // step 2 t + 1
+    vc.start(vb + b0 + kHalf, 1, s1w, v1, vs);
+    window_step<E, D>(st, sb, sa, pa, pb, kl + b0, vl + a0, q, c);
+    land(t);
+    if (t + 3 < ntiles) kc.start(kb + b0, 0, s3w, k3, ks);  // step 2 t + 2
+    if (t + 2 < ntiles) vc.start(vb + a0, 0, s2w, v2, vs);
+    mask(sa, first + kKeys * (t + 1), 0, s1w);
+    window_step<E, D>(st, sa, sb, pb, pa, kl + b0 + kHalf, vl + a0 + kHalf, q, c);
+    mask(sb, first + kKeys * (t + 1), 1, s1w);
+    land(t);
+    k2 = k3, v1 = v2;
+    s1w = s2w, s2w = s3w;
+  }
+  const uint32_t a0 = (t & 1) * 2 * kHalf;
+  window_step<E, D>(st, sb, sa, pa, pb, kl + 2 * kHalf - a0, vl + a0, q, c);
+  mfma_fence(st.acc);
+#pragma unroll
+  for (int i = 0; i < NC; ++i)  // P.V of the last half
+    st.acc[i % ND] = E::mfma32(v_op_x<D>(vl + a0 + kHalf, i / ND, i % ND), pb[i / ND], st.acc[i % ND]);
 }
 
 }  // namespace solattn
