@@ -58,12 +58,13 @@ struct PagedArgs {
                              // here, the others `length` keys (null: all of them)
   int length, pages, page, max_pages;
   Divisor by_page;
+  int near;                  // pages' and slots' strides are within 32 bits
   uint16_t* o;
   int64_t so_b, so_h;
   float* part;               // parts > 1: [B][H][parts][D] sums, then [B][H][parts][2] max and sum
   int64_t part_ml;           // where the latter begin
   int B, H, Hkv, D, group, tiles, split;
-  Divisor by_tiles, by_hkv, by_split;
+  Divisor by_tiles, by_hkv, by_split, by_run;  // by_run: workgroups of the same own keys
   int window, sinks;         // window 0: none
   float c;                   // scale log2(e)
   // Keys in common: of `per` sequences each the first `shared`, cut into psplit parts, for
@@ -266,6 +267,8 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
     slot = static_cast<int>(j - pg * a.page);
     return a.table ? a.table[w.b * a.table_b + pg] : w.b;
   };
+  const uint8_t* const khead = a.k + hk * a.sk_h;
+  const uint8_t* const vhead = a.v + hk * a.sv_h + ES * vch;
   int kslot[KB], vslot[KB], kid[KB], vid[KB];
   const auto find = [&](int st) __attribute__((always_inline)) {
     const int base = base_of(st);
@@ -303,36 +306,51 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
     uint4 kr[KB][2][KL];
     uint32_t vr[KB][8][VW];
     uint2 ke[KB], ve[KB];  // exponents of the keys 8 g + 0..7
-    const int last = a.page - 1;  // a slot past the page's end (a whole-sequence page) repeats its last
+    const auto load_k = [&](int u, int t, const uint8_t* at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int cc = 0; cc < KL; ++cc) {
+        const int ch = Q8 ? 64 * cc + 16 * g : 32 * cc + 8 * g;
+        kr[u][t][cc] = *reinterpret_cast<const uint4*>(at + (kFull || ch < a.D ? ES * ch : 0));
+      }
+    };
+    const auto load_v = [&](int u, int i, const uint8_t* at) __attribute__((always_inline)) {
+      if constexpr (VW == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        vr[u][i][0] = x.x, vr[u][i][1] = x.y, vr[u][i][2] = x.z, vr[u][i][3] = x.w;
+      } else if constexpr (VW == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        vr[u][i][0] = x.x, vr[u][i][1] = x.y;
+      } else {
+        vr[u][i][0] = *reinterpret_cast<const uint32_t*>(at);
+      }
+    };
+    // A lane's rows of K are those at col % 4 and 4 further, of V eight: a slot apart, but where a
+    // whole-sequence page ends among them, whose last row is read again. (Every row's place by
+    // itself, in 64 bits: 82 multiplications a step, more time than all the rest of it.)
 #pragma unroll
     for (int u = 0; u < KB; ++u) {
       vok[u] = vid[u] >= 0 && vid[u] < a.pages;
-      const int64_t kpage = kid[u] >= 0 && kid[u] < a.pages ? kid[u] : 0, vpage = vok[u] ? vid[u] : 0;
+      const uint32_t kpage = kid[u] >= 0 && kid[u] < a.pages ? kid[u] : 0, vpage = vok[u] ? vid[u] : 0;
+      const int kleft = a.page - 1 - kslot[u], vleft = a.page - 1 - vslot[u];
+      const auto times = [](uint32_t x, int64_t stride) { return static_cast<uint64_t>(x) * static_cast<uint32_t>(stride); };
+      if (a.near && (Q8 || !__any(min(kleft, vleft) < 7))) {
+        const uint8_t* kp = khead + times(kpage, a.sk_p) + times(kslot[u] + (col & 3), a.sk_s);
+        load_k(u, 0, kp);
+        load_k(u, 1, kp + 4 * a.sk_s);
+        const uint8_t* vp = vhead + times(vpage, a.sv_p) + times(vslot[u], a.sv_s);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t* kp = a.k + kpage * a.sk_p + static_cast<int64_t>(min(kslot[u] + 4 * t + (col & 3), last)) * a.sk_s + hk * a.sk_h;
+        for (int i = 0; i < 8; ++i, vp += a.sv_s) load_v(u, i, vp);
+      } else {
+        const uint8_t* kp = khead + static_cast<uint64_t>(kpage) * a.sk_p;
+        const uint8_t* vp = vhead + static_cast<uint64_t>(vpage) * a.sv_p;
 #pragma unroll
-        for (int cc = 0; cc < KL; ++cc) {
-          const int ch = Q8 ? 64 * cc + 16 * g : 32 * cc + 8 * g;
-          kr[u][t][cc] = *reinterpret_cast<const uint4*>(kp + (kFull || ch < a.D ? ES * ch : 0));
-        }
-      }
+        for (int t = 0; t < 2; ++t) load_k(u, t, kp + (kslot[u] + min(4 * t + (col & 3), kleft)) * a.sk_s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint8_t* vp = a.v + vpage * a.sv_p + static_cast<int64_t>(min(vslot[u] + i, last)) * a.sv_s + hk * a.sv_h + ES * vch;
-        if constexpr (VW == 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vp);
-          vr[u][i][0] = x.x, vr[u][i][1] = x.y, vr[u][i][2] = x.z, vr[u][i][3] = x.w;
-        } else if constexpr (VW == 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vp);
-          vr[u][i][0] = x.x, vr[u][i][1] = x.y;
-        } else {
-          vr[u][i][0] = *reinterpret_cast<const uint32_t*>(vp);
-        }
+        for (int i = 0; i < 8; ++i) load_v(u, i, vp + (vslot[u] + min(i, vleft)) * a.sv_s);
       }
       if constexpr (Q8) {
-        ke[u] = *reinterpret_cast<const uint2*>(a.ks + vpage * a.ks_p + hk * a.ks_h + vslot[u]);
-        ve[u] = *reinterpret_cast<const uint2*>(a.vs + vpage * a.vs_p + hk * a.vs_h + vslot[u]);
+        ke[u] = *reinterpret_cast<const uint2*>(a.ks + hk * a.ks_h + times(vpage, a.ks_p) + vslot[u]);
+        ve[u] = *reinterpret_cast<const uint2*>(a.vs + hk * a.vs_h + times(vpage, a.vs_p) + vslot[u]);
       }
     }
     if (st + kWaves < w.step1) find(st + kWaves);
@@ -591,6 +609,14 @@ paged_kernel(const PagedArgs a) {
     }
     n -= a.pitems;
   }
+  if constexpr (kCodes<C>) {
+    // kv heads of the same keys on one XCD, side by side: their rows and exponents share
+    // lines (32 ragged sequences of 4 heads of 64 channels, pages of 16: 54.6 -> 45.5 us).
+    const uint32_t x = n & 7u;
+    uint32_t i = n >> 3;
+    const uint32_t in_run = a.by_run.split(i), run = 8 * i + x;  // runs of the kv heads, dealt round robin
+    if (run < (static_cast<uint32_t>(a.B * a.split) & ~7u)) n = run * a.by_run.d + in_run;
+  }
   const int tile = a.by_tiles.split(n);
   w.hk = a.by_hkv.split(n);
   const int split = a.by_split.split(n);
@@ -813,6 +839,10 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.lengths = p.lengths, a.length = static_cast<int>(p.length);
   a.pages = static_cast<int>(p.pages), a.page = static_cast<int>(p.page_size), a.max_pages = static_cast<int>(p.max_pages);
   a.by_page = divisor(p.page_size);
+  const auto u32 = [](int64_t x) { return x >= 0 && x < (1ll << 32); };
+  a.near = u32(a.sk_p) && u32(a.sk_s) && u32(a.sv_p) && u32(a.sv_s);
+  SOLATTN_REQUIRE(!p.cache_type || (u32(p.ks_p) && u32(p.vs_p)), SOLATTN_EUNSUPPORTED,
+                  "%s: pages' scales 2^32 bytes apart", what);
   a.o = p.o, a.so_b = p.so_b, a.so_h = p.so_h;
   a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.Hkv = static_cast<int>(Hkv), a.D = static_cast<int>(D);
   a.group = static_cast<int>(H / Hkv);
@@ -820,7 +850,7 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.c = p.scale * kLog2e;
   const Cut c = cut(B, H, Hkv, D, p.max_pages * p.page_size, p.window, p.sinks, p.shared, p.groups, p.cache_type);
   a.tiles = static_cast<int>(c.tiles), a.split = static_cast<int>(c.split);
-  a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split);
+  a.by_tiles = divisor(c.tiles), a.by_hkv = divisor(Hkv), a.by_split = divisor(c.split), a.by_run = divisor(Hkv * c.tiles);
   a.parts = static_cast<int>(c.parts());
   const int64_t need = c.part_bytes(B, H, D);
   SOLATTN_REQUIRE(need == 0 || (p.workspace && p.workspace_bytes >= need), SOLATTN_ESIZE,
