@@ -26,7 +26,7 @@ namespace solattn {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kBlock = 32;      // keys of a block of products
+constexpr int kStep = 32;       // keys of a wave's step
 constexpr int kMaxSplits = 64;  // parts of a row over its own keys
 constexpr int kMaxShared = 64;  // and over shared ones
 constexpr int kGroups = 16;     // query columns of a tile
@@ -35,11 +35,6 @@ constexpr int kGroups = 16;     // query columns of a tile
 struct SameType {};
 template <typename C>
 constexpr bool kCodes = !__is_same(C, SameType);
-// Keys of a wave's step: 16 KiB of 128 channels are in flight either way.
-template <typename C>
-constexpr int kBlocks = kCodes<C> ? 2 : 1;
-template <typename C>
-constexpr int kStep = kBlock * kBlocks<C>;
 
 struct PagedArgs {
   const uint16_t* q;
@@ -135,9 +130,8 @@ struct Visible {
   int sinks_end;       // <= low
   int sink_steps, first, steps;  // the window's steps begin at key `first`
 };
-template <typename C>
 __device__ __forceinline__ Visible visible(int len, int low, int sinks) {
-  constexpr int S = kStep<C>;
+  constexpr int S = kStep;
   Visible s;
   s.len = len, s.low = min(low, len);
   s.sinks_end = min(sinks, s.low);
@@ -178,10 +172,10 @@ struct Work {
 };
 
 // The part's steps of `keys` shared ones, on sequence b's pages.
-template <typename C, bool TILED>
+template <bool TILED>
 __device__ __forceinline__ void shared_steps(const PagedArgs& a, Work& w, int b, int keys) {
   w.b = b;
-  w.vis = visible<C>(keys, 0, 0);
+  w.vis = visible(keys, 0, 0);
   if constexpr (TILED) w.vis.steps = (keys + kKeys - 1) / kKeys;
   const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
   w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
@@ -214,7 +208,7 @@ __device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
 template <typename E, typename C, int DP, bool kFull, int NT, bool MANY>
 __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Work& w) {
   constexpr bool Q8 = kCodes<C>;
-  constexpr int KB = kBlocks<C>, S = kStep<C>;
+  constexpr int S = kStep;
   constexpr int NC = DP / 32;           // products of a score tile
   constexpr int KL = Q8 ? NC / 2 : NC;  // 16-byte pieces of a key that a lane reads
   constexpr int CH = DP / 16;           // channels of a lane's V piece = operands of the second product
@@ -269,14 +263,11 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
   };
   const uint8_t* const khead = a.k + hk * a.sk_h;
   const uint8_t* const vhead = a.v + hk * a.sv_h + ES * vch;
-  int kslot[KB], vslot[KB], kid[KB], vid[KB];
+  int kslot, vslot, kid, vid;
   const auto find = [&](int st) __attribute__((always_inline)) {
     const int base = base_of(st);
-#pragma unroll
-    for (int u = 0; u < KB; ++u) {
-      kid[u] = slot_of(base + kBlock * u + 8 * (col >> 2), kslot[u]);
-      vid[u] = slot_of(base + kBlock * u + 8 * g, vslot[u]);
-    }
+    kid = slot_of(base + 8 * (col >> 2), kslot);
+    vid = slot_of(base + 8 * g, vslot);
   };
   if (w.step0 + wave < w.step1) find(w.step0 + wave);
   int safe = 0;  // MANY: keys that every column sees
@@ -284,7 +275,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
     int b, len;
     longest(a, w.seq, b, len);
     if (b != w.seq || len < vis.len) {
-      shared_steps<C, false>(a, w, b, min(len, vis.len));
+      shared_steps<false>(a, w, b, min(len, vis.len));
       if (w.step0 >= w.step1) return no_keys<true>(a, w);
       if (w.step0 + wave < w.step1) find(w.step0 + wave);
     }
@@ -302,109 +293,96 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
     const int base = base_of(st);
     const int lo = sink ? 0 : vis.low, end = sink ? vis.sinks_end : vis.len;  // visible: lo <= j < end
     // Keys of page ids outside the cache are not visible (a key's score lane holds its V piece too).
-    bool vok[KB];
-    uint4 kr[KB][2][KL];
-    uint32_t vr[KB][8][VW];
-    uint2 ke[KB], ve[KB];  // exponents of the keys 8 g + 0..7
-    const auto load_k = [&](int u, int t, const uint8_t* at) __attribute__((always_inline)) {
+    uint4 kr[2][KL];
+    uint32_t vr[8][VW];
+    uint2 ke, ve;  // exponents of the keys 8 g + 0..7
+    const auto load_k = [&](int t, const uint8_t* at) __attribute__((always_inline)) {
 #pragma unroll
       for (int cc = 0; cc < KL; ++cc) {
         const int ch = Q8 ? 64 * cc + 16 * g : 32 * cc + 8 * g;
-        kr[u][t][cc] = *reinterpret_cast<const uint4*>(at + (kFull || ch < a.D ? ES * ch : 0));
+        kr[t][cc] = *reinterpret_cast<const uint4*>(at + (kFull || ch < a.D ? ES * ch : 0));
       }
     };
-    const auto load_v = [&](int u, int i, const uint8_t* at) __attribute__((always_inline)) {
+    const auto load_v = [&](int i, const uint8_t* at) __attribute__((always_inline)) {
       if constexpr (VW == 4) {
         const uint4 x = *reinterpret_cast<const uint4*>(at);
-        vr[u][i][0] = x.x, vr[u][i][1] = x.y, vr[u][i][2] = x.z, vr[u][i][3] = x.w;
+        vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
       } else if constexpr (VW == 2) {
         const uint2 x = *reinterpret_cast<const uint2*>(at);
-        vr[u][i][0] = x.x, vr[u][i][1] = x.y;
+        vr[i][0] = x.x, vr[i][1] = x.y;
       } else {
-        vr[u][i][0] = *reinterpret_cast<const uint32_t*>(at);
+        vr[i][0] = *reinterpret_cast<const uint32_t*>(at);
       }
     };
     // A lane's rows of K are those at col % 4 and 4 further, of V eight: a slot apart, but where a
     // whole-sequence page ends among them, whose last row is read again. (Every row's place by
     // itself, in 64 bits: 82 multiplications a step, more time than all the rest of it.)
+    const bool vok = vid >= 0 && vid < a.pages;
+    const uint32_t kpage = kid >= 0 && kid < a.pages ? kid : 0, vpage = vok ? vid : 0;
+    const int kleft = a.page - 1 - kslot, vleft = a.page - 1 - vslot;
+    const auto times = [](uint32_t x, int64_t stride) { return static_cast<uint64_t>(x) * static_cast<uint32_t>(stride); };
+    if (a.near && (Q8 || !__any(min(kleft, vleft) < 7))) {
+      const uint8_t* kp = khead + times(kpage, a.sk_p) + times(kslot + (col & 3), a.sk_s);
+      load_k(0, kp);
+      load_k(1, kp + 4 * a.sk_s);
+      const uint8_t* vp = vhead + times(vpage, a.sv_p) + times(vslot, a.sv_s);
 #pragma unroll
-    for (int u = 0; u < KB; ++u) {
-      vok[u] = vid[u] >= 0 && vid[u] < a.pages;
-      const uint32_t kpage = kid[u] >= 0 && kid[u] < a.pages ? kid[u] : 0, vpage = vok[u] ? vid[u] : 0;
-      const int kleft = a.page - 1 - kslot[u], vleft = a.page - 1 - vslot[u];
-      const auto times = [](uint32_t x, int64_t stride) { return static_cast<uint64_t>(x) * static_cast<uint32_t>(stride); };
-      if (a.near && (Q8 || !__any(min(kleft, vleft) < 7))) {
-        const uint8_t* kp = khead + times(kpage, a.sk_p) + times(kslot[u] + (col & 3), a.sk_s);
-        load_k(u, 0, kp);
-        load_k(u, 1, kp + 4 * a.sk_s);
-        const uint8_t* vp = vhead + times(vpage, a.sv_p) + times(vslot[u], a.sv_s);
+      for (int i = 0; i < 8; ++i, vp += a.sv_s) load_v(i, vp);
+    } else {
+      const uint8_t* kp = khead + static_cast<uint64_t>(kpage) * a.sk_p;
+      const uint8_t* vp = vhead + static_cast<uint64_t>(vpage) * a.sv_p;
 #pragma unroll
-        for (int i = 0; i < 8; ++i, vp += a.sv_s) load_v(u, i, vp);
-      } else {
-        const uint8_t* kp = khead + static_cast<uint64_t>(kpage) * a.sk_p;
-        const uint8_t* vp = vhead + static_cast<uint64_t>(vpage) * a.sv_p;
+      for (int t = 0; t < 2; ++t) load_k(t, kp + (kslot + min(4 * t + (col & 3), kleft)) * a.sk_s);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) load_k(u, t, kp + (kslot[u] + min(4 * t + (col & 3), kleft)) * a.sk_s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) load_v(u, i, vp + (vslot[u] + min(i, vleft)) * a.sv_s);
-      }
-      if constexpr (Q8) {
-        ke[u] = *reinterpret_cast<const uint2*>(a.ks + hk * a.ks_h + times(vpage, a.ks_p) + vslot[u]);
-        ve[u] = *reinterpret_cast<const uint2*>(a.vs + hk * a.vs_h + times(vpage, a.vs_p) + vslot[u]);
-      }
+      for (int i = 0; i < 8; ++i) load_v(i, vp + (vslot + min(i, vleft)) * a.sv_s);
+    }
+    if constexpr (Q8) {
+      ke = *reinterpret_cast<const uint2*>(a.ks + hk * a.ks_h + times(vpage, a.ks_p) + vslot);
+      ve = *reinterpret_cast<const uint2*>(a.vs + hk * a.vs_h + times(vpage, a.vs_p) + vslot);
     }
     if (st + kWaves < w.step1) find(st + kWaves);
     // scores of this lane: key base + 32 u + 8 g + i in element i % 4 of tile i / 4
-    f32x4 s[NT][KB][2];
-#pragma unroll
-    for (int u = 0; u < KB; ++u)
+    f32x4 s[NT][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc) {
           bf16x8 kop;
           if constexpr (Q8) {
-            const uint4 x = kr[u][i][cc >> 1];
+            const uint4 x = kr[i][cc >> 1];
             const uint32_t lo2 = cc & 1 ? x.z : x.x, hi2 = cc & 1 ? x.w : x.y;
             kop = __builtin_bit_cast(bf16x8, make_uint4(C::template pair<E>(lo2, 0), C::template pair<E>(lo2, 2),
                                                         C::template pair<E>(hi2, 0), C::template pair<E>(hi2, 2)));
           } else {
-            kop = __builtin_bit_cast(bf16x8, kr[u][i][cc]);
+            kop = __builtin_bit_cast(bf16x8, kr[i][cc]);
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if (cc == 0) s[t][u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            s[t][u][i] = E::mfma16(kop, q[t][cc], s[t][u][i]);
+            if (cc == 0) s[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            s[t][i] = E::mfma16(kop, q[t][cc], s[t][i]);
           }
         }
     const float c = Q8 ? 1.f : a.c;  // codes: the factor is the key's
     if constexpr (Q8) {
 #pragma unroll
-      for (int u = 0; u < KB; ++u)
-#pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float f = power_at(i < 4 ? ke[u].x : ke[u].y, i & 3) * a.c;
+          const float f = power_at(i < 4 ? ke.x : ke.y, i & 3) * a.c;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) s[t][u][i >> 2][i & 3] *= f;
+          for (int t = 0; t < NT; ++t) s[t][i >> 2][i & 3] *= f;
         }
     }
-    bool bad = false;
-#pragma unroll
-    for (int u = 0; u < KB; ++u) bad = bad || !vok[u];
-    if (base < lo || base + S > (MANY ? safe : end) || __any(bad)) {
-#pragma unroll
-      for (int u = 0; u < KB; ++u)
+    if (base < lo || base + S > (MANY ? safe : end) || __any(!vok)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int j = base + kBlock * u + 8 * g + i;
-          const bool on = vok[u] && j >= lo && j < end;
+          const int j = base + 8 * g + i;
+          const bool on = vok && j >= lo && j < end;
 #pragma unroll
           for (int t = 0; t < NT; ++t)
-            s[t][u][i >> 2][i & 3] = on && (!MANY || j < hi[t]) ? s[t][u][i >> 2][i & 3] : -INFINITY;
+            s[t][i >> 2][i & 3] = on && (!MANY || j < hi[t]) ? s[t][i >> 2][i & 3] : -INFINITY;
 #pragma unroll
-          for (int r = 0; r < VW; ++r) vr[u][i][r] = on ? vr[u][i][r] : 0u;  // 0 P of a value that may be anything
+          for (int r = 0; r < VW; ++r) vr[i][r] = on ? vr[i][r] : 0u;  // 0 P of a value that may be anything
           if constexpr (Q8) {
-            uint32_t& e = i < 4 ? ve[u].x : ve[u].y;
+            uint32_t& e = i < 4 ? ve.x : ve.y;
             e = on ? e : e & ~(0xFFu << (8 * (i & 3)));
           }
         }
@@ -414,9 +392,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
     for (int t = 0; t < NT; ++t) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < KB; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[t][u][i >> 2][i & 3]);
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
       const float m_new = fmaxf(m[t], over_groups_max(mx) * c);
       if (__any(m_new != m[t])) {
         const float alpha = weight_of(m[t], m_new);
@@ -427,46 +403,43 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
       }
       neg[t] = m[t] == -INFINITY ? 0.f : -m[t];
     }
+    // P, of codes times V's powers in two bf16 parts: fp16 does not have their range, and
+    // the sums are as near as in fp16.
+    bf16x8 pb[NT][NP];
 #pragma unroll
-    for (int u = 0; u < KB; ++u) {
-      // P, of codes times V's powers in two bf16 parts: fp16 does not have their range, and
-      // the sums are as near as in fp16.
-      bf16x8 pb[NT][NP];
+    for (int t = 0; t < NT; ++t) {
+      float p[8];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u][i >> 2][i & 3], c, neg[t]));
-          l[t] += p[i];
-          if constexpr (Q8) p[i] *= power_at(i < 4 ? ve[u].x : ve[u].y, i & 3);
-        }
-        uint32_t x[4], y[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = Q8 ? Bf16::pack(p[2 * r], p[2 * r + 1]) : E::pack(p[2 * r], p[2 * r + 1]);
-          if constexpr (NP == 2) y[r] = Bf16::pack(p[2 * r] - Bf16::lo(x[r]), p[2 * r + 1] - Bf16::hi(x[r]));
-        }
-        pb[t][0] = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
-        if constexpr (NP == 2) pb[t][1] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], c, neg[t]));
+        l[t] += p[i];
+        if constexpr (Q8) p[i] *= power_at(i < 4 ? ve.x : ve.y, i & 3);
       }
+      uint32_t x[4], y[4];
 #pragma unroll
-      for (int j = 0; j < CH; ++j) {  // channel j of the lane's piece, its eight keys
-        uint32_t x[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (Q8)
-            x[r] = C::across(vr[u][2 * r][j >> 2], vr[u][2 * r + 1][j >> 2], j & 3);
-          else
-            x[r] = __builtin_amdgcn_perm(vr[u][2 * r + 1][j >> 1], vr[u][2 * r][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-        }
-        const bf16x8 vop = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int n = 0; n < NP; ++n)
-            acc[t][j] = Q8 ? Bf16::mfma16(vop, pb[t][n], acc[t][j]) : E::mfma16(vop, pb[t][n], acc[t][j]);
+      for (int r = 0; r < 4; ++r) {
+        x[r] = Q8 ? Bf16::pack(p[2 * r], p[2 * r + 1]) : E::pack(p[2 * r], p[2 * r + 1]);
+        if constexpr (NP == 2) y[r] = Bf16::pack(p[2 * r] - Bf16::lo(x[r]), p[2 * r + 1] - Bf16::hi(x[r]));
       }
+      pb[t][0] = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+      if constexpr (NP == 2) pb[t][1] = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {  // channel j of the lane's piece, its eight keys
+      uint32_t x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (Q8)
+          x[r] = C::across(vr[2 * r][j >> 2], vr[2 * r + 1][j >> 2], j & 3);
+        else
+          x[r] = __builtin_amdgcn_perm(vr[2 * r + 1][j >> 1], vr[2 * r][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+      }
+      const bf16x8 vop = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+          acc[t][j] = Q8 ? Bf16::mfma16(vop, pb[t][n], acc[t][j]) : E::mfma16(vop, pb[t][n], acc[t][j]);
     }
   }
 
@@ -542,7 +515,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Wo
     int best, len;
     longest(a, w.seq, best, len);
     if (best != w.seq || len < w.vis.len) {
-      shared_steps<C, true>(a, w, best, min(len, w.vis.len));
+      shared_steps<true>(a, w, best, min(len, w.vis.len));
       if (w.step0 >= w.step1) return no_keys<true>(a, w);
       pg.table = a.table + w.b * a.table_b, pg.end = w.vis.len;
       if constexpr (!kCodes<C>) pg.fetch_ids(ring.ids, w.step0 * kKeys, 0);
@@ -598,7 +571,7 @@ paged_kernel(const PagedArgs a) {
       w.col0 = tile * 16 * PT;
       w.ncol = min(16 * PT, a.per * a.group - w.col0);
       // (a part that the longest sequence may have keys for; whether it does is found out there)
-      shared_steps<C, TILED>(a, w, w.seq, all_shared(a));
+      shared_steps<TILED>(a, w, w.seq, all_shared(a));
       if (w.step0 >= w.step1)
         no_keys<true>(a, w);
       else if constexpr (TILED)
@@ -625,7 +598,7 @@ paged_kernel(const PagedArgs a) {
   w.col0 = tile * kGroups;
   w.ncol = min(kGroups, a.group - w.col0);
   const int len = sequence_length(a, w.b);
-  w.vis = visible<C>(len, PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0, PT > 0 ? 0 : a.sinks);
+  w.vis = visible(len, PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0, PT > 0 ? 0 : a.sinks);
   const int per = a.by_split.of(w.vis.steps + a.split - 1);
   w.step0 = split * per, w.step1 = min(w.step0 + per, w.vis.steps);
   if (w.step0 >= w.step1 && a.parts > 1)
@@ -717,45 +690,54 @@ __global__ void __launch_bounds__(kJoinThreads) paged_wide_join_kernel(const Pag
 // 4096 each 275 -> 284. Four of 32768 to 131072: within two 281, four 250, eight 258.)
 // No split is longer than 4096 keys as far as there may be 64 of them: one long sequence
 // in a large batch is not left to one workgroup a head.
-int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks, int64_t limit) {
+// Over codes twice as many (half as many again in a batch): a split of as many keys is
+// half the bytes (eight sequences of up to 32760 keys 80 -> 73 us, 48 of up to 4100 58 ->
+// 56; four of 131072 148 -> 143; twice that in a batch: 64 of up to 7800 39 -> 41).
+int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks, bool codes) {
   const int64_t keys = window && window < most && sinks < most - window ? window + sinks : most;
-  const int64_t steps = cdiv(keys, kBlock) + 1;
-  int64_t n = (B < 16 ? 1024 : 2048) / (B * Hkv * tiles);
+  const int64_t steps = cdiv(keys, kStep) + 1;
+  int64_t n = (B < 16 ? codes ? 2048 : 1024 : codes ? 3072 : 2048) / (B * Hkv * tiles);
   if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);
   if (n > steps / kWaves) n = steps / kWaves;
-  if (n > limit) n = limit;
+  if (n > kMaxSplits) n = kMaxSplits;
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
-#ifndef PS
-#define PS 512
-#endif
-#ifndef TILED_FROM
-#define TILED_FROM 64
-#endif
 // How a call is cut.
 struct Cut {
   int64_t tiles, split;
-  int64_t ctiles, ptiles, psplit;  // shared keys: tiles of 16 columns in a workgroup, tiles of columns, splits
+  int64_t ctiles, ptiles, psplit;  // shared keys (0: none): tiles of 16 columns in a workgroup, tiles of columns, splits
   int64_t parts() const { return psplit + split; }
   int64_t part_bytes(int64_t B, int64_t H, int64_t D) const { return parts() > 1 ? B * H * parts() * (D + 2) * 4 : 0; }
 };
-Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window, int64_t sinks, int64_t shared, int64_t groups, int cache_type) {
+// Shared keys: up to 16 columns are one tile, up to 64 tiles of 32, whose keys come straight
+// from HBM; more are tiles of 128 in LDS (of 64 or 128 channels). Splits end with a round of
+// a workgroup's steps (four waves; a tile): a wave with a step more than the others is
+// waited for.
+Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t window, int64_t sinks, int64_t shared,
+        int64_t groups, int cache_type) {
   Cut c{};
   c.tiles = cdiv(H / Hkv, kGroups);
-  if (shared > 0) {
-    const int64_t cols = B / groups * (H / Hkv);
-    c.ctiles = cols > kGroups ? cols > TILED_FROM && (D == 64 || D == 128) ? kTiled : 2 : 1;
-    c.ptiles = cdiv(cols, kGroups * c.ctiles);
-    // whole rounds of a workgroup's steps: a wave with a step more than the others is waited for
-    const int64_t steps = cdiv(shared, c.ctiles == kTiled ? kKeys : cache_type ? 2 * kBlock : kBlock);
-    const int64_t round = c.ctiles == kTiled ? 1 : kWaves;
-    int64_t n = PS / (groups * Hkv * c.ptiles);
+  if (shared > keys) shared = keys;
+  if (shared > 0) keys -= shared;
+  c.split = splits(B, Hkv, c.tiles, keys, window, sinks, cache_type != 0);
+  if (shared <= 0) return c;
+  const int64_t cols = B / groups * (H / Hkv);
+  const bool tiled = cols > 4 * kGroups && (D == 64 || D == 128);
+  c.ctiles = tiled ? kTiled : cols > kGroups ? 2 : 1;
+  c.ptiles = cdiv(cols, kGroups * c.ctiles);
+  const int64_t steps = cdiv(shared, tiled ? kKeys : kStep), round = tiled ? 1 : kWaves, items = groups * Hkv * c.ptiles;
+  const auto within = [&](int64_t most) {
+    int64_t n = most / items;
     n = n < 1 ? 1 : n > kMaxShared ? kMaxShared : n;
-    c.psplit = cdiv(steps, round * cdiv(steps, round * n));
-    keys = keys > shared ? keys - shared : 0;
-  }
-  c.split = splits(B, Hkv, c.tiles, keys, window, sinks, kMaxSplits);
+    return cdiv(steps, round * cdiv(steps, round * n));
+  };
+  // One workgroup a CU: 8 sequences of 24 heads behind 4100 keys 14 us, within two 15; behind
+  // 32760 36 and 36. Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
+  // behind 32760 keys 62 against 70; 32 behind 4100 21 against 18), one and a half where own
+  // keys take the other places meanwhile (256 of up to 500 of their own 171 against 184).
+  c.psplit = within(256);
+  if (tiled && steps >= 12 * within(512)) c.psplit = within(B * Hkv * c.tiles * c.split >= 1024 ? 384 : 512);
   return c;
 }
 
@@ -809,7 +791,7 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
                       (!p.table || p.page_size % 8 == 0),
                   SOLATTN_EINVAL, "%s: %lld pages of %lld (a multiple of 8)", what, (long long)p.pages,
                   (long long)p.page_size);
-  SOLATTN_REQUIRE(p.page_size < (1ll << 31) && p.max_pages < (1ll << 31) && p.max_pages * p.page_size < (1ll << 31) - (p.cache_type ? 2 : 1) * kBlock,
+  SOLATTN_REQUIRE(p.page_size < (1ll << 31) && p.max_pages < (1ll << 31) && p.max_pages * p.page_size < (1ll << 31) - kStep,
                   SOLATTN_EUNSUPPORTED, "%s: sequences beyond 2^31 keys", what);
   SOLATTN_REQUIRE(p.shared >= 0 && p.shared < (1ll << 31), SOLATTN_EINVAL, "%s: %lld shared keys", what, (long long)p.shared);
   SOLATTN_REQUIRE(p.shared == 0 || (p.window == 0 && p.sinks == 0), SOLATTN_EINVAL, "%s: shared keys and a window", what);
@@ -860,7 +842,7 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   a.part = static_cast<float*>(p.workspace);
   a.part_ml = B * H * c.parts() * D;
   int64_t grid = B * Hkv * c.tiles * c.split;
-  if (p.shared > 0) {
+  if (c.psplit > 0) {
     const int64_t items = p.groups * Hkv * c.ptiles * c.psplit;
     grid += items;
     SOLATTN_REQUIRE(grid < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
