@@ -311,6 +311,34 @@ def test_paged_bad_pages(paged, dev, kind):
     assert (call(table, n, kc[:0], vc[:0], ks[:0], vs[:0]) == 0).all()
 
 
+@pytest.mark.parametrize("kind", [None] + c8.KINDS, ids=["same", "int8", "e4m3"])
+@pytest.mark.parametrize("B,H,Hkv,D,page", [(3, 64, 64, 64, 16), (70, 16, 8, 64, 8), (256, 8, 8, 128, 16), (300, 4, 4, 64, 32)])
+def test_paged_ragged_batches(paged, dev, kind, B, H, Hkv, D, page):
+    """Launches whose workgroups go by length: idle slots, equal and very different lengths."""
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, 600, (B,), generator=g).tolist()
+    lengths[0], lengths[-1], lengths[B // 2] = 0, 0, 1000
+    lengths[1] = lengths[2] = 300
+    L = max(lengths)
+    n = ints(lengths, dev)
+    q = randn((B, 1, H, D), 3, dev, BF, 2.0)
+    if kind is None:
+        most = -(-L // page)
+        k, v = (randn((B, most * page, Hkv, D), s, dev) for s in (1, 2))
+        table = torch.arange(B * most, dtype=torch.int32, device=dev).reshape(B, most)
+        got = paged.paged_attn(q, k.view(B * most, page, Hkv, D), v.view(B * most, page, Hkv, D), table, n)
+        k, v = k[:, :L], v[:, :L]
+    else:
+        (kc, ks, vc, vs), (k, v), table = filled(B, L, page, Hkv, D, kind, dev, lengths, spread=False)
+        got = paged.paged_attn(q, kc, vc, table, n, k_scale=ks, v_scale=vs)
+    on = (torch.arange(L, device=dev) < n[:, None])[:, None]
+    for b0 in range(0, B, 64):
+        s = slice(b0, b0 + 64)
+        o, p, (_, _, vh) = ref.attention(q[s], k[s], v[s], on[s], D ** -0.5)
+        ref.close(got[s], o, (ref if kind is None else c8).forward_bound(o, p, vh, BF), "o")
+    assert (got[n == 0] == 0).all()
+
+
 # ------------------------------------------------------------------ shared keys
 # per, groups, prefix, rests, page, H, Hkv, D, dtype
 SHARED = [
@@ -381,6 +409,77 @@ def test_shared(paged, dev, kind, case):
     bound = ref.forward_bound(o, p, vh, dtype) if once else c8.forward_bound(o, p, vh, dtype)
     ref.close(got, o, bound, "o")
     assert (got[n == 0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", [None] + c8.KINDS, ids=["same", "int8", "e4m3"])
+@pytest.mark.parametrize("page,D", [(8, 128), (64, 64), (24, 128)])
+def test_shared_long(paged, dev, kind, page, D):
+    """Many tiles of rows over a long prefix, pages that are none of the cache's among its own."""
+    prefix, rests, H, Hkv = 40000, [3, 70], 256, 2
+    B, L = 2, prefix + max(rests)
+    most = -(-L // page)
+    n = ints([prefix + r for r in rests], dev)
+    q = randn((B, 1, H, D), 3, dev, BF, 2.0)
+    table = torch.randperm(B * most, generator=torch.Generator().manual_seed(3)).to(torch.int32).reshape(B, most).to(dev)
+    table[0, :prefix // page] = table[1, :prefix // page]
+    bad = torch.tensor([5, 700 // page * 3, prefix // page // 2], device=dev)
+    k, v = (randn((B * most, page, Hkv, D), s, dev) for s in (1, 2))
+    scales = {}
+    if kind is not None:
+        coded = [c8.encode(x, kind) for x in (k, v)]
+        k, v = (c8.values(*c).to(BF) for c in coded)
+        (kc, vc), (ks, vs) = ([c[0] for c in coded], [c[1].transpose(1, 2).contiguous().view(c8.E8) for c in coded])
+        scales = dict(k_scale=ks, v_scale=vs)
+    else:
+        kc, vc = k, v
+    rows = [torch.stack([x[table[b].long()].flatten(0, 1)[:L] for b in range(B)]) for x in (k, v)]
+    for x in rows:
+        x[:, :prefix] = x[1:, :prefix]
+    table[:, bad] = ints([-1, B * most, -5], dev)
+    on = (torch.arange(L, device=dev) < n[:, None])[:, None].clone()
+    for p in bad.tolist():
+        on[..., p * page:(p + 1) * page] = False
+    got = paged.paged_attn(q, kc, vc, table, n, shared=prefix, **scales)
+    o, p, (_, _, vh) = ref.attention(q, *rows, on, D ** -0.5)
+    ref.close(got, o, ref.forward_bound(o, p, vh, BF), "o")  # (many rows: P in one rounding)
+
+
+@pytest.mark.parametrize("kind", [None, F8], ids=["same", "e4m3"])
+@pytest.mark.parametrize("page,D", [(8, 64), (16, 128)])
+def test_shared_in_one_part(paged, dev, kind, page, D):
+    """So many rows that none of the keys are split: one part of more than 128 tiles, whose page ids
+    are held 64 tiles at a time."""
+    B, H, n = 512, 128, 8300
+    most = -(-n // page)
+    q = randn((B, 1, H, D), 3, dev, BF, 2.0)
+    table = torch.randperm(most, generator=torch.Generator().manual_seed(5)).to(torch.int32).to(dev)[None].repeat(B, 1)
+    k, v = (randn((most, page, 1, D), s, dev) for s in (1, 2))
+    scales = {}
+    kc, vc = k, v
+    if kind is not None:
+        coded = [c8.encode(x, kind) for x in (k, v)]
+        k, v = (c8.values(*c).to(BF) for c in coded)
+        (kc, vc), (ks, vs) = ([c[0] for c in coded], [c[1].transpose(1, 2).contiguous().view(c8.E8) for c in coded])
+        scales = dict(k_scale=ks, v_scale=vs)
+    table[:, 40] = -1
+    at = table[0].long().clamp_min(0)
+    kd, vd = (x[at].flatten(0, 1)[:n, 0].double() for x in (k, v))
+    on = torch.ones(n, dtype=torch.bool, device=dev)
+    on[40 * page:41 * page] = False
+    lengths = torch.full((B,), n, dtype=torch.int32, device=dev)
+    lengths[7] = 0
+    got = paged.paged_attn(q, kc, vc, table, lengths, shared=n, **scales)
+    assert (got[7] == 0).all()
+    got[7] = got[6]
+    u = ref.half_step(BF)
+    for b in range(0, B, 64):
+        rows = q[b:b + 64].clone()
+        if b == 0:
+            rows[7] = rows[6]
+        p = torch.softmax((rows.flatten(0, 2).double() @ kd.T * D ** -0.5).masked_fill(~on, float("-inf")), -1)
+        o, pv = p @ vd, p @ vd.abs()
+        bound = (u * (2 * o.abs() + pv) + 2 * 2.0 ** -13 * pv) * 1.01  # that of _operators.forward_bound
+        ref.close(got[b:b + 64].flatten(0, 2), o, bound, "o")
 
 
 @pytest.mark.parametrize("shared", [1, 31, 64, 500, 2 ** 40])
