@@ -17,7 +17,22 @@ constexpr uint32_t kTinyRow = (127u - 110u) << 23;  // bits of 2^-110
 constexpr uint32_t kInfBits = 0x7F800000u;
 
 __device__ __forceinline__ float power_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-__device__ __forceinline__ float power_at(uint32_t word, int i) { return power_of((word >> (8 * i)) & 0xFFu); }
+// The power of byte i of a word, in one instruction (an AND and a shift where the compiler chooses).
+__device__ __forceinline__ float power_at(uint32_t word, int i) {
+  uint32_t x;
+#define SOLATTN_BYTE_SHL(sel) \
+  asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:" sel : "=v"(x) : "v"(23), "v"(word))
+  if (i == 0)
+    SOLATTN_BYTE_SHL("BYTE_0");
+  else if (i == 1)
+    SOLATTN_BYTE_SHL("BYTE_1");
+  else if (i == 2)
+    SOLATTN_BYTE_SHL("BYTE_2");
+  else
+    SOLATTN_BYTE_SHL("BYTE_3");
+#undef SOLATTN_BYTE_SHL
+  return __uint_as_float(x);
+}
 
 // Exponent byte of a row whose largest magnitude has the bits `top`; unit: what the factor
 // of the codes (2^-that) is multiplied with them as.

@@ -714,13 +714,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_wide_join_kernel(const Pag
 // 4096 each 275 -> 284. Four of 32768 to 131072: within two 281, four 250, eight 258.)
 // No split is longer than 4096 keys as far as there may be 64 of them: one long sequence
 // in a large batch is not left to one workgroup a head.
-// Over codes twice as many (half as many again in a batch): a split of as many keys is
-// half the bytes (eight sequences of up to 32760 keys 80 -> 73 us, 48 of up to 4100 58 ->
-// 56; four of 131072 148 -> 143; twice that in a batch: 64 of up to 7800 39 -> 41).
+// Over codes eight in any batch: a split of as many keys is half the bytes (eight sequences
+// of up to 32760 keys 80 -> 73 us, four of 131072 148 -> 143; more than eight, 32 of up to
+// 16384 39 -> 41, fewer 46).
 int splits(int64_t B, int64_t Hkv, int64_t tiles, int64_t most, int64_t window, int64_t sinks, bool codes) {
   const int64_t keys = window && window < most && sinks < most - window ? window + sinks : most;
   const int64_t steps = cdiv(keys, kStep) + 1;
-  int64_t n = (B < 16 ? codes ? 2048 : 1024 : codes ? 3072 : 2048) / (B * Hkv * tiles);
+  int64_t n = (B < 16 && !codes ? 1024 : 2048) / (B * Hkv * tiles);
   if (n < cdiv(keys, 4096)) n = cdiv(keys, 4096);
   if (n > steps / kWaves) n = steps / kWaves;
   if (n > kMaxSplits) n = kMaxSplits;
