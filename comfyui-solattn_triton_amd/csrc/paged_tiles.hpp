@@ -284,7 +284,8 @@ template <int N>
 __device__ __forceinline__ void wait_copies() {
   __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
 }
-__device__ __forceinline__ void tile_barrier() { asm volatile("s_barrier" ::: "memory"); }
+// Behind it no wave reads LDS any more: the compiler does not wait for its reads here by itself.
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <typename E, int D>
 __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (&q)[D / 16], TileLds<D>& lds,
