@@ -365,58 +365,58 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
       ve = *reinterpret_cast<const uint2*>(a.vs + hk * a.vs_h + times(vpage, a.vs_p) + vslot);
     }
     if (st + kWaves < w.step1) find(st + kWaves);
-    // scores of this lane: key base + 32 u + 8 g + i in element i % 4 of tile i / 4
+    // scores of this lane: key base + 8 g + i in element i % 4 of tile i / 4
     f32x4 s[NT][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
-          bf16x8 kop;
-          if constexpr (Q8) {
-            const uint4 x = kr[i][cc >> 1];
-            const uint32_t lo2 = cc & 1 ? x.z : x.x, hi2 = cc & 1 ? x.w : x.y;
-            kop = __builtin_bit_cast(bf16x8, make_uint4(C::template pair<E>(lo2, 0), C::template pair<E>(lo2, 2),
-                                                        C::template pair<E>(hi2, 0), C::template pair<E>(hi2, 2)));
-          } else {
-            kop = __builtin_bit_cast(bf16x8, kr[i][cc]);
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (cc == 0) s[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            s[t][i] = E::mfma16(kop, q[t][cc], s[t][i]);
-          }
+      for (int cc = 0; cc < NC; ++cc) {
+        bf16x8 kop;
+        if constexpr (Q8) {
+          const uint4 x = kr[i][cc >> 1];
+          const uint32_t lo2 = cc & 1 ? x.z : x.x, hi2 = cc & 1 ? x.w : x.y;
+          kop = __builtin_bit_cast(bf16x8, make_uint4(C::template pair<E>(lo2, 0), C::template pair<E>(lo2, 2),
+                                                      C::template pair<E>(hi2, 0), C::template pair<E>(hi2, 2)));
+        } else {
+          kop = __builtin_bit_cast(bf16x8, kr[i][cc]);
         }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (cc == 0) s[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+          s[t][i] = E::mfma16(kop, q[t][cc], s[t][i]);
+        }
+      }
     const float c = Q8 ? 1.f : a.c;  // codes: the factor is the key's
     if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float f = power_at(i < 4 ? ke.x : ke.y, i & 3) * a.c;
+      for (int i = 0; i < 8; ++i) {
+        const float f = power_at(i < 4 ? ke.x : ke.y, i & 3) * a.c;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) s[t][i >> 2][i & 3] *= f;
-        }
+        for (int t = 0; t < NT; ++t) s[t][i >> 2][i & 3] *= f;
+      }
     }
     if (base < lo || base + S > (MANY ? safe : end) || __any(!vok)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = base + 8 * g + i;
-          const bool on = vok && j >= lo && j < end;
+      for (int i = 0; i < 8; ++i) {
+        const int j = base + 8 * g + i;
+        const bool on = vok && j >= lo && j < end;
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            s[t][i >> 2][i & 3] = on && (!MANY || j < hi[t]) ? s[t][i >> 2][i & 3] : -INFINITY;
+        for (int t = 0; t < NT; ++t)
+          s[t][i >> 2][i & 3] = on && (!MANY || j < hi[t]) ? s[t][i >> 2][i & 3] : -INFINITY;
 #pragma unroll
-          for (int r = 0; r < VW; ++r) vr[i][r] = on ? vr[i][r] : 0u;  // 0 P of a value that may be anything
-          if constexpr (Q8) {
-            uint32_t& e = i < 4 ? ve.x : ve.y;
-            e = on ? e : e & ~(0xFFu << (8 * (i & 3)));
-          }
+        for (int r = 0; r < VW; ++r) vr[i][r] = on ? vr[i][r] : 0u;  // 0 P of a value that may be anything
+        if constexpr (Q8) {
+          uint32_t& e = i < 4 ? ve.x : ve.y;
+          e = on ? e : e & ~(0xFFu << (8 * (i & 3)));
         }
+      }
     }
     float neg[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
       const float m_new = fmaxf(m[t], over_groups_max(mx) * c);
       if (__any(m_new != m[t])) {
         const float alpha = weight_of(m[t], m_new);
@@ -551,8 +551,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Wo
   RowState<D / 32> st;
   if constexpr (kCodes<C>) {
     const uint32_t kb = lds_addr(lds), vb = kb + 2 * kKeys * D;
-    attend_tiles<E, D, HalfDecode<E, C, D, kByRow>, HalfDecode<E, C, D, kTransposed>>(st, q, kb, vb, ks, vs, pg, w.step0,
-                                                                                     w.step1 - w.step0, hi, safe, a.c);
+    attend_codes<E, C, D>(st, q, kb, vb, ks, vs, pg, w.step0, w.step1 - w.step0, hi, safe, a.c);
   } else {
     attend_ring<E, D>(st, q, ring, ks, vs, pg, w.step0, w.step1 - w.step0, hi, safe, a.c);
   }

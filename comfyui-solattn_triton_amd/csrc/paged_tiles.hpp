@@ -3,13 +3,19 @@
 // windowed forward has (window_common.hpp). A row is a head of one of the sequences that
 // share the keys.
 //
-// What differs is where keys come from: a lane finds the place of one key of a tile of 64
-// well ahead of its copy, and the copies of a half (rows of eight consecutive keys a wave
-// at most, so of one page) take their scalar bases from these lanes. (Bases found by each
-// copy in scalar arithmetic: some 40 scalar instructions a copy, 160 a step of 16 matrix
-// instructions.) Keys past the end or on pages that are none of the cache's are rows of
-// zeros, and masked. Codes go through registers and become 16-bit values there, once for
-// all the rows that read the tile.
+// Bound: the matrix instructions, 4 D operations a row and key, beside the exponentials of
+// the scores. 256 sequences of 24 heads over 8, of 128 channels, behind 32760 keys alone:
+// 16-bit values 146 us, 0.70 PFLOP/s (0.9-0.97 between the first tile's latency and the
+// parts' way out); e4m3 173, whose conversions stand between the products.
+//
+// What differs from the windowed forward is where keys come from: a lane finds the place of
+// one key of a tile of 64 well ahead of its copy, and the copies of a half (rows of eight
+// consecutive keys a wave at most, so of one page) take their scalar bases from these lanes.
+// (Bases found by each copy in scalar arithmetic: some 40 scalar instructions a copy, 160 a
+// step of 16 matrix instructions.) Keys past the end or on pages that are none of the
+// cache's are rows of zeros, and masked. 16-bit values are copied straight into LDS
+// (attend_ring); codes go through registers and become 16-bit values there, once for all
+// the rows that read the tile (attend_codes).
 #pragma once
 
 #include "cache8.hpp"
@@ -69,26 +75,30 @@ struct TilePages {
       to[s & 1][i] = id >= 0 && id < pages ? id : -1;
     }
   }
-  template <bool CODES>
-  __device__ __forceinline__ TileRows rows(int id, int j0, const TileSource& s) const {
-    const uint32_t j = static_cast<uint32_t>(j0 + (static_cast<int>(threadIdx.x) & 63));
-    const uint32_t slot = j - by_page.of(j) * by_page.d;
-    const uint8_t* at = id >= 0 ? s.p + id * s.page + slot * s.slot : reinterpret_cast<const uint8_t*>(zero_row);
-    TileRows r;
-    r.lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at));
-    r.hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at) >> 32);
-    r.power = 0.f;
-    if constexpr (CODES)
-      if (id >= 0) r.power = power_of(s.e[id * s.e_page + slot]);
-    return r;
-  }
 };
 
-// Copies of half `hf` of a tile into the half buffer at dst: start() asks for the rows,
-// finish() has them in LDS, or on their way there.
+// A key's row, of page `id` (-1: a row of zeros).
+__device__ __forceinline__ TileRows row_at(const TileSource& s, int id, uint32_t slot) {
+  const uint64_t at = id >= 0 ? reinterpret_cast<uint64_t>(s.p) + id * s.page + slot * s.slot : reinterpret_cast<uint64_t>(zero_row);
+  return {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32), 0.f};
+}
+
+// Scores of a half from key j0 on: keys that are not visible (`seen` has a bit for each) or
+// not below `hi` become -inf; every row sees the keys below `safe`.
+__device__ __forceinline__ void mask_half(f32x16& s, int j0, uint32_t seen, int hi, int safe) {
+  if (seen == ~0u && j0 + 32 <= safe) return;
+  const int half = (threadIdx.x & 63) >> 5;
+  const uint32_t bits = (seen >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const uint32_t w = bit_word(bits, r);
+    s[r] = __uint_as_float((__float_as_uint(s[r]) & w) | (__float_as_uint(-INFINITY) & ~w));
+  }
+}
+
+// Copies half `hf` of a tile of 16-bit values into the half buffer at dst.
 template <int D, int HOW>
-struct HalfCopy {  // 16-bit values, straight into LDS
-  static constexpr bool kCodes = false;
+struct HalfCopy {
   static constexpr int C = D / 8, R = 64 / C, U = 32 / (kTileThreads / C);  // pieces of a row; rows of a wave's copy; copies
   uint32_t off;
   __device__ __forceinline__ void init(const TileSource& s) {
@@ -109,23 +119,24 @@ struct HalfCopy {  // 16-bit values, straight into LDS
         g2l16(rows.of_lane(32 * hf + g0 + (threadIdx.x & 63) / C) + piece(), dst + g0 * 2 * D);
     }
   }
-  __device__ __forceinline__ void finish(uint32_t) const {}
 };
+
+// The same of codes, 16 of a row a thread: start() asks for them, finish() has their values
+// in LDS.
 template <typename E, typename CODES, int D, int HOW>
-struct HalfDecode {  // codes, 16 of a row a thread, through registers
-  static constexpr bool kCodes = true;
+struct HalfDecode {
   static constexpr int C = D / 16;
   uint4 w;
   float power;
   uint32_t to0, to1;  // where the piece's two halves go
   bool mine;
-  __device__ __forceinline__ void init(const TileSource&) {
+  __device__ __forceinline__ void init() {
     const int e = threadIdx.x, row = e / C % 32, pc = e % C;
     mine = D == 128 || (e < 32 * C) == (HOW == kByRow);  // 64 channels: half the threads for K, half for V
     to0 = row * 2 * D + swz<D, HOW>(row, 2 * pc) * 16;
     to1 = row * 2 * D + swz<D, HOW>(row, 2 * pc + 1) * 16;
   }
-  __device__ __forceinline__ void start(uint32_t, int hf, uint64_t, const TileRows& rows, const TileSource&) {
+  __device__ __forceinline__ void start(int hf, const TileRows& rows) {
     const int e = threadIdx.x, row = 32 * hf + e / C % 32;
     power = __shfl(rows.power, row);
     const uint8_t* at = rows.of_lane(row);
@@ -150,44 +161,33 @@ struct HalfDecode {  // codes, 16 of a row a thread, through registers
 // The keys of tiles tile0 .. tile0 + ntiles - 1 (64 each, the last may end early) for this
 // lane's row (32 wave + lane % 32 of the workgroup's), which sees those below `hi`; every
 // row of the workgroup sees those below `safe`. st: the row's O^T, maximum and sum.
-template <typename E, int D, typename KCopy, typename VCopy>
-__device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const bf16x8 (&q)[D / 16], uint32_t kb, uint32_t vb,
+template <typename E, typename CODES, int D>
+__device__ __forceinline__ void attend_codes(RowState<D / 32>& st, const bf16x8 (&q)[D / 16], uint32_t kb, uint32_t vb,
                                              const TileSource& ks, const TileSource& vs, const TilePages& pg,
                                              int tile0, int ntiles, int hi, int safe, float c) {
   constexpr int ND = D / 32, NC = D / 16;
   constexpr uint32_t kHalf = kKeys * D;  // bytes of half a tile
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const uint32_t kl = k_lane<D>(kb, lane & 31, half), vl = v_lane<D>(vb, lane);
-  constexpr bool Q8 = KCopy::kCodes;
   const int first = tile0 * kKeys;
-  KCopy kc;
-  VCopy vc;
-  kc.init(ks);
-  vc.init(vs);
+  HalfDecode<E, CODES, D, kByRow> kc;
+  HalfDecode<E, CODES, D, kTransposed> vc;
+  kc.init();
+  vc.init();
   st.m = kNoMax;
   st.l = 0.f;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt) st.acc[dt] = f32x16{};
   const auto key0 = [&](int t) __attribute__((always_inline)) { return first + kKeys * min(t, ntiles - 1); };
   const auto ids_of = [&](int t) __attribute__((always_inline)) { return pg.ids(key0(t)); };
-  const auto krows = [&](int id, int t) __attribute__((always_inline)) { return pg.template rows<Q8>(id, key0(t), ks); };
-  const auto vrows = [&](int id, int t) __attribute__((always_inline)) { return pg.template rows<Q8>(id, key0(t), vs); };
-  const auto land = [&]() __attribute__((always_inline)) {
-    wait_tile_copies();
-    __syncthreads();
+  const auto rows = [&](int id, int t, const TileSource& s) __attribute__((always_inline)) {
+    const uint32_t j = static_cast<uint32_t>(key0(t) + lane), slot = j - pg.by_page.of(j) * pg.by_page.d;
+    TileRows r = row_at(s, id, slot);
+    if (id >= 0) r.power = power_of(s.e[id * s.e_page + slot]);
+    return r;
   };
-  // Scores of half hf of the tile from j0 on: keys that are not visible become -inf.
-  const auto mask = [&](f32x16& s, int j0, int hf, uint64_t seen) __attribute__((always_inline)) {
-    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * hf));
-    j0 += 32 * hf;
-    if (mine != ~0u || j0 + 32 > safe) {
-      const uint32_t bits = (mine >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t w = bit_word(bits, r);
-        s[r] = __uint_as_float((__float_as_uint(s[r]) & w) | (__float_as_uint(-INFINITY) & ~w));
-      }
-    }
+  const auto mask = [&](f32x16& s, int t, int hf, uint64_t seen) __attribute__((always_inline)) {
+    mask_half(s, first + kKeys * t + 32 * hf, static_cast<uint32_t>(seen >> (32 * hf)), hi, safe);
   };
   // In round t: K's rows of the tiles t + 1 and t + 2, V's of t and t + 1; those of a tile
   // further on are found here, the ids of t + 4 asked for.
@@ -197,30 +197,30 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const bf16x8 
   {
     const int i0 = ids_of(0), i1 = ids_of(1);
     i2 = ids_of(2), i3 = ids_of(3);
-    const TileRows k0 = krows(i0, 0);
-    v0 = vrows(i0, 0);
+    const TileRows k0 = rows(i0, 0, ks);
+    v0 = rows(i0, 0, vs);
     s0w = __ballot(i0 >= 0), s1w = __ballot(i1 >= 0), s2w = __ballot(i2 >= 0), s3w = __ballot(i3 >= 0);
-    kc.start(kb, 0, s0w, k0, ks);
+    kc.start(0, k0);
     kc.finish(kb);
-    kc.start(kb + kHalf, 1, s0w, k0, ks);
+    kc.start(1, k0);
     kc.finish(kb + kHalf);
-    vc.start(vb, 0, s0w, v0, vs);
+    vc.start(0, v0);
     vc.finish(vb);
-    k1 = krows(i1, 1), v1 = vrows(i1, 1), k2 = krows(i2, 2);
+    k1 = rows(i1, 1, ks), v1 = rows(i1, 1, vs), k2 = rows(i2, 2, ks);
   }
   f32x16 sa, sb;  // scores of even and odd halves
   bf16x8 pa[2], pb[2];
-  land();
+  __syncthreads();
   {  // step 0, without a stream: both halves are scored, the running max is the whole tile's
     f32x16 x0 = {}, x1 = {};
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) x0 = E::mfma32(k_op_x<D>(kl, 0, cc), q[cc], x0);
     __syncthreads();  // every wave is done with K(0)
-    if (ntiles > 1) kc.start(kb, 0, s1w, k1, ks);
+    if (ntiles > 1) kc.start(0, k1);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) x1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], x1);
-    mask(x0, first, 0, s0w);
-    mask(x1, first, 1, s0w);
+    mask(x0, 0, 0, s0w);
+    mask(x1, 0, 1, s0w);
     float mx = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(x0[r], x1[r]));
@@ -234,36 +234,36 @@ __device__ __forceinline__ void attend_tiles(RowState<D / 32>& st, const bf16x8 
     if (ntiles > 1) kc.finish(kb);
   }
   mfma_fence(st.acc);  // O's zeros are in their registers before the asm MFMAs that add to them
-  land();
+  __syncthreads();
   int t = 0;
 #pragma unroll 1
   for (; t < ntiles - 1; ++t) {
     i4 = ids_of(t + 4);
-    const TileRows k3 = krows(i3, t + 3), v2 = vrows(i2, t + 2);
+    const TileRows k3 = rows(i3, t + 3, ks), v2 = rows(i2, t + 2, vs);
     // step 2 t + 1: K of half 2 t + 3, V of 2 t + 1
-    kc.start(kb + kHalf, 1, s1w, k1, ks);
-    vc.start(vb + kHalf, 1, s0w, v0, vs);
+    kc.start(1, k1);
+    vc.start(1, v0);
     window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, c);
     kc.finish(kb + kHalf);
     vc.finish(vb + kHalf);
-    land();
+    __syncthreads();
     // step 2 t + 2: K of half 2 t + 4, V of 2 t + 2
-    if (t + 2 < ntiles) kc.start(kb, 0, s2w, k2, ks);
-    vc.start(vb, 0, s1w, v1, vs);
-    mask(sa, first + kKeys * (t + 1), 0, s1w);
+    if (t + 2 < ntiles) kc.start(0, k2);
+    vc.start(0, v1);
+    mask(sa, t + 1, 0, s1w);
     window_step<E, D>(st, sa, sb, pb, pa, kl + kHalf, vl + kHalf, q, c);
-    mask(sb, first + kKeys * (t + 1), 1, s1w);
+    mask(sb, t + 1, 1, s1w);
     if (t + 2 < ntiles) kc.finish(kb);
     vc.finish(vb);
-    land();
+    __syncthreads();
     i2 = i3, i3 = i4;
     k1 = k2, k2 = k3, v0 = v1, v1 = v2;
     s0w = s1w, s1w = s2w, s2w = s3w, s3w = __ballot(i4 >= 0);
   }
-  vc.start(vb + kHalf, 1, s0w, v0, vs);
+  vc.start(1, v0);
   window_step<E, D>(st, sb, sa, pa, pb, kl, vl, q, c);
   vc.finish(vb + kHalf);
-  land();
+  __syncthreads();
   mfma_fence(st.acc);
 #pragma unroll
   for (int i = 0; i < NC; ++i)  // P.V of the last half
@@ -312,28 +312,15 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
     t = min(t, ntiles - 1);
     const int j = first + kKeys * t + lane;
     const uint32_t page = pg.by_page.of(static_cast<uint32_t>(j));
-    const int slot = static_cast<int>(static_cast<uint32_t>(j) - page * pg.by_page.d);
+    const uint32_t slot = static_cast<uint32_t>(j) - page * pg.by_page.d;
     const int sg = t / kIdTiles;
     int id = lds.ids[sg & 1][min(static_cast<int>(page) - pg.page0(first, sg), kIds - 1)];
     id = j < pg.end ? id : -1;
     seen = __ballot(id >= 0);
-    const uint8_t* at = id >= 0 ? s.p + id * s.page + slot * s.slot : reinterpret_cast<const uint8_t*>(zero_row);
-    TileRows r;
-    r.lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at));
-    r.hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(at) >> 32);
-    return r;
+    return row_at(s, id, slot);
   };
-  const auto mask = [&](f32x16& s, int j0, int hf, uint64_t seen) __attribute__((always_inline)) {
-    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * hf));
-    j0 += 32 * hf;
-    if (mine != ~0u || j0 + 32 > safe) {
-      const uint32_t bits = (mine >> (4 * half)) & ~bits_from(hi - j0 - 4 * half);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t w = bit_word(bits, r);
-        s[r] = __uint_as_float((__float_as_uint(s[r]) & w) | (__float_as_uint(-INFINITY) & ~w));
-      }
-    }
+  const auto mask = [&](f32x16& s, int t, int hf, uint64_t seen) __attribute__((always_inline)) {
+    mask_half(s, first + kKeys * t + 32 * hf, static_cast<uint32_t>(seen >> (32 * hf)), hi, safe);
   };
   wait_copies<0>();
   tile_barrier();
@@ -372,8 +359,8 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
     if (ntiles > 1) vc.start(vb + 2 * kHalf, 0, s1w, v1, vs);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) x1 = E::mfma32(k_op_x<D>(kl + kHalf, 0, cc), q[cc], x1);
-    mask(x0, first, 0, s0w);
-    mask(x1, first, 1, s0w);
+    mask(x0, 0, 0, s0w);
+    mask(x1, 0, 1, s0w);
     float mx = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(x0[r], x1[r]));
@@ -399,9 +386,9 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
     land(t);
     if (t + 3 < ntiles) kc.start(kb + b0, 0, s3w, k3, ks);  // step 2 t + 2
     if (t + 2 < ntiles) vc.start(vb + a0, 0, s2w, v2, vs);
-    mask(sa, first + kKeys * (t + 1), 0, s1w);
+    mask(sa, t + 1, 0, s1w);
     window_step<E, D>(st, sa, sb, pb, pa, kl + b0 + kHalf, vl + a0 + kHalf, q, c);
-    mask(sb, first + kKeys * (t + 1), 1, s1w);
+    mask(sb, t + 1, 1, s1w);
     land(t);
     k2 = k3, v1 = v2;
     s1w = s2w, s2w = s3w;
