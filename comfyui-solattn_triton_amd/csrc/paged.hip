@@ -1,17 +1,29 @@
 // Attention of one new token of each sequence over a key-value cache, paged or
-// contiguous: the visible keys are split over workgroups and waves, each with an
-// online softmax of its own, and joined.
+// contiguous, of 16-bit values or of 8-bit codes: the visible keys are split over
+// workgroups and waves, each with an online softmax of its own, and joined.
 //
 // Per sequence b the token sits at position len - 1 and sees the keys j < len,
 // with a window those with j >= len - window or j < sinks. A query head shares its
 // kv head with group - 1 others; these (up to 16) are the columns of the tiles.
+// Sequences may have their first keys in common (`shared` of them, runs of `per`
+// sequences): the heads of all of a run are then the columns of these keys, which
+// are read once for 16 columns, for 32, or for 128 (paged_tiles.hpp), and what is
+// behind them is attended as before, in the same launch; the join takes both.
 //
 // Bound: HBM, 2 Hkv D values a visible key; the matrix instructions do 16 query
-// columns whether they exist or not, 256 of their cycles for 16 KiB of cache. Four
-// sequences of 32768 to 131072 tokens, 24 heads over 8, bf16: 232-251 us, 5.3-5.8
-// TB/s (a large copy reaches 5.0); 32 of 512 to 16384, 16 heads of 64 over 4, pages of
-// 16: 65-68 us, 4.1 TB/s, of it the kernel 54 and the join and its launch the rest; one
-// sequence with a window of 4096: 10.2 us, two launches of the host's (kernels 5.9 and 4.7).
+// columns whether they exist or not, 256 of their cycles for 16 KiB of a 16-bit cache.
+//   bf16: four sequences of 32768 to 131072 tokens, 24 heads over 8 of 128 channels:
+//     238-251 us, 5.3-5.6 TB/s (a large copy reaches 5.0-5.15); 32 of 512 to 16384, 16
+//     heads of 64 over 4, pages of 16: 63 us; one sequence with a window of 4096: 10.2
+//     us, two launches of the host's (kernels 5.9 and 4.7).
+//   Codes: the four, e4m3: 138 us, 4.9 TB/s, kernel 134. The 32, int8: 39 us, 3.6 TB/s,
+//     kernel 31 and join 5; there the vector units are at 56-70%, with a byte's way to a
+//     16-bit float (two instructions a pair of e4m3, four of int8). One with a window of
+//     4096: 8.7 us, kernels 6.0 and 2.8.
+//   Shared keys: 8 sequences of 24 heads over 8 behind 4096 bf16 keys: 13 us (22 as if
+//     nothing was shared), latency: 10.6 of it the kernel, a chain of lengths, page ids,
+//     keys and steps, and 2-4 the join. 64 in groups over int8: 21 us (48), the
+//     conversions again. 256 behind 32760 bf16 keys: 172 us (2600), products.
 // A wave takes 32 keys at a time straight from HBM into operand registers, no LDS:
 //   S^T = K Q^T (v_mfma_f32_16x16x32): row r of tile t is key 8 (r/4) + 4 t + r%4
 //     of the 32, so lane (q, g) = (lane % 16, lane / 16) gets the scores of the
@@ -19,7 +31,9 @@
 //   O^T += V^T P^T: a lane reads the same keys 8 g + 0..7, D / 16 channels each,
 //     and transposes them in registers (v_perm_b32), one A operand per channel of
 //     the D / 16: row i of operand j is channel (D / 16) i + j.
-// The row's statistics need an exchange between the lanes g only.
+// The row's statistics need an exchange between the lanes g only. Codes become operands
+// as they are (integers up to 127 and e4m3's values are exact in 16 bits); K's power of
+// two multiplies the score, V's the weight.
 #include "paged_tiles.hpp"
 
 namespace solattn {

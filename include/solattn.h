@@ -490,7 +490,11 @@ int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint
  * strides are those of pages and heads.
  * Written rows: the smallest power of two that keeps the row's largest magnitude within
  * 127 or 448 (below 2^-110: a row of zeros), codes rounded to nearest even. A row that
- * holds a NaN or an infinity reads as NaN in every channel.
+ * holds a NaN or an infinity reads as NaN in every channel. Its byte is
+ * 255, with codes 0 or e4m3's NaN; zeros have byte 0 and codes 0. Other codes beside these
+ * two bytes mean nothing.
+ * A value is exact in 16 bits: in bf16, and in fp16 within fp16's range (an fp16 call
+ * may round values below 2^-14 and those from 65520 on to infinities).
  *
  * solattn_qk_norm_rope_append with such a cache; k' is rounded once, from fp32. */
 int solattn_qk_norm_rope_append8(

@@ -27,7 +27,8 @@ CACHE = [
     (dict(dtype=3), EINVAL, b"dtype"), (dict(ct=0), EINVAL, b"cache type"), (dict(ct=3), EINVAL, b"cache type"),
     (dict(T=0), EINVAL, b"sizes"), (dict(D=24), EUNSUPPORTED, b"head_dim"), (dict(D=144), EUNSUPPORTED, b"head_dim"),
     (dict(B=1 << 31), EUNSUPPORTED, b"many"), (dict(B=1 << 20, T=1 << 12), EUNSUPPORTED, b"many"),
-    (dict(B=TOP, T=TOP), EUNSUPPORTED, b"many"), (dict(table=None), EINVAL, b"page table"), (dict(n=None), EINVAL, b"lengths"),
+    (dict(B=TOP, T=TOP), EUNSUPPORTED, b"many"), (dict(B=1 << 20, T=1 << 5), EUNSUPPORTED, b"one launch"),
+    (dict(B=1 << 20, T=1 << 6, D=64), EUNSUPPORTED, b"one launch"), (dict(table=None), EINVAL, b"page table"), (dict(n=None), EINVAL, b"lengths"),
     (dict(pages=-1), EUNSUPPORTED, b"pages"), (dict(page=0), EUNSUPPORTED, b"pages"), (dict(most=1 << 28), EUNSUPPORTED, b"2^31"),
     (dict(most=TOP), EUNSUPPORTED, b"2^31"), (dict(x=None), EINVAL, b"null k"), (dict(x=A + 8), EINVAL, b"k must be 16-byte"),
     (dict(c=None), EINVAL, b"null k_cache"), (dict(c=A + 8), EINVAL, b"k_cache must be 16-byte"),
@@ -99,14 +100,14 @@ def test_paged_refusals(capi, kw, rc, text):
 
 
 def test_paged_workspace(capi):
-    """A row's parts over shared keys and over its own, 64 at most; sizes that no call takes have none."""
+    """A row's parts over shared keys and over its own, 64 at most of each; sizes that no call takes have none."""
     L = capi.LIB
     need = L.solattn_paged_attn_shared_workspace_bytes
     for B, H, Hkv, D, most, shared, groups in ((8, 24, 8, 128, 70, 4100, 1), (256, 24, 8, 128, 520, 32760, 1), (64, 16, 4, 64, 525, 8000, 4),
                                                (1, 1, 1, 64, 1000, 60000, 1), (2, 1, 1, 64, 1 << 20, 1 << 25, 1), (4, 8, 8, 128, 4, 64, 4)):
         row = B * H * (D + 2) * 4
         size = need(B, H, Hkv, D, most, 64, 0, 0, 0, shared, groups)
-        assert size % row == 0 and 2 <= size // row <= 64
+        assert size % row == 0 and 2 <= size // row <= 128
     for args in ((4, 4, 2, 128, 64, 16, 0, 0, 0, 5, 3), (4, 4, 2, 128, 64, 16, 0, 0, 0, -1, 1), (4, 4, 2, 128, 64, 16, 0, 0, 0, TOP, 1),
                  (TOP, 2, 1, 128, 64, 16, 0, 0, 0, 5, 1), (4, 4, 2, 128, TOP, TOP, 0, 0, 0, 5, 1), (4, 4, 2, TOP, 64, 16, 0, 0, 0, 5, 1),
                  (4, 4, 2, 128, 64, 16, 0, 0, 0, 5, 0), (4, 4, 2, 128, 64, 16, 0, 0, 0, 5, -2)):
