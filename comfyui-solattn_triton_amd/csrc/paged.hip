@@ -543,7 +543,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Wo
   bf16x8 q[D / 16];
   load_row<D>(q, a.q + b * a.sq_b + h * a.sq_h, half);
   int hi = sequence_length(a, b);
-  const auto near = [](int64_t slot) { return slot >= 0 && slot < (1 << 28); };
+  const auto near = [&](int64_t slot) { return a.near && slot < (1 << 28); };
   const TileSource ks{a.k + w.hk * a.sk_h, a.sk_p, a.sk_s, a.ks + w.hk * a.ks_h, a.ks_p, near(a.sk_s)};
   const TileSource vs{a.v + w.hk * a.sv_h, a.sv_p, a.sv_s, a.vs + w.hk * a.vs_h, a.vs_p, near(a.sv_s)};
   TilePages pg{a.table + w.b * a.table_b, a.by_page, a.pages, w.vis.len};

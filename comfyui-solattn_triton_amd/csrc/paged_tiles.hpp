@@ -33,7 +33,7 @@ struct TileSource {
   int64_t page, slot;
   const uint8_t* e;  // codes: exponents
   int64_t e_page;
-  bool near;         // a few slots are within 32 bits
+  bool near;         // strides are within 32 bits, and a few slots
 };
 
 // Where a tile's keys are, a lane each: rows' addresses and, of codes, their powers of two.
@@ -79,7 +79,13 @@ struct TilePages {
 
 // A key's row, of page `id` (-1: a row of zeros).
 __device__ __forceinline__ TileRows row_at(const TileSource& s, int id, uint32_t slot) {
-  const uint64_t at = id >= 0 ? reinterpret_cast<uint64_t>(s.p) + id * s.page + slot * s.slot : reinterpret_cast<uint64_t>(zero_row);
+  uint64_t at = reinterpret_cast<uint64_t>(s.p);
+  if (s.near)
+    at += static_cast<uint64_t>(static_cast<uint32_t>(id)) * static_cast<uint32_t>(s.page) +
+          static_cast<uint64_t>(slot) * static_cast<uint32_t>(s.slot);
+  else
+    at += id * s.page + slot * s.slot;
+  at = id >= 0 ? at : reinterpret_cast<uint64_t>(zero_row);
   return {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32), 0.f};
 }
 
@@ -308,16 +314,22 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
   st.l = 0.f;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt) st.acc[dt] = f32x16{};
-  const auto rows = [&](int t, const TileSource& s, uint64_t& seen) __attribute__((always_inline)) {
-    t = min(t, ntiles - 1);
-    const int j = first + kKeys * t + lane;
-    const uint32_t page = pg.by_page.of(static_cast<uint32_t>(j));
-    const uint32_t slot = static_cast<uint32_t>(j) - page * pg.by_page.d;
+  // Where this lane's key of tile t is (t may pass the last tile: nothing is read there). The
+  // ids come from LDS, so a tile's are asked for a round before its rows' places are needed.
+  struct Key {
+    int id;
+    uint32_t slot;
+  };
+  const auto key_of = [&](int t) __attribute__((always_inline)) {
+    const uint32_t j = min(static_cast<uint32_t>(first + lane) + kKeys * t, static_cast<uint32_t>(pg.end));
+    const uint32_t page = pg.by_page.of(j);
     const int sg = t / kIdTiles;
-    int id = lds.ids[sg & 1][min(static_cast<int>(page) - pg.page0(first, sg), kIds - 1)];
-    id = j < pg.end ? id : -1;
-    seen = __ballot(id >= 0);
-    return row_at(s, id, slot);
+    const uint32_t i = page - pg.page0(first, sg);
+    return Key{lds.ids[sg & 1][min(i, static_cast<uint32_t>(kIds - 1))], j - page * pg.by_page.d};
+  };
+  const auto seen_of = [&](Key& k, int t) __attribute__((always_inline)) {
+    k.id = static_cast<uint32_t>(first + lane) + kKeys * t < static_cast<uint32_t>(pg.end) ? k.id : -1;
+    return __ballot(k.id >= 0);
   };
   const auto mask = [&](f32x16& s, int t, int hf, uint64_t seen) __attribute__((always_inline)) {
     mask_half(s, first + kKeys * t + 32 * hf, static_cast<uint32_t>(seen >> (32 * hf)), hi, safe);
@@ -326,17 +338,21 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
   tile_barrier();
   // Round t copies the second half of tile t + 2 and the first of t + 3 for K, of t + 1 and
   // t + 2 for V.
-  uint64_t s0w, s1w, s2w, s3w, unused;  // visible keys of the tiles t, t + 1, t + 2, t + 3
+  uint64_t s0w, s1w, s2w, s3w;  // visible keys of the tiles t, t + 1, t + 2, t + 3
   TileRows k2, k3, v1, v2;
+  Key key2, key3;
   {
-    const TileRows k0 = rows(0, ks, s0w), k1 = rows(1, ks, s1w), v0 = rows(0, vs, unused);
+    Key key0 = key_of(0), key1 = key_of(1);
+    key2 = key_of(2), key3 = key_of(3);
+    s0w = seen_of(key0, 0), s1w = seen_of(key1, 1), s2w = seen_of(key2, 2);
+    const TileRows k0 = row_at(ks, key0.id, key0.slot), k1 = row_at(ks, key1.id, key1.slot), v0 = row_at(vs, key0.id, key0.slot);
     kc.start(kb, 0, s0w, k0, ks);
     kc.start(kb + kHalf, 1, s0w, k0, ks);
     if (ntiles > 1) kc.start(kb + 2 * kHalf, 0, s1w, k1, ks);
     vc.start(vb, 0, s0w, v0, vs);
     if (ntiles > 1) kc.start(kb + 3 * kHalf, 1, s1w, k1, ks);
     vc.start(vb + kHalf, 1, s0w, v0, vs);
-    k2 = rows(2, ks, s2w), v1 = rows(1, vs, unused);
+    k2 = row_at(ks, key2.id, key2.slot), v1 = row_at(vs, key1.id, key1.slot);
   }
   // All but the newest two steps' copies are there; near the end, where steps ask for
   // fewer, all are.
@@ -379,7 +395,9 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
   for (; t < ntiles - 1; ++t) {
     if (t % kIdTiles == kIdTiles / 2 && (t / kIdTiles + 1) * kIdTiles < ntiles) pg.fetch_ids(lds.ids, first, t / kIdTiles + 1);
     const uint32_t a0 = (t & 1) * 2 * kHalf, b0 = 2 * kHalf - a0;  // halves 2 t and 2 t + 2 of the rings
-    k3 = rows(t + 3, ks, s3w), v2 = rows(t + 2, vs, unused);
+    const Key key4 = key_of(t + 4);
+    s3w = seen_of(key3, t + 3);
+    k3 = row_at(ks, key3.id, key3.slot), v2 = row_at(vs, key2.id, key2.slot);
     if (t + 2 < ntiles) kc.start(kb + a0 + kHalf, 1, s2w, k2, ks);  // step 2 t + 1
     vc.start(vb + b0 + kHalf, 1, s1w, v1, vs);
     window_step<E, D>(st, sb, sa, pa, pb, kl + b0, vl + a0, q, c);
@@ -390,7 +408,7 @@ __device__ __forceinline__ void attend_ring(RowState<D / 32>& st, const bf16x8 (
     window_step<E, D>(st, sa, sb, pb, pa, kl + b0 + kHalf, vl + a0 + kHalf, q, c);
     mask(sb, t + 1, 1, s1w);
     land(t);
-    k2 = k3, v1 = v2;
+    k2 = k3, v1 = v2, key2 = key3, key3 = key4;
     s1w = s2w, s2w = s3w;
   }
   const uint32_t a0 = (t & 1) * 2 * kHalf;
