@@ -771,10 +771,14 @@ Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t wind
   };
   // One workgroup a CU: 8 sequences of 24 heads behind 4100 keys 14 us, within two 15; behind
   // 32760 36 and 36. Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
-  // behind 32760 keys 62 against 70; 32 behind 4100 21 against 18), one and a half where own
-  // keys take the other places meanwhile (256 of up to 500 of their own 171 against 184).
+  // behind 32760 keys 62 against 70; 32 behind 4100 21 against 18), one and a half where
+  // enough own keys take the other places meanwhile. That is by what both take, own bytes
+  // against products: 256 sequences behind 32760 with up to 250 / 500 / 1000 of their own 163 /
+  // 171 / 219 us, within two 163 / 187 / 245; behind 131071 with 500 / 2000 564 / 616 and 522 /
+  // 645; over e4m3 with 500 196 and 190; 512 of 16 heads of 64 over 4 with 240 148 and 122.
   c.psplit = within(256);
-  if (tiled && steps >= 12 * within(512)) c.psplit = within(B * Hkv * c.tiles * c.split >= 1024 ? 384 : 512);
+  if (tiled && steps >= 12 * within(512))
+    c.psplit = within(150 * keys * (cache_type ? 1 : 2) > shared * (H / Hkv) ? 384 : 512);
   return c;
 }
 
