@@ -769,16 +769,23 @@ Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t wind
     n = n < 1 ? 1 : n > kMaxShared ? kMaxShared : n;
     return cdiv(steps, round * cdiv(steps, round * n));
   };
-  // One workgroup a CU: 8 sequences of 24 heads behind 4100 keys 14 us, within two 15; behind
-  // 32760 36 and 36. Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
+  // One workgroup a CU where two would leave a wave less than some four steps: 8 sequences of
+  // 24 heads behind 4100 keys 13.2 us, within two 15. Else two: 64 in four runs of 16 heads of
+  // 64 behind 8000 int8 / e4m3 / fp16 keys 22.5 / 21.4 / 22.4 us, within two 20.4 / 19.4 / 19.1;
+  // 16 behind 32760 int8 / bf16 keys 38 / 43 and 35 / 43; 64 in eight runs behind 4100 31 and
+  // 32. Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
   // behind 32760 keys 62 against 70; 32 behind 4100 21 against 18), one and a half where
   // enough own keys take the other places meanwhile. That is by what both take, own bytes
   // against products: 256 sequences behind 32760 with up to 250 / 500 / 1000 of their own 163 /
   // 171 / 219 us, within two 163 / 187 / 245; behind 131071 with 500 / 2000 564 / 616 and 522 /
   // 645; over e4m3 with 500 196 and 190; 512 of 16 heads of 64 over 4 with 240 148 and 122.
-  c.psplit = within(256);
-  if (tiled && steps >= 12 * within(512))
-    c.psplit = within(150 * keys * (cache_type ? 1 : 2) > shared * (H / Hkv) ? 384 : 512);
+  const int64_t two = within(512);
+  if (!tiled)
+    c.psplit = steps > 3 * kWaves * two ? two : within(256);
+  else if (steps < 12 * two)
+    c.psplit = within(256);
+  else
+    c.psplit = 150 * keys * (cache_type ? 1 : 2) > shared * (H / Hkv) ? within(384) : two;
   return c;
 }
 
