@@ -16,14 +16,14 @@
 //     238-251 us, 5.3-5.6 TB/s (a large copy reaches 5.0-5.15); 32 of 512 to 16384, 16
 //     heads of 64 over 4, pages of 16: 63 us; one sequence with a window of 4096: 10.2
 //     us, two launches of the host's (kernels 5.9 and 4.7).
-//   Codes: the four, e4m3: 138 us, 4.9 TB/s, kernel 134. The 32, int8: 39 us, 3.6 TB/s,
-//     kernel 31 and join 5; there the vector units are at 56-70%, with a byte's way to a
-//     16-bit float (two instructions a pair of e4m3, four of int8). One with a window of
-//     4096: 8.7 us, kernels 6.0 and 2.8.
+//   Codes: the four, e4m3: 138 us, 4.9 TB/s, kernel 134. The 32, int8: 38-39 us, 3.6 TB/s,
+//     kernel 29-33 and join 5 (the vector units, 60% busy with a byte's way to a 16-bit
+//     float, are not what it waits for: fewer of their instructions, or sequences of one
+//     length, took as long). One with a window of 4096: 8.9 us, kernels 6.0 and 2.7.
 //   Shared keys: 8 sequences of 24 heads over 8 behind 4096 bf16 keys: 13 us (22 as if
 //     nothing was shared), latency: 10.6 of it the kernel, a chain of lengths, page ids,
-//     keys and steps, and 2-4 the join. 64 in groups over int8: 21 us (48), the
-//     conversions again. 256 behind 32760 bf16 keys: 172 us (2600), products.
+//     keys and steps, and 2-4 the join. 64 in groups over int8: 19-20 us (48), latency
+//     beside the conversions. 256 behind 32760 bf16 keys: 167 us (2600), products.
 // A wave takes 32 keys at a time straight from HBM into operand registers, no LDS:
 //   S^T = K Q^T (v_mfma_f32_16x16x32): row r of tile t is key 8 (r/4) + 4 t + r%4
 //     of the 32, so lane (q, g) = (lane % 16, lane / 16) gets the scores of the
@@ -773,7 +773,8 @@ Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t wind
   // 24 heads behind 4100 keys 13.2 us, within two 15. Else two: 64 in four runs of 16 heads of
   // 64 behind 8000 int8 / e4m3 / fp16 keys 22.5 / 21.4 / 22.4 us, within two 20.4 / 19.4 / 19.1;
   // 16 behind 32760 int8 / bf16 keys 38 / 43 and 35 / 43; 64 in eight runs behind 4100 31 and
-  // 32. Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
+  // 32. One again for more columns of other head dims than 64 and 128 (192 of 96 channels
+  // behind 8000 35 us, within two 38). Tiles: two where that leaves each twelve tiles (64 sequences of 24 heads
   // behind 32760 keys 62 against 70; 32 behind 4100 21 against 18), one and a half where
   // enough own keys take the other places meanwhile. That is by what both take, own bytes
   // against products: 256 sequences behind 32760 with up to 250 / 500 / 1000 of their own 163 /
@@ -781,7 +782,7 @@ Cut cut(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t keys, int64_t wind
   // 645; over e4m3 with 500 196 and 190; 512 of 16 heads of 64 over 4 with 240 148 and 122.
   const int64_t two = within(512);
   if (!tiled)
-    c.psplit = steps > 3 * kWaves * two ? two : within(256);
+    c.psplit = cols <= 4 * kGroups && steps > 3 * kWaves * two ? two : within(256);
   else if (steps < 12 * two)
     c.psplit = within(256);
   else

@@ -5,8 +5,9 @@
 //
 // Bound: the matrix instructions, 4 D operations a row and key, beside the exponentials of
 // the scores. 256 sequences of 24 heads over 8, of 128 channels, behind 32760 keys alone:
-// 16-bit values 146 us, 0.70 PFLOP/s (0.9-0.97 between the first tile's latency and the
-// parts' way out); e4m3 173, whose conversions stand between the products.
+// 16-bit values 143 us, 0.72 PFLOP/s (0.95 between the first tile's latency and the parts'
+// way out: behind 131071 keys 467 us, matrix instructions in 39% of the cycles, vector ones
+// in 43%, either in 63%); e4m3 some 10% more, whose conversions stand between the products.
 //
 // What differs from the windowed forward is where keys come from: a lane finds the place of
 // one key of a tile of 64 well ahead of its copy, and the copies of a half (rows of eight

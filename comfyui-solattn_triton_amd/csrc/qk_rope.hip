@@ -12,8 +12,8 @@
 //
 // Bound: HBM; for a few tokens the launch. 32760 tokens of 24 + 24 heads of 128
 // channels, bf16: 156 us, 5.25 TB/s (a large copy reaches 5.0-5.15); 16004 tokens of 24
-// heads over 8 into int8 pages: 61 us, 4.9 TB/s, 13% of the lanes' time in vector
-// instructions; one token of each of
+// heads over 8 into int8 pages: 61 us, 4.9 TB/s, vector
+// instructions in 57% of the cycles; one token of each of
 // four sequences into its pages: 7 us a call (the host's), the kernel 4.9; gradients of 8200
 // tokens of 16 + 4 heads of 64, fp16: 17 us and 4.9 for the weights' join, 3.7 TB/s.
 // A lane holds 8 channels, so a row is LPR = 16 lanes (8 up to 64
