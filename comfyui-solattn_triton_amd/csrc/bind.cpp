@@ -640,8 +640,9 @@ Tensor paged_attn(const Tensor& q0, const Tensor& k, const Tensor& v, const Tens
   const Tensor ks = tensor(k_scale), vs = tensor(v_scale);
   check(lib.paged_attn_shared(
             ptr_as<U16>(q), q.stride(0), q.stride(2), ptr(k), STRIDES(k), ptr(v), STRIDES(v), pages, page, cache_type,
-            SCALES(ks), SCALES(vs), ptr_as<int32_t>(table), table.stride(0), max_pages, ptr_as<int32_t>(lengths), B, H, Hkv, D, type_code(q), w, sinks, shared, groups,
-            static_cast<float>(scale), ptr(ws), need, ptr_as<U16>(out), out.stride(0), out.stride(2), stream_of(q)),
+            SCALES(ks), SCALES(vs), ptr_as<int32_t>(table), table.stride(0), max_pages, ptr_as<int32_t>(lengths), B, H,
+            Hkv, D, type_code(q), w, sinks, shared, groups, static_cast<float>(scale), ptr(ws), need, ptr_as<U16>(out),
+            out.stride(0), out.stride(2), stream_of(q)),
         "solattn_paged_attn");
   return out;
 }

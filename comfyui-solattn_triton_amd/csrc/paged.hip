@@ -899,7 +899,10 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
     a.psplit = static_cast<int>(c.psplit), a.ptiles = static_cast<int>(c.ptiles), a.pitems = static_cast<int>(items);
     a.by_ptiles = divisor(c.ptiles), a.by_psplit = divisor(c.psplit), a.by_group = divisor(a.group);
   }
-  SOLATTN_REQUIRE(grid < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
+  const bool wide = p.cache_type != 0 || p.shared != 0;  // (the others keep their order of sums)
+  constexpr int64_t most = (1ll << 32) / (kWaves * 64);  // (a launch has less than 2^32 threads)
+  static_assert(kJoinThreads == kWaves * 64, "one bound");
+  SOLATTN_REQUIRE(grid < most && (!wide || B * H < most), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   // More workgroups than are there at once: those of the longest sequences first, so that none
   // of theirs begin when the others end (32 ragged sequences of bf16 keys 69 -> 63 us, eight
   // over e4m3 72 -> 66, four of up to 131072 144 -> 138).
@@ -909,7 +912,7 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(grid)), dim3(kWaves * 64), 0, s, a);
   if (int rc = check_launch(what)) return rc;
   if (a.parts == 1) return SOLATTN_OK;
-  if (p.cache_type == 0 && p.shared == 0) {  // (the order of sums of the calls without codes and shared keys)
+  if (!wide) {
     hipLaunchKernelGGL(bf ? paged_join_kernel<Bf16> : paged_join_kernel<Fp16>,
                        dim3(static_cast<uint32_t>(cdiv(B * H, 4))), dim3(256), 0, s, a);
     return check_launch(what);
