@@ -9,8 +9,9 @@ Probe" measures per-block error, ``attention_sol`` is registered as
 The kernel-level API (``sol_attn``, ``sol_attn_int8``, ``prepare``,
 ``fused_preprocess``, ``quantize_bthd``, ``quantize_v_per_channel``,
 ``morton_perm``; beside the sparse path ``qk_norm_rope``, ``qk_norm_rope_append``,
-``window_attn`` and ``paged_attn``) lives in the submodules and needs no ComfyUI; the
-node layer below is defined when ComfyUI is importable.
+``window_attn``, ``paged_attn``, ``cache_append`` and ``cache_read``) lives in the
+submodules and needs no ComfyUI; the node layer below is defined when ComfyUI is
+importable.
 """
 
 import logging
