@@ -4,12 +4,12 @@
 // Bound: HBM; for a few tokens the launch and three dependent rounds of memory (length,
 // page id, row). A lane holds 8 channels, a row is LPR = 16 lanes (8 up to 64 channels), so
 // that the largest magnitude is four lane moves away and a row needs no second pass; k's and
-// v's rows of the same place are worked on together and share the page's id. One row a lane
-// group and no loop: the launch has thousands of workgroups where bandwidth counts, and one
-// round where latency does.
+// v's rows of the same place are worked on together and share the page's id. One or two rows a
+// lane group and no loop: the launch has thousands of workgroups where bandwidth counts, and
+// one round where latency does.
 //   Append, 12133 tokens of 24 heads of 128, bf16 to e4m3: 46-48 us, 4.7-4.9 TB/s (a large
 //   copy reaches 5.15); two chunks of 1000, 4 heads of 64: 2.8-3.5 us.
-//   Read, four sequences of up to 32760 tokens, 8 heads of 128, e4m3 to bf16: 133-146 us, 4.8-5.3 TB/s; the
+//   Read, four sequences of up to 32760 tokens, 8 heads of 128, e4m3 to bf16: 134 us, 5.3 TB/s; the
 //   last 1333 of eight, 4 heads of 64: 5.3-5.7 us.
 #include "cache8.hpp"
 
@@ -76,26 +76,46 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const CacheArgs 
   put_row<E, C, LPR>(a, a.v, a.vc, p, l, active);
 }
 
-template <typename E, typename C>
-__device__ __forceinline__ void get_row(const Rows& dst, const CodePages& from, const Place& p, int l) {
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (p.page >= 0) {
-    const uint2 c = *reinterpret_cast<const uint2*>(from.codes + p.page * from.p + p.slot * from.s + p.h * from.h + 8 * l);
-    const float power = power_of(from.exps[p.page * from.ep + p.h * from.eh + p.slot]);
-    w = make_uint4(C::template scaled<E>(c.x, 0, power), C::template scaled<E>(c.x, 2, power),
-                   C::template scaled<E>(c.y, 0, power), C::template scaled<E>(c.y, 2, power));
-  }
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst.p) + p.b * dst.b + p.t * dst.t + p.h * dst.h + 8 * l) = w;
-}
-
+// Two rows of k and of v a lane group, whose loads are all on their way before the first
+// store (four sequences of up to 32760 e4m3 tokens: a row of k, then one of v 144 us, one of
+// both 136, two of both 134, four 141).
+constexpr int kReadRows = 2;
 template <typename E, typename C, int LPR>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheArgs a) {
+  constexpr int G = 64 / LPR;  // rows of a wave's access
   const int l = threadIdx.x & (LPR - 1);
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
-  if (row >= a.rows || 8 * l >= a.D) return;
-  const Place p = place(a, row, false);
-  get_row<E, C>(a.k, a.kc, p, l);
-  get_row<E, C>(a.v, a.vc, p, l);
+  if (8 * l >= a.D) return;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  const int64_t row = wave * (G * kReadRows) + (threadIdx.x & 63) / LPR;
+  Place p[kReadRows];
+#pragma unroll
+  for (int u = 0; u < kReadRows; ++u) p[u] = place(a, min(row + u * G, a.rows - 1), false);
+  uint2 kc[kReadRows], vc[kReadRows];
+  float kp[kReadRows], vp[kReadRows];
+#pragma unroll
+  for (int u = 0; u < kReadRows; ++u) {
+    kc[u] = vc[u] = make_uint2(0, 0), kp[u] = vp[u] = 0.f;
+    if (p[u].page < 0) continue;
+    const auto codes = [&](const CodePages& from) {
+      return *reinterpret_cast<const uint2*>(from.codes + p[u].page * from.p + p[u].slot * from.s + p[u].h * from.h + 8 * l);
+    };
+    const auto power = [&](const CodePages& from) {
+      return power_of(from.exps[p[u].page * from.ep + p[u].h * from.eh + p[u].slot]);
+    };
+    kc[u] = codes(a.kc), vc[u] = codes(a.vc);
+    kp[u] = power(a.kc), vp[u] = power(a.vc);
+  }
+#pragma unroll
+  for (int u = 0; u < kReadRows; ++u) {
+    if (row + u * G >= a.rows) return;
+    const auto put = [&](const Rows& dst, const uint2& c, float power) {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst.p) + p[u].b * dst.b + p[u].t * dst.t + p[u].h * dst.h + 8 * l) =
+          make_uint4(C::template scaled<E>(c.x, 0, power), C::template scaled<E>(c.x, 2, power),
+                     C::template scaled<E>(c.y, 0, power), C::template scaled<E>(c.y, 2, power));
+    };
+    put(a.k, kc[u], kp[u]);
+    put(a.v, vc[u], vp[u]);
+  }
 }
 
 int setup(CacheArgs& a, int64_t B, int64_t T, int64_t Hkv, int64_t D, int dtype, bool fp32, int64_t pages,
@@ -193,7 +213,7 @@ extern "C" int solattn_cache_read(const void* k_cache, int64_t skc_p, int64_t sk
   const bool wide = D > 64;
   const auto kern = dtype == SOLATTN_BF16 ? SOLATTN_BY_CODES(cache_read_kernel, Bf16, cache_type, wide)
                                           : SOLATTN_BY_CODES(cache_read_kernel, Fp16, cache_type, wide);
-  const int64_t blocks = cdiv(a.rows, kThreads / (wide ? 16 : 8));
+  const int64_t blocks = cdiv(a.rows, kReadRows * (kThreads / (wide ? 16 : 8)));
   hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), a);
   return check_launch("cache_read");
 }
