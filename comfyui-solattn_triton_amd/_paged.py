@@ -34,8 +34,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ``groups``, for each run of B / groups sequences. They are read once for a run, from
     the pages of its longest sequence (the first of these); the others' pages for them are
     not looked at, so their tables may name the same pages or copies. A sequence may be
-    shorter (an idle slot's length 0); a NaN or infinity in ``v`` at a shared key behind
-    its end can reach it then, if it is not empty. Not together with a window or sinks.
+    shorter than ``shared`` (an idle slot's length 0): it sees its own keys of them. Not
+    together with a window or sinks.
     """
     return native.paged_attn(q, k_cache, v_cache, page_table, lengths, window, sinks, scale, k_scale, v_scale, shared,
                              groups)

@@ -8,7 +8,10 @@
 // Sequences may have their first keys in common (`shared` of them, runs of `per`
 // sequences): the heads of all of a run are then the columns of these keys, which
 // are read once for 16 columns, for 32, or for 128 (paged_tiles.hpp), and what is
-// behind them is attended as before, in the same launch; the join takes both.
+// behind them is attended as before, in the same launch; the join takes both. A column sees
+// a part of the shared keys whole or not at all: of a sequence that ends inside a part, what it
+// has of that part is with its own keys. (One product for all columns would take 0 times what
+// is behind its end, and that may be a NaN or an infinity that another sequence does see.)
 //
 // Bound: HBM, 2 Hkv D values a visible key; the matrix instructions do 16 query
 // columns whether they exist or not, 256 of their cycles for 16 KiB of a 16-bit cache.
@@ -194,6 +197,15 @@ __device__ __forceinline__ void longest(const PagedArgs& a, int first, int& b, i
   len = __builtin_amdgcn_readfirstlane(top);
 }
 
+// Steps of a part of `keys` shared ones.
+template <bool TILED>
+__device__ __forceinline__ int shared_part(const PagedArgs& a, int keys) {
+  constexpr int S = TILED ? kKeys : kStep;
+  return a.by_psplit.of((keys + S - 1) / S + a.psplit - 1);
+}
+// Of a column with `len` keys: how many of the keys that the part ends with (`end`) it may see, all or none.
+__device__ __forceinline__ int sees(int len, int end) { return len >= end ? INT32_MAX : 0; }
+
 // A workgroup's keys and columns. The columns of own keys are the heads of one sequence
 // that share a kv head, those of shared keys the heads of all its sequences.
 struct Work {
@@ -215,7 +227,7 @@ __device__ __forceinline__ void shared_steps(const PagedArgs& a, Work& w, int b,
   w.b = b;
   w.vis = visible(keys, 0, 0);
   if constexpr (TILED) w.vis.steps = (keys + kKeys - 1) / kKeys;
-  const int per = a.by_psplit.of(w.vis.steps + a.psplit - 1);
+  const int per = shared_part<TILED>(a, keys);
   w.step0 = w.part * per, w.step1 = min(w.step0 + per, w.vis.steps);
 }
 // What shared keys mostly are: all of them, on the first sequence's pages. The first page
@@ -262,7 +274,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
   // Channels of product cc that this lane holds of q and of a key: eight from
   // 32 cc + 8 g on, of codes, read 16 bytes at a time, from 64 (cc / 2) + 16 g + 8 (cc % 2).
   bf16x8 q[NT][NC];
-  int hi[NT];  // MANY: keys that a column sees
+  int hi[NT];  // MANY: the sequence's length, then keys of the part that the column sees
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     int b, h;
@@ -318,9 +330,10 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
       if (w.step0 + wave < w.step1) find(w.step0 + wave);
     }
     safe = vis.len;
+    const int end = min(w.step1 * S, vis.len);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      hi[t] = min(hi[t], vis.len);
+      hi[t] = sees(hi[t], end);
       safe = min(safe, hi[t]);
     }
     safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
@@ -559,7 +572,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Wo
       if constexpr (!kCodes<C>) pg.fetch_ids(ring.ids, w.step0 * kKeys, 0);
     }
   }
-  hi = min(hi, w.vis.len);
+  hi = sees(hi, min(w.step1 * kKeys, w.vis.len));
   const int safe = __builtin_amdgcn_readfirstlane(static_cast<int>(
       over_wave(static_cast<uint32_t>(hi), [](uint32_t x, uint32_t y) { return min(x, y); })));
   RowState<D / 32> st;
@@ -635,7 +648,17 @@ paged_kernel(const PagedArgs a) {
   w.col0 = tile * kGroups;
   w.ncol = min(kGroups, a.group - w.col0);
   const int len = sequence_length(a, w.b);
-  w.vis = visible(len, PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0, PT > 0 ? 0 : a.sinks);
+  int low = PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0;
+  if constexpr (PT > 0) {
+    if (len > 0 && len < all_shared(a)) {  // from where the part begins that it ends in, on the pages of the longest
+      int best, top;
+      longest(a, w.seq - w.seq % a.per, best, top);
+      const int keys = min(top, all_shared(a)), part = shared_part<TILED>(a, keys) * (TILED ? kKeys : kStep);
+      low = len < keys ? len - len % part : len;
+      w.b = best;
+    }
+  }
+  w.vis = visible(len, low, PT > 0 ? 0 : a.sinks);
   const int per = a.by_split.of(w.vis.steps + a.split - 1);
   w.step0 = split * per, w.step1 = min(w.step0 + per, w.vis.steps);
   if (w.step0 >= w.step1 && a.parts > 1)

@@ -537,8 +537,8 @@ int solattn_cache_read(const void* k_cache, int64_t skc_p, int64_t skc_s, int64_
  * whose sequences have keys in common: of each of `groups` runs of B / groups sequences
  * the first `shared` keys are the same, and are read once, from the pages of the run's
  * longest sequence (the first of these); the other sequences' pages for them are not
- * looked at. With shared > 0: no window. A NaN or infinity in v at a key behind the end
- * of a sequence that is shorter than `shared` (but not empty) can reach it. */
+ * looked at; a sequence that is shorter than `shared` sees lengths[b] of them. With
+ * shared > 0: no window. */
 int64_t solattn_paged_attn_shared_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
                                             int64_t page_size, int64_t window, int64_t sinks,
                                             int cache_type, int64_t shared, int64_t groups);

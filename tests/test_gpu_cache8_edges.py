@@ -1,0 +1,135 @@
+"""What the 8-bit cache and attention over shared keys do at their edges: values that a
+sequence must not see, values beyond fp16's range, runs that are shorter than the shared
+keys, wide tables and far pages. Bounds and references as in test_gpu_cache8.py."""
+
+import importlib
+
+import pytest
+import torch
+
+import _cache8 as c8
+import _operators as ref
+
+pytestmark = pytest.mark.gpu
+
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+I8, F8 = c8.KINDS
+CODES = pytest.mark.parametrize("kind", c8.KINDS, ids=["int8", "e4m3"])
+KINDS = pytest.mark.parametrize("kind", [None] + c8.KINDS, ids=["same", "int8", "e4m3"])
+
+
+@pytest.fixture(scope="module")
+def rope(pkg):
+    return importlib.import_module(f"{pkg.__name__}._qk_rope")
+
+
+@pytest.fixture(scope="module")
+def paged(pkg):
+    return importlib.import_module(f"{pkg.__name__}._paged")
+
+
+@pytest.fixture(scope="module")
+def cache(pkg):
+    return importlib.import_module(f"{pkg.__name__}._cache")
+
+
+def randn(shape, seed, dev, dtype=BF, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(dev)
+
+
+def ints(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def raw(t):
+    return t.view(torch.uint8)
+
+
+class Pages:
+    """Rows k, v [B, L, Hkv, D] (fp32) in scattered pages, of `kind` (None: of dtype); at:
+    whose rows a sequence's are. k, v become what the cache holds, in float64."""
+
+    def __init__(self, k, v, at, page, kind, dtype, wide=0):
+        dev, (B, L, Hkv, D) = k.device, k.shape
+        self.most = -(-L // page) + wide
+        self.table = c8.tables(B, self.most, dev, seed=L)[torch.as_tensor(at, device=dev)]
+        own = c8.tables(B, self.most, dev, seed=L)
+        self.scales, out = {}, []
+        for name, x in (("k", k), ("v", v)):
+            x = torch.nn.functional.pad(x, (0, 0, 0, 0, 0, self.most * page - L))
+            if kind is None:
+                c, e, x = x.to(dtype), None, x.to(dtype).double()
+                held = torch.empty(B * self.most, page, Hkv, D, dtype=dtype, device=dev)
+                held[own.long().flatten()] = c.reshape(B * self.most, page, Hkv, D)
+            else:
+                c, e = c8.encode(x, kind)
+                x = c8.values(c, e)
+                held, s = c8.empty(B * self.most, page, Hkv, D, kind, dev)
+                raw(held)[own.long().flatten()] = raw(c).reshape(B * self.most, page, Hkv, D)
+                raw(s)[own.long().flatten()] = e.reshape(B * self.most, page, Hkv).transpose(1, 2)
+                self.scales[f"{name}_scale"] = s
+            setattr(self, name, held)
+            out.append(x[torch.as_tensor(at, device=dev)][:, :L])
+        self.rows = out
+
+    def attn(self, paged, q, n, **kw):
+        return paged.paged_attn(q, self.k, self.v, self.table, n, **self.scales, **kw)
+
+
+def seen(n, L):
+    return (torch.arange(L, device=n.device) < n[:, None])[:, None]
+
+
+def bound(kind, o, p, v, dtype, columns, D):
+    """P is rounded once over 16-bit pages and over tiles (more than 64 columns), else kept in two parts."""
+    once = kind is None or (columns > 64 and D in (64, 128))
+    return (ref if once else c8).forward_bound(o, p, v, dtype)
+
+
+# ------------------------------------------------------ keys behind a sequence's end
+# run's lengths, shared, groups, H, Hkv, D, page, dtype: 2 and 15 columns, two tiles of 16, more than 64 by tiles
+# of 128 rows or, of other head dims, by tiles of 32
+ENDS = [
+    ([320, 1, 0, 290, 289, 64, 96], 290, 1, 2, 1, 128, 16, BF),
+    ([1200, 1000, 999, 513, 512, 511, 128], 1000, 1, 12, 4, 64, 24, FP),
+    ([100, 2100, 2000, 1990, 1024, 7, 2000, 1536], 2000, 2, 24, 8, 128, 64, BF),
+    ([3000, 2900, 2048, 2047, 2049, 64, 0, 1], 2900, 1, 32, 2, 128, 64, BF),
+    ([640, 641, 700, 63, 64, 65, 127, 128, 129, 320], 641, 1, 16, 2, 64, 8, FP),
+    ([900, 850, 33, 450], 850, 1, 40, 2, 96, 16, BF),
+    ([500, 499, 64, 500, 0], 2000, 1, 40, 2, 128, 16, BF),
+]
+
+
+@KINDS
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")], ids=["nan", "inf"])
+@pytest.mark.parametrize("case", ENDS, ids=[str(i) for i in range(len(ENDS))])
+def test_shared_keys_behind_the_end_of_a_sequence(paged, dev, kind, case, poison):
+    """NaN or infinities in shared rows that a sequence does not have do not reach it, in k or in v: the
+    sequences that end before them are exact, the others NaN or infinite."""
+    run, shared, groups, H, Hkv, D, page, dtype = case
+    lengths = run * groups
+    B, per, L = len(lengths), len(run), max(run)
+    q = randn((B, 1, H, D), 3, dev, dtype, 2.0)
+    k, v = (randn((B, L, Hkv, D), s, dev, F32) for s in (1, 2))
+    longest = run.index(L)
+    first = [b // per * per + longest for b in range(B)]
+    for x in (k, v):
+        x[:, :min(shared, L)] = x[first, :min(shared, L)]
+    n = ints(lengths, dev)
+    on = seen(n, L)
+    ends = sorted({m for m in run if 0 < m < min(shared, L)})
+    for bad in (ends[0], ends[len(ends) // 2], ends[-1]):  # the first key that one of the sequences does not have
+        for which in ("k", "v"):
+            kp, vp = k.clone(), v.clone()
+            (kp if which == "k" else vp)[:, bad, :, 3 % D] = poison
+            pages = Pages(kp, vp, range(B), page, kind, dtype)
+            print("[ends]", kind, case, poison, bad, which, flush=True)
+            got = pages.attn(paged, q, n, shared=shared, groups=groups)
+            safe = n <= bad
+            rows = [x.masked_fill(~on.transpose(1, 2)[..., None], 0).nan_to_num(0.0, 0.0, 0.0) for x in pages.rows]
+            o, p, (_, _, vh) = ref.attention(q, *rows, on, D ** -0.5)
+            tol = bound(kind, o, p, vh, dtype, per * (H // Hkv), D)
+            ref.close(got[safe], o[safe], tol[safe], "sequences that end before it")
+            if which == "v":  # (an infinity in k may be a score of minus infinity)
+                assert not torch.isfinite(got[~safe]).flatten(1).all(1).any()
