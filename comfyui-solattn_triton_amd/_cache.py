@@ -4,12 +4,13 @@ half the memory and half the reads of a 16-bit one. No counterpart in the refere
 k_cache, v_cache: codes [pages, page_size, Hkv, D] of ``torch.int8`` or
 ``torch.float8_e4m3fn``; k_scale, v_scale: ``torch.float8_e8m0fnu`` [pages, Hkv,
 page_size], a power of two for each row. A cached value is ``code * scale``, which bf16
-holds exactly, and fp16 within its range (a call with fp16 queries, or a read in fp16, may
-round values below 2^-14, and makes those from 65520 on infinities). Of a written row the scale is the smallest power of two that keeps its
-largest magnitude within 127 (int8) or 448 (e4m3) codes, the codes are the nearest (ties
-to even): int8 is off by at most 1/127 of the row's largest value, e4m3 by 1/16 of each
-value or 2^-17 of the row's largest. Rows below 2^-110 become zeros; a
-row with a NaN or an infinity reads as NaN throughout.
+holds exactly, and fp16 within its range: a read in fp16, and a call with fp16 queries over
+keys that sequences share, may round values below 2^-14; a read makes those from 65520 on
+infinities, a call takes them as they are. Of a written row the scale is the smallest power
+of two that keeps its largest magnitude within 127 (int8) or 448 (e4m3) codes, the codes are
+the nearest (ties to even): int8 is off by at most 1/127 of the row's largest value, e4m3 by
+1/16 of each value or 2^-17 of the row's largest. Rows below 2^-110 become zeros; a row with
+a NaN or an infinity reads as NaN throughout.
 
 Written here or, with norms and rotation in the same pass, by
 ``_qk_rope.qk_norm_rope_append``; attended by ``_paged.paged_attn``, or read back for

@@ -86,6 +86,7 @@ __device__ __forceinline__ void put_codes(const float (&x)[8], const CodePages& 
 struct Int8Codes {
   static constexpr uint32_t kPast = 0x01FFFFu;  // 0x800000 - 0x7E0000 - 1
   static constexpr int kShift = 6;
+  static constexpr uint32_t kFp16Byte = 127 + 8;  // fp16 holds 128 2^8, not 128 2^9
   // Eight values times the row's unit as codes; bad: the row holds a NaN or an infinity.
   static __device__ __forceinline__ uint2 encode(const float (&x)[8], float unit, bool bad) {
     uint32_t w[2];
@@ -122,6 +123,7 @@ struct Int8Codes {
 struct Fp8Codes {
   static constexpr uint32_t kPast = 0x1FFFFFu;  // 0x800000 - 0x600000 - 1
   static constexpr int kShift = 8;
+  static constexpr uint32_t kFp16Byte = 127 + 7;  // fp16 holds 448 2^7, not 448 2^8
   static __device__ __forceinline__ uint2 encode(const float (&x)[8], float unit, bool bad) {
     uint32_t w[2];
 #pragma unroll

@@ -254,9 +254,10 @@ __device__ __forceinline__ void no_keys(const PagedArgs& a, const Work& w) {
 }
 
 // DP: the head dim that the registers hold; D < DP (kFull false) leaves the rest zero.
-// NT: tiles of 16 columns. MANY: the columns are of several sequences.
+// NT: tiles of 16 columns. MANY: the columns are of several sequences; found: w has the longest
+// one's pages and steps already.
 template <typename E, typename C, int DP, bool kFull, int NT, bool MANY>
-__device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Work& w) {
+__device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Work& w, bool found = false) {
   constexpr bool Q8 = kCodes<C>;
   constexpr int S = kStep;
   constexpr int NC = DP / 32;           // products of a score tile
@@ -322,12 +323,14 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
   if (w.step0 + wave < w.step1) find(w.step0 + wave);
   int safe = 0;  // MANY: keys that every column sees
   if constexpr (MANY) {
-    int b, len;
-    longest(a, w.seq, b, len);
-    if (b != w.seq || len < vis.len) {
-      shared_steps<false>(a, w, b, min(len, vis.len));
-      if (w.step0 >= w.step1) return no_keys<true>(a, w);
-      if (w.step0 + wave < w.step1) find(w.step0 + wave);
+    if (!found) {
+      int b, len;
+      longest(a, w.seq, b, len);
+      if (b != w.seq || len < vis.len) {
+        shared_steps<false>(a, w, b, min(len, vis.len));
+        if (w.step0 >= w.step1) return no_keys<true>(a, w);
+        if (w.step0 + wave < w.step1) find(w.step0 + wave);
+      }
     }
     safe = vis.len;
     const int end = min(w.step1 * S, vis.len);
@@ -545,7 +548,37 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
   }
 }
 
-// The same for 128 columns of several sequences, by tiles in LDS: steps of 64 keys.
+// Whether fp16 holds the largest values of codes of a part's keys [first, end). Two bytes a key
+// and two rounds of memory in front of the first tile: 256 fp16 sequences of 24 heads behind
+// 32760 int8 keys 204 -> 197 us, of 16 heads of 64 behind 8000 of e4m3 42.1 -> 42.5. Where one
+// page of these is beyond fp16 they take 307 and 55.
+template <typename C>
+__device__ __forceinline__ bool fp16_holds(const PagedArgs& a, const Work& w, uint32_t* any, int first, int end) {
+  bool over = false;
+  for (int j = first + 8 * static_cast<int>(threadIdx.x); j < end; j += 8 * kWaves * 64) {
+    const uint32_t pg = a.by_page.of(static_cast<uint32_t>(j));
+    const int64_t slot = j - static_cast<int64_t>(pg) * a.page, id = a.table[w.b * a.table_b + pg];
+    if (id < 0 || id >= a.pages) continue;
+    const uint2 k = *reinterpret_cast<const uint2*>(a.ks + w.hk * a.ks_h + id * a.ks_p + slot);
+    const uint2 v = *reinterpret_cast<const uint2*>(a.vs + w.hk * a.vs_h + id * a.vs_p + slot);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t kb = (i < 4 ? k.x : k.y) >> (8 * (i & 3)) & 0xFFu, vb = (i < 4 ? v.x : v.y) >> (8 * (i & 3)) & 0xFFu;
+      over = over || (j + i < end && max(kb, vb) > C::kFp16Byte);
+    }
+  }
+  any[wave_id()] = __any(over);
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) all |= any[i];
+  __syncthreads();  // (the LDS is the tiles')
+  return all == 0;
+}
+
+// The same for 128 columns of several sequences, by tiles in LDS: steps of 64 keys. Codes
+// become values of the queries' type there, which fp16 may not hold: a part that has such keys
+// goes as fewer columns do, where the powers stay apart, 32 columns at a time.
 constexpr int kTiled = kTileRows / kGroups;  // its tiles of columns
 template <typename E, typename C, int D>
 __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Work& w) {
@@ -570,6 +603,20 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, uint8_t* lds, Wo
       if (w.step0 >= w.step1) return no_keys<true>(a, w);
       pg.table = a.table + w.b * a.table_b, pg.end = w.vis.len;
       if constexpr (!kCodes<C>) pg.fetch_ids(ring.ids, w.step0 * kKeys, 0);
+    }
+  }
+  if constexpr (kCodes<C> && __is_same(E, Fp16)) {
+    if (!fp16_holds<C>(a, w, reinterpret_cast<uint32_t*>(lds), w.step0 * kKeys, min(w.step1 * kKeys, w.vis.len))) {
+      const int col0 = w.col0, ncol = w.ncol;
+      w.vis = visible(w.vis.len, 0, 0);
+      w.step0 *= kKeys / kStep, w.step1 = min(w.step1 * (kKeys / kStep), w.vis.steps);
+#pragma unroll 1
+      for (int c = 0; c < ncol; c += 2 * kGroups) {
+        if (c) __syncthreads();  // (the last columns' sums are read from LDS)
+        w.col0 = col0 + c, w.ncol = min(2 * kGroups, ncol - c);
+        attend<E, C, D, true, 2, true>(a, *reinterpret_cast<PagedLds<D>*>(lds), w, true);
+      }
+      return;
     }
   }
   hi = sees(hi, min(w.step1 * kKeys, w.vis.len));

@@ -493,8 +493,9 @@ int solattn_paged_attn(const uint16_t* q, int64_t sq_b, int64_t sq_h, const uint
  * holds a NaN or an infinity reads as NaN in every channel. Its byte is
  * 255, with codes 0 or e4m3's NaN; zeros have byte 0 and codes 0. Other codes beside these
  * two bytes mean nothing.
- * A value is exact in 16 bits: in bf16, and in fp16 within fp16's range (an fp16 call
- * may round values below 2^-14 and those from 65520 on to infinities).
+ * A value is exact in 16 bits: in bf16, and in fp16 within fp16's range. An fp16 read, and
+ * an fp16 call over shared keys, may round values below 2^-14; a read rounds those from
+ * 65520 on to infinities, a call takes them as they are.
  *
  * solattn_qk_norm_rope_append with such a cache; k' is rounded once, from fp32. */
 int solattn_qk_norm_rope_append8(

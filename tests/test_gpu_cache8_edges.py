@@ -133,3 +133,37 @@ def test_shared_keys_behind_the_end_of_a_sequence(paged, dev, kind, case, poison
             ref.close(got[safe], o[safe], tol[safe], "sequences that end before it")
             if which == "v":  # (an infinity in k may be a score of minus infinity)
                 assert not torch.isfinite(got[~safe]).flatten(1).all(1).any()
+
+
+# ------------------------------------------------------- values that fp16 does not have
+@CODES
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B", [5, 20, 40])  # 10 columns, 40, 80 (by tiles of 128 rows)
+def test_fp16_queries_over_values_beyond_fp16(paged, cache, dev, kind, D, B):
+    """fp16 rows at the type's largest value, which their codes round up beyond it, and rows of a bf16
+    model far beyond: finite results, the same whatever the number of columns."""
+    H, Hkv, page, L = 4, 2, 16, 700
+    most = -(-L // page)
+    table = torch.arange(most, dtype=torch.int32, device=dev)[None].repeat(B, 1)
+    n = ints([L] * B, dev)
+    q = randn((B, 1, H, D), 3, dev, FP)
+    q[..., 5] = 0
+    for dtype, top, keys in ((FP, 65504.0, L), (BF, 1e6, L), (FP, 65504.0, 1)):
+        k, v = (randn((1, L, Hkv, D), s, dev, F32) for s in (1, 2))
+        k[:, 7:7 + keys:3, :, 5] = top       # no query looks at this channel
+        v[:, 10:10 + keys:7, :, 3] = top / 8  # a seventh of the weights: within fp16 together
+        v[:, 400:400 + keys:7, 0, 9] = -top / 8
+        v[:, 100, :, 11] = top
+        v[:, 300, :, 11] = -top
+        (kc, ks), (vc, vs) = (c8.empty(most, page, Hkv, D, kind, dev) for _ in "kv")
+        cache.cache_append(k.to(dtype), v.to(dtype), kc, vc, table[:1], n[:1], ks, vs)
+        rows = [c8.values(c.flatten(0, 1)[:L], raw(s).transpose(1, 2).flatten(0, 1)[:L])[None].expand(B, -1, -1, -1)
+                for c, s in ((kc, ks), (vc, vs))]
+        assert rows[0].abs().max() > 65520 and rows[1].abs().max() > 65520
+        o, p, (_, _, vh) = ref.attention(q, *rows, seen(n, L), D ** -0.5)
+        assert o.abs().max() < 65000
+        apart = paged.paged_attn(q, kc, vc, table, n, k_scale=ks, v_scale=vs)
+        ref.close(apart, o, c8.forward_bound(o, p, vh, FP), "not shared")
+        for shared in (L, 333):
+            got = paged.paged_attn(q, kc, vc, table, n, shared=shared, k_scale=ks, v_scale=vs)
+            ref.close(got, o, bound(kind, o, p, vh, FP, B * (H // Hkv), D), f"{dtype}, {shared} shared")
