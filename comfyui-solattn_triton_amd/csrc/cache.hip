@@ -130,7 +130,9 @@ int setup(CacheArgs& a, int64_t B, int64_t T, int64_t Hkv, int64_t D, int dtype,
   constexpr int64_t top = 1ll << 31;
   SOLATTN_REQUIRE(B < top && T < top && Hkv < top && B * T < top && B * T * Hkv < top, SOLATTN_EUNSUPPORTED,
                   "%s: too many tokens or heads", what);
-  SOLATTN_REQUIRE(B * T * Hkv * (D > 64 ? 16 : 8) < 2 * top, SOLATTN_EUNSUPPORTED, "%s: too many rows for one launch", what);
+  static_assert(kThreads == kLaunchThreads, "one bound");
+  SOLATTN_REQUIRE(cdiv(B * T * Hkv, kThreads / (D > 64 ? 16 : 8)) < kMostBlocks, SOLATTN_EUNSUPPORTED,
+                  "%s: too many rows for one launch", what);
   SOLATTN_REQUIRE(a.table && a.lengths, SOLATTN_EINVAL, "%s: null page table or lengths", what);
   SOLATTN_REQUIRE(pages >= 0 && pages < top && page_size > 0 && page_size < top && max_pages >= 0 && max_pages < top &&
                       max_pages * page_size < top,

@@ -102,6 +102,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A launch has less than 2^32 threads: workgroups of kLaunchThreads, fewer than kMostBlocks.
+constexpr int kLaunchThreads = 256;
+constexpr int64_t kMostBlocks = (1ll << 32) / kLaunchThreads;
+
 constexpr int kMaxWords = 512;  // mask words of a query block: NT <= 16384 (the forwards' limit)
 // moments_kernel's 32-bit offsets into the |v| maxima: heads that a V scale can have.
 constexpr int kMaxVScaleHeads = 32768;

@@ -970,9 +970,9 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
     a.by_ptiles = divisor(c.ptiles), a.by_psplit = divisor(c.psplit), a.by_group = divisor(a.group);
   }
   const bool wide = p.cache_type != 0 || p.shared != 0;  // (the others keep their order of sums)
-  constexpr int64_t most = (1ll << 32) / (kWaves * 64);  // (a launch has less than 2^32 threads)
-  static_assert(kJoinThreads == kWaves * 64, "one bound");
-  SOLATTN_REQUIRE(grid < most && (!wide || B * H < most), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
+  const int64_t join_grid = a.parts == 1 ? 0 : wide ? B * H : cdiv(B * H, 4);
+  static_assert(kJoinThreads == kLaunchThreads && kWaves * 64 == kLaunchThreads, "one bound");
+  SOLATTN_REQUIRE(grid < kMostBlocks && join_grid < kMostBlocks, SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   // More workgroups than are there at once: those of the longest sequences first, so that none
   // of theirs begin when the others end (32 ragged sequences of bf16 keys 69 -> 63 us, eight
   // over e4m3 72 -> 66, four of up to 131072 144 -> 138).
@@ -984,11 +984,11 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   if (a.parts == 1) return SOLATTN_OK;
   if (!wide) {
     hipLaunchKernelGGL(bf ? paged_join_kernel<Bf16> : paged_join_kernel<Fp16>,
-                       dim3(static_cast<uint32_t>(cdiv(B * H, 4))), dim3(256), 0, s, a);
+                       dim3(static_cast<uint32_t>(join_grid)), dim3(256), 0, s, a);
     return check_launch(what);
   }
   const auto join = bf ? wide_join_of<Bf16>(D, a.parts) : wide_join_of<Fp16>(D, a.parts);
-  hipLaunchKernelGGL(join, dim3(static_cast<uint32_t>(B * H)), dim3(kJoinThreads), 0, s, a);
+  hipLaunchKernelGGL(join, dim3(static_cast<uint32_t>(join_grid)), dim3(kJoinThreads), 0, s, a);
   return check_launch(what);
 }
 

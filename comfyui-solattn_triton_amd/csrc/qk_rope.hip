@@ -447,7 +447,8 @@ int64_t wave_count(const RopeArgs& a) { return (a.tokens * a.split + a.tpw - 1) 
 template <typename KEPT>
 int launch(const RopeArgs& a, int dtype, hipStream_t s, const char* what) {
   const int64_t blocks = cdiv(wave_count(a), kRopeThreads / 64);
-  SOLATTN_REQUIRE(blocks < (1ll << 31), SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
+  static_assert(kRopeThreads == kLaunchThreads, "one bound");
+  SOLATTN_REQUIRE(blocks < kMostBlocks, SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   const dim3 grid(static_cast<uint32_t>(blocks)), block(kRopeThreads);
   const bool wide = a.D > 64;
   const auto kern = dtype == SOLATTN_BF16   ? (wide ? qk_rope_kernel<Bf16, 16, KEPT> : qk_rope_kernel<Bf16, 8, KEPT>)

@@ -100,6 +100,28 @@ def test_paged_refusals(capi, kw, rc, text):
     _said(capi, _paged(capi.LIB, **kw), rc, text)
 
 
+def test_launches_of_2_to_the_32_threads(capi):
+    """The fewest rows whose workgroups, rounded up, are 2^24 of 256 threads; nothing is launched before a
+    join that cannot be."""
+    L, s = capi.LIB, (512, 512, 128)
+    for D, T in ((128, (1 << 28) - 15), (64, (1 << 29) - 31)):
+        o, ss = _cache_args(dict(D=D, T=T, B=1, Hkv=1)), (128, 16)
+        rest = (o["pages"], o["page"], o["ct"], A, *ss, A, *ss, A, 4, o["most"], A)
+        _said(capi, L.solattn_cache_append(A, *s, A, *s, 1, T, 1, D, 0, A, *o["cs"], A, *o["cs"], *rest, None), EUNSUPPORTED,
+              b"one launch")
+        _said(capi, L.solattn_cache_read(A, *o["cs"], A, *o["cs"], *rest, None, 1, T, 1, D, 0, A, *s, A, *s, None), EUNSUPPORTED,
+              b"one launch")
+    T = (1 << 26) - 3  # a wave a token
+    _said(capi, L.solattn_qk_norm_rope_append8(
+        A, *s, A, *s, A, *s, 1, T, 4, 4, 128, 0, A, A, None, None, 0, 0, 0, 1e-6, A, *s, A, *s, A, *s, 4, 16, 1, A, 64, 16, A, 64, 16,
+        A, 2, 2, A, None), EUNSUPPORTED, b"grid")
+    _said(capi, L.solattn_qk_norm_rope(A, *s, A, *s, 1, T, 4, 4, 128, 0, A, A, None, None, 0, 0, 0, None, 0, 1e-6, A, *s, A, *s, None),
+          EUNSUPPORTED, b"grid")
+    # 2^23 workgroups of two parts, 2^26 rows to join, four a workgroup; over codes a workgroup each
+    for ct, B in ((0, 1 << 22), (1, 1 << 20)):
+        _said(capi, _paged(L, ct=ct, B=B, H=16, Hkv=1, most=512, need=TOP), EUNSUPPORTED, b"grid")
+
+
 def test_paged_workspace(capi):
     """A row's parts over shared keys and over its own, 64 at most of each; sizes that no call takes have none."""
     L = capi.LIB
