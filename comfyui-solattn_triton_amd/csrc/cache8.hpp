@@ -130,7 +130,7 @@ struct Fp8Codes {
     for (int h = 0; h < 2; ++h) {
       const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h] * unit, x[4 * h + 1] * unit, 0, false);
       w[h] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h + 2] * unit, x[4 * h + 3] * unit, lo, true));
-      if (bad) w[h] = 0x7F7F7F7Fu;
+      if (unit == 0.f) w[h] = bad ? 0x7F7F7F7Fu : 0u;  // (a row of zeros: without the signs that -x * 0 has)
     }
     return make_uint2(w[0], w[1]);
   }

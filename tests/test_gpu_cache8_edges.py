@@ -167,3 +167,19 @@ def test_fp16_queries_over_values_beyond_fp16(paged, cache, dev, kind, D, B):
         for shared in (L, 333):
             got = paged.paged_attn(q, kc, vc, table, n, shared=shared, k_scale=ks, v_scale=vs)
             ref.close(got, o, bound(kind, o, p, vh, FP, B * (H // Hkv), D), f"{dtype}, {shared} shared")
+
+
+# ----------------------------------------------------------------- codes of nothing
+@CODES
+def test_rows_of_next_to_nothing_are_codes_of_zero(rope, cache, dev, kind):
+    """Byte 0 goes with codes 0, whatever the signs of the values were."""
+    x = -torch.full((1, 3, 1, 32), 2.0 ** -112, device=dev)
+    x[0, 1] = -0.0
+    x[0, 2, 0, 1::2] *= -1
+    table, n = torch.zeros(1, 1, dtype=torch.int32, device=dev), ints([3], dev)
+    for write in (lambda *c: cache.cache_append(x, x, c[0], c[2], table, n, c[1], c[3]),
+                  lambda *c: rope.qk_norm_rope_append(x, x * 0, x, c[0], c[2], table, n, k_scale=c[1], v_scale=c[3])):
+        (kc, ks), (vc, vs) = (c8.empty(1, 8, 1, 32, kind, dev) for _ in "kv")
+        write(kc, ks, vc, vs)
+        for codes, byte in ((kc, ks), (vc, vs)):
+            assert (raw(codes)[0, :3] == 0).all() and (raw(byte)[0, 0, :3] == 0).all()
