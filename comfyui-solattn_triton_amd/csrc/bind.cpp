@@ -421,7 +421,7 @@ Tensor qk_norm_rope_append(const Tensor& q0, const Tensor& k0, const Tensor& v0,
   const int64_t pages = none ? 0 : k_cache.size(0), page = k_cache.size(1);
   const c10::OptionalDeviceGuard guard(q.device());
   if (codes) {
-    const Tensor &ks = none ? table : *k_scale, &vs = none ? table : *v_scale;
+    const Tensor &ks = none ? q : *k_scale, &vs = none ? q : *v_scale;
     const auto stride = [none](const Tensor& t, int d) { return none ? 0 : t.stride(d); };
     check(lib.qk_norm_rope_append8(
               ptr(q), STRIDES(q), ptr(k), STRIDES(k), ptr(v), STRIDES(v), B, T, H, Hkv, q.size(3), type_code(q),

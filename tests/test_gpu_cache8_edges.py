@@ -183,3 +183,14 @@ def test_rows_of_next_to_nothing_are_codes_of_zero(rope, cache, dev, kind):
         write(kc, ks, vc, vs)
         for codes, byte in ((kc, ks), (vc, vs)):
             assert (raw(codes)[0, :3] == 0).all() and (raw(byte)[0, 0, :3] == 0).all()
+
+
+def test_append_without_pages_anywhere(rope, cache, dev):
+    """A cache without pages and tables without columns: q', and nothing is written."""
+    (kc, ks), (vc, vs) = (c8.empty(0, 16, 2, 64, I8, dev) for _ in "kv")
+    y = randn((2, 1, 2, 64), 1, dev)
+    t, n = torch.zeros(2, 0, dtype=torch.int32, device=dev), ints([5, 0], dev)
+    got = rope.qk_norm_rope_append(y, y, y, kc, vc, t, n, k_scale=ks, v_scale=vs)
+    same = [torch.zeros(0, 16, 2, 64, dtype=BF, device=dev) for _ in "kv"]
+    assert torch.equal(got, rope.qk_norm_rope_append(y, y, y, *same, t, n))
+    cache.cache_append(y, y, kc, vc, t, n, ks, vs)
