@@ -194,3 +194,134 @@ def test_append_without_pages_anywhere(rope, cache, dev):
     same = [torch.zeros(0, 16, 2, 64, dtype=BF, device=dev) for _ in "kv"]
     assert torch.equal(got, rope.qk_norm_rope_append(y, y, y, *same, t, n))
     cache.cache_append(y, y, kc, vc, t, n, ks, vs)
+
+
+# --------------------------------------- runs that are shorter than the shared keys said
+@KINDS
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shared", [1, 64, 500, 5000, 2 ** 40])
+@pytest.mark.parametrize("groups,lengths", [
+    (1, [33, 640, 1, 0, 500, 64]), (2, [33, 600, 640, 0, 0, -4]), (2, [0, 0, 0, 500, 4200, 64]), (3, [1, 0, 9000, 8999, 0, 63]),
+], ids=["one", "idle behind", "idle before", "three"])
+def test_tiles_of_shorter_runs(paged, dev, kind, D, shared, groups, lengths):
+    """More than 64 columns: the longest of a run is not the first, a run is idle beside a live one,
+    `shared` is more than any sequence holds, so that parts leave and page ids are found again."""
+    B, H, Hkv, page, L = len(lengths), 128, 2, 16, max(lengths)
+    per = B // groups
+    if per * (H // Hkv) <= 64:
+        pytest.fail("no tiles")
+    k, v = (randn((groups, L, Hkv, D), s, dev, F32) for s in (1, 2))
+    at = [b // per for b in range(B)]
+    k, v = k.repeat_interleave(per, 0), v.repeat_interleave(per, 0)
+    pages = Pages(k, v, [a * per for a in at], page, kind, BF)
+    n, q = ints(lengths, dev), randn((B, 1, H, D), 3, dev)
+    got = pages.attn(paged, q, n, shared=shared, groups=groups)
+    on = seen(n, L)
+    o, p, (_, _, vh) = ref.attention(q, *pages.rows, on, D ** -0.5)
+    ref.close(got, o, bound(kind, o, p, vh, BF, per * (H // Hkv), D), "o")
+    assert (got[n <= 0] == 0).all()
+    assert torch.equal(pages.attn(paged, q, n, shared=shared, groups=groups), got), "the same bits again"
+
+
+@KINDS
+@pytest.mark.parametrize("H,Hkv,D", [(2, 1, 128), (20, 2, 64), (64, 2, 64), (64, 2, 128), (64, 2, 80)])
+def test_idle_slots_beside_poison(paged, dev, kind, H, Hkv, D):
+    """NaN in the shared values reaches those that see them, not the idle slots beside them."""
+    k, v = (randn((1, 320, Hkv, D), s, dev, F32).repeat(5, 1, 1, 1) for s in (1, 2))
+    v[:, 53] = float("nan")
+    pages = Pages(k, v, [0] * 5, 16, kind, BF)
+    got = pages.attn(paged, randn((5, 1, H, D), 3, dev), ints([320, 0, 300, 0, 0], dev), shared=290)
+    assert got[[0, 2]].isnan().all() and (got[[1, 3, 4]] == 0).all()
+
+
+# ------------------------------------------------------------- bounds, sizes, places
+@CODES
+@pytest.mark.parametrize("per,prefix,rest,page,H,Hkv,D,dtype", [
+    (6, 700, 40, 16, 9, 3, 128, BF), (8, 4100, 30, 64, 24, 8, 128, BF), (16, 777, 10, 16, 16, 4, 64, FP), (32, 333, 60, 8, 8, 4, 64, BF),
+    (60, 513, 17, 64, 1, 1, 128, FP), (7, 300, 20, 16, 10, 2, 16, BF), (20, 300, 20, 16, 10, 5, 48, FP), (70, 100, 9, 8, 4, 4, 32, BF),
+])
+def test_few_columns_keep_two_parts(paged, dev, kind, per, prefix, rest, page, H, Hkv, D, dtype):
+    """Up to 64 columns, or of other head dims, P is kept in two parts over codes: the bound of that."""
+    L = prefix + rest
+    k, v = (randn((1, L, Hkv, D), s, dev, F32).repeat(per, 1, 1, 1) for s in (1, 2))
+    pages = Pages(k, v, [0] * per, page, kind, dtype)
+    q, n = randn((per, 1, H, D), 3, dev, dtype, 2.0), ints([L - b % rest for b in range(per)], dev)
+    o, p, (_, _, vh) = ref.attention(q, *pages.rows, seen(n, L), D ** -0.5)
+    ref.close(pages.attn(paged, q, n, shared=prefix), o, c8.forward_bound(o, p, vh, dtype), "o")
+
+
+@KINDS
+@pytest.mark.parametrize("B,groups,shared,H,Hkv,D", [
+    (6, 1, 0, 8, 2, 128), (40, 1, 0, 16, 4, 64), (8, 1, 1000, 24, 8, 128), (32, 4, 700, 16, 4, 64), (60, 1, 900, 24, 8, 128),
+    (30, 1, 900, 24, 8, 96),
+])
+def test_wide_tables(paged, dev, kind, B, groups, shared, H, Hkv, D):
+    """Tables far wider than any sequence is long: many parts, most of them without keys."""
+    page, L = 16, 1200
+    per = B // groups
+    at = [b // per * per for b in range(B)]
+    k, v = (randn((B, L, Hkv, D), s, dev, F32) for s in (1, 2))
+    for x in (k, v):
+        x[:, :shared] = x[at, :shared]
+    pages = Pages(k, v, range(B), page, kind, BF, wide=2000 // B * 8)
+    n = ints([L - 13 * (b % 10) for b in range(B)], dev)
+    pages.table[:, -(-L // page):] = -7
+    q = randn((B, 1, H, D), 3, dev)
+    o, p, (_, _, vh) = ref.attention(q, *pages.rows, seen(n, L), D ** -0.5)
+    ref.close(pages.attn(paged, q, n, shared=shared, groups=groups), o, bound(kind, o, p, vh, BF, per * (H // Hkv), D), "o")
+
+
+@KINDS
+@pytest.mark.parametrize("far", ["pages", "slots"])
+@pytest.mark.parametrize("B", [2, 20, 40])  # 4, 40 and 80 columns
+def test_strides_beyond_32_bits(paged, dev, kind, far, B):
+    """Pages 2^32 bytes apart, and slots 2^28 apart, as a view into a larger cache has them."""
+    H, Hkv, D, page, pages = 4, 2, 64, 8, 3
+    dtype = BF if kind is None else kind
+    size = 2 if kind is None else 1
+    strides = ((1 << 32) // size, Hkv * D, D, 1) if far == "pages" else ((1 << 31) // size, (1 << 28) // size, D, 1)
+    extent = sum((a - 1) * b for a, b in zip((pages, page, Hkv, D), strides)) + 1
+    k, v = (randn((1, pages * page, Hkv, D), s, dev, F32) for s in (1, 2))
+    held, scales, rows = [], {}, []
+    for name, x in (("k", k), ("v", v)):
+        view = torch.empty(extent, dtype=dtype, device=dev).as_strided((pages, page, Hkv, D), strides)
+        if kind is None:
+            view.copy_(x.view(pages, page, Hkv, D))
+            x = x.to(dtype).double()
+        else:
+            c, e = c8.encode(x, kind)
+            raw(view).copy_(raw(c).view(pages, page, Hkv, D))
+            scales[f"{name}_scale"] = e.view(pages, page, Hkv).transpose(1, 2).contiguous().view(c8.E8)
+            x = c8.values(c, e)
+        held.append(view)
+        rows.append(x.expand(B, -1, -1, -1))
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None].repeat(B, 1)
+    n = ints([24 - b % 5 for b in range(B)], dev)
+    q = randn((B, 1, H, D), 3, dev)
+    o, p, (_, _, vh) = ref.attention(q, *rows, seen(n, 24), D ** -0.5)
+    for shared in (0, 17):
+        print("[far]", kind, far, B, shared, flush=True)
+        got = paged.paged_attn(q, *held, table, n, shared=shared, **scales)
+        ref.close(got, o, bound(kind, o, p, vh, BF, B * 2, D), "o")
+
+
+@KINDS
+def test_tiles_captured_and_replayed(paged, dev, kind):
+    """A captured call over tiles, replayed on other lengths, queries and tables with eager work between the
+    replays: the eager bits every time."""
+    B, H, Hkv, D, page, L, shared = 24, 24, 8, 128, 16, 800, 600
+    k, v = (randn((1, L, Hkv, D), s, dev, F32).repeat(B, 1, 1, 1) for s in (1, 2))
+    pages = Pages(k, v, [0] * B, page, kind, FP)
+    q, n = randn((B, 1, H, D), 3, dev, FP), ints([L - b for b in range(B)], dev)
+    pages.attn(paged, q, n, shared=shared)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = pages.attn(paged, q, n, shared=shared)
+    for i in range(4):
+        q.copy_(randn(tuple(q.shape), 10 + i, dev, FP))
+        n.copy_(ints([max(0, L - 30 * i * (b % 24) - b) for b in range(B)], dev))
+        pages.table.copy_(pages.table.roll(1, 1))
+        g.replay()
+        torch.cuda.synchronize()
+        first = out.clone()
+        assert torch.isfinite(first).all() and torch.equal(pages.attn(paged, q, n, shared=shared), first)
