@@ -70,7 +70,7 @@ struct PagedArgs {
                              // here, the others `length` keys (null: all of them)
   int length, pages, page, max_pages;
   Divisor by_page;
-  int ranked;                // longest sequences first
+  int ranked;                // longest sequences first, where one has that many keys (0: never)
   int near;                  // pages' and slots' strides are within 32 bits
   uint16_t* o;
   int64_t so_b, so_h;
@@ -143,22 +143,37 @@ __device__ __forceinline__ int sequence_length(const PagedArgs& a, int b) {
 }
 
 // The sequence with the r-th largest length of up to 256 (of as many times 128 keys: the
-// first), r from 0: built bit by bit from what lanes with up to four sequences each say.
+// first), r from 0: built bit by bit from what lanes with up to four sequences each say. Where
+// none has `ranked` keys, or the longest is not a quarter above the mean, sequence r: there is
+// nothing to gain, and the search takes its own time.
 constexpr int kRanked = 256;
 __device__ __forceinline__ int by_length(const PagedArgs& a, int r) {
+  constexpr int U = kRanked / 64;
   const int lane = threadIdx.x & 63;
-  uint32_t key[kRanked / 64];  // unique; 0 is none (sequence 255 of length 0 is the last in any case)
+  int len[U];
+  bool few = true;
 #pragma unroll
-  for (int u = 0; u < kRanked / 64; ++u) {
+  for (int u = 0; u < U; ++u) len[u] = 64 * u < a.B ? a.lengths[min(lane + 64 * u, a.B - 1)] : 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) few = few && !__any(len[u] >= a.ranked);
+  if (few) return r;
+  uint32_t key[U], top = 0, total = 0;  // keys: unique; 0 is none (sequence 255 of length 0 is the last in any case)
+  const int cap = a.max_pages * a.page;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
     const int i = lane + 64 * u;
-    key[u] = 64 * u < a.B && i < a.B ? static_cast<uint32_t>(sequence_length(a, i)) / 128 << 8 | (kRanked - 1 - i) : 0u;
+    key[u] = i < a.B ? static_cast<uint32_t>(min(max(len[u], 0), cap)) / 128 << 8 | (kRanked - 1 - i) : 0u;
+    top = max(top, key[u]), total += key[u] >> 8;
   }
+  top = __builtin_amdgcn_readfirstlane(over_wave(top, [](uint32_t x, uint32_t y) { return max(x, y); }));
+  total = __builtin_amdgcn_readfirstlane(over_wave(total, [](uint32_t x, uint32_t y) { return x + y; }));
+  if (4ull * a.B * (top >> 8) <= 5ull * total) return r;
   uint32_t nth = 0;
-  for (int bit = 39 - __builtin_clz(static_cast<uint32_t>(a.max_pages) * a.page / 128 | 1); bit >= 0; --bit) {
+  for (int bit = 31 - __builtin_clz(top | 1); bit >= 0; --bit) {
     const uint32_t with = nth | 1u << bit;
     int n = 0;
 #pragma unroll
-    for (int u = 0; u < kRanked / 64; ++u)
+    for (int u = 0; u < U; ++u)
       if (64 * u < a.B) n += __popcll(__ballot(key[u] >= with));
     if (n > r) nth = with;
   }
@@ -498,9 +513,9 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
   }
 
   // Join the waves, a tile of columns at a time: O[q][channel], channel CH (4 g + i) + j in
-  // acc[j][i]. A thread takes eight channels of a column.
-  constexpr int L = DP / 8;
-  const int qc = threadIdx.x / L, ch = 8 * (threadIdx.x % L);
+  // acc[j][i]. A thread takes four channels of a column.
+  constexpr int L = DP / 4;
+  const int ch = 4 * (threadIdx.x % L);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t) __syncthreads();
@@ -516,34 +531,30 @@ __device__ __forceinline__ void attend(const PagedArgs& a, PagedLds<DP>& lds, Wo
       lds.l[wave][col] = sum_l;
     }
     __syncthreads();
-    if (qc >= min(kGroups, w.ncol - 16 * t) || (!kFull && ch >= a.D)) continue;
-    float top = lds.m[0][qc];
+    if (!kFull && ch >= a.D) continue;
+    for (int qc = threadIdx.x / L; qc < min(kGroups, w.ncol - 16 * t); qc += kWaves * 64 / L) {
+      float top = lds.m[0][qc];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds.m[i][qc]);
-    float o[8] = {}, sum = 0.f;
+      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, lds.m[i][qc]);
+      float o[4] = {}, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float f = weight_of(lds.m[i][qc], top);
-      const float4 x = *reinterpret_cast<const float4*>(&lds.o[i][qc][ch]);
-      const float4 y = *reinterpret_cast<const float4*>(&lds.o[i][qc][ch + 4]);
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
-      sum = fmaf(lds.l[i][qc], f, sum);
-    }
-    int b, h;
-    w.row(a, 16 * t + qc, MANY, b, h);
-    if (a.parts > 1) {
-      const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
-      float4* to = reinterpret_cast<float4*>(a.part + at * a.D + ch);
-      to[0] = make_float4(o[0], o[1], o[2], o[3]);
-      to[1] = make_float4(o[4], o[5], o[6], o[7]);
-      if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
-    } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
-      *reinterpret_cast<uint4*>(a.o + b * a.so_b + h * a.so_h + ch) =
-          make_uint4(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv), E::pack(o[4] * inv, o[5] * inv),
-                     E::pack(o[6] * inv, o[7] * inv));
+      for (int i = 0; i < kWaves; ++i) {
+        const float f = weight_of(lds.m[i][qc], top);
+        const float4 x = *reinterpret_cast<const float4*>(&lds.o[i][qc][ch]);
+        o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]), o[2] = fmaf(x.z, f, o[2]), o[3] = fmaf(x.w, f, o[3]);
+        sum = fmaf(lds.l[i][qc], f, sum);
+      }
+      int b, h;
+      w.row(a, 16 * t + qc, MANY, b, h);
+      if (a.parts > 1) {
+        const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.parts + w.part;
+        *reinterpret_cast<float4*>(a.part + at * a.D + ch) = make_float4(o[0], o[1], o[2], o[3]);
+        if (ch == 0) *reinterpret_cast<float2*>(a.part + a.part_ml + 2 * at) = make_float2(top, sum);
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zeros
+        *reinterpret_cast<uint2*>(a.o + b * a.so_b + h * a.so_h + ch) =
+            make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
+      }
     }
   }
 }
@@ -653,7 +664,9 @@ paged_kernel(const PagedArgs a) {
   constexpr size_t kLds = kTileLds > sizeof(PagedLds<DP>) ? kTileLds : sizeof(PagedLds<DP>);
   __shared__ __align__(256) uint8_t lds_bytes[kLds];
   PagedLds<DP>& lds = *reinterpret_cast<PagedLds<DP>*>(lds_bytes);
-  fetch_arguments(a);
+  // (over 16-bit pages the compiler's own loads are sooner done, 128 sequences of 128 keys 14.9 ->
+  // 14.5 us; over codes and behind shared keys they are not, 39.4 -> 39.0)
+  if constexpr (PT > 0 || kCodes<C>) fetch_arguments(a);
   uint32_t n = blockIdx.x;
   Work w;
   if constexpr (PT > 0) {
@@ -975,8 +988,14 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   SOLATTN_REQUIRE(grid < kMostBlocks && join_grid < kMostBlocks, SOLATTN_EUNSUPPORTED, "%s: grid too large", what);
   // More workgroups than are there at once: those of the longest sequences first, so that none
   // of theirs begin when the others end (32 ragged sequences of bf16 keys 69 -> 63 us, eight
-  // over e4m3 72 -> 66, four of up to 131072 144 -> 138).
-  a.ranked = a.table && c.psplit == 0 && B > 1 && B <= kRanked && grid > 1024;
+  // over e4m3 72 -> 66, four of up to 131072 144 -> 138). Only where a sequence is long enough
+  // that the batch holds some 2^26 values of k, and the longer the more sequences there are to
+  // search: 128 ragged ones of up to 4096 bf16 keys of 8 heads 223 -> 199, of up to 512 29 -> 32;
+  // 256 of up to 128 16.6 -> 21.9, behind tables of 32768 keys 44 -> 98 (looked at and left: 48).
+  int64_t from = cdiv(1ll << 27, B * Hkv * D);
+  if (from < 4 * B) from = 4 * B;
+  const bool ranked = p.table && c.psplit == 0 && B > 1 && B <= kRanked && grid > 1024 && from <= p.max_pages * p.page_size;
+  a.ranked = ranked ? static_cast<int>(from) : 0;
   const bool bf = p.dtype == SOLATTN_BF16;
   const auto kern = bf ? kernel_of<Bf16>(D, c.ctiles, p.cache_type) : kernel_of<Fp16>(D, c.ctiles, p.cache_type);
   hipLaunchKernelGGL(kern, dim3(static_cast<uint32_t>(grid)), dim3(kWaves * 64), 0, s, a);

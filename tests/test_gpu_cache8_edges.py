@@ -325,3 +325,38 @@ def test_tiles_captured_and_replayed(paged, dev, kind):
         torch.cuda.synchronize()
         first = out.clone()
         assert torch.isfinite(first).all() and torch.equal(pages.attn(paged, q, n, shared=shared), first)
+
+
+@KINDS
+@pytest.mark.parametrize("B,H,Hkv,D,page,lengths", [
+    (64, 8, 8, 128, 16, "ragged 3000"), (64, 8, 8, 128, 64, "equal 2500"), (64, 16, 8, 128, 16, "one 3000"), (64, 8, 8, 128, 16, "ragged 1000"),
+    (256, 4, 4, 128, 16, "ragged 1400"), (5, 32, 32, 128, 64, "ragged 7000"), (130, 8, 8, 64, 8, "ragged 2500"),
+])
+def test_longest_first(paged, dev, kind, B, H, Hkv, D, page, lengths):
+    """Batches whose workgroups go by length, and those that do not: few keys, sequences of one length; idle
+    slots, lengths past the table and below 0 among them."""
+    how, L = lengths.split()
+    L = int(L)
+    g = torch.Generator().manual_seed(B)
+    n = {"ragged": torch.randint(0, L, (B,), generator=g), "equal": torch.full((B,), L), "one": torch.full((B,), 5)}[how].int()
+    n[B // 3] = L
+    if how == "ragged":
+        n[1], n[B - 1] = 0, -9
+    want = n.clamp(0, L)
+    if how == "ragged":
+        n[B // 3] = 2 ** 31 - 1
+    k, v = (randn((1, L, Hkv, D), s, dev, F32).expand(B, -1, -1, -1).clone() for s in (1, 2))
+    k *= 1 + torch.arange(B, device=dev)[:, None, None, None] % 5 / 4
+    v += torch.arange(B, device=dev)[:, None, None, None] % 7 - 3
+    most = -(-L // page)
+    want = torch.where(n > L, torch.tensor(most * page), want).to(dev)
+    k, v = (torch.nn.functional.pad(x, (0, 0, 0, 0, 0, most * page - L)) for x in (k, v))
+    pages = Pages(k, v, range(B), page, kind, BF)
+    q = randn((B, 1, H, D), 3, dev)
+    got = pages.attn(paged, q, n.to(dev))
+    on = seen(want, most * page)
+    for b0 in range(0, B, 16):
+        s = slice(b0, b0 + 16)
+        o, p, (_, _, vh) = ref.attention(q[s], *(x[s] for x in pages.rows), on[s], D ** -0.5)
+        ref.close(got[s], o, bound(kind, o, p, vh, BF, 1, D), "o")
+    assert (got[want == 0] == 0).all()
