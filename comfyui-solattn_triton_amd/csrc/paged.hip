@@ -923,7 +923,9 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
                       (!p.table || p.page_size % 8 == 0),
                   SOLATTN_EINVAL, "%s: %lld pages of %lld (a multiple of 8)", what, (long long)p.pages,
                   (long long)p.page_size);
-  SOLATTN_REQUIRE(p.page_size < (1ll << 31) && p.max_pages < (1ll << 31) && p.max_pages * p.page_size < (1ll << 31) - kStep,
+  // (what is counted past the last key: the rest of a step; of shared keys a tile's, or the next of 256 threads' eight)
+  const int64_t past = p.shared ? 8 * kWaves * 64 : kStep;
+  SOLATTN_REQUIRE(p.page_size < (1ll << 31) && p.max_pages < (1ll << 31) && p.max_pages * p.page_size < (1ll << 31) - past,
                   SOLATTN_EUNSUPPORTED, "%s: sequences beyond 2^31 keys", what);
   SOLATTN_REQUIRE(p.shared >= 0 && p.shared < (1ll << 31), SOLATTN_EINVAL, "%s: %lld shared keys", what, (long long)p.shared);
   SOLATTN_REQUIRE(p.shared == 0 || (p.window == 0 && p.sinks == 0), SOLATTN_EINVAL, "%s: shared keys and a window", what);

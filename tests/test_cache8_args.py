@@ -91,7 +91,8 @@ def _paged(L, B=4, H=4, Hkv=2, D=128, dtype=0, ct=1, page=16, pages=9, most=64, 
     (dict(shared=5, groups=0), EINVAL, b"groups"), (dict(shared=5, groups=3), EINVAL, b"groups"), (dict(page=12), EINVAL, b"multiple of 8"),
     (dict(dtype=2), EINVAL, b"dtype"), (dict(H=3), EINVAL, b"heads"), (dict(B=1 << 31, shared=4), EUNSUPPORTED, b"grid"),
     (dict(B=1 << 30, H=1, Hkv=1, shared=4, groups=1 << 30), EUNSUPPORTED, b"grid"), (dict(B=1 << 24, H=1, Hkv=1, need=TOP), EUNSUPPORTED, b"grid"),
-    (dict(scale=0.0), EINVAL, b"scale"),
+    (dict(scale=0.0), EINVAL, b"scale"), (dict(most=(1 << 27) - 2), EUNSUPPORTED, b"2^31 keys"),
+    (dict(most=(1 << 27) - 128, shared=4), EUNSUPPORTED, b"2^31 keys"), (dict(most=(1 << 27) - 3, shared=4), EUNSUPPORTED, b"2^31 keys"),
     (dict(shared=500, need=0), ESIZE, b"workspace"), (dict(shared=500, ws=A + 16), EINVAL, b"256"), (dict(q=A + 8), EINVAL, b"aligned"),
 ])
 def test_paged_refusals(capi, kw, rc, text):
