@@ -35,7 +35,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ``lengths`` (int32 [B]) counts them too: token t is at position lengths[b] - T + t, slot
     position % page_size of page ``page_table[b, position // page_size]``. A token before
     position 0, past the page table or on a page id that the cache does not have writes
-    nothing. Has no gradient.
+    nothing. No two tokens of a call may have the same slot of the same page: what it holds
+    then is a mixture of both. Has no gradient.
     """
     native.cache_append(k, v, k_cache, v_cache, page_table, lengths, k_scale, v_scale)
 

@@ -6,8 +6,9 @@
 // Of a row with largest magnitude a, 2^(b - 127) is the smallest power of two with
 // a <= 127 2^(b - 127) (int8) or 448 2^(b - 127) (e4m3); codes are rounded to nearest
 // even, from 32 bits: by half a step at most, 2^(b - 128) of int8, 2^-4 of a value of e4m3
-// (2^(b - 137) below its smallest normal). Rows below 2^-110 are zeros (b = 0, codes 0). A row with a NaN or an infinity
-// reads as NaN: b = 255 (the bits of an infinity) and codes 0 (int8) or NaN (e4m3).
+// (2^(b - 137) below its smallest normal). Rows below 2^-110 are zeros (b = 0, codes 0).
+// A row with a NaN or an infinity reads as NaN: b = 255 (the bits of an infinity) and codes
+// 0 (int8) or NaN (e4m3).
 #pragma once
 
 #include "elem.hpp"

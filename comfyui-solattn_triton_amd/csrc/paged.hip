@@ -879,10 +879,10 @@ auto kernel_of(int64_t D) {
   if constexpr (PT == kTiled)
     return D == 128 ? paged_kernel<E, C, 128, true, PT> : paged_kernel<E, C, 64, true, PT>;
   else
-  return D == 128 ? paged_kernel<E, C, 128, true, PT>
-         : D == 64 ? paged_kernel<E, C, 64, true, PT>
-         : D > 64  ? paged_kernel<E, C, 128, false, PT>
-                   : paged_kernel<E, C, 64, false, PT>;
+    return D == 128  ? paged_kernel<E, C, 128, true, PT>
+           : D == 64 ? paged_kernel<E, C, 64, true, PT>
+           : D > 64  ? paged_kernel<E, C, 128, false, PT>
+                     : paged_kernel<E, C, 64, false, PT>;
 }
 template <typename E, typename C>
 auto kernel_of(int64_t D, int64_t ctiles) {

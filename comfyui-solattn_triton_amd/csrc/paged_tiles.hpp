@@ -16,7 +16,9 @@
 // step of 16 matrix instructions.) Keys past the end or on pages that are none of the
 // cache's are rows of zeros, and masked. 16-bit values are copied straight into LDS
 // (attend_ring); codes go through registers and become 16-bit values there, once for all
-// the rows that read the tile (attend_codes).
+// the rows that read the tile (attend_codes). P is rounded once to the queries' type, as in
+// the windowed forward: a second part would double the products with V, half of what bounds
+// a tile.
 #pragma once
 
 #include "cache8.hpp"

@@ -393,7 +393,8 @@ int solattn_qk_norm_rope(const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h
  * v as it is, to slot position % page_size of page page_table[b][position /
  * page_size]. k_cache, v_cache: [pages][page_size][Hkv][D] with the strides given.
  * Tokens before position 0, past the table, or whose page id is not in
- * [0, pages) are not written (their rows of qo are finite but mean nothing). */
+ * [0, pages) are not written (their rows of qo are finite but mean nothing). No two
+ * tokens of a call may have the same slot of the same page: it holds a mixture of both then. */
 int solattn_qk_norm_rope_append(
     const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_b,
     int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int64_t B,
