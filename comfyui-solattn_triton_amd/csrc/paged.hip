@@ -145,20 +145,27 @@ __device__ __forceinline__ int sequence_length(const PagedArgs& a, int b) {
 // The sequence with the r-th largest length of up to 256 (of as many times 128 keys: the
 // first), r from 0: built bit by bit from what lanes with up to four sequences each say. Where
 // none has `ranked` keys, or the longest is not a quarter above the mean, sequence r: there is
-// nothing to gain, and the search takes its own time.
+// nothing to gain, and the search takes its own time. Its length comes out of the lane that has
+// it: another round of memory would be most of a short sequence's time.
 constexpr int kRanked = 256;
-__device__ __forceinline__ int by_length(const PagedArgs& a, int r) {
+__device__ __forceinline__ int by_length(const PagedArgs& a, int r, int& length) {
   constexpr int U = kRanked / 64;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, cap = a.max_pages * a.page;
   int len[U];
   bool few = true;
 #pragma unroll
   for (int u = 0; u < U; ++u) len[u] = 64 * u < a.B ? a.lengths[min(lane + 64 * u, a.B - 1)] : 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) few = few && !__any(len[u] >= a.ranked);
-  if (few) return r;
+  const auto found = [&](int b) __attribute__((always_inline)) {
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) n = b >> 6 == u ? __builtin_amdgcn_readlane(len[u], b & 63) : n;
+    length = min(max(n, 0), cap);
+    return b;
+  };
+  if (few) return found(r);
   uint32_t key[U], top = 0, total = 0;  // keys: unique; 0 is none (sequence 255 of length 0 is the last in any case)
-  const int cap = a.max_pages * a.page;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = lane + 64 * u;
@@ -167,7 +174,7 @@ __device__ __forceinline__ int by_length(const PagedArgs& a, int r) {
   }
   top = __builtin_amdgcn_readfirstlane(over_wave(top, [](uint32_t x, uint32_t y) { return max(x, y); }));
   total = __builtin_amdgcn_readfirstlane(over_wave(total, [](uint32_t x, uint32_t y) { return x + y; }));
-  if (4ull * a.B * (top >> 8) <= 5ull * total) return r;
+  if (4ull * a.B * (top >> 8) <= 5ull * total) return found(r);
   uint32_t nth = 0;
   for (int bit = 31 - __builtin_clz(top | 1); bit >= 0; --bit) {
     const uint32_t with = nth | 1u << bit;
@@ -177,7 +184,7 @@ __device__ __forceinline__ int by_length(const PagedArgs& a, int r) {
       if (64 * u < a.B) n += __popcll(__ballot(key[u] >= with));
     if (n > r) nth = with;
   }
-  return kRanked - 1 - static_cast<int>(nth & (kRanked - 1));
+  return found(kRanked - 1 - static_cast<int>(nth & (kRanked - 1)));
 }
 
 // The visible keys as steps: first those of the sinks below the window, then the window's.
@@ -704,10 +711,14 @@ paged_kernel(const PagedArgs a) {
   w.hk = a.by_hkv.split(n);
   const int split = a.by_split.split(n);
   w.part = a.psplit + split;
-  w.b = w.seq = a.ranked ? by_length(a, n) : static_cast<int>(n);
+  int len;
+  if (a.ranked)
+    w.b = by_length(a, n, len);
+  else
+    w.b = static_cast<int>(n), len = sequence_length(a, w.b);
+  w.seq = w.b;
   w.col0 = tile * kGroups;
   w.ncol = min(kGroups, a.group - w.col0);
-  const int len = sequence_length(a, w.b);
   int low = PT > 0 ? a.shared : a.window ? max(len - a.window, 0) : 0;
   if constexpr (PT > 0) {
     if (len > 0 && len < all_shared(a)) {  // from where the part begins that it ends in, on the pages of the longest
@@ -992,11 +1003,14 @@ int paged_attn(const PagedCall& p, hipStream_t s, const char* what) {
   // of theirs begin when the others end (32 ragged sequences of bf16 keys 69 -> 63 us, eight
   // over e4m3 72 -> 66, four of up to 131072 144 -> 138). Only where a sequence is long enough
   // that the batch holds some 2^26 values of k, and the longer the more sequences there are to
-  // search: 128 ragged ones of up to 4096 bf16 keys of 8 heads 223 -> 199, of up to 512 29 -> 32;
-  // 256 of up to 128 16.6 -> 21.9, behind tables of 32768 keys 44 -> 98 (looked at and left: 48).
+  // search: 128 ragged ones of up to 4096 bf16 keys of 8 heads 223 -> 199, of up to 512 29 -> 32.
+  // Nor in a launch of 8192 or more, which one workgroup's keys are too little of (256 of up to
+  // 1024 keys of 32 heads 391 -> 394) and which a wide table makes of short sequences (256 of 64
+  // keys behind tables of 32768: 41 us, 48 where their lengths are only looked at).
   int64_t from = cdiv(1ll << 27, B * Hkv * D);
   if (from < 4 * B) from = 4 * B;
-  const bool ranked = p.table && c.psplit == 0 && B > 1 && B <= kRanked && grid > 1024 && from <= p.max_pages * p.page_size;
+  const bool ranked = p.table && c.psplit == 0 && B > 1 && B <= kRanked && grid > 1024 && grid < 8192 &&
+                      from <= p.max_pages * p.page_size;
   a.ranked = ranked ? static_cast<int>(from) : 0;
   const bool bf = p.dtype == SOLATTN_BF16;
   const auto kern = bf ? kernel_of<Bf16>(D, c.ctiles, p.cache_type) : kernel_of<Fp16>(D, c.ctiles, p.cache_type);
