@@ -17,16 +17,17 @@
 // columns whether they exist or not, 256 of their cycles for 16 KiB of a 16-bit cache.
 //   bf16: four sequences of 32768 to 131072 tokens, 24 heads over 8 of 128 channels:
 //     238-251 us, 5.3-5.6 TB/s (a large copy reaches 5.0-5.15); 32 of 512 to 16384, 16
-//     heads of 64 over 4, pages of 16: 63 us; one sequence with a window of 4096: 10.2
-//     us, two launches of the host's (kernels 5.9 and 4.7).
-//   Codes: the four, e4m3: 138 us, 4.9 TB/s, kernel 134. The 32, int8: 38-39 us, 3.6 TB/s,
-//     kernel 29-33 and join 5 (the vector units, 60% busy with a byte's way to a 16-bit
+//     heads of 64 over 4, pages of 16: 64 us; one sequence with a window of 4096: 10.2
+//     us, two launches of the host's (kernels 6.5 and 4.5).
+//   Codes: the four, e4m3: 138 us, 4.9 TB/s, kernel 135. The 32, int8: 39 us, 3.6 TB/s,
+//     kernel 30-37 and join 5 (the vector units, 60% busy with a byte's way to a 16-bit
 //     float, are not what it waits for: fewer of their instructions, or sequences of one
-//     length, took as long). One with a window of 4096: 8.9 us, kernels 6.0 and 2.7.
+//     length, took as long). One with a window of 4096: 8.9 us, kernels 6.1 and 2.8.
 //   Shared keys: 8 sequences of 24 heads over 8 behind 4096 bf16 keys: 13 us (22 as if
 //     nothing was shared), latency: 10.6 of it the kernel, a chain of lengths, page ids,
-//     keys and steps, and 2-4 the join. 64 in groups over int8: 19-20 us (48), latency
-//     beside the conversions. 256 behind 32760 bf16 keys: 167 us (2600), products.
+//     keys and steps, and 2-4 the join. 64 in groups over int8: 19-21 us (48), latency
+//     beside the conversions. 256 behind 32760 bf16 keys: 170-178 us, in some runs up to 192
+//     (2600), products.
 // A wave takes 32 keys at a time straight from HBM into operand registers, no LDS:
 //   S^T = K Q^T (v_mfma_f32_16x16x32): row r of tile t is key 8 (r/4) + 4 t + r%4
 //     of the 32, so lane (q, g) = (lane % 16, lane / 16) gets the scores of the
