@@ -48,8 +48,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
     Hkv, D]. A token before position 0 (an idle slot's length 0), past the page table
     or on a page id that the cache does not have writes nothing, and its q' means
     nothing. No two tokens of a call may have the same slot of the same page: what it
-    holds then is a mixture of both. Positions past the end of ``cos`` turn by its last row: it has to cover
-    the sequences. Has no gradient.
+    holds then is a mixture of both. Positions past the end of ``cos`` turn by its last
+    row: it has to cover the sequences. Has no gradient.
 
     With ``k_scale`` and ``v_scale`` the caches are of 8 bits (``_cache``): k' and v are
     rounded to codes, k' once, from 32 bits.
